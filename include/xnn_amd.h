@@ -16,7 +16,8 @@
  *   - `shift` is the integer image shift packed as three signed 10-bit fields
  *     (x | y << 10 | z << 20), range [-512, 511] per axis.
  *   - `pos` and `cell` share the geometry dtype; per-edge/per-node features use
- *     the compute dtype. Dtype codes: XNN_F32 = 0, XNN_F64 = 1.
+ *     the compute dtype. Dtype codes: XNN_F32 = 0, XNN_F64 = 1; the attention operators
+ *     at the end take XNN_F32, XNN_BF16 = 2 and XNN_F16 = 3 (sums in float32).
  *   - CSR "plans": ptr_dst (N+1) and optional perm_dst (E) list the edges of
  *     every receiver; ptr_src/perm_src list the edges of every sender. A NULL
  *     perm means the edges are already in that order.
@@ -36,7 +37,7 @@ extern "C" {
 typedef struct ihipStream_t* xnn_stream_t; /* == hipStream_t */
 
 enum { XNN_OK = 0, XNN_EINVAL = 1, XNN_ECAPACITY = 2, XNN_EHIP = 3 };
-enum { XNN_F32 = 0, XNN_F64 = 1 };
+enum { XNN_F32 = 0, XNN_F64 = 1, XNN_BF16 = 2, XNN_F16 = 3 };
 enum { XNN_BASIS_BESSEL = 0, XNN_BASIS_GAUSSIAN = 1 };
 /* Envelopes multiply the radial basis and are zero for r >= cutoff (cutoff.py:41, 125);
  * XNN_ENV_NONE is the unit step (r < cutoff) with no smooth decay. */
@@ -1146,6 +1147,105 @@ int xnn_atm_energy_backward_tangent(
  * vectors (bohr). Synchronous; for roofline figures (flops per triangle x triangles). */
 int xnn_atm_count(const void* plan, int64_t n_edges, int64_t n_atoms, int64_t max_tiles,
                   const double* edge_vec, double cutoff, int64_t* counts, xnn_stream_t stream);
+
+/* ---- attention over atoms -------------------------------------------------------------
+ * The operators of an attention block over the atoms of a batch; no counterpart on the
+ * reference's per-edge path. Element types XNN_F32, XNN_BF16 and XNN_F16, arithmetic and sums
+ * in float32, each output rounded once; every sum in a fixed order. */
+
+/* Heads of one projection: element d of head h of token t is
+ * data[t * token_stride + h * head_stride + d] (strides in elements). */
+typedef struct {
+  const void* data;
+  int64_t token_stride, head_stride;
+  int32_t n_heads;
+} xnn_heads;
+
+/* The row tiles of a batch (xnn_attention_plan): three int32 a tile, the first row, the end
+ * and the begin of its structure; max_atoms is the longest structure. */
+typedef struct {
+  int64_t n_tokens, max_atoms, n_tiles64, n_tiles128;
+  const int32_t *tiles64, *tiles128;
+} xnn_attention_tiles;
+
+/* out[t] = scale * table[ids[t]], out (n, n_channels), table (n_rows, n_channels); an id
+ * outside the table gives a row of NaN. */
+int xnn_embedding(int dtype, const int64_t* ids, int64_t n, const void* table, int64_t n_rows,
+                  int64_t n_channels, float scale, void* out, xnn_stream_t stream);
+
+/* Bytes of the workspace of xnn_embedding_grad. */
+int xnn_embedding_grad_work_size(int64_t n, int64_t n_rows, int64_t n_channels, size_t* bytes);
+
+/* grad_table[v] = scale * sum of grad_out[t] over the t with ids[t] = v (zero where there is
+ * none; ids outside the table count nowhere), summed over the sorted ids. `work` is aligned
+ * to 16 bytes. */
+int xnn_embedding_grad(int dtype, const int64_t* ids, int64_t n, const void* grad_out,
+                       int64_t n_rows, int64_t n_channels, float scale, void* grad_table,
+                       void* work, size_t work_bytes, xnn_stream_t stream);
+
+/* out[e] = residual[e] + keep(e) x[e] 65536 / (65536 - drop); residual may be NULL. keep(e):
+ * half word e % 8 (low half of word 0 first) of the Philox4x32-10 block with counter (e / 8,
+ * offset) and key seed is at least `drop` (0 ... 65536). `offset_add` (device, may be NULL) is
+ * added to offset: a captured graph advances it. The gradient of x is the same call on the
+ * cotangent without a residual. */
+int xnn_dropout_add(int dtype, const void* x, const void* residual, int64_t n, int32_t drop,
+                    uint64_t seed, uint64_t offset, const int64_t* offset_add, void* out,
+                    xnn_stream_t stream);
+
+/* Root-mean-square norm of every head of q and k over head_dim (at most 128), times q_weight /
+ * k_weight (head_dim), and the rotation of its first `rotated` elements (even) by the angles
+ * whose cosines and sines are row positions[t] (positions NULL: row t, n_rows = n_tokens) of
+ * cos, sin (n_rows, rotated / 2): pairs (i, i + rotated / 2), or (2 i, 2 i + 1) when
+ * interleaved. q_out (n_tokens, heads, head_dim), k_out with k's heads, contiguous. A position
+ * outside the tables gives NaN. */
+int xnn_head_norm_rotate(int dtype, const xnn_heads* q, const xnn_heads* k, int64_t n_tokens,
+                         int32_t head_dim, int32_t rotated, const void* q_weight,
+                         const void* k_weight, const float* cos, const float* sin, int64_t n_rows,
+                         const int64_t* positions, float eps, int32_t interleaved, void* q_out,
+                         void* k_out, xnn_stream_t stream);
+
+/* Bytes of the workspace of xnn_head_norm_rotate_backward. */
+int xnn_head_norm_rotate_backward_work_size(int32_t head_dim, size_t* bytes);
+
+/* Gradients for the cotangents grad_q, grad_k (contiguous, as the outputs): d_q, d_k
+ * (contiguous), d_q_weight and d_k_weight (both or neither; neither needs no work), d_cos and
+ * d_sin (both or neither; only without positions). */
+int xnn_head_norm_rotate_backward(int dtype, const xnn_heads* q, const xnn_heads* k,
+                                  int64_t n_tokens, int32_t head_dim, int32_t rotated,
+                                  const void* q_weight, const void* k_weight, const float* cos,
+                                  const float* sin, int64_t n_rows, const int64_t* positions,
+                                  float eps, int32_t interleaved, const void* grad_q,
+                                  const void* grad_k, void* d_q, void* d_k, void* d_q_weight,
+                                  void* d_k_weight, float* d_cos, float* d_sin, void* work,
+                                  size_t work_bytes, xnn_stream_t stream);
+
+/* Tiles of 64 and 128 rows of a batch of structures of n_atoms[b] consecutive tokens each: ptr
+ * (B + 1), tile_ptr (2 (B + 1)), the lists of three int32 a tile with room for n_tokens / 64 + B
+ * and n_tokens / 128 + B tiles, and info (5): tiles of 64, tiles of 128, longest structure,
+ * status (0; 1: a negative or too large count; 2: the counts do not sum to n_tokens), sum. */
+int xnn_attention_plan(const int64_t* n_atoms, int64_t n_structures, int64_t n_tokens, int64_t* ptr,
+                       int64_t* tile_ptr, int32_t* tiles64, int64_t capacity64, int32_t* tiles128,
+                       int64_t capacity128, int64_t* info, xnn_stream_t stream);
+
+/* Attention of every token to the tokens of its structure that `mask` (n_tokens bytes, zero
+ * leaves a key out; NULL keeps all) keeps: out_i = sum_j p_ij v_j with p the softmax over j of
+ * scale q_i . k_j; rows without keys are zero. head_dim at most 128; q's heads are a multiple of
+ * those of k and v, which they share in order. out (n_tokens, heads, head_dim) contiguous; lse
+ * (heads, n_tokens) for the backward pass (NULL: not wanted). */
+int xnn_attention(int dtype, const xnn_heads* q, const xnn_heads* k, const xnn_heads* v,
+                  int64_t n_tokens, int32_t head_dim, const xnn_attention_tiles* plan,
+                  const uint8_t* mask, float scale, void* out, float* lse, xnn_stream_t stream);
+
+/* Bytes of the workspace of xnn_attention_backward. */
+int xnn_attention_backward_work_size(int64_t n_tokens, int32_t n_heads, size_t* bytes);
+
+/* Gradients of xnn_attention for the cotangent `grad`, from its inputs and its outputs out and
+ * lse (out, grad, dq, dk and dv contiguous); the probabilities are formed again. */
+int xnn_attention_backward(int dtype, const xnn_heads* q, const xnn_heads* k, const xnn_heads* v,
+                           int64_t n_tokens, int32_t head_dim, const xnn_attention_tiles* plan,
+                           const uint8_t* mask, float scale, const void* out, const float* lse,
+                           const void* grad, void* dq, void* dk, void* dv, void* work,
+                           size_t work_bytes, xnn_stream_t stream);
 
 #ifdef __cplusplus
 }

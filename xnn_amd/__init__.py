@@ -19,6 +19,9 @@ from .models import (InteratomicPotential, ModelConfig, ShEdgePotential, build_m
 from .outputs import ForceStressOutput
 from .radial import FullyConnectedNet, RadialNet, set_recompute_radial
 from .conv import ConvTensorProduct
+from .attention import (AttentionPlan, attention_plan, dropout_add, embedding, head_norm_rotate,
+                        structure_attention)
+from .atom_attention import AtomAttention, AtomAttentionPotential, SpeciesEmbedding
 from .irreps import Irrep, Irreps, tp_out_irreps_with_instructions, wigner_3j
 
 __all__ = [
@@ -32,5 +35,7 @@ __all__ = [
     "InteratomicPotential", "ModelConfig", "ShEdgePotential", "build_model", "get_model_class",
     "register_model", "ForceStressOutput",
     "FullyConnectedNet", "RadialNet", "set_recompute_radial", "ConvTensorProduct",
+    "AttentionPlan", "attention_plan", "dropout_add", "embedding", "head_norm_rotate",
+    "structure_attention", "AtomAttention", "AtomAttentionPotential", "SpeciesEmbedding",
     "Irrep", "Irreps", "tp_out_irreps_with_instructions", "wigner_3j",
 ]

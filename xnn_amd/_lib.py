@@ -17,7 +17,7 @@ LIBRARY = os.path.join(HERE, "libxnn_amd.so")
 ABI_VERSION = 2
 
 XNN_OK, XNN_EINVAL, XNN_ECAPACITY, XNN_EHIP = 0, 1, 2, 3
-XNN_F32, XNN_F64 = 0, 1
+XNN_F32, XNN_F64, XNN_BF16, XNN_F16 = 0, 1, 2, 3
 BASIS = {"bessel": 0, "gaussian": 1}
 ENVELOPE = {"polynomial": 0, "cosine": 1, "none": 2}
 
@@ -101,6 +101,21 @@ class ShPairModel(ctypes.Structure):
     _fields_ = [("prm", ctypes.POINTER(FeaturizeParams)), ("rbf_table", vp), ("n_channels", i32),
                 ("W", vp), ("U", vp), ("atom_ref", vp), ("n_atom_ref", i64)]
 
+
+class Heads(ctypes.Structure):
+    """``xnn_heads``."""
+    _fields_ = [("data", vp), ("token_stride", i64), ("head_stride", i64), ("n_heads", i32)]
+
+
+class AttentionTiles(ctypes.Structure):
+    """``xnn_attention_tiles``."""
+    _fields_ = [("n_tokens", i64), ("max_atoms", i64), ("n_tiles64", i64), ("n_tiles128", i64),
+                ("tiles64", vp), ("tiles128", vp)]
+
+
+_heads, _tiles = ctypes.POINTER(Heads), ctypes.POINTER(AttentionTiles)
+u64 = ctypes.c_uint64
+f32 = ctypes.c_float
 
 # name -> argtypes (restype int unless listed in _RESTYPES)
 _SIGNATURES = {
@@ -258,6 +273,20 @@ _SIGNATURES = {
     "xnn_graph_plan_workspace_bytes": [i64, i64, i64, i32],
     "xnn_graph_plan": [vp, vp, i64, i64, vp, vp, i64, vp, vp, c_int, vp, vp, vp, vp, vp, vp, vp,
                        vp, vp, vp, vp, vp, sz, vp],
+    "xnn_embedding": [c_int, vp, i64, vp, i64, i64, f32, vp, vp],
+    "xnn_embedding_grad_work_size": [i64, i64, i64, vp],
+    "xnn_embedding_grad": [c_int, vp, i64, vp, i64, i64, f32, vp, vp, sz, vp],
+    "xnn_dropout_add": [c_int, vp, vp, i64, i32, u64, u64, vp, vp, vp],
+    "xnn_head_norm_rotate": [c_int, _heads, _heads, i64, i32, i32, vp, vp, vp, vp, i64, vp, f32,
+                             i32, vp, vp, vp],
+    "xnn_head_norm_rotate_backward_work_size": [i32, vp],
+    "xnn_head_norm_rotate_backward": [c_int, _heads, _heads, i64, i32, i32, vp, vp, vp, vp, i64, vp,
+                                      f32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp],
+    "xnn_attention_plan": [vp, i64, i64, vp, vp, vp, i64, vp, i64, vp, vp],
+    "xnn_attention": [c_int, _heads, _heads, _heads, i64, i32, _tiles, vp, f32, vp, vp, vp],
+    "xnn_attention_backward_work_size": [i64, i32, vp],
+    "xnn_attention_backward": [c_int, _heads, _heads, _heads, i64, i32, _tiles, vp, f32, vp, vp, vp,
+                               vp, vp, vp, vp, sz, vp],
 }
 _RESTYPES = {"xnn_last_error": ctypes.c_char_p, "xnn_scan_workspace_bytes": sz,
              "xnn_edge_plan_workspace_bytes": sz, "xnn_graph_plan_workspace_bytes": sz,
@@ -382,6 +411,17 @@ def dtype_code(dtype: torch.dtype) -> int:
     if dtype == torch.float64:
         return XNN_F64
     raise TypeError(f"unsupported dtype {dtype} (float32 or float64)")
+
+
+STORAGE = {torch.float32: XNN_F32, torch.bfloat16: XNN_BF16, torch.float16: XNN_F16}
+
+
+def storage_code(dtype: torch.dtype) -> int:
+    """The dtype code of an attention operator's tensors."""
+    try:
+        return STORAGE[dtype]
+    except KeyError:
+        raise TypeError(f"unsupported dtype {dtype} (float32, bfloat16 or float16)") from None
 
 
 calls: dict = {}

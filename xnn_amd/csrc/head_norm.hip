@@ -1,0 +1,426 @@
+// Norms of queries and keys for each head with the rotation in the same pass, and the backward
+// pass (gfx950, wave64).
+//
+//   n = x / sqrt(mean_d x^2 + eps),  u = w n,  (a, b) -> (a c - b s, a s + b c)
+//
+// over the D elements of one head of one token; the first R elements form R / 2 pairs (i, i + R/2)
+// or (2 i, 2 i + 1) turned by the angle whose cosine and sine are row `positions[t]` (or t) of the
+// tables, the other elements are not turned. Backward, with g the cotangent turned back:
+//
+//   dx = r (w g - n mean_d(w g n)),  dw = sum_{t, heads} g n,
+//   dc = sum_heads (ga a + gb b),    ds = sum_heads (gb a - ga b)
+//
+// A stream over queries and keys in one launch: a head lies in the registers of G lanes, 2 N
+// elements a lane in two accesses of N (both members of a pair in one lane), so the sums over
+// d are exchanges within G lanes and the sums over heads exchanges across the lanes of the token.
+// All arithmetic is float32 and every sum has a fixed order.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "common.h"
+#include "device.h"
+#include "storage.h"
+
+namespace xnn {
+
+constexpr int kNormBlocks = 1024;  // blocks of the backward pass, at most (their weight sums are joined)
+
+struct HeadArgs {
+  const void *q, *k, *gq, *gk, *wq, *wk;
+  int64_t q_token, q_head, k_token, k_head;
+  int64_t n_tokens, n_rows;
+  const int64_t* positions;
+  const float *cos, *sin;
+  int heads, kv_heads, D, R;
+  int lanes, parallel;             // lanes of a head, heads a token has in flight
+  float eps;
+  void *q_out, *k_out;
+  float *d_cos, *d_sin, *part;
+};
+
+template <int N>
+struct Unit {                      // the 2 N elements of one lane
+  float a[N], b[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void load_unit(const T* p, int o0, int o1, int D, Unit<N>& x) {
+  load_pack<T, N>(p + o0, x.a);
+  if (o1 < D) {
+    load_pack<T, N>(p + o1, x.b);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) x.b[j] = 0.0f;
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_unit(T* p, int o0, int o1, int D, const Unit<N>& x) {
+  store_pack<T, N>(p + o0, x.a);
+  if (o1 < D) store_pack<T, N>(p + o1, x.b);
+}
+
+// member `m` of pair `p` of a unit's elements
+template <int N, bool INTER>
+__device__ __forceinline__ float& member(Unit<N>& x, int p, int m) {
+  if (!INTER || N == 1) return m == 0 ? x.a[p] : x.b[p];
+  const int e = 2 * p + m;
+  return e < N ? x.a[e] : x.b[e - N];
+}
+
+__device__ __forceinline__ float lanes_sum(float x, int lanes) {
+  for (int o = 1; o < lanes; o <<= 1) x += __shfl_xor(x, o);
+  return x;
+}
+
+template <typename T, int N, bool INTER, bool BACK>
+__global__ __launch_bounds__(256) void head_norm_kernel(HeadArgs h) {
+  const int lane = threadIdx.x & (kWave - 1), wave = wave_in_block();
+  const int per_token = h.lanes * h.parallel, tokens = kWave / per_token;
+  const int u = lane % h.lanes, slot = (lane / h.lanes) % h.parallel;
+  const int all = h.heads + h.kv_heads, D = h.D;
+  const int o0 = INTER || 2 * u * N >= h.R ? 2 * u * N : u * N;
+  const int o1 = INTER || 2 * u * N >= h.R ? o0 + N : h.R / 2 + u * N;
+  const bool mine = 2 * u * N < D, turned = 2 * u * N < h.R;
+  Unit<N> wq, wk, dwq, dwk;
+#pragma unroll
+  for (int j = 0; j < N; ++j) wq.a[j] = wq.b[j] = wk.a[j] = wk.b[j] = 0.0f;
+  dwq = dwk = wq;
+  if (mine) {
+    load_unit<T, N>((const T*)h.wq, o0, o1, D, wq);
+    load_unit<T, N>((const T*)h.wk, o0, o1, D, wk);
+  }
+  const int64_t step = (int64_t)gridDim.x * 4 * tokens;
+  for (int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) * tokens; t0 < h.n_tokens; t0 += step) {
+    const int64_t t = t0 + lane / per_token;
+    const bool live = mine && t < h.n_tokens;
+    float c[N], s[N], dc[N], ds[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      c[j] = 1.0f;
+      s[j] = dc[j] = ds[j] = 0.0f;
+    }
+    if (live && turned) {
+      const int64_t row = h.positions != nullptr ? h.positions[t] : t;
+      if (row >= 0 && row < h.n_rows) {
+        load_pack<float, N>(h.cos + row * (h.R / 2) + u * N, c);
+        load_pack<float, N>(h.sin + row * (h.R / 2) + u * N, s);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) c[j] = s[j] = __builtin_nanf("");
+      }
+    }
+    for (int i0 = 0; i0 < all; i0 += h.parallel) {
+      const int i = i0 + slot;
+      const bool on = live && i < all, is_q = i < h.heads;
+      const int64_t head = is_q ? i : i - h.heads;
+      Unit<N> x;
+#pragma unroll
+      for (int j = 0; j < N; ++j) x.a[j] = x.b[j] = 0.0f;
+      if (on)
+        load_unit<T, N>(is_q ? (const T*)h.q + t * h.q_token + head * h.q_head
+                             : (const T*)h.k + t * h.k_token + head * h.k_head,
+                        o0, o1, D, x);
+      const int64_t at = (is_q ? t * h.heads + head : t * h.kv_heads + head) * D;
+      Unit<N> g = x;
+      if (BACK && on) load_unit<T, N>((const T*)(is_q ? h.gq : h.gk) + at, o0, o1, D, g);
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < N; ++j) sum += x.a[j] * x.a[j] + x.b[j] * x.b[j];
+      const float r = 1.0f / sqrtf(lanes_sum(sum, h.lanes) / (float)D + h.eps);
+      Unit<N> w;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        w.a[j] = is_q ? wq.a[j] : wk.a[j];
+        w.b[j] = is_q ? wq.b[j] : wk.b[j];
+        x.a[j] *= r;                                       // x is n from here
+        x.b[j] *= r;
+      }
+      if (!BACK) {
+        Unit<N> y = x;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          y.a[j] *= w.a[j];
+          y.b[j] *= w.b[j];
+        }
+        if (turned) {
+#pragma unroll
+          for (int p = 0; p < N; ++p) {
+            const float a = member<N, INTER>(y, p, 0), b = member<N, INTER>(y, p, 1);
+            member<N, INTER>(y, p, 0) = a * c[p] - b * s[p];
+            member<N, INTER>(y, p, 1) = a * s[p] + b * c[p];
+          }
+        }
+        if (on) store_unit<T, N>((T*)(is_q ? h.q_out : h.k_out) + at, o0, o1, D, y);
+        continue;
+      }
+      if (turned && on) {
+#pragma unroll
+        for (int p = 0; p < N; ++p) {
+          const float ga = member<N, INTER>(g, p, 0), gb = member<N, INTER>(g, p, 1);
+          const float a = member<N, INTER>(x, p, 0) * member<N, INTER>(w, p, 0);
+          const float b = member<N, INTER>(x, p, 1) * member<N, INTER>(w, p, 1);
+          dc[p] += ga * a + gb * b;
+          ds[p] += gb * a - ga * b;
+          member<N, INTER>(g, p, 0) = ga * c[p] + gb * s[p];
+          member<N, INTER>(g, p, 1) = gb * c[p] - ga * s[p];
+        }
+      }
+      float dot = 0.0f;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float na = on ? g.a[j] * x.a[j] : 0.0f, nb = on ? g.b[j] * x.b[j] : 0.0f;
+        dwq.a[j] += is_q ? na : 0.0f;
+        dwq.b[j] += is_q ? nb : 0.0f;
+        dwk.a[j] += is_q ? 0.0f : na;
+        dwk.b[j] += is_q ? 0.0f : nb;
+        dot += na * w.a[j] + nb * w.b[j];
+      }
+      dot = lanes_sum(dot, h.lanes) / (float)D;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        x.a[j] = r * (g.a[j] * w.a[j] - x.a[j] * dot);
+        x.b[j] = r * (g.b[j] * w.b[j] - x.b[j] * dot);
+      }
+      if (on) store_unit<T, N>((T*)(is_q ? h.q_out : h.k_out) + at, o0, o1, D, x);
+    }
+    if (BACK && h.d_cos != nullptr) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        for (int o = h.lanes; o < per_token; o <<= 1) {
+          dc[j] += __shfl_xor(dc[j], o);
+          ds[j] += __shfl_xor(ds[j], o);
+        }
+      }
+      if (live && turned && slot == 0) {
+        store_pack<float, N>(h.d_cos + t * (h.R / 2) + u * N, dc);
+        store_pack<float, N>(h.d_sin + t * (h.R / 2) + u * N, ds);
+      }
+    }
+  }
+  if (BACK && h.part != nullptr) {
+    // the block's sums over tokens and heads: across the lanes of a wave, then its waves in order
+    __shared__ float sums[4][2][128];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      for (int o = h.lanes; o < kWave; o <<= 1) {
+        dwq.a[j] += __shfl_xor(dwq.a[j], o);
+        dwq.b[j] += __shfl_xor(dwq.b[j], o);
+        dwk.a[j] += __shfl_xor(dwk.a[j], o);
+        dwk.b[j] += __shfl_xor(dwk.b[j], o);
+      }
+      if (mine && lane < h.lanes) {
+        sums[wave][0][o0 + j] = dwq.a[j];
+        sums[wave][1][o0 + j] = dwk.a[j];
+        if (o1 < D) {
+          sums[wave][0][o1 + j] = dwq.b[j];
+          sums[wave][1][o1 + j] = dwk.b[j];
+        }
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * D; i += 256) {
+      const int m = i / D, d = i - m * D;
+      h.part[(int64_t)blockIdx.x * 2 * D + i] =
+          (sums[0][m][d] + sums[1][m][d]) + (sums[2][m][d] + sums[3][m][d]);
+    }
+  }
+}
+
+// the blocks' weight sums added in float64: sixteen of them at a time, then those in order
+template <typename T>
+__global__ __launch_bounds__(256) void head_weight_kernel(const float* __restrict__ part, int blocks,
+                                                          int D, T* __restrict__ dwq,
+                                                          T* __restrict__ dwk) {
+  __shared__ double s[16][17];
+  const int x = threadIdx.x % 16, y = threadIdx.x / 16;
+  const int i = blockIdx.x * 16 + x;
+  double v = 0.0;
+  if (i < 2 * D)
+#pragma unroll 4
+    for (int b = y; b < blocks; b += 16) v += part[(int64_t)b * 2 * D + i];
+  s[y][x] = v;
+  __syncthreads();
+  if (y == 0 && i < 2 * D) {
+    double r = 0.0;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) r += s[q][x];
+    if (i < D)
+      dwq[i] = (T)(float)r;
+    else
+      dwk[i - D] = (T)(float)r;
+  }
+}
+
+static int pow2_at_least(int n) {
+  int p = 1;
+  while (p < n) p *= 2;
+  return p;
+}
+
+// The widest access that the addresses, strides and pair layout allow; fills in the lanes.
+template <typename T>
+static int head_width(HeadArgs& h, bool back) {
+  const uintptr_t at = (uintptr_t)h.q | (uintptr_t)h.k | (uintptr_t)h.wq | (uintptr_t)h.wk |
+                       (uintptr_t)h.q_out | (uintptr_t)h.k_out |
+                       (back ? (uintptr_t)h.gq | (uintptr_t)h.gk : 0);
+  const uintptr_t tables = (uintptr_t)h.cos | (uintptr_t)h.sin | (uintptr_t)h.d_cos | (uintptr_t)h.d_sin;
+  const int64_t strides = h.q_token | h.q_head | h.k_token | h.k_head;
+  int n = 16 / sizeof(T);
+  while (n > 1 && (at % (n * sizeof(T)) != 0 || tables % 16 != 0 || strides % n != 0 ||
+                   h.D % (2 * n) != 0 || h.R % (2 * n) != 0))
+    n /= 2;
+  h.lanes = pow2_at_least((h.D + 2 * n - 1) / (2 * n));
+  h.parallel = std::min(kWave / h.lanes, pow2_at_least(h.heads + h.kv_heads));
+  return n;
+}
+
+static int norm_blocks(const HeadArgs& h, int64_t most) {
+  const int64_t per = 4 * (kWave / (h.lanes * h.parallel));
+  return (int)std::min<int64_t>((h.n_tokens + per - 1) / per, most);
+}
+
+template <typename T, bool BACK>
+static void head_norm_launch(const HeadArgs& h, int n, int inter, int blocks, hipStream_t s) {
+#define XNN_HEAD_LAUNCH(N)                                                                         \
+  do {                                                                                             \
+    if (inter)                                                                                     \
+      hipLaunchKernelGGL((head_norm_kernel<T, N, true, BACK>), dim3(blocks), dim3(256), 0, s, h);  \
+    else                                                                                           \
+      hipLaunchKernelGGL((head_norm_kernel<T, N, false, BACK>), dim3(blocks), dim3(256), 0, s, h); \
+  } while (0)
+  if constexpr (sizeof(T) == 2) {
+    if (n == 8) {
+      XNN_HEAD_LAUNCH(8);
+      return;
+    }
+  }
+  if (n == 4)
+    XNN_HEAD_LAUNCH(4);
+  else if (n == 2)
+    XNN_HEAD_LAUNCH(2);
+  else
+    XNN_HEAD_LAUNCH(1);
+#undef XNN_HEAD_LAUNCH
+}
+
+static size_t norm_work_bytes(int D) { return (size_t)kNormBlocks * 2 * D * sizeof(float); }
+
+static int head_args(HeadArgs& h, const xnn_heads* q, const xnn_heads* k, int64_t n_tokens,
+                     int32_t head_dim, int32_t rotated, const void* q_weight, const void* k_weight,
+                     const float* cos, const float* sin, int64_t n_rows, const int64_t* positions,
+                     float eps) {
+  XNN_REQUIRE(q && k, "NULL heads");
+  XNN_REQUIRE(n_tokens >= 0 && n_rows >= 0, "negative size");
+  XNN_REQUIRE(q->n_heads >= 1 && k->n_heads >= 1, "no heads");
+  XNN_REQUIRE(head_dim >= 1 && head_dim <= 128, "head_dim must be in [1, 128]");
+  XNN_REQUIRE(rotated >= 0 && rotated <= head_dim && rotated % 2 == 0,
+              "rotated must be even and at most head_dim");
+  if (n_tokens > 0) {
+    XNN_REQUIRE(positions != nullptr || rotated == 0 || n_rows == n_tokens,
+                "without positions the tables have a row a token");
+    XNN_REQUIRE(q->data && k->data && q_weight && k_weight, "NULL input");
+    XNN_REQUIRE(rotated == 0 || n_rows == 0 || (cos && sin), "NULL table");
+  }
+  h = HeadArgs{};
+  h.q = q->data;
+  h.k = k->data;
+  h.q_token = q->token_stride;
+  h.q_head = q->head_stride;
+  h.k_token = k->token_stride;
+  h.k_head = k->head_stride;
+  h.heads = q->n_heads;
+  h.kv_heads = k->n_heads;
+  h.n_tokens = n_tokens;
+  h.n_rows = n_rows;
+  h.positions = positions;
+  h.cos = cos;
+  h.sin = sin;
+  h.D = head_dim;
+  h.R = rotated;
+  h.wq = q_weight;
+  h.wk = k_weight;
+  h.eps = eps;
+  return XNN_OK;
+}
+
+}  // namespace xnn
+
+using namespace xnn;
+
+extern "C" {
+
+int xnn_head_norm_rotate(int dtype, const xnn_heads* q, const xnn_heads* k, int64_t n_tokens,
+                         int32_t head_dim, int32_t rotated, const void* q_weight,
+                         const void* k_weight, const float* cos, const float* sin, int64_t n_rows,
+                         const int64_t* positions, float eps, int32_t interleaved, void* q_out,
+                         void* k_out, xnn_stream_t stream) {
+  XNN_REQUIRE(is_storage(dtype), "dtype must be XNN_F32, XNN_BF16 or XNN_F16");
+  HeadArgs h;
+  const int status = head_args(h, q, k, n_tokens, head_dim, rotated, q_weight, k_weight, cos, sin,
+                               n_rows, positions, eps);
+  if (status != XNN_OK || n_tokens == 0) return status;
+  XNN_REQUIRE(q_out && k_out, "NULL output");
+  h.q_out = q_out;
+  h.k_out = k_out;
+  XNN_STORAGE_DISPATCH(dtype, T, {
+    const int n = head_width<T>(h, false);
+    head_norm_launch<T, false>(h, n, interleaved, norm_blocks(h, 1 << 20), as_hip(stream));
+  });
+  XNN_LAUNCH_CHECK();
+  return XNN_OK;
+}
+
+int xnn_head_norm_rotate_backward_work_size(int32_t head_dim, size_t* bytes) {
+  XNN_REQUIRE(head_dim >= 1 && head_dim <= 128, "head_dim must be in [1, 128]");
+  XNN_REQUIRE(bytes != nullptr, "NULL size");
+  *bytes = norm_work_bytes(head_dim);
+  return XNN_OK;
+}
+
+int xnn_head_norm_rotate_backward(int dtype, const xnn_heads* q, const xnn_heads* k,
+                                  int64_t n_tokens, int32_t head_dim, int32_t rotated,
+                                  const void* q_weight, const void* k_weight, const float* cos,
+                                  const float* sin, int64_t n_rows, const int64_t* positions,
+                                  float eps, int32_t interleaved, const void* grad_q,
+                                  const void* grad_k, void* d_q, void* d_k, void* d_q_weight,
+                                  void* d_k_weight, float* d_cos, float* d_sin, void* work,
+                                  size_t work_bytes, xnn_stream_t stream) {
+  XNN_REQUIRE(is_storage(dtype), "dtype must be XNN_F32, XNN_BF16 or XNN_F16");
+  HeadArgs h;
+  const int status = head_args(h, q, k, n_tokens, head_dim, rotated, q_weight, k_weight, cos, sin,
+                               n_rows, positions, eps);
+  if (status != XNN_OK) return status;
+  XNN_REQUIRE((d_q_weight == nullptr) == (d_k_weight == nullptr),
+              "the weights' gradients go together");
+  XNN_REQUIRE((d_cos == nullptr) == (d_sin == nullptr), "the tables' gradients go together");
+  XNN_REQUIRE(d_cos == nullptr || positions == nullptr,
+              "tables read by position have no gradient here");
+  XNN_REQUIRE(n_tokens == 0 || (grad_q && grad_k && d_q && d_k), "NULL cotangent or gradient");
+  if (d_q_weight != nullptr)
+    XNN_REQUIRE(work && work_bytes >= norm_work_bytes(head_dim), "work too small");
+  h.gq = grad_q;
+  h.gk = grad_k;
+  h.q_out = d_q;
+  h.k_out = d_k;
+  h.d_cos = d_cos;
+  h.d_sin = d_sin;
+  h.part = d_q_weight != nullptr ? (float*)work : nullptr;
+  hipStream_t s = as_hip(stream);
+  XNN_STORAGE_DISPATCH(dtype, T, {
+    int blocks = 0;
+    if (n_tokens > 0) {
+      const int n = head_width<T>(h, true);
+      blocks = norm_blocks(h, kNormBlocks);
+      head_norm_launch<T, true>(h, n, interleaved, blocks, s);
+    }
+    if (d_q_weight != nullptr)
+      hipLaunchKernelGGL(head_weight_kernel<T>, dim3((2 * head_dim + 15) / 16), dim3(256), 0, s,
+                         (const float*)work, blocks, head_dim, (T*)d_q_weight, (T*)d_k_weight);
+  });
+  XNN_LAUNCH_CHECK();
+  return XNN_OK;
+}
+
+}  // extern "C"
