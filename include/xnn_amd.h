@@ -1227,17 +1227,25 @@ int xnn_attention_plan(const int64_t* n_atoms, int64_t n_structures, int64_t n_t
                        int64_t* tile_ptr, int32_t* tiles64, int64_t capacity64, int32_t* tiles128,
                        int64_t capacity128, int64_t* info, xnn_stream_t stream);
 
+/* Bytes of the workspace of xnn_attention (0 where it needs none: only long structures of few
+ * tiles are walked in parts that are joined). */
+int xnn_attention_work_size(int64_t n_tokens, int32_t n_heads, int32_t head_dim,
+                            const xnn_attention_tiles* plan, size_t* bytes);
+
 /* Attention of every token to the tokens of its structure that `mask` (n_tokens bytes, zero
  * leaves a key out; NULL keeps all) keeps: out_i = sum_j p_ij v_j with p the softmax over j of
  * scale q_i . k_j; rows without keys are zero. head_dim at most 128; q's heads are a multiple of
  * those of k and v, which they share in order. out (n_tokens, heads, head_dim) contiguous; lse
- * (heads, n_tokens) for the backward pass (NULL: not wanted). */
+ * (heads, n_tokens) for the backward pass (NULL: not wanted). `work` is aligned to 16 bytes. */
 int xnn_attention(int dtype, const xnn_heads* q, const xnn_heads* k, const xnn_heads* v,
                   int64_t n_tokens, int32_t head_dim, const xnn_attention_tiles* plan,
-                  const uint8_t* mask, float scale, void* out, float* lse, xnn_stream_t stream);
+                  const uint8_t* mask, float scale, void* out, float* lse, void* work,
+                  size_t work_bytes, xnn_stream_t stream);
 
 /* Bytes of the workspace of xnn_attention_backward. */
-int xnn_attention_backward_work_size(int64_t n_tokens, int32_t n_heads, size_t* bytes);
+int xnn_attention_backward_work_size(int64_t n_tokens, int32_t n_heads, int32_t n_kv_heads,
+                                     int32_t head_dim, const xnn_attention_tiles* plan,
+                                     size_t* bytes);
 
 /* Gradients of xnn_attention for the cotangent `grad`, from its inputs and its outputs out and
  * lse (out, grad, dq, dk and dv contiguous); the probabilities are formed again. */

@@ -19,7 +19,7 @@ def _refused(lib, code, text):
 
 
 BUF = (ctypes.c_double * 64)()
-SIZE = ctypes.c_size_t()
+SIZE, SPLIT = ctypes.c_size_t(), ctypes.c_size_t()
 
 
 def test_embedding_arguments(lib):
@@ -83,7 +83,7 @@ def test_attention_arguments(lib):
 
     def call(dtype=0, H=4, K=2, KV=2, T=10, D=16, p=None, scale=0.25, out=BUF, q=None):
         return lib.xnn_attention(dtype, _heads(H, q), _heads(K), _heads(KV), T, D, p or plan(), None,
-                                 scale, out, None, None)
+                                 scale, out, None, None, 0, None)
     _refused(lib, call(dtype=1), b"dtype")
     _refused(lib, call(D=0), b"head_dim")
     _refused(lib, call(D=129), b"head_dim")
@@ -99,7 +99,10 @@ def test_attention_arguments(lib):
     assert call(T=0, p=plan(tokens=0, tiles=False), out=None) == 0
     _refused(lib, lib.xnn_attention_plan(BUF, 2, 100, BUF, BUF, BUF, 2, BUF, 2, BUF, None), b"too small")
     _refused(lib, lib.xnn_attention_plan(BUF, 2, 1 << 31, BUF, BUF, BUF, 2, BUF, 2, BUF, None), b"too many")
-    assert lib.xnn_attention_backward_work_size(10, 4, ctypes.byref(SIZE)) == 0
+    assert lib.xnn_attention_backward_work_size(10, 4, 2, 16, plan(), ctypes.byref(SIZE)) == 0
+    long = ctypes.byref(_lib.AttentionTiles(9000, 9000, 141, 71, None, None))
+    assert lib.xnn_attention_work_size(9000, 4, 32, long, ctypes.byref(SPLIT)) == 0 and SPLIT.value > 0
+    assert lib.xnn_attention_work_size(10, 4, 16, plan(), ctypes.byref(SPLIT)) == 0 and SPLIT.value == 0
     _refused(lib, lib.xnn_attention_backward(0, _heads(4), _heads(2), _heads(2), 10, 16, plan(), None,
                                              0.25, BUF, BUF, BUF, BUF, BUF, BUF, BUF, SIZE.value - 1,
                                              None), b"too small")

@@ -321,6 +321,17 @@ class AttentionPlan:
         self.c = _lib.AttentionTiles(self.n_tokens, self.max_atoms, self.tiles64.shape[0],
                                      self.tiles128.shape[0], self.tiles64.data_ptr(),
                                      self.tiles128.data_ptr())
+        self._bytes = {}
+
+    def work_bytes(self, name: str, *sizes: int) -> int:
+        """Bytes of a workspace for this plan: a function of the sizes alone."""
+        need = self._bytes.get((name, sizes))
+        if need is None:
+            c = ctypes.c_size_t()
+            _lib.check(name, getattr(_lib.load(), name)(self.n_tokens, *sizes, ctypes.byref(self.c),
+                                                        ctypes.byref(c)))
+            need = self._bytes[name, sizes] = c.value
+        return need
 
 
 def attention_plan(n_atoms: Tensor, n_tokens: Optional[int] = None) -> AttentionPlan:
@@ -360,10 +371,13 @@ def _attention_args(q, k, v, plan, mask, scale):
             None if mask is None else mask.data_ptr(), scale)
 
 
-def _attention(q, args, want_lse):
+def _attention(q, plan, args, want_lse):
     out = q.new_empty(q.shape)
+    size = plan.work_bytes("xnn_attention_work_size", q.shape[1], q.shape[2])
+    work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device) if want_lse else None
-    _lib.call("xnn_attention", *args, out.data_ptr(), _lib.ptr(lse), _stream(q))
+    _lib.call("xnn_attention", *args, out.data_ptr(), _lib.ptr(lse),
+              _lib.ptr(work), size, _stream(q))
     return out, lse
 
 
@@ -371,7 +385,7 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, plan, mask, scale):
         ctx.plan, ctx.scale = plan, scale
-        out, lse = _attention(q, _attention_args(q, k, v, plan, mask, scale), True)
+        out, lse = _attention(q, plan, _attention_args(q, k, v, plan, mask, scale), True)
         ctx.save_for_backward(q, k, v, mask, out, lse)
         return out
 
@@ -381,7 +395,8 @@ class _Attention(torch.autograd.Function):
         q, k, v, mask, out, lse = ctx.saved_tensors
         grad = grad.contiguous()
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-        work, size = _workspace("xnn_attention_backward_work_size", q.device, q.shape[0], q.shape[1])
+        size = ctx.plan.work_bytes("xnn_attention_backward_work_size", q.shape[1], k.shape[1], q.shape[2])
+        work = torch.empty(size, dtype=torch.uint8, device=q.device)
         _lib.call("xnn_attention_backward", *_attention_args(q, k, v, ctx.plan, mask, ctx.scale),
                   out.data_ptr(), lse.data_ptr(), grad.data_ptr(), dq.data_ptr(), dk.data_ptr(),
                   dv.data_ptr(), work.data_ptr(), size, _stream(q))
@@ -427,4 +442,4 @@ def structure_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan,
     q, k, v = _unit_stride(q), _unit_stride(k), _unit_stride(v)
     if _wanted(q, k, v):
         return _Attention.apply(q, k, v, plan, mask, scale)
-    return _attention(q, _attention_args(q, k, v, plan, mask, scale), False)[0]
+    return _attention(q, plan, _attention_args(q, k, v, plan, mask, scale), False)[0]

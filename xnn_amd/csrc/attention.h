@@ -9,16 +9,21 @@
 // the operand of the next one, because the order of a contraction index is free as long as both
 // operands use the same: the walked row of operand element e is the one the product left there.
 //
-//   walk(tile) x own   = tile (natural rows from LDS, 16 bytes a lane)  x  own (registers)
-//   own^T += tile^T x weights: tile read across its rows (float32: one element a lane and row;
-//            16 bits: the transposing LDS read, four rows a lane)
+//   walk(tile) x own       = tile (rows from LDS, 16 bytes a lane)  x  own (registers)
+//   own^T     += tile^T x weights: tile read across its rows by the transposing LDS read
 //
-// float32 uses v_mfma_f32_32x32x2_f32 (products and sums in float32), 16 bits
-// v_mfma_f32_32x32x16_{bf16,f16} (sums in float32).
+// 16-bit types use v_mfma_f32_32x32x16_{bf16,f16} (sums in float32). float32 is taken apart into
+// three bfloat16 planes of 8 bits each by truncation, x = h + m + l exactly, and a product is the
+// six plane products of order 2^-16 and larger (h h, h m, m h, h l, l h, m m; the dropped ones
+// are 2^-24 of it, as a float32 rounding): six instructions of the 16-bit rate in place of eight of
+// a sixteenth of it, 2.7 times the rate of v_mfma_f32_32x32x2_f32. An operand that is not finite
+// makes the products it enters NaN.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
+
+#include <algorithm>
 
 #include "common.h"
 #include "device.h"
@@ -28,6 +33,8 @@ namespace xnn {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -41,125 +48,193 @@ __host__ __device__ constexpr int tile_row(int r, int half) {
   return 8 * (r / 4) + 4 * half + r % 4;
 }
 
-// 16 bytes of one row a lane: the unit of loads and of operands
 template <typename T>
-struct Mma;
+struct Store {                     // bfloat16, float16: one plane, the value itself
+  typedef T Element;
+  static constexpr int kPlanes = 1;
+};
 template <>
-struct Mma<float> {
-  typedef f32x4 Frag;
-  static __device__ __forceinline__ void mma(Frag a, Frag b, f32x16& c) {
+struct Store<float> {
+  typedef bf16_t Element;
+  static constexpr int kPlanes = 3;
+};
+template <typename E>
+struct FragOf {
+  typedef bf16x8 type;
+};
+template <>
+struct FragOf<f16_t> {
+  typedef f16x8 type;
+};
+// the eight elements of a lane in an operand of one instruction, and its planes
+template <typename T>
+using Frag = typename FragOf<typename Store<T>::Element>::type;
+template <typename T, int PLANES = Store<T>::kPlanes>
+struct Operand {
+  Frag<T> p[PLANES];
+};
+
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// c += a b over the plane products of order max(NA, NB) - 1 and lower, the smallest first
+template <typename T, int NA, int NB>
+__device__ __forceinline__ void mma(const Operand<T, NA>& a, const Operand<T, NB>& b, f32x16& c) {
+  constexpr int kMost = NA > NB ? NA : NB;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
-  }
-};
-template <>
-struct Mma<bf16_t> {
-  typedef bf16x8 Frag;
-  static __device__ __forceinline__ void mma(Frag a, Frag b, f32x16& c) {
-    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-  }
-};
-template <>
-struct Mma<f16_t> {
-  typedef f16x8 Frag;
-  static __device__ __forceinline__ void mma(Frag a, Frag b, f32x16& c) {
-    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-  }
-};
+  for (int order = kMost - 1; order >= 0; --order)
+#pragma unroll
+    for (int i = 0; i <= order; ++i)
+      if (i < NA && order - i < NB) c = mfma(a.p[i], b.p[order - i], c);
+}
+
+// the upper halves of two float32, the first in the low half: truncated bfloat16s
+__device__ __forceinline__ uint32_t upper_halves(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+__device__ __forceinline__ float truncated(float x) {
+  return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+}
+
+// the planes of two float32
+__device__ __forceinline__ void planes_of(float a, float b, uint32_t (&out)[3]) {
+  out[0] = upper_halves(a, b);
+  a -= truncated(a);
+  b -= truncated(b);
+  out[1] = upper_halves(a, b);
+  a -= truncated(a);
+  b -= truncated(b);
+  out[2] = upper_halves(a, b);
+}
 
 // Sizes of a head padded to DP elements (16, 32, 64 or 128; zeros beyond the head)
 template <typename T, int DP>
 struct Head {
-  static constexpr int kPer = 16 / sizeof(T);            // elements of 16 bytes
-  static constexpr int kSteps = DP * sizeof(T) / 32;     // operands along the head (natural)
+  static constexpr int kPlanes = Store<T>::kPlanes;
+  static constexpr int kSteps = DP / 16;                 // operands along the head
   static constexpr int kBlocks = (DP + 31) / 32;         // 32-element blocks of an output
   static constexpr int kWide = kBlocks * 32;             // elements of a staged row
-  static constexpr int kRow = kWide * sizeof(T) + 16;    // its bytes: 16 more spread the banks
-  static constexpr int kFrags = sizeof(T);               // operands along 32 walked rows
+  static constexpr int kRow = kWide * 2 + 16;            // its bytes in a plane: 16 more spread the banks
+  // walked rows of a staged tile: 64, or 32 where three planes of 64 would leave a CU one block
+  static constexpr int kTile = kPlanes == 3 && DP == 128 ? 32 : 64;
+  static constexpr int kPlane = kTile * kRow;
+  // waves of a SIMD: two share its matrix core and vector unit where their registers fit
+  static constexpr int kOccupancy = DP <= 32 || (kPlanes == 1 && DP == 64) ? 2 : 1;
+  static constexpr int kBytes = kPlanes * kPlane;
 };
 
-// operand f of the weights: registers of a 32 x 32 product, rounded to T
-template <typename T>
-__device__ __forceinline__ typename Mma<T>::Frag weight_frag(const f32x16& p, int f) {
-  typename Mma<T>::Frag out;
-  constexpr int kPer = 16 / sizeof(T);
+// Operand f (of two) along the 32 walked rows of a product's registers, the weights of the next
+// product. WP planes: float32 in three; 16 bits in one, rounded to nearest, or in two, the second
+// one the rounding error of the first.
+template <typename T, int WP>
+__device__ __forceinline__ Operand<T, WP> weight_operand(const f32x16& p, int f) {
+  Operand<T, WP> out;
+  if constexpr (sizeof(T) == 4) {
+    u32x4 w[3];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) out[i] = (T)p[f * kPer + i];
+    for (int i = 0; i < 4; ++i) {
+      uint32_t x[3];
+      planes_of(p[8 * f + 2 * i], p[8 * f + 2 * i + 1], x);
+#pragma unroll
+      for (int n = 0; n < 3; ++n) w[n][i] = x[n];
+    }
+#pragma unroll
+    for (int n = 0; n < 3; ++n) out.p[n] = __builtin_bit_cast(Frag<T>, w[n]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out.p[0][i] = (T)p[8 * f + i];
+    if constexpr (WP == 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out.p[1][i] = (T)(p[8 * f + i] - (float)out.p[0][i]);
+    }
+  }
   return out;
 }
 
-// operand `step` along the head of walked row `row` (natural order)
+// operand `step` along the head of walked row `row`
 template <typename T, int DP>
-__device__ __forceinline__ typename Mma<T>::Frag natural_frag(const char* tile, int row, int step,
-                                                              int half) {
-  return *reinterpret_cast<const typename Mma<T>::Frag*>(tile + row * Head<T, DP>::kRow +
-                                                         32 * step + 16 * half);
-}
-
-// operand f along the 32 walked rows from `row0`, transposed: own side's elements 32 block + lane % 32
-template <typename T, int DP>
-__device__ __forceinline__ typename Mma<T>::Frag transposed_frag(const char* tile, int row0,
-                                                                 int block, int f, int lane) {
-  constexpr int kRow = Head<T, DP>::kRow;
-  const int half = lane / 32;
-  if constexpr (sizeof(T) == 4) {
-    const char* p = tile + (row0 + 8 * f + 4 * half) * kRow + (32 * block + lane % 32) * 4;
-    f32x4 out;
+__device__ __forceinline__ Operand<T> natural_operand(const char* tile, int row, int step, int half) {
+  Operand<T> out;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = *reinterpret_cast<const float*>(p + i * kRow);
-    return out;
-  } else {
-    // sixteen lanes read four rows of sixteen elements and get a column of four each
-    const int l = lane % 16;
-    const char* p = tile + (row0 + 16 * f + 4 * half + l / 4) * kRow +
-                    (32 * block + 16 * ((lane / 16) & 1) + 4 * (l % 4)) * 2;
-    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * kRow));
-    const s16x8 both = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-    return __builtin_bit_cast(typename Mma<T>::Frag, both);
-  }
+  for (int n = 0; n < Store<T>::kPlanes; ++n)
+    out.p[n] = *reinterpret_cast<const Frag<T>*>(tile + n * Head<T, DP>::kPlane +
+                                                 row * Head<T, DP>::kRow + 32 * step + 16 * half);
+  return out;
 }
 
-// 16 bytes of a row from element d on, zeros beyond the head's D elements
-template <typename T>
-__device__ __forceinline__ typename Mma<T>::Frag load_frag(const T* row, int d, int D, bool vec) {
-  typedef typename Mma<T>::Frag Frag;
-  constexpr int kPer = 16 / sizeof(T);
-  Frag out;
+// operand f along the 32 walked rows from `row0`, for the head's elements 32 block + lane % 32:
+// sixteen lanes read four rows of sixteen elements and get a column of four each
+template <typename T, int DP>
+__device__ __forceinline__ Operand<T> transposed_operand(const char* tile, int row0, int block, int f,
+                                                         int lane) {
+  constexpr int kRow = Head<T, DP>::kRow;
+  typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+  const int l = lane % 16;
+  const char* p = tile + (row0 + 16 * f + 4 * (lane / 32) + l / 4) * kRow +
+                  (32 * block + 16 * ((lane / 16) & 1) + 4 * (l % 4)) * 2;
+  Operand<T> out;
+#pragma unroll
+  for (int n = 0; n < Store<T>::kPlanes; ++n) {
+    const char* q = p + n * Head<T, DP>::kPlane;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)q);
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(q + 8 * kRow));
+    out.p[n] = __builtin_bit_cast(Frag<T>, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  return out;
+}
+
+// N elements of a row from element d on, zeros beyond the head's D elements
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_row(const T* row, int d, int D, bool vec) {
+  Pack<T, N> out;
   if (vec) {
     if (d < D) {
-      out = *reinterpret_cast<const Frag*>(row + d);
+      out = *reinterpret_cast<const Pack<T, N>*>(row + d);
     } else {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) out[i] = (T)0.0f;
+      for (int i = 0; i < N; ++i) out.v[i] = (T)0.0f;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) out[i] = d + i < D ? row[d + i] : (T)0.0f;
+    for (int i = 0; i < N; ++i) out.v[i] = d + i < D ? row[d + i] : (T)0.0f;
   }
   return out;
 }
 
-// the own row's operands in registers, zeros where the row does not exist
+// The own row's operands, zeros where the row does not exist. Scores are in base 2: float32 takes
+// `scale` into the operands here (one more rounding of each, no product a score); 16 bits would
+// lose the operands' last bits and scales the scores.
 template <typename T, int DP>
-__device__ __forceinline__ void load_own(const T* base, int64_t stride, int64_t row, bool live,
-                                         int D, bool vec, int half,
-                                         typename Mma<T>::Frag (&out)[Head<T, DP>::kSteps]) {
-  constexpr int kPer = Head<T, DP>::kPer;
+__device__ __forceinline__ void load_own(const T* base, int64_t stride, int64_t row, bool live, int D,
+                                         bool vec, int half, float scale,
+                                         Operand<T> (&out)[Head<T, DP>::kSteps]) {
+  const T* p = base + (live ? row : 0) * stride;
+  D = live ? D : 0;
 #pragma unroll
-  for (int c = 0; c < Head<T, DP>::kSteps; ++c)
-    out[c] = load_frag<T>(base + (live ? row : 0) * stride, (2 * c + half) * kPer, live ? D : 0, vec);
-}
-
-// Scores in base 2. float32 takes the scale into the own row's operands once (one more rounding of
-// each, no product a score); 16 bits would lose the operands' last bits and scale the scores.
-template <typename T, int DP>
-__device__ __forceinline__ void scale_own(float scale,
-                                          typename Mma<T>::Frag (&own)[Head<T, DP>::kSteps]) {
-  if constexpr (sizeof(T) == 4) {
+  for (int c = 0; c < Head<T, DP>::kSteps; ++c) {
+    const int d = 16 * c + 8 * half;
+    if constexpr (sizeof(T) == 4) {
+      u32x4 w[3];
 #pragma unroll
-    for (int c = 0; c < Head<T, DP>::kSteps; ++c) own[c] *= scale;
+      for (int i = 0; i < 2; ++i) {
+        const Pack<T, 4> x = load_row<T, 4>(p, d + 4 * i, D, vec);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t y[3];
+          planes_of(x.v[2 * j] * scale, x.v[2 * j + 1] * scale, y);
+#pragma unroll
+          for (int n = 0; n < 3; ++n) w[n][2 * i + j] = y[n];
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 3; ++n) out[c].p[n] = __builtin_bit_cast(Frag<T>, w[n]);
+    } else {
+      out[c].p[0] = __builtin_bit_cast(Frag<T>, load_row<T, 8>(p, d, D, vec));
+    }
   }
 }
 template <typename T>
@@ -172,38 +247,63 @@ __device__ __forceinline__ float weight(float s, float scale, float base) {
   return __builtin_amdgcn_exp2f(sizeof(T) == 4 ? s - base : fmaf(s, scale, -base));
 }
 
-// Rows [first, first + ROWS) of one head into LDS; zeros beyond `end`, beyond the head and in rows
-// that `skip` (a mask's zeros, NULL: none) leaves out, so that what they hold reaches no sum.
-template <typename T, int DP, int ROWS, int THREADS>
-__device__ __forceinline__ void stage(const T* base, int64_t stride, int64_t first, int64_t end,
-                                      int D, bool vec, const uint8_t* mask, char* tile) {
+// A tile of walked rows on its way to LDS: fetched to registers before the products of the tile
+// before, written after them, so that the products cover the memory latency. Rows beyond `end`,
+// elements beyond the head and rows that the mask (NULL: none) leaves out become zeros, so that
+// what they hold reaches no sum.
+template <typename T, int DP, int THREADS>
+struct Stage {
   typedef Head<T, DP> S;
-  constexpr int kChunks = S::kWide / S::kPer;
-#pragma unroll
-  for (int i0 = 0; i0 < ROWS * kChunks; i0 += THREADS) {
-    const int i = i0 + threadIdx.x;
-    if (ROWS * kChunks % THREADS != 0 && i >= ROWS * kChunks) break;
-    const int r = i / kChunks, c = i % kChunks;
-    const int64_t row = first + r;
-    const bool live = row < end && (mask == nullptr || mask[row] != 0);
-    *reinterpret_cast<typename Mma<T>::Frag*>(tile + r * S::kRow + 16 * c) =
-        load_frag<T>(base + (live ? row : 0) * stride, c * S::kPer, live ? D : 0, vec);
-  }
-}
+  static constexpr int kPer = 16 / sizeof(T);
+  static constexpr int kChunks = S::kWide / kPer;          // 16-byte pieces of a row
+  static constexpr int kCount = (S::kTile * kChunks + THREADS - 1) / THREADS;
+  static constexpr bool kEven = S::kTile * kChunks % THREADS == 0;
+  Pack<T, kPer> x[kCount];
 
-// one bit a walked row of a tile of 64: rows before `end` that the mask keeps (the whole wave calls)
+  __device__ __forceinline__ void fetch(const T* base, int64_t stride, int64_t first, int64_t end,
+                                        int D, bool vec, const uint8_t* mask) {
+#pragma unroll
+    for (int n = 0; n < kCount; ++n) {
+      const int i = n * THREADS + threadIdx.x;
+      const int64_t row = first + i / kChunks;
+      const bool live = row < end && (kEven || i < S::kTile * kChunks) &&
+                        (mask == nullptr || mask[row] != 0);
+      x[n] = load_row<T, kPer>(base + (live ? row : 0) * stride, i % kChunks * kPer, live ? D : 0, vec);
+    }
+  }
+  __device__ __forceinline__ void commit(char* tile) const {
+#pragma unroll
+    for (int n = 0; n < kCount; ++n) {
+      const int i = n * THREADS + threadIdx.x;
+      if (!kEven && i >= S::kTile * kChunks) break;
+      char* p = tile + i / kChunks * S::kRow + i % kChunks * kPer * 2;
+      if constexpr (sizeof(T) == 4) {
+        uint32_t a[3], b[3];
+        planes_of(x[n].v[0], x[n].v[1], a);
+        planes_of(x[n].v[2], x[n].v[3], b);
+#pragma unroll
+        for (int m = 0; m < 3; ++m) *reinterpret_cast<u32x2*>(p + m * S::kPlane) = u32x2{a[m], b[m]};
+      } else {
+        *reinterpret_cast<Pack<T, kPer>*>(p) = x[n];
+      }
+    }
+  }
+};
+
+// one bit a walked row of a tile: rows before `end` that the mask keeps (the whole wave calls)
+template <int ROWS>
 __device__ __forceinline__ uint64_t live_rows(int64_t first, int64_t end, const uint8_t* mask,
                                               int lane) {
   const int64_t row = first + lane;
-  return __ballot(row < end && (mask == nullptr || mask[row] != 0));
+  return __ballot(lane < ROWS && row < end && (mask == nullptr || mask[row] != 0));
 }
 
 // the wave's result, own rows as columns: element 32 b + row(r) of own row `out` = acc[b][r] * factor
-template <typename T, int DP>
-__device__ __forceinline__ void store_own(T* out, const f32x16 (&acc)[Head<T, DP>::kBlocks],
-                                          float factor, int D, bool vec, int half) {
+template <typename T, int BLOCKS>
+__device__ __forceinline__ void store_own(T* out, const f32x16 (&acc)[BLOCKS], float factor, int D,
+                                          bool vec, int half) {
 #pragma unroll
-  for (int b = 0; b < Head<T, DP>::kBlocks; ++b) {
+  for (int b = 0; b < BLOCKS; ++b) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = 32 * b + 8 * g + 4 * half;
@@ -230,32 +330,73 @@ struct AttentionArgs {
   int64_t n_tiles;
   const uint8_t* mask;
   int heads, kv_heads, D;
+  int splits;                      // parts of the walked side, each with results of its own
   bool vec, vec_out;
   bool head_major;                 // blocks walk a head's tiles in turn, not a tile's heads
   float scale;
   float *lse, *delta;              // (heads, tokens): base-2 logarithm of the sums; rows' dot products
+  float *part, *part_lse;          // of the parts: results, logarithms
   void *dq, *dk, *dv, *result;
 };
 
 struct Tile {
   int64_t first, end, begin;
-  int head;
+  int head, split;
 };
 
-// the block's tile and head; consecutive slots lie in one XCD and share its L2
+// the block's tile, head and part; consecutive slots lie in one XCD and share its L2
 __device__ __forceinline__ bool block_tile(const AttentionArgs& a, int heads, Tile& t) {
-  const int64_t slot = xcd_slot();
-  if (slot >= a.n_tiles * heads) return false;
-  const int64_t tile = a.head_major ? slot % a.n_tiles : slot / heads;
-  t.head = (int)(a.head_major ? slot / a.n_tiles : slot % heads);
+  int64_t slot = xcd_slot(), tile;
+  if (slot >= a.n_tiles * heads * a.splits) return false;
+  if (a.head_major) {
+    tile = slot % a.n_tiles;
+    slot /= a.n_tiles;
+    t.split = (int)(slot % a.splits);
+    t.head = (int)(slot / a.splits);
+  } else {
+    t.head = (int)(slot % heads);
+    slot /= heads;
+    t.split = (int)(slot % a.splits);
+    tile = slot / a.splits;
+  }
   t.first = a.tiles[3 * tile];
   t.end = a.tiles[3 * tile + 1];
   t.begin = a.tiles[3 * tile + 2];
   return true;
 }
 
-// The checks and the choices that forward and backward share. `rows`: of a tile, 128 where that
-// still gives every SIMD of the chip (1,024) a wave, 64 below and where no structure is longer.
+// part `split` of `n` walked tiles: [from, to)
+__device__ __forceinline__ void walk_part(int64_t n, const AttentionArgs& a, int split, int64_t& from,
+                                          int64_t& to) {
+  from = n * split / a.splits;
+  to = n * (split + 1) / a.splits;
+}
+
+constexpr int kCus = 256;
+constexpr int kMostSplits = 16;
+constexpr int kSplitRows = 512;    // walked rows of a part, at least
+
+// Parts of the walked side, for `blocks` blocks without: as few as give every CU two blocks and
+// leave none idle for more than a tenth of the time (blocks of equal length over the chip's 256 CUs).
+// 9,000 rows of 4 heads (284 blocks): 5 parts.
+inline int attention_splits(int64_t blocks, int64_t walked) {
+  const int64_t most = std::min<int64_t>(kMostSplits, walked / kSplitRows);
+  int best = 1;
+  double best_use = 0.0;
+  for (int s = 1; s <= std::max<int64_t>(most, 1); ++s) {
+    const int64_t n = blocks * s;
+    const double use = (double)n / ((n + kCus - 1) / kCus * kCus) * (n < 2 * kCus ? 0.6 : 1.0);
+    if (use > best_use + 0.03) {
+      best = s;
+      best_use = use;
+    }
+    if (best_use >= 0.9) break;
+  }
+  return best;
+}
+
+// The checks and the choices that forward and backward share. `rows` of a tile: 64 where no structure
+// is longer (half the block would idle), otherwise 128.
 inline int attention_args(AttentionArgs& a, int dtype, const xnn_heads* q, const xnn_heads* k,
                           const xnn_heads* v, int64_t n_tokens, int32_t head_dim,
                           const xnn_attention_tiles* plan, const uint8_t* mask, float scale,
@@ -274,7 +415,7 @@ inline int attention_args(AttentionArgs& a, int dtype, const xnn_heads* q, const
   XNN_REQUIRE(q->data && k->data && v->data, "NULL input");
   XNN_REQUIRE(plan->tiles64 && plan->tiles128 && plan->n_tiles64 > 0 && plan->n_tiles128 > 0,
               "empty plan");
-  XNN_REQUIRE(plan->n_tiles64 * q->n_heads <= (int64_t)1 << 30, "too many tiles");
+  XNN_REQUIRE(plan->n_tiles64 * q->n_heads <= (int64_t)1 << 26, "too many tiles");
   a.q = q->data;
   a.k = k->data;
   a.v = v->data;
@@ -290,17 +431,23 @@ inline int attention_args(AttentionArgs& a, int dtype, const xnn_heads* q, const
   a.D = head_dim;
   a.mask = mask;
   a.scale = scale;
+  a.splits = 1;
   const int per = 16 / storage_bytes(dtype);
   a.vec = ((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 &&
           (a.q_token | a.q_head | a.k_token | a.k_head | a.v_token | a.v_head) % per == 0 &&
           head_dim % per == 0;
-  rows = plan->max_atoms <= 64 || plan->n_tiles128 * q->n_heads * 4 < 1024 ? 64 : 128;
+  rows = plan->max_atoms <= 64 ? 64 : 128;
   a.tiles = rows == 64 ? plan->tiles64 : plan->tiles128;
   a.n_tiles = rows == 64 ? plan->n_tiles64 : plan->n_tiles128;
   // keys and values of all heads of a structure within half an XCD's 4 MB of L2: its heads side by
   // side (they share the lines of packed projections), otherwise one head after the other
   a.head_major = plan->max_atoms * a.kv_heads * head_dim * storage_bytes(dtype) * 2 > (2 << 20);
   return XNN_OK;
+}
+
+// blocks of a launch without parts
+inline int64_t attention_blocks(const xnn_attention_tiles* plan, int heads) {
+  return (plan->max_atoms <= 64 ? plan->n_tiles64 : plan->n_tiles128) * heads;
 }
 
 }  // namespace xnn

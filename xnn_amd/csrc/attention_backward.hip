@@ -20,11 +20,10 @@
 namespace xnn {
 
 template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(WAVES* kWave) void attention_dq_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void attention_dq_kernel(AttentionArgs a) {
   typedef Head<T, DP> S;
-  constexpr int kTile = 64;
-  __shared__ __align__(16) char k_tile[kTile * S::kRow];
-  __shared__ __align__(16) char v_tile[kTile * S::kRow];
+  __shared__ __align__(16) char k_tile[S::kBytes];
+  __shared__ __align__(16) char v_tile[S::kBytes];
   Tile t;
   if (!block_tile(a, a.heads, t)) return;
   const int lane = threadIdx.x & (kWave - 1), half = lane / 32;
@@ -33,20 +32,32 @@ __global__ __launch_bounds__(WAVES* kWave) void attention_dq_kernel(AttentionArg
   const int64_t kv = t.head / (a.heads / a.kv_heads);
   const T* k = (const T*)a.k + kv * a.k_head;
   const T* v = (const T*)a.v + kv * a.v_head;
-  typename Mma<T>::Frag q[S::kSteps], g[S::kSteps];
-  load_own<T, DP>((const T*)a.q + t.head * a.q_head, a.q_token, row, live, a.D, a.vec, half, q);
-  const int64_t out_stride = (int64_t)a.heads * a.D;
-  load_own<T, DP>((const T*)a.grad + (int64_t)t.head * a.D, out_stride, row, live, a.D, a.vec_out, half, g);
+  const float scale = a.scale * kLog2e;
+  int64_t from, to;
+  walk_part((t.end - t.begin + S::kTile - 1) / S::kTile, a, t.split, from, to);
+  from = t.begin + from * S::kTile;
+  to = min(t.end, t.begin + to * S::kTile);
+  Stage<T, DP, WAVES * kWave> next_k, next_v;
+  uint64_t next_keep = 0;
+  if (from < to) {
+    next_k.fetch(k, a.k_token, from, to, a.D, a.vec, a.mask);
+    next_v.fetch(v, a.v_token, from, to, a.D, a.vec, a.mask);
+    next_keep = live_rows<S::kTile>(from, to, a.mask, lane);
+  }
+  Operand<T> q[S::kSteps], g[S::kSteps];
+  const int64_t out_stride = (int64_t)a.heads * a.D, at_head = (int64_t)t.head * a.D;
+  load_own<T, DP>((const T*)a.q + t.head * a.q_head, a.q_token, row, live, a.D, a.vec, half, scale, q);
+  load_own<T, DP>((const T*)a.grad + at_head, out_stride, row, live, a.D, a.vec_out, half, 1.0f, g);
   // d_i by the products that form g_i . v_j, out_i in the place of v_j: where one key has all the
   // weight the two are the same bits and its gradient is exactly zero. The wave's 32 x 32 tile of
   // out . g holds the rows' own products on its diagonal.
   float delta = 0.0f;
   {
-    typename Mma<T>::Frag o[S::kSteps];
-    load_own<T, DP>((const T*)a.out + (int64_t)t.head * a.D, out_stride, row, live, a.D, a.vec_out, half, o);
+    Operand<T> o[S::kSteps];
+    load_own<T, DP>((const T*)a.out + at_head, out_stride, row, live, a.D, a.vec_out, half, 1.0f, o);
     f32x16 all = {};
 #pragma unroll
-    for (int c = 0; c < S::kSteps; ++c) Mma<T>::mma(o[c], g[c], all);
+    for (int c = 0; c < S::kSteps; ++c) mma<T>(o[c], g[c], all);
 #pragma unroll
     for (int r = 0; r < 16; ++r) delta = tile_row(r, half) == lane % 32 ? all[r] : delta;
     const float other = __shfl_xor(delta, 32);
@@ -55,38 +66,40 @@ __global__ __launch_bounds__(WAVES* kWave) void attention_dq_kernel(AttentionArg
   float lse = live ? a.lse[(int64_t)t.head * a.n_tokens + row] : -INFINITY;
   const bool empty = lse == -INFINITY;
   if (empty) lse = INFINITY;                               // every probability of the row is zero
-  if (live && half == 0) a.delta[(int64_t)t.head * a.n_tokens + row] = delta;
+  if (live && half == 0 && t.split == 0) a.delta[(int64_t)t.head * a.n_tokens + row] = delta;
   f32x16 dq[S::kBlocks] = {};
-  const float scale = a.scale * kLog2e;
-  scale_own<T, DP>(scale, q);
-  for (int64_t j0 = t.begin; j0 < t.end; j0 += kTile) {
+  for (int64_t j0 = from; j0 < to; j0 += S::kTile) {
     __syncthreads();
-    stage<T, DP, kTile, WAVES * kWave>(k, a.k_token, j0, t.end, a.D, a.vec, a.mask, k_tile);
-    stage<T, DP, kTile, WAVES * kWave>(v, a.v_token, j0, t.end, a.D, a.vec, a.mask, v_tile);
-    const uint64_t keep = live_rows(j0, t.end, a.mask, lane);
+    next_k.commit(k_tile);
+    next_v.commit(v_tile);
+    const uint64_t keep = next_keep;
     __syncthreads();
+    if (j0 + S::kTile < to) {
+      next_k.fetch(k, a.k_token, j0 + S::kTile, to, a.D, a.vec, a.mask);
+      next_v.fetch(v, a.v_token, j0 + S::kTile, to, a.D, a.vec, a.mask);
+      next_keep = live_rows<S::kTile>(j0 + S::kTile, to, a.mask, lane);
+    }
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < S::kTile / 32; ++b) {
       f32x16 p = {}, dp = {};
 #pragma unroll
       for (int c = 0; c < S::kSteps; ++c) {
-        Mma<T>::mma(natural_frag<T, DP>(k_tile, 32 * b + lane % 32, c, half), q[c], p);
-        Mma<T>::mma(natural_frag<T, DP>(v_tile, 32 * b + lane % 32, c, half), g[c], dp);
+        mma<T>(natural_operand<T, DP>(k_tile, 32 * b + lane % 32, c, half), q[c], p);
+        mma<T>(natural_operand<T, DP>(v_tile, 32 * b + lane % 32, c, half), g[c], dp);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        p[r] = weight<T>(p[r], scale, lse) * (dp[r] - delta);
-      if (keep != ~0ull) {
+      for (int r = 0; r < 16; ++r) p[r] = weight<T>(p[r], scale, lse) * (dp[r] - delta);
+      if (keep != (~0ull >> (64 - S::kTile))) {
         const uint64_t mine = keep >> (32 * b + 4 * half);
 #pragma unroll
         for (int r = 0; r < 16; ++r) p[r] = (mine >> tile_row(r, 0)) & 1 ? p[r] : 0.0f;
       }
 #pragma unroll
-      for (int f = 0; f < S::kFrags; ++f) {
-        const typename Mma<T>::Frag w = weight_frag<T>(p, f);
+      for (int f = 0; f < 2; ++f) {
+        const Operand<T> w = weight_operand<T, Store<T>::kPlanes>(p, f);
 #pragma unroll
         for (int d = 0; d < S::kBlocks; ++d)
-          Mma<T>::mma(transposed_frag<T, DP>(k_tile, 32 * b, d, f, lane), w, dq[d]);
+          mma<T>(transposed_operand<T, DP>(k_tile, 32 * b, d, f, lane), w, dq[d]);
       }
     }
   }
@@ -97,71 +110,89 @@ __global__ __launch_bounds__(WAVES* kWave) void attention_dq_kernel(AttentionArg
 #pragma unroll
       for (int r = 0; r < 16; ++r) dq[d][r] = 0.0f;
   }
-  store_own<T, DP>((T*)a.dq + (row * a.heads + t.head) * a.D, dq, a.scale, a.D, a.vec_out, half);
+  const int64_t at = (row * a.heads + t.head) * a.D;
+  if (a.splits > 1)
+    store_own(a.part + (int64_t)t.split * a.n_tokens * a.heads * a.D + at, dq, a.scale, a.D,
+              a.D % 4 == 0, half);
+  else
+    store_own((T*)a.dq + at, dq, a.scale, a.D, a.vec_out, half);
 }
 
 template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(WAVES* kWave) void attention_dkv_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void attention_dkv_kernel(AttentionArgs a) {
   typedef Head<T, DP> S;
-  constexpr int kTile = 64;                                // query rows of a staged tile
-  __shared__ __align__(16) char q_tile[kTile * S::kRow];
-  __shared__ __align__(16) char g_tile[kTile * S::kRow];
-  __shared__ __align__(16) float lse_tile[kTile], delta_tile[kTile];
+  __shared__ __align__(16) char q_tile[S::kBytes];
+  __shared__ __align__(16) char g_tile[S::kBytes];
+  __shared__ __align__(16) float lse_tile[S::kTile], delta_tile[S::kTile];
   Tile t;
   if (!block_tile(a, a.kv_heads, t)) return;
   const int lane = threadIdx.x & (kWave - 1), half = lane / 32;
   const int64_t key = t.first + kOwn * wave_in_block() + lane % 32;
   const bool live = key < t.end;
   const bool kept = live && (a.mask == nullptr || a.mask[key] != 0);
-  typename Mma<T>::Frag k[S::kSteps], v[S::kSteps];
-  load_own<T, DP>((const T*)a.k + t.head * a.k_head, a.k_token, key, kept, a.D, a.vec, half, k);
-  load_own<T, DP>((const T*)a.v + t.head * a.v_head, a.v_token, key, kept, a.D, a.vec, half, v);
-  f32x16 dk[S::kBlocks] = {}, dv[S::kBlocks] = {};
   const float scale = a.scale * kLog2e;
-  scale_own<T, DP>(scale, k);
   const int group = a.heads / a.kv_heads;
   const int64_t out_stride = (int64_t)a.heads * a.D;
-  for (int h = t.head * group; h < (t.head + 1) * group; ++h) {
-    const T* q = (const T*)a.q + h * a.q_head;
-    const T* g = (const T*)a.grad + (int64_t)h * a.D;
-    for (int64_t i0 = t.begin; i0 < t.end; i0 += kTile) {
-      __syncthreads();
-      stage<T, DP, kTile, WAVES * kWave>(q, a.q_token, i0, t.end, a.D, a.vec, nullptr, q_tile);
-      stage<T, DP, kTile, WAVES * kWave>(g, out_stride, i0, t.end, a.D, a.vec_out, nullptr, g_tile);
-      if (threadIdx.x < kTile) {
-        const int64_t i = i0 + threadIdx.x;
-        const float l = i < t.end ? a.lse[(int64_t)h * a.n_tokens + i] : -INFINITY;
-        lse_tile[threadIdx.x] = l == -INFINITY ? INFINITY : l;
-        delta_tile[threadIdx.x] = i < t.end ? a.delta[(int64_t)h * a.n_tokens + i] : 0.0f;
+  // the walk: the rows of every head that shares these keys
+  const int64_t per = (t.end - t.begin + S::kTile - 1) / S::kTile;
+  int64_t from, to;
+  walk_part(per * group, a, t.split, from, to);
+  Stage<T, DP, WAVES * kWave> next_q, next_g;
+  float next_lse = 0.0f, next_delta = 0.0f;
+  const auto fetch = [&](int64_t n) {
+    const int h = t.head * group + (int)(n / per);
+    const int64_t i0 = t.begin + n % per * S::kTile;
+    next_q.fetch((const T*)a.q + h * a.q_head, a.q_token, i0, t.end, a.D, a.vec, nullptr);
+    next_g.fetch((const T*)a.grad + (int64_t)h * a.D, out_stride, i0, t.end, a.D, a.vec_out, nullptr);
+    const int64_t i = i0 + threadIdx.x;
+    if (threadIdx.x < S::kTile) {
+      next_lse = i < t.end ? a.lse[(int64_t)h * a.n_tokens + i] : -INFINITY;
+      next_delta = i < t.end ? a.delta[(int64_t)h * a.n_tokens + i] : 0.0f;
+    }
+  };
+  if (from < to) fetch(from);
+  Operand<T> k[S::kSteps], v[S::kSteps];
+  load_own<T, DP>((const T*)a.k + t.head * a.k_head, a.k_token, key, kept, a.D, a.vec, half, scale, k);
+  load_own<T, DP>((const T*)a.v + t.head * a.v_head, a.v_token, key, kept, a.D, a.vec, half, 1.0f, v);
+  f32x16 dk[S::kBlocks] = {}, dv[S::kBlocks] = {};
+  for (int64_t n = from; n < to; ++n) {
+    __syncthreads();
+    next_q.commit(q_tile);
+    next_g.commit(g_tile);
+    if (threadIdx.x < S::kTile) {
+      // a row beyond the structure or without keys: every probability is zero
+      lse_tile[threadIdx.x] = next_lse == -INFINITY ? INFINITY : next_lse;
+      delta_tile[threadIdx.x] = next_delta;
+    }
+    __syncthreads();
+    if (n + 1 < to) fetch(n + 1);
+#pragma unroll
+    for (int b = 0; b < S::kTile / 32; ++b) {
+      f32x16 p = {}, dp = {};
+#pragma unroll
+      for (int c = 0; c < S::kSteps; ++c) {
+        mma<T>(natural_operand<T, DP>(q_tile, 32 * b + lane % 32, c, half), k[c], p);
+        mma<T>(natural_operand<T, DP>(g_tile, 32 * b + lane % 32, c, half), v[c], dp);
       }
-      __syncthreads();
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        f32x16 p = {}, dp = {};
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const f32x4 l = *(const f32x4*)(lse_tile + 32 * b + 8 * q4 + 4 * half);
+        const f32x4 d = *(const f32x4*)(delta_tile + 32 * b + 8 * q4 + 4 * half);
 #pragma unroll
-        for (int c = 0; c < S::kSteps; ++c) {
-          Mma<T>::mma(natural_frag<T, DP>(q_tile, 32 * b + lane % 32, c, half), k[c], p);
-          Mma<T>::mma(natural_frag<T, DP>(g_tile, 32 * b + lane % 32, c, half), v[c], dp);
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * q4 + j;
+          p[r] = weight<T>(p[r], scale, l[j]);
+          dp[r] = p[r] * (dp[r] - d[j]);
         }
+      }
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          const f32x4 l = *(const f32x4*)(lse_tile + 32 * b + 8 * q4 + 4 * half);
-          const f32x4 d = *(const f32x4*)(delta_tile + 32 * b + 8 * q4 + 4 * half);
+      for (int f = 0; f < 2; ++f) {
+        const Operand<T> w = weight_operand<T, Store<T>::kPlanes>(p, f);
+        const Operand<T> dw = weight_operand<T, Store<T>::kPlanes>(dp, f);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = 4 * q4 + j;
-            p[r] = weight<T>(p[r], scale, l[j]);
-            dp[r] = p[r] * (dp[r] - d[j]);
-          }
-        }
-#pragma unroll
-        for (int f = 0; f < S::kFrags; ++f) {
-          const typename Mma<T>::Frag w = weight_frag<T>(p, f), dw = weight_frag<T>(dp, f);
-#pragma unroll
-          for (int d = 0; d < S::kBlocks; ++d) {
-            Mma<T>::mma(transposed_frag<T, DP>(g_tile, 32 * b, d, f, lane), w, dv[d]);
-            Mma<T>::mma(transposed_frag<T, DP>(q_tile, 32 * b, d, f, lane), dw, dk[d]);
-          }
+        for (int d = 0; d < S::kBlocks; ++d) {
+          mma<T>(transposed_operand<T, DP>(g_tile, 32 * b, d, f, lane), w, dv[d]);
+          mma<T>(transposed_operand<T, DP>(q_tile, 32 * b, d, f, lane), dw, dk[d]);
         }
       }
     }
@@ -174,21 +205,74 @@ __global__ __launch_bounds__(WAVES* kWave) void attention_dkv_kernel(AttentionAr
       for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.0f;
   }
   const int64_t at = (key * a.kv_heads + t.head) * a.D;
-  store_own<T, DP>((T*)a.dk + at, dk, a.scale, a.D, a.vec_out, half);
-  store_own<T, DP>((T*)a.dv + at, dv, 1.0f, a.D, a.vec_out, half);
+  if (a.splits > 1) {
+    const int64_t one = a.n_tokens * a.kv_heads * a.D;
+    store_own(a.part + t.split * one + at, dk, a.scale, a.D, a.D % 4 == 0, half);
+    store_own(a.part + (a.splits + t.split) * one + at, dv, 1.0f, a.D, a.D % 4 == 0, half);
+  } else {
+    store_own((T*)a.dk + at, dk, a.scale, a.D, a.vec_out, half);
+    store_own((T*)a.dv + at, dv, 1.0f, a.D, a.vec_out, half);
+  }
+}
+
+// out[i] = sum over the parts in order, N elements a thread; blockIdx.y: the first or the second of
+// two gradients, whose parts follow each other
+template <typename T, int N>
+__global__ __launch_bounds__(256) void attention_sum_kernel(const float* __restrict__ part, int64_t n,
+                                                            int splits, T* __restrict__ a,
+                                                            T* __restrict__ b) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N;
+  if (i >= n) return;
+  part += (int64_t)blockIdx.y * splits * n;
+  float sum[N] = {};
+  for (int s = 0; s < splits; ++s) {
+    float x[N];
+    load_pack<float, N>(part + s * n + i, x);
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum[j] += x[j];
+  }
+  store_pack<T, N>((blockIdx.y == 0 ? a : b) + i, sum);
+}
+
+template <typename T>
+static void attention_sum(const AttentionArgs& a, int64_t n, void* x, void* y, hipStream_t s) {
+  const unsigned both = y == nullptr ? 1 : 2;
+  if (a.vec_out)
+    hipLaunchKernelGGL((attention_sum_kernel<T, 4>), dim3((unsigned)((n / 4 + 255) / 256), both),
+                       dim3(256), 0, s, a.part, n, a.splits, (T*)x, (T*)y);
+  else
+    hipLaunchKernelGGL((attention_sum_kernel<T, 1>), dim3((unsigned)((n + 255) / 256), both),
+                       dim3(256), 0, s, a.part, n, a.splits, (T*)x, (T*)y);
 }
 
 template <typename T, int DP>
-static void attention_backward_launch(const AttentionArgs& a, int rows, hipStream_t s) {
-  const dim3 q_grid((unsigned)xcd_blocks(a.n_tiles * a.heads));
-  const dim3 k_grid((unsigned)xcd_blocks(a.n_tiles * a.kv_heads));
-  if (rows == 64) {
+static void attention_backward_launch(AttentionArgs a, int rows, int q_splits, int k_splits,
+                                      hipStream_t s) {
+  const dim3 q_grid((unsigned)xcd_blocks(a.n_tiles * a.heads * q_splits));
+  const dim3 k_grid((unsigned)xcd_blocks(a.n_tiles * a.kv_heads * k_splits));
+  a.splits = q_splits;
+  if (rows == 64)
     hipLaunchKernelGGL((attention_dq_kernel<T, DP, 2>), q_grid, dim3(128), 0, s, a);
-    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 2>), k_grid, dim3(128), 0, s, a);
-  } else {
+  else
     hipLaunchKernelGGL((attention_dq_kernel<T, DP, 4>), q_grid, dim3(256), 0, s, a);
+  if (q_splits > 1) attention_sum<T>(a, a.n_tokens * a.heads * a.D, a.dq, nullptr, s);
+  a.splits = k_splits;
+  if (rows == 64)
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 2>), k_grid, dim3(128), 0, s, a);
+  else
     hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 4>), k_grid, dim3(256), 0, s, a);
-  }
+  if (k_splits > 1) attention_sum<T>(a, a.n_tokens * a.kv_heads * a.D, a.dk, a.dv, s);
+}
+
+// the rows' dot products, then the parts of the queries' gradients and after those the parts of the
+// keys' and values' (one after the other in the same place)
+static int64_t delta_floats(int64_t n_tokens, int heads) { return (n_tokens * heads + 3) / 4 * 4; }
+
+static size_t backward_bytes(int64_t n_tokens, int heads, int kv_heads, int D, int q_splits,
+                             int k_splits) {
+  const int64_t q = q_splits == 1 ? 0 : (int64_t)q_splits * heads;
+  const int64_t k = k_splits == 1 ? 0 : (int64_t)2 * k_splits * kv_heads;
+  return sizeof(float) * (size_t)(delta_floats(n_tokens, heads) + std::max(q, k) * n_tokens * D);
 }
 
 }  // namespace xnn
@@ -197,10 +281,17 @@ using namespace xnn;
 
 extern "C" {
 
-int xnn_attention_backward_work_size(int64_t n_tokens, int32_t n_heads, size_t* bytes) {
-  XNN_REQUIRE(n_tokens >= 0 && n_heads >= 1, "sizes out of range");
-  XNN_REQUIRE(bytes != nullptr, "NULL size");
-  *bytes = sizeof(float) * (size_t)n_tokens * (size_t)n_heads;
+int xnn_attention_backward_work_size(int64_t n_tokens, int32_t n_heads, int32_t n_kv_heads,
+                                     int32_t head_dim, const xnn_attention_tiles* plan,
+                                     size_t* bytes) {
+  XNN_REQUIRE(plan && bytes, "NULL plan or size");
+  XNN_REQUIRE(n_tokens >= 0 && n_heads >= 1 && n_kv_heads >= 1 && n_heads % n_kv_heads == 0 &&
+                  head_dim >= 1,
+              "sizes out of range");
+  const int q = attention_splits(attention_blocks(plan, n_heads), plan->max_atoms);
+  const int k = attention_splits(attention_blocks(plan, n_kv_heads),
+                                 plan->max_atoms * (n_heads / n_kv_heads));
+  *bytes = backward_bytes(n_tokens, n_heads, n_kv_heads, head_dim, q, k);
   return XNN_OK;
 }
 
@@ -214,7 +305,12 @@ int xnn_attention_backward(int dtype, const xnn_heads* q, const xnn_heads* k, co
   const int status = attention_args(a, dtype, q, k, v, n_tokens, head_dim, plan, mask, scale, rows);
   if (status != XNN_OK || n_tokens == 0) return status;
   XNN_REQUIRE(out && lse && grad && dq && dk && dv && work, "NULL input, output or work");
-  XNN_REQUIRE(work_bytes >= sizeof(float) * (size_t)n_tokens * (size_t)q->n_heads, "work too small");
+  const int q_splits = attention_splits(attention_blocks(plan, a.heads), plan->max_atoms);
+  const int k_splits = attention_splits(attention_blocks(plan, a.kv_heads),
+                                        plan->max_atoms * (a.heads / a.kv_heads));
+  XNN_REQUIRE(work_bytes >= backward_bytes(n_tokens, a.heads, a.kv_heads, head_dim, q_splits, k_splits),
+              "work too small");
+  XNN_REQUIRE((uintptr_t)work % 16 == 0, "work must be aligned to 16 bytes");
   a.out = out;
   a.lse = const_cast<float*>(lse);
   a.grad = grad;
@@ -222,18 +318,19 @@ int xnn_attention_backward(int dtype, const xnn_heads* q, const xnn_heads* k, co
   a.dk = dk;
   a.dv = dv;
   a.delta = (float*)work;
+  a.part = a.delta + delta_floats(n_tokens, a.heads);
   a.vec_out = head_dim % (16 / storage_bytes(dtype)) == 0 &&
               ((uintptr_t)out | (uintptr_t)grad | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0;
   hipStream_t s = as_hip(stream);
   XNN_STORAGE_DISPATCH(dtype, T, {
     if (head_dim <= 16)
-      attention_backward_launch<T, 16>(a, rows, s);
+      attention_backward_launch<T, 16>(a, rows, q_splits, k_splits, s);
     else if (head_dim <= 32)
-      attention_backward_launch<T, 32>(a, rows, s);
+      attention_backward_launch<T, 32>(a, rows, q_splits, k_splits, s);
     else if (head_dim <= 64)
-      attention_backward_launch<T, 64>(a, rows, s);
+      attention_backward_launch<T, 64>(a, rows, q_splits, k_splits, s);
     else
-      attention_backward_launch<T, 128>(a, rows, s);
+      attention_backward_launch<T, 128>(a, rows, q_splits, k_splits, s);
   });
   XNN_LAUNCH_CHECK();
   return XNN_OK;
