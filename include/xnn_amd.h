@@ -1164,8 +1164,8 @@ typedef struct {
 /* The row tiles of a batch (xnn_attention_plan): three int32 a tile, the first row, the end
  * and the begin of its structure; max_atoms is the longest structure. */
 typedef struct {
-  int64_t n_tokens, max_atoms, n_tiles64, n_tiles128;
-  const int32_t *tiles64, *tiles128;
+  int64_t n_tokens, max_atoms, n_tiles32, n_tiles128;
+  const int32_t *tiles32, *tiles128;
 } xnn_attention_tiles;
 
 /* out[t] = scale * table[ids[t]], out (n, n_channels), table (n_rows, n_channels); an id
@@ -1219,13 +1219,14 @@ int xnn_head_norm_rotate_backward(int dtype, const xnn_heads* q, const xnn_heads
                                   void* d_k_weight, float* d_cos, float* d_sin, void* work,
                                   size_t work_bytes, xnn_stream_t stream);
 
-/* Tiles of 64 and 128 rows of a batch of structures of n_atoms[b] consecutive tokens each: ptr
- * (B + 1), tile_ptr (2 (B + 1)), the lists of three int32 a tile with room for n_tokens / 64 + B
- * and n_tokens / 128 + B tiles, and info (5): tiles of 64, tiles of 128, longest structure,
- * status (0; 1: a negative or too large count; 2: the counts do not sum to n_tokens), sum. */
+/* Tiles of 32 and 128 rows of a batch of structures of n_atoms[b] consecutive tokens each, the
+ * longer structures first: ptr (B + 1), tile_ptr (2 (B + 1)), order (B), the lists of three int32 a
+ * tile with room for n_tokens / 32 + B and n_tokens / 128 + B tiles, and info (5): tiles of 32,
+ * tiles of 128, longest structure, status (0; 1: a negative or too large count; 2: the counts do
+ * not sum to n_tokens), sum. */
 int xnn_attention_plan(const int64_t* n_atoms, int64_t n_structures, int64_t n_tokens, int64_t* ptr,
-                       int64_t* tile_ptr, int32_t* tiles64, int64_t capacity64, int32_t* tiles128,
-                       int64_t capacity128, int64_t* info, xnn_stream_t stream);
+                       int64_t* tile_ptr, int64_t* order, int32_t* tiles32, int64_t capacity32,
+                       int32_t* tiles128, int64_t capacity128, int64_t* info, xnn_stream_t stream);
 
 /* Bytes of the workspace of xnn_attention (0 where it needs none: only long structures of few
  * tiles are walked in parts that are joined). */

@@ -77,9 +77,9 @@ def test_head_norm_arguments(lib):
 def test_attention_arguments(lib):
     from xnn_amd import _lib
 
-    def plan(tokens=10, n64=1, n128=1, tiles=True):
+    def plan(tokens=10, n32=1, n128=1, tiles=True):
         at = ctypes.addressof(BUF) if tiles else None
-        return ctypes.byref(_lib.AttentionTiles(tokens, 10, n64, n128, at, at))
+        return ctypes.byref(_lib.AttentionTiles(tokens, 10, n32, n128, at, at))
 
     def call(dtype=0, H=4, K=2, KV=2, T=10, D=16, p=None, scale=0.25, out=BUF, q=None):
         return lib.xnn_attention(dtype, _heads(H, q), _heads(K), _heads(KV), T, D, p or plan(), None,
@@ -90,15 +90,15 @@ def test_attention_arguments(lib):
     _refused(lib, call(H=3), b"multiple")
     _refused(lib, call(KV=1), b"multiple")
     _refused(lib, call(T=9), b"another number")
-    _refused(lib, call(p=plan(n64=0)), b"empty plan")
+    _refused(lib, call(p=plan(n32=0)), b"empty plan")
     _refused(lib, call(p=plan(tiles=False)), b"empty plan")
     for scale in (0.0, -1.0, float("inf"), float("nan")):
         _refused(lib, call(scale=scale), b"scale")
     _refused(lib, call(out=None), b"NULL output")
     _refused(lib, call(q=0), b"NULL input")
     assert call(T=0, p=plan(tokens=0, tiles=False), out=None) == 0
-    _refused(lib, lib.xnn_attention_plan(BUF, 2, 100, BUF, BUF, BUF, 2, BUF, 2, BUF, None), b"too small")
-    _refused(lib, lib.xnn_attention_plan(BUF, 2, 1 << 31, BUF, BUF, BUF, 2, BUF, 2, BUF, None), b"too many")
+    _refused(lib, lib.xnn_attention_plan(BUF, 2, 100, BUF, BUF, BUF, BUF, 2, BUF, 2, BUF, None), b"too small")
+    _refused(lib, lib.xnn_attention_plan(BUF, 2, 1 << 31, BUF, BUF, BUF, BUF, 2, BUF, 2, BUF, None), b"too many")
     assert lib.xnn_attention_backward_work_size(10, 4, 2, 16, plan(), ctypes.byref(SIZE)) == 0
     long = ctypes.byref(_lib.AttentionTiles(9000, 9000, 141, 71, None, None))
     assert lib.xnn_attention_work_size(9000, 4, 32, long, ctypes.byref(SPLIT)) == 0 and SPLIT.value > 0

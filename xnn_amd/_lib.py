@@ -109,8 +109,8 @@ class Heads(ctypes.Structure):
 
 class AttentionTiles(ctypes.Structure):
     """``xnn_attention_tiles``."""
-    _fields_ = [("n_tokens", i64), ("max_atoms", i64), ("n_tiles64", i64), ("n_tiles128", i64),
-                ("tiles64", vp), ("tiles128", vp)]
+    _fields_ = [("n_tokens", i64), ("max_atoms", i64), ("n_tiles32", i64), ("n_tiles128", i64),
+                ("tiles32", vp), ("tiles128", vp)]
 
 
 _heads, _tiles = ctypes.POINTER(Heads), ctypes.POINTER(AttentionTiles)
@@ -282,7 +282,7 @@ _SIGNATURES = {
     "xnn_head_norm_rotate_backward_work_size": [i32, vp],
     "xnn_head_norm_rotate_backward": [c_int, _heads, _heads, i64, i32, i32, vp, vp, vp, vp, i64, vp,
                                       f32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp],
-    "xnn_attention_plan": [vp, i64, i64, vp, vp, vp, i64, vp, i64, vp, vp],
+    "xnn_attention_plan": [vp, i64, i64, vp, vp, vp, vp, i64, vp, i64, vp, vp],
     "xnn_attention_work_size": [i64, i32, i32, _tiles, vp],
     "xnn_attention": [c_int, _heads, _heads, _heads, i64, i32, _tiles, vp, f32, vp, vp, vp, sz, vp],
     "xnn_attention_backward_work_size": [i64, i32, i32, i32, _tiles, vp],

@@ -313,13 +313,13 @@ class AttentionPlan:
     n_tokens: int
     n_structures: int
     max_atoms: int
-    tiles64: Tensor                  # (tiles, 3) int32: first row, end and begin of its structure
+    tiles32: Tensor                  # (tiles, 3) int32: first row, end and begin of its structure
     tiles128: Tensor
     ptr: Tensor                      # (B + 1,) int64
 
     def __post_init__(self):
-        self.c = _lib.AttentionTiles(self.n_tokens, self.max_atoms, self.tiles64.shape[0],
-                                     self.tiles128.shape[0], self.tiles64.data_ptr(),
+        self.c = _lib.AttentionTiles(self.n_tokens, self.max_atoms, self.tiles32.shape[0],
+                                     self.tiles128.shape[0], self.tiles32.data_ptr(),
                                      self.tiles128.data_ptr())
         self._bytes = {}
 
@@ -348,20 +348,20 @@ def attention_plan(n_atoms: Tensor, n_tokens: Optional[int] = None) -> Attention
     if n_tokens < 0:
         raise ValueError(f"negative number of atoms ({n_tokens})")
     B = n_atoms.shape[0]
-    caps = [n_tokens // 64 + B, n_tokens // 128 + B]
+    caps = [n_tokens // 32 + B, n_tokens // 128 + B]
     ints = torch.empty(3 * sum(caps), dtype=torch.int32, device=device)
-    longs = torch.empty(3 * (B + 1) + 5, dtype=torch.int64, device=device)
-    ptr, tile_ptr, info = longs.split([B + 1, 2 * (B + 1), 5])
+    longs = torch.empty(4 * B + 8, dtype=torch.int64, device=device)
+    ptr, tile_ptr, order, info = longs.split([B + 1, 2 * (B + 1), B, 5])
     lists = ints.split([3 * c for c in caps])
     _lib.call("xnn_attention_plan", n_atoms.data_ptr(), B, n_tokens, ptr.data_ptr(),
-              tile_ptr.data_ptr(), lists[0].data_ptr(), caps[0], lists[1].data_ptr(), caps[1],
+              tile_ptr.data_ptr(), order.data_ptr(), lists[0].data_ptr(), caps[0], lists[1].data_ptr(), caps[1],
               info.data_ptr(), _stream(n_atoms))
-    n64, n128, longest, status, total = info.tolist()
+    n32, n128, longest, status, total = info.tolist()
     if status == 1:
         raise ValueError(f"n_atoms holds a count outside [0, {n_tokens}]")
     if status == 2:
         raise ValueError(f"n_atoms sums to {total}, the batch has {n_tokens} atoms")
-    return AttentionPlan(n_tokens, B, longest, lists[0][:3 * n64].view(-1, 3),
+    return AttentionPlan(n_tokens, B, longest, lists[0][:3 * n32].view(-1, 3),
                          lists[1][:3 * n128].view(-1, 3), ptr)
 
 

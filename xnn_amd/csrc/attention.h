@@ -31,6 +31,7 @@
 
 namespace xnn {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -112,15 +113,15 @@ __device__ __forceinline__ void planes_of(float a, float b, uint32_t (&out)[3]) 
 }
 
 // Sizes of a head padded to DP elements (16, 32, 64 or 128; zeros beyond the head)
-template <typename T, int DP>
+template <typename T, int DP, int TILE = 64>
 struct Head {
   static constexpr int kPlanes = Store<T>::kPlanes;
   static constexpr int kSteps = DP / 16;                 // operands along the head
   static constexpr int kBlocks = (DP + 31) / 32;         // 32-element blocks of an output
-  static constexpr int kWide = kBlocks * 32;             // elements of a staged row
+  static constexpr int kWide = DP;                       // elements of a staged row
   static constexpr int kRow = kWide * 2 + 16;            // its bytes in a plane: 16 more spread the banks
-  // walked rows of a staged tile: 64, or 32 where three planes of 64 would leave a CU one block
-  static constexpr int kTile = kPlanes == 3 && DP == 128 ? 32 : 64;
+  // walked rows of a staged tile: 32 also where three planes of 64 would leave a CU one block
+  static constexpr int kTile = kPlanes == 3 && DP == 128 ? 32 : TILE;
   static constexpr int kPlane = kTile * kRow;
   // waves of a SIMD: two share its matrix core and vector unit where their registers fit
   static constexpr int kOccupancy = DP <= 32 || (kPlanes == 1 && DP == 64) ? 2 : 1;
@@ -145,41 +146,49 @@ __device__ __forceinline__ Operand<T, WP> weight_operand(const f32x16& p, int f)
 #pragma unroll
     for (int n = 0; n < 3; ++n) out.p[n] = __builtin_bit_cast(Frag<T>, w[n]);
   } else {
+    typedef T Two __attribute__((ext_vector_type(2)));
+    u32x4 w[WP];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out.p[0][i] = (T)p[8 * f + i];
-    if constexpr (WP == 2) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) out.p[1][i] = (T)(p[8 * f + i] - (float)out.p[0][i]);
+    for (int i = 0; i < 4; ++i) {
+      const f32x2 x = {p[8 * f + 2 * i], p[8 * f + 2 * i + 1]};
+      const Two y = __builtin_convertvector(x, Two);
+      w[0][i] = __builtin_bit_cast(uint32_t, y);
+      if constexpr (WP == 2)
+        w[1][i] = __builtin_bit_cast(
+            uint32_t, __builtin_convertvector(x - __builtin_convertvector(y, f32x2), Two));
     }
+#pragma unroll
+    for (int n = 0; n < WP; ++n) out.p[n] = __builtin_bit_cast(Frag<T>, w[n]);
   }
   return out;
 }
 
 // operand `step` along the head of walked row `row`
-template <typename T, int DP>
+template <typename T, typename S>
 __device__ __forceinline__ Operand<T> natural_operand(const char* tile, int row, int step, int half) {
   Operand<T> out;
 #pragma unroll
-  for (int n = 0; n < Store<T>::kPlanes; ++n)
-    out.p[n] = *reinterpret_cast<const Frag<T>*>(tile + n * Head<T, DP>::kPlane +
-                                                 row * Head<T, DP>::kRow + 32 * step + 16 * half);
+  for (int n = 0; n < S::kPlanes; ++n)
+    out.p[n] = *reinterpret_cast<const Frag<T>*>(tile + n * S::kPlane + row * S::kRow + 32 * step +
+                                                 16 * half);
   return out;
 }
 
 // operand f along the 32 walked rows from `row0`, for the head's elements 32 block + lane % 32:
-// sixteen lanes read four rows of sixteen elements and get a column of four each
-template <typename T, int DP>
+// sixteen lanes read four rows of sixteen elements and get a column of four each (a head of 16 gives
+// the upper lanes the same columns again: outputs beyond the head, which are not stored)
+template <typename T, typename S>
 __device__ __forceinline__ Operand<T> transposed_operand(const char* tile, int row0, int block, int f,
                                                          int lane) {
-  constexpr int kRow = Head<T, DP>::kRow;
+  constexpr int kRow = S::kRow;
   typedef __attribute__((address_space(3))) s16x4* lds_ptr;
   const int l = lane % 16;
   const char* p = tile + (row0 + 16 * f + 4 * (lane / 32) + l / 4) * kRow +
-                  (32 * block + 16 * ((lane / 16) & 1) + 4 * (l % 4)) * 2;
+                  (32 * block + (S::kWide == 16 ? 0 : 16 * ((lane / 16) & 1)) + 4 * (l % 4)) * 2;
   Operand<T> out;
 #pragma unroll
-  for (int n = 0; n < Store<T>::kPlanes; ++n) {
-    const char* q = p + n * Head<T, DP>::kPlane;
+  for (int n = 0; n < S::kPlanes; ++n) {
+    const char* q = p + n * S::kPlane;
     const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)q);
     const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(q + 8 * kRow));
     out.p[n] = __builtin_bit_cast(Frag<T>, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -188,10 +197,10 @@ __device__ __forceinline__ Operand<T> transposed_operand(const char* tile, int r
 }
 
 // N elements of a row from element d on, zeros beyond the head's D elements
-template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> load_row(const T* row, int d, int D, bool vec) {
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ Pack<T, N> load_row(const T* row, int d, int D) {
   Pack<T, N> out;
-  if (vec) {
+  if constexpr (VEC) {
     if (d < D) {
       out = *reinterpret_cast<const Pack<T, N>*>(row + d);
     } else {
@@ -208,9 +217,9 @@ __device__ __forceinline__ Pack<T, N> load_row(const T* row, int d, int D, bool 
 // The own row's operands, zeros where the row does not exist. Scores are in base 2: float32 takes
 // `scale` into the operands here (one more rounding of each, no product a score); 16 bits would
 // lose the operands' last bits and scales the scores.
-template <typename T, int DP>
+template <typename T, int DP, bool VEC>
 __device__ __forceinline__ void load_own(const T* base, int64_t stride, int64_t row, bool live, int D,
-                                         bool vec, int half, float scale,
+                                         int half, float scale,
                                          Operand<T> (&out)[Head<T, DP>::kSteps]) {
   const T* p = base + (live ? row : 0) * stride;
   D = live ? D : 0;
@@ -221,7 +230,7 @@ __device__ __forceinline__ void load_own(const T* base, int64_t stride, int64_t 
       u32x4 w[3];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const Pack<T, 4> x = load_row<T, 4>(p, d + 4 * i, D, vec);
+        const Pack<T, 4> x = load_row<T, 4, VEC>(p, d + 4 * i, D);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           uint32_t y[3];
@@ -233,7 +242,7 @@ __device__ __forceinline__ void load_own(const T* base, int64_t stride, int64_t 
 #pragma unroll
       for (int n = 0; n < 3; ++n) out[c].p[n] = __builtin_bit_cast(Frag<T>, w[n]);
     } else {
-      out[c].p[0] = __builtin_bit_cast(Frag<T>, load_row<T, 8>(p, d, D, vec));
+      out[c].p[0] = __builtin_bit_cast(Frag<T>, load_row<T, 8, VEC>(p, d, D));
     }
   }
 }
@@ -247,44 +256,68 @@ __device__ __forceinline__ float weight(float s, float scale, float base) {
   return __builtin_amdgcn_exp2f(sizeof(T) == 4 ? s - base : fmaf(s, scale, -base));
 }
 
+// the larger of a lane's value and that of the lane 32 away
+__device__ __forceinline__ float max_xor32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // A tile of walked rows on its way to LDS: fetched to registers before the products of the tile
-// before, written after them, so that the products cover the memory latency. Rows beyond `end`,
-// elements beyond the head and rows that the mask (NULL: none) leaves out become zeros, so that
-// what they hold reaches no sum.
-template <typename T, int DP, int THREADS>
+// before, written after them, so that the products cover the memory latency. A thread moves the same
+// 16 bytes of every kStep-th row. Rows beyond the structure, elements beyond the head and rows that
+// the mask (NULL: none) leaves out become zeros as they are written, so that what they hold reaches
+// no sum; their loads go to the tile's first row, which exists.
+template <typename T, typename S, int THREADS, bool VEC>
 struct Stage {
-  typedef Head<T, DP> S;
   static constexpr int kPer = 16 / sizeof(T);
   static constexpr int kChunks = S::kWide / kPer;          // 16-byte pieces of a row
-  static constexpr int kCount = (S::kTile * kChunks + THREADS - 1) / THREADS;
-  static constexpr bool kEven = S::kTile * kChunks % THREADS == 0;
+  static constexpr int kStep = THREADS / kChunks;
+  static constexpr int kCount = (S::kTile + kStep - 1) / kStep;
+  static_assert(THREADS % kChunks == 0, "a thread keeps its place in the rows");
   Pack<T, kPer> x[kCount];
+  bool keep[kCount];
+  int row, at;                                             // its first row, its element of a row
+  int64_t offset;
 
-  __device__ __forceinline__ void fetch(const T* base, int64_t stride, int64_t first, int64_t end,
-                                        int D, bool vec, const uint8_t* mask) {
+  __device__ __forceinline__ void init(int64_t stride, int D) {
+    row = threadIdx.x / kChunks;
+    at = threadIdx.x % kChunks * kPer;
+    offset = row * stride + (at < D ? at : 0);
+  }
+  // `tile`: the first of `rows` rows, `mask` its byte
+  __device__ __forceinline__ void fetch(const T* tile, int64_t stride, int64_t rows, int D,
+                                        const uint8_t* mask) {
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {
-      const int i = n * THREADS + threadIdx.x;
-      const int64_t row = first + i / kChunks;
-      const bool live = row < end && (kEven || i < S::kTile * kChunks) &&
-                        (mask == nullptr || mask[row] != 0);
-      x[n] = load_row<T, kPer>(base + (live ? row : 0) * stride, i % kChunks * kPer, live ? D : 0, vec);
+      const int r = row + n * kStep;
+      keep[n] = at < D && r < rows && r < S::kTile;
+      if (mask != nullptr) keep[n] = keep[n] && mask[r < rows ? r : 0] != 0;
+      const T* p = keep[n] ? tile + n * kStep * stride + offset : tile;
+      if constexpr (VEC) {
+        x[n] = *reinterpret_cast<const Pack<T, kPer>*>(p);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) x[n].v[j] = keep[n] && at + j < D ? p[j] : (T)0.0f;
+      }
     }
   }
   __device__ __forceinline__ void commit(char* tile) const {
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {
-      const int i = n * THREADS + threadIdx.x;
-      if (!kEven && i >= S::kTile * kChunks) break;
-      char* p = tile + i / kChunks * S::kRow + i % kChunks * kPer * 2;
+      const int r = row + n * kStep;
+      if (S::kTile % kStep != 0 && r >= S::kTile) break;
+      char* p = tile + r * S::kRow + at * 2;
+      u32x4 w = __builtin_bit_cast(u32x4, x[n]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = keep[n] ? w[j] : 0u;
       if constexpr (sizeof(T) == 4) {
         uint32_t a[3], b[3];
-        planes_of(x[n].v[0], x[n].v[1], a);
-        planes_of(x[n].v[2], x[n].v[3], b);
+        planes_of(__uint_as_float(w[0]), __uint_as_float(w[1]), a);
+        planes_of(__uint_as_float(w[2]), __uint_as_float(w[3]), b);
 #pragma unroll
         for (int m = 0; m < 3; ++m) *reinterpret_cast<u32x2*>(p + m * S::kPlane) = u32x2{a[m], b[m]};
       } else {
-        *reinterpret_cast<Pack<T, kPer>*>(p) = x[n];
+        *reinterpret_cast<u32x4*>(p) = w;
       }
     }
   }
@@ -344,10 +377,10 @@ struct Tile {
   int head, split;
 };
 
-// the block's tile, head and part; consecutive slots lie in one XCD and share its L2
-__device__ __forceinline__ bool block_tile(const AttentionArgs& a, int heads, Tile& t) {
-  int64_t slot = xcd_slot(), tile;
-  if (slot >= a.n_tiles * heads * a.splits) return false;
+// The block's tile, head and part. The plan lists the tiles of longer structures first, and blocks
+// start in their order: the long ones do not come last.
+__device__ __forceinline__ void block_tile(const AttentionArgs& a, int heads, Tile& t) {
+  int64_t slot = blockIdx.x, tile;
   if (a.head_major) {
     tile = slot % a.n_tiles;
     slot /= a.n_tiles;
@@ -362,7 +395,6 @@ __device__ __forceinline__ bool block_tile(const AttentionArgs& a, int heads, Ti
   t.first = a.tiles[3 * tile];
   t.end = a.tiles[3 * tile + 1];
   t.begin = a.tiles[3 * tile + 2];
-  return true;
 }
 
 // part `split` of `n` walked tiles: [from, to)
@@ -395,12 +427,30 @@ inline int attention_splits(int64_t blocks, int64_t walked) {
   return best;
 }
 
-// The checks and the choices that forward and backward share. `rows` of a tile: 64 where no structure
-// is longer (half the block would idle), otherwise 128.
+// Rows of a block: 32, one wave, where no structure is longer than 64 (the other waves of a larger
+// block would idle) and one wave's registers hold a tile on its way, otherwise 128.
+inline bool short_head(int bytes, int D) { return bytes * D <= 128; }
+inline int attention_rows(const xnn_attention_tiles* plan, int bytes, int D) {
+  return plan->max_atoms <= 64 && short_head(bytes, D) ? 32 : 128;
+}
+
+// blocks of a launch without parts
+inline int64_t attention_blocks(const xnn_attention_tiles* plan, int heads) {
+  return plan->n_tiles128 * heads;                         // short structures have no parts
+}
+
+// the tiles of a launch; rows that are not moved 16 bytes at a time are always walked by 128
+inline int attention_pick(AttentionArgs& a, const xnn_attention_tiles* plan, int dtype) {
+  const int rows = a.vec ? attention_rows(plan, storage_bytes(dtype), a.D) : 128;
+  a.tiles = rows == 32 ? plan->tiles32 : plan->tiles128;
+  a.n_tiles = rows == 32 ? plan->n_tiles32 : plan->n_tiles128;
+  return rows;
+}
+
+// the checks and the choices that forward and backward share
 inline int attention_args(AttentionArgs& a, int dtype, const xnn_heads* q, const xnn_heads* k,
                           const xnn_heads* v, int64_t n_tokens, int32_t head_dim,
-                          const xnn_attention_tiles* plan, const uint8_t* mask, float scale,
-                          int& rows) {
+                          const xnn_attention_tiles* plan, const uint8_t* mask, float scale) {
   XNN_REQUIRE(is_storage(dtype), "dtype must be XNN_F32, XNN_BF16 or XNN_F16");
   XNN_REQUIRE(q && k && v && plan, "NULL heads or plan");
   XNN_REQUIRE(n_tokens >= 0 && n_tokens < ((int64_t)1 << 31) - 128, "token count out of range");
@@ -413,9 +463,9 @@ inline int attention_args(AttentionArgs& a, int dtype, const xnn_heads* q, const
   a = AttentionArgs{};
   if (n_tokens == 0) return XNN_OK;
   XNN_REQUIRE(q->data && k->data && v->data, "NULL input");
-  XNN_REQUIRE(plan->tiles64 && plan->tiles128 && plan->n_tiles64 > 0 && plan->n_tiles128 > 0,
+  XNN_REQUIRE(plan->tiles32 && plan->tiles128 && plan->n_tiles32 > 0 && plan->n_tiles128 > 0,
               "empty plan");
-  XNN_REQUIRE(plan->n_tiles64 * q->n_heads <= (int64_t)1 << 26, "too many tiles");
+  XNN_REQUIRE(plan->n_tiles32 * q->n_heads <= (int64_t)1 << 26, "too many tiles");
   a.q = q->data;
   a.k = k->data;
   a.v = v->data;
@@ -436,18 +486,10 @@ inline int attention_args(AttentionArgs& a, int dtype, const xnn_heads* q, const
   a.vec = ((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 &&
           (a.q_token | a.q_head | a.k_token | a.k_head | a.v_token | a.v_head) % per == 0 &&
           head_dim % per == 0;
-  rows = plan->max_atoms <= 64 ? 64 : 128;
-  a.tiles = rows == 64 ? plan->tiles64 : plan->tiles128;
-  a.n_tiles = rows == 64 ? plan->n_tiles64 : plan->n_tiles128;
   // keys and values of all heads of a structure within half an XCD's 4 MB of L2: its heads side by
   // side (they share the lines of packed projections), otherwise one head after the other
   a.head_major = plan->max_atoms * a.kv_heads * head_dim * storage_bytes(dtype) * 2 > (2 << 20);
   return XNN_OK;
-}
-
-// blocks of a launch without parts
-inline int64_t attention_blocks(const xnn_attention_tiles* plan, int heads) {
-  return (plan->max_atoms <= 64 ? plan->n_tiles64 : plan->n_tiles128) * heads;
 }
 
 }  // namespace xnn

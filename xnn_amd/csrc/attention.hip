@@ -18,87 +18,114 @@
 namespace xnn {
 
 // ---------------------------------------------------------------- plan
-// tile counts of lists of 64 and 128 rows; info: tiles of each list, longest structure, status
-__global__ __launch_bounds__(1024) void attention_plan_count_kernel(
-    const int64_t* __restrict__ n_atoms, int64_t n_structures, int64_t n_tokens,
-    int64_t* __restrict__ ptr, int64_t* __restrict__ tile_ptr, int64_t* __restrict__ info) {
-  __shared__ int64_t sums[3][16];
-  __shared__ int64_t top[16];
-  __shared__ int bad[16];
+constexpr int kLengths = 1024;     // classes of lengths, 32 rows each (the last: all longer ones)
+
+__device__ __forceinline__ int64_t atoms_of(const int64_t* n_atoms, int64_t b, int64_t n_tokens,
+                                            bool& wrong) {
+  const int64_t n = n_atoms[b];
+  const bool bad = n < 0 || n > n_tokens;
+  wrong |= bad;
+  return bad ? 0 : n;
+}
+
+// exclusive sum over the block's 1,024 threads, and the total
+__device__ __forceinline__ int64_t block_before(int64_t x, int64_t* sums, int64_t& total) {
   const int lane = threadIdx.x & (kWave - 1), wave = wave_in_block();
-  const int64_t per = (n_structures + 1023) / 1024;
-  const int64_t b0 = min(n_structures, threadIdx.x * per), b1 = min(n_structures, b0 + per);
-  int64_t s[3] = {0, 0, 0}, most = 0;
-  bool wrong = false;
-  for (int64_t b = b0; b < b1; ++b) {
-    int64_t n = n_atoms[b];
-    wrong |= n < 0 || n > n_tokens;
-    n = n < 0 || n > n_tokens ? 0 : n;
-    s[0] += n;
-    s[1] += (n + 63) / 64;
-    s[2] += (n + 127) / 128;
-    most = max(most, n);
-  }
-  int64_t x[3];
-  for (int q = 0; q < 3; ++q) {
-    x[q] = s[q];
-    for (int o = 1; o < kWave; o <<= 1) {
-      const int64_t y = __shfl_up(x[q], o);
-      if (lane >= o) x[q] += y;
-    }
-    if (lane == kWave - 1) sums[q][wave] = x[q];
-  }
-  for (int o = 1; o < kWave; o <<= 1) most = max(most, (int64_t)__shfl_xor(most, o));
-  wrong = __any(wrong);
-  if (lane == 0) {
-    top[wave] = most;
-    bad[wave] = wrong;
+  int64_t y = x;
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int64_t z = __shfl_up(y, o);
+    if (lane >= o) y += z;
   }
   __syncthreads();
-  int64_t at[3];
-  for (int q = 0; q < 3; ++q) {
-    at[q] = x[q] - s[q];
-    for (int w = 0; w < wave; ++w) at[q] += sums[q][w];
+  if (lane == kWave - 1) sums[wave] = y;
+  __syncthreads();
+  int64_t before = y - x;
+  total = 0;
+  for (int w = 0; w < 16; ++w) {
+    if (w < wave) before += sums[w];
+    total += sums[w];
   }
+  return before;
+}
+
+// One block: where each structure's rows begin (ptr), the structures by falling length (order; those
+// of one class in any order, which moves no result: every tile has an owner), the tiles of 32 and of
+// 128 rows before each of them (tile_ptr), info: tiles of each list, longest structure, status, rows
+__global__ __launch_bounds__(1024) void attention_plan_count_kernel(
+    const int64_t* __restrict__ n_atoms, int64_t n_structures, int64_t n_tokens,
+    int64_t* __restrict__ ptr, int64_t* __restrict__ tile_ptr, int64_t* order,
+    int64_t* __restrict__ info) {
+  __shared__ int64_t sums[16];
+  __shared__ int count[kLengths], wrong_any;
+  __shared__ unsigned long long longest;
+  const int tid = threadIdx.x;
+  const int64_t per = (n_structures + 1023) / 1024;
+  const int64_t b0 = min(n_structures, tid * per), b1 = min(n_structures, b0 + per);
+  count[tid] = 0;
+  if (tid == 0) {
+    wrong_any = 0;
+    longest = 0;
+  }
+  __syncthreads();
+  const auto class_of = [](int64_t n) { return (int)(kLengths - 1 - min((n + 31) / 32, (int64_t)kLengths - 1)); };
+  int64_t s = 0, most = 0;
+  bool wrong = false;
   for (int64_t b = b0; b < b1; ++b) {
-    int64_t n = n_atoms[b];
-    n = n < 0 || n > n_tokens ? 0 : n;
-    ptr[b] = at[0];
-    tile_ptr[b] = at[1];
-    tile_ptr[n_structures + 1 + b] = at[2];
-    at[0] += n;
-    at[1] += (n + 63) / 64;
-    at[2] += (n + 127) / 128;
+    const int64_t n = atoms_of(n_atoms, b, n_tokens, wrong);
+    s += n;
+    most = max(most, n);
+    atomicAdd(&count[class_of(n)], 1);
   }
-  if (threadIdx.x == 0) {
-    int64_t total[3] = {0, 0, 0}, longest = 0;
-    bool any = false;
-    for (int w = 0; w < 16; ++w) {
-      for (int q = 0; q < 3; ++q) total[q] += sums[q][w];
-      longest = max(longest, top[w]);
-      any |= bad[w] != 0;
+  if (wrong) atomicOr(&wrong_any, 1);
+  atomicMax(&longest, (unsigned long long)most);
+  int64_t rows;
+  int64_t at = block_before(s, sums, rows);
+  for (int64_t b = b0; b < b1; ++b) {
+    ptr[b] = at;
+    at += atoms_of(n_atoms, b, n_tokens, wrong);
+  }
+  int64_t all;
+  const int before = (int)block_before(count[tid], sums, all);
+  count[tid] = before;
+  __syncthreads();
+  for (int64_t b = b0; b < b1; ++b)
+    order[atomicAdd(&count[class_of(atoms_of(n_atoms, b, n_tokens, wrong))], 1)] = b;
+  __threadfence_block();
+  __syncthreads();
+  int64_t tiles[2];
+  for (int list = 0; list < 2; ++list) {
+    const int64_t size = list == 0 ? 32 : 128;
+    s = 0;
+    for (int64_t i = b0; i < b1; ++i) s += (atoms_of(n_atoms, order[i], n_tokens, wrong) + size - 1) / size;
+    at = block_before(s, sums, tiles[list]);
+    int64_t* out = tile_ptr + list * (n_structures + 1);
+    for (int64_t i = b0; i < b1; ++i) {
+      out[i] = at;
+      at += (atoms_of(n_atoms, order[i], n_tokens, wrong) + size - 1) / size;
     }
-    ptr[n_structures] = total[0];
-    tile_ptr[n_structures] = total[1];
-    tile_ptr[2 * n_structures + 1] = total[2];
-    info[0] = total[1];
-    info[1] = total[2];
-    info[2] = longest;
-    info[3] = any ? 1 : total[0] != n_tokens ? 2 : 0;
-    info[4] = total[0];
+    if (tid == 0) out[n_structures] = tiles[list];
+  }
+  if (tid == 0) {
+    ptr[n_structures] = rows;
+    info[0] = tiles[0];
+    info[1] = tiles[1];
+    info[2] = (int64_t)longest;
+    info[3] = wrong_any ? 1 : rows != n_tokens ? 2 : 0;
+    info[4] = rows;
   }
 }
 
 // one thread a tile: (first row, end of its structure, begin of its structure)
 __global__ __launch_bounds__(256) void attention_plan_fill_kernel(
-    const int64_t* __restrict__ ptr, const int64_t* __restrict__ tile_ptr, int64_t n_structures,
-    const int64_t* __restrict__ info, int64_t capacity64, int64_t capacity128,
-    int32_t* __restrict__ tiles64, int32_t* __restrict__ tiles128) {
+    const int64_t* __restrict__ ptr, const int64_t* __restrict__ tile_ptr,
+    const int64_t* __restrict__ order, int64_t n_structures, const int64_t* __restrict__ info,
+    int64_t capacity32, int64_t capacity128, int32_t* __restrict__ tiles32,
+    int32_t* __restrict__ tiles128) {
   if (info[3] != 0) return;
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int list = t < capacity64 ? 0 : 1;
-  const int64_t i = list == 0 ? t : t - capacity64;
-  if (i >= (list == 0 ? capacity64 : capacity128) || i >= info[list]) return;
+  const int list = t < capacity32 ? 0 : 1;
+  const int64_t i = list == 0 ? t : t - capacity32;
+  if (i >= (list == 0 ? capacity32 : capacity128) || i >= info[list]) return;
   const int64_t* p = tile_ptr + list * (n_structures + 1);
   int64_t lo = 0, hi = n_structures;                        // p[lo] <= i < p[hi]
   while (hi - lo > 1) {
@@ -108,24 +135,26 @@ __global__ __launch_bounds__(256) void attention_plan_fill_kernel(
     else
       hi = mid;
   }
-  int32_t* out = (list == 0 ? tiles64 : tiles128) + 3 * i;
-  out[0] = (int32_t)(ptr[lo] + (i - p[lo]) * (list == 0 ? 64 : 128));
-  out[1] = (int32_t)ptr[lo + 1];
-  out[2] = (int32_t)ptr[lo];
+  const int64_t b = order[lo];
+  int32_t* out = (list == 0 ? tiles32 : tiles128) + 3 * i;
+  out[0] = (int32_t)(ptr[b] + (i - p[lo]) * (list == 0 ? 32 : 128));
+  out[1] = (int32_t)ptr[b + 1];
+  out[2] = (int32_t)ptr[b];
 }
 
 // ---------------------------------------------------------------- forward
-template <typename T, int DP, int WAVES>
+template <typename T, int DP, int WAVES, int TILE, bool VEC>
 __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void attention_kernel(AttentionArgs a) {
-  typedef Head<T, DP> S;
+  typedef Head<T, DP, TILE> S;
   constexpr int kParts = S::kTile / 32;                    // 32-row products of a tile
   __shared__ __align__(16) char k_tile[S::kBytes];
   __shared__ __align__(16) char v_tile[S::kBytes];
   Tile t;
-  if (!block_tile(a, a.heads, t)) return;
+  block_tile(a, a.heads, t);
   const int lane = threadIdx.x & (kWave - 1), half = lane / 32;
   const int64_t row = t.first + kOwn * wave_in_block() + lane % 32;
   const bool live = row < t.end;
+  const bool busy = t.first + kOwn * wave_in_block() < t.end;   // the wave has rows
   const int64_t kv = t.head / (a.heads / a.kv_heads);
   const T* k = (const T*)a.k + kv * a.k_head;
   const T* v = (const T*)a.v + kv * a.v_head;
@@ -134,15 +163,19 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   walk_part((t.end - t.begin + S::kTile - 1) / S::kTile, a, t.split, from, to);
   from = t.begin + from * S::kTile;
   to = min(t.end, t.begin + to * S::kTile);
-  Stage<T, DP, WAVES * kWave> next_k, next_v;
+  Stage<T, S, WAVES * kWave, VEC> next_k, next_v;
   uint64_t next_keep = 0;
-  if (from < to) {
-    next_k.fetch(k, a.k_token, from, to, a.D, a.vec, a.mask);
-    next_v.fetch(v, a.v_token, from, to, a.D, a.vec, a.mask);
-    next_keep = live_rows<S::kTile>(from, to, a.mask, lane);
-  }
+  next_k.init(a.k_token, a.D);
+  next_v.init(a.v_token, a.D);
+  const auto fetch = [&](int64_t j0) {
+    const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + j0;
+    next_k.fetch(k + j0 * a.k_token, a.k_token, to - j0, a.D, mask);
+    next_v.fetch(v + j0 * a.v_token, a.v_token, to - j0, a.D, mask);
+    next_keep = live_rows<S::kTile>(j0, to, a.mask, lane);
+  };
+  if (from < to) fetch(from);
   Operand<T> q[S::kSteps];
-  load_own<T, DP>((const T*)a.q + t.head * a.q_head, a.q_token, row, live, a.D, a.vec, half, scale, q);
+  load_own<T, DP, VEC>((const T*)a.q + t.head * a.q_head, a.q_token, row, live, a.D, half, scale, q);
   f32x16 o[S::kBlocks] = {};
   float top = -INFINITY, sum = 0.0f;                       // the sum over this lane's keys only
   for (int64_t j0 = from; j0 < to; j0 += S::kTile) {
@@ -151,17 +184,14 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
     next_v.commit(v_tile);
     const uint64_t keep = next_keep;
     __syncthreads();
-    if (j0 + S::kTile < to) {
-      next_k.fetch(k, a.k_token, j0 + S::kTile, to, a.D, a.vec, a.mask);
-      next_v.fetch(v, a.v_token, j0 + S::kTile, to, a.D, a.vec, a.mask);
-      next_keep = live_rows<S::kTile>(j0 + S::kTile, to, a.mask, lane);
-    }
+    if (j0 + S::kTile < to) fetch(j0 + S::kTile);
+    if (!busy) continue;
     f32x16 p[kParts] = {};
 #pragma unroll
     for (int c = 0; c < S::kSteps; ++c)
 #pragma unroll
       for (int b = 0; b < kParts; ++b)
-        mma<T>(natural_operand<T, DP>(k_tile, 32 * b + lane % 32, c, half), q[c], p[b]);
+        mma<T>(natural_operand<T, S>(k_tile, 32 * b + lane % 32, c, half), q[c], p[b]);
     if (keep != (~0ull >> (64 - S::kTile))) {
       const uint64_t mine = keep >> (4 * half);
 #pragma unroll
@@ -175,7 +205,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
     for (int b = 0; b < kParts; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) m = fmaxf(m, p[b][r]);
-    m = score<T>(fmaxf(m, __shfl_xor(m, 32)), scale);
+    m = score<T>(max_xor32(m), scale);
     const float next = fmaxf(top, m);
     const float base = next == -INFINITY ? 0.0f : next;    // nothing kept so far
     if (__any(next != top)) {                              // rare once the walk is under way
@@ -201,10 +231,10 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
         const Operand<T> w = weight_operand<T, Store<T>::kPlanes>(p[b], f);
 #pragma unroll
         for (int d = 0; d < S::kBlocks; ++d)
-          mma<T>(transposed_operand<T, DP>(v_tile, 32 * b, d, f, lane), w, o[d]);
+          mma<T>(transposed_operand<T, S>(v_tile, 32 * b, d, f, lane), w, o[d]);
       }
   }
-  sum += __shfl_xor(sum, 32);
+  sum = add_xor32(sum);
   if (!live) return;
   const bool empty = sum == 0.0f;
   const float factor = empty ? 0.0f : 1.0f / sum;
@@ -252,11 +282,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
 
 template <typename T, int DP>
 static void attention_launch(const AttentionArgs& a, int rows, hipStream_t s) {
-  const dim3 grid((unsigned)xcd_blocks(a.n_tiles * a.heads * a.splits));
-  if (rows == 64)
-    hipLaunchKernelGGL((attention_kernel<T, DP, 2>), grid, dim3(128), 0, s, a);
-  else
-    hipLaunchKernelGGL((attention_kernel<T, DP, 4>), grid, dim3(256), 0, s, a);
+  const dim3 grid((unsigned)(a.n_tiles * a.heads * a.splits));
+  if (!a.vec)
+    hipLaunchKernelGGL((attention_kernel<T, DP, 4, 64, false>), grid, dim3(256), 0, s, a);
+  else if (rows == 128)
+    hipLaunchKernelGGL((attention_kernel<T, DP, 4, 64, true>), grid, dim3(256), 0, s, a);
+  else if constexpr (sizeof(T) * DP <= 128)
+    hipLaunchKernelGGL((attention_kernel<T, DP, 1, 32, true>), grid, dim3(64), 0, s, a);
   if (a.splits == 1) return;
   const int64_t n = a.n_tokens * a.heads;
   if (a.vec_out)
@@ -278,22 +310,24 @@ using namespace xnn;
 extern "C" {
 
 int xnn_attention_plan(const int64_t* n_atoms, int64_t n_structures, int64_t n_tokens, int64_t* ptr,
-                       int64_t* tile_ptr, int32_t* tiles64, int64_t capacity64, int32_t* tiles128,
-                       int64_t capacity128, int64_t* info, xnn_stream_t stream) {
+                       int64_t* tile_ptr, int64_t* order, int32_t* tiles32, int64_t capacity32,
+                       int32_t* tiles128, int64_t capacity128, int64_t* info, xnn_stream_t stream) {
   XNN_REQUIRE(n_structures >= 0 && n_tokens >= 0, "negative size");
-  XNN_REQUIRE(n_tokens < ((int64_t)1 << 31) - 128, "too many tokens");
-  XNN_REQUIRE(ptr && tile_ptr && info && (n_structures == 0 || n_atoms), "NULL input or output");
-  XNN_REQUIRE(capacity64 >= n_tokens / 64 + n_structures &&
+  XNN_REQUIRE(n_tokens < ((int64_t)1 << 31) - 128 && n_structures < (int64_t)1 << 31,
+              "too many tokens or structures");
+  XNN_REQUIRE(ptr && tile_ptr && info && (n_structures == 0 || (n_atoms && order)),
+              "NULL input or output");
+  XNN_REQUIRE(capacity32 >= n_tokens / 32 + n_structures &&
                   capacity128 >= n_tokens / 128 + n_structures,
               "a tile list is too small");
-  XNN_REQUIRE((capacity64 == 0 || tiles64) && (capacity128 == 0 || tiles128), "NULL tile list");
+  XNN_REQUIRE((capacity32 == 0 || tiles32) && (capacity128 == 0 || tiles128), "NULL tile list");
   hipStream_t s = as_hip(stream);
   hipLaunchKernelGGL(attention_plan_count_kernel, dim3(1), dim3(1024), 0, s, n_atoms, n_structures,
-                     n_tokens, ptr, tile_ptr, info);
-  const int64_t all = capacity64 + capacity128;
+                     n_tokens, ptr, tile_ptr, order, info);
+  const int64_t all = capacity32 + capacity128;
   if (all > 0)
     hipLaunchKernelGGL(attention_plan_fill_kernel, dim3((unsigned)((all + 255) / 256)), dim3(256), 0,
-                       s, ptr, tile_ptr, n_structures, info, capacity64, capacity128, tiles64,
+                       s, ptr, tile_ptr, order, n_structures, info, capacity32, capacity128, tiles32,
                        tiles128);
   XNN_LAUNCH_CHECK();
   return XNN_OK;
@@ -313,8 +347,7 @@ int xnn_attention(int dtype, const xnn_heads* q, const xnn_heads* k, const xnn_h
                   const uint8_t* mask, float scale, void* out, float* lse, void* work,
                   size_t work_bytes, xnn_stream_t stream) {
   AttentionArgs a;
-  int rows = 0;
-  const int status = attention_args(a, dtype, q, k, v, n_tokens, head_dim, plan, mask, scale, rows);
+  const int status = attention_args(a, dtype, q, k, v, n_tokens, head_dim, plan, mask, scale);
   if (status != XNN_OK || n_tokens == 0) return status;
   XNN_REQUIRE(out != nullptr, "NULL output");
   a.splits = attention_splits(attention_blocks(plan, a.heads), plan->max_atoms);
@@ -328,6 +361,7 @@ int xnn_attention(int dtype, const xnn_heads* q, const xnn_heads* k, const xnn_h
   a.part = (float*)work;
   a.part_lse = a.part + (size_t)a.splits * n_tokens * a.heads * head_dim;
   a.vec_out = head_dim % 4 == 0 && (uintptr_t)out % 16 == 0;
+  const int rows = attention_pick(a, plan, dtype);
   hipStream_t s = as_hip(stream);
   XNN_STORAGE_DISPATCH(dtype, T, {
     if (head_dim <= 16)

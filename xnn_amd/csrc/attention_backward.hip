@@ -19,16 +19,17 @@
 
 namespace xnn {
 
-template <typename T, int DP, int WAVES>
+template <typename T, int DP, int WAVES, int TILE, bool VEC>
 __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void attention_dq_kernel(AttentionArgs a) {
-  typedef Head<T, DP> S;
+  typedef Head<T, DP, TILE> S;
   __shared__ __align__(16) char k_tile[S::kBytes];
   __shared__ __align__(16) char v_tile[S::kBytes];
   Tile t;
-  if (!block_tile(a, a.heads, t)) return;
+  block_tile(a, a.heads, t);
   const int lane = threadIdx.x & (kWave - 1), half = lane / 32;
   const int64_t row = t.first + kOwn * wave_in_block() + lane % 32;
   const bool live = row < t.end;
+  const bool busy = t.first + kOwn * wave_in_block() < t.end;   // the wave has rows
   const int64_t kv = t.head / (a.heads / a.kv_heads);
   const T* k = (const T*)a.k + kv * a.k_head;
   const T* v = (const T*)a.v + kv * a.v_head;
@@ -37,24 +38,28 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   walk_part((t.end - t.begin + S::kTile - 1) / S::kTile, a, t.split, from, to);
   from = t.begin + from * S::kTile;
   to = min(t.end, t.begin + to * S::kTile);
-  Stage<T, DP, WAVES * kWave> next_k, next_v;
+  Stage<T, S, WAVES * kWave, VEC> next_k, next_v;
   uint64_t next_keep = 0;
-  if (from < to) {
-    next_k.fetch(k, a.k_token, from, to, a.D, a.vec, a.mask);
-    next_v.fetch(v, a.v_token, from, to, a.D, a.vec, a.mask);
-    next_keep = live_rows<S::kTile>(from, to, a.mask, lane);
-  }
+  next_k.init(a.k_token, a.D);
+  next_v.init(a.v_token, a.D);
+  const auto fetch = [&](int64_t j0) {
+    const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + j0;
+    next_k.fetch(k + j0 * a.k_token, a.k_token, to - j0, a.D, mask);
+    next_v.fetch(v + j0 * a.v_token, a.v_token, to - j0, a.D, mask);
+    next_keep = live_rows<S::kTile>(j0, to, a.mask, lane);
+  };
+  if (from < to) fetch(from);
   Operand<T> q[S::kSteps], g[S::kSteps];
   const int64_t out_stride = (int64_t)a.heads * a.D, at_head = (int64_t)t.head * a.D;
-  load_own<T, DP>((const T*)a.q + t.head * a.q_head, a.q_token, row, live, a.D, a.vec, half, scale, q);
-  load_own<T, DP>((const T*)a.grad + at_head, out_stride, row, live, a.D, a.vec_out, half, 1.0f, g);
+  load_own<T, DP, VEC>((const T*)a.q + t.head * a.q_head, a.q_token, row, live, a.D, half, scale, q);
+  load_own<T, DP, VEC>((const T*)a.grad + at_head, out_stride, row, live, a.D, half, 1.0f, g);
   // d_i by the products that form g_i . v_j, out_i in the place of v_j: where one key has all the
   // weight the two are the same bits and its gradient is exactly zero. The wave's 32 x 32 tile of
   // out . g holds the rows' own products on its diagonal.
   float delta = 0.0f;
   {
     Operand<T> o[S::kSteps];
-    load_own<T, DP>((const T*)a.out + at_head, out_stride, row, live, a.D, a.vec_out, half, 1.0f, o);
+    load_own<T, DP, VEC>((const T*)a.out + at_head, out_stride, row, live, a.D, half, 1.0f, o);
     f32x16 all = {};
 #pragma unroll
     for (int c = 0; c < S::kSteps; ++c) mma<T>(o[c], g[c], all);
@@ -74,18 +79,15 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
     next_v.commit(v_tile);
     const uint64_t keep = next_keep;
     __syncthreads();
-    if (j0 + S::kTile < to) {
-      next_k.fetch(k, a.k_token, j0 + S::kTile, to, a.D, a.vec, a.mask);
-      next_v.fetch(v, a.v_token, j0 + S::kTile, to, a.D, a.vec, a.mask);
-      next_keep = live_rows<S::kTile>(j0 + S::kTile, to, a.mask, lane);
-    }
+    if (j0 + S::kTile < to) fetch(j0 + S::kTile);
+    if (!busy) continue;
 #pragma unroll
     for (int b = 0; b < S::kTile / 32; ++b) {
       f32x16 p = {}, dp = {};
 #pragma unroll
       for (int c = 0; c < S::kSteps; ++c) {
-        mma<T>(natural_operand<T, DP>(k_tile, 32 * b + lane % 32, c, half), q[c], p);
-        mma<T>(natural_operand<T, DP>(v_tile, 32 * b + lane % 32, c, half), g[c], dp);
+        mma<T>(natural_operand<T, S>(k_tile, 32 * b + lane % 32, c, half), q[c], p);
+        mma<T>(natural_operand<T, S>(v_tile, 32 * b + lane % 32, c, half), g[c], dp);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) p[r] = weight<T>(p[r], scale, lse) * (dp[r] - delta);
@@ -99,7 +101,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
         const Operand<T> w = weight_operand<T, Store<T>::kPlanes>(p, f);
 #pragma unroll
         for (int d = 0; d < S::kBlocks; ++d)
-          mma<T>(transposed_operand<T, DP>(k_tile, 32 * b, d, f, lane), w, dq[d]);
+          mma<T>(transposed_operand<T, S>(k_tile, 32 * b, d, f, lane), w, dq[d]);
       }
     }
   }
@@ -118,17 +120,18 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
     store_own((T*)a.dq + at, dq, a.scale, a.D, a.vec_out, half);
 }
 
-template <typename T, int DP, int WAVES>
+template <typename T, int DP, int WAVES, int TILE, bool VEC>
 __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void attention_dkv_kernel(AttentionArgs a) {
-  typedef Head<T, DP> S;
+  typedef Head<T, DP, TILE> S;
   __shared__ __align__(16) char q_tile[S::kBytes];
   __shared__ __align__(16) char g_tile[S::kBytes];
   __shared__ __align__(16) float lse_tile[S::kTile], delta_tile[S::kTile];
   Tile t;
-  if (!block_tile(a, a.kv_heads, t)) return;
+  block_tile(a, a.kv_heads, t);
   const int lane = threadIdx.x & (kWave - 1), half = lane / 32;
   const int64_t key = t.first + kOwn * wave_in_block() + lane % 32;
   const bool live = key < t.end;
+  const bool busy = t.first + kOwn * wave_in_block() < t.end;   // the wave has keys
   const bool kept = live && (a.mask == nullptr || a.mask[key] != 0);
   const float scale = a.scale * kLog2e;
   const int group = a.heads / a.kv_heads;
@@ -137,13 +140,16 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   const int64_t per = (t.end - t.begin + S::kTile - 1) / S::kTile;
   int64_t from, to;
   walk_part(per * group, a, t.split, from, to);
-  Stage<T, DP, WAVES * kWave> next_q, next_g;
+  Stage<T, S, WAVES * kWave, VEC> next_q, next_g;
   float next_lse = 0.0f, next_delta = 0.0f;
+  next_q.init(a.q_token, a.D);
+  next_g.init(out_stride, a.D);
   const auto fetch = [&](int64_t n) {
     const int h = t.head * group + (int)(n / per);
     const int64_t i0 = t.begin + n % per * S::kTile;
-    next_q.fetch((const T*)a.q + h * a.q_head, a.q_token, i0, t.end, a.D, a.vec, nullptr);
-    next_g.fetch((const T*)a.grad + (int64_t)h * a.D, out_stride, i0, t.end, a.D, a.vec_out, nullptr);
+    next_q.fetch((const T*)a.q + h * a.q_head + i0 * a.q_token, a.q_token, t.end - i0, a.D, nullptr);
+    next_g.fetch((const T*)a.grad + (int64_t)h * a.D + i0 * out_stride, out_stride, t.end - i0, a.D,
+                 nullptr);
     const int64_t i = i0 + threadIdx.x;
     if (threadIdx.x < S::kTile) {
       next_lse = i < t.end ? a.lse[(int64_t)h * a.n_tokens + i] : -INFINITY;
@@ -152,8 +158,8 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   };
   if (from < to) fetch(from);
   Operand<T> k[S::kSteps], v[S::kSteps];
-  load_own<T, DP>((const T*)a.k + t.head * a.k_head, a.k_token, key, kept, a.D, a.vec, half, scale, k);
-  load_own<T, DP>((const T*)a.v + t.head * a.v_head, a.v_token, key, kept, a.D, a.vec, half, 1.0f, v);
+  load_own<T, DP, VEC>((const T*)a.k + t.head * a.k_head, a.k_token, key, kept, a.D, half, scale, k);
+  load_own<T, DP, VEC>((const T*)a.v + t.head * a.v_head, a.v_token, key, kept, a.D, half, 1.0f, v);
   f32x16 dk[S::kBlocks] = {}, dv[S::kBlocks] = {};
   for (int64_t n = from; n < to; ++n) {
     __syncthreads();
@@ -166,13 +172,14 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
     }
     __syncthreads();
     if (n + 1 < to) fetch(n + 1);
+    if (!busy) continue;
 #pragma unroll
     for (int b = 0; b < S::kTile / 32; ++b) {
       f32x16 p = {}, dp = {};
 #pragma unroll
       for (int c = 0; c < S::kSteps; ++c) {
-        mma<T>(natural_operand<T, DP>(q_tile, 32 * b + lane % 32, c, half), k[c], p);
-        mma<T>(natural_operand<T, DP>(g_tile, 32 * b + lane % 32, c, half), v[c], dp);
+        mma<T>(natural_operand<T, S>(q_tile, 32 * b + lane % 32, c, half), k[c], p);
+        mma<T>(natural_operand<T, S>(g_tile, 32 * b + lane % 32, c, half), v[c], dp);
       }
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
@@ -191,8 +198,8 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
         const Operand<T> dw = weight_operand<T, Store<T>::kPlanes>(dp, f);
 #pragma unroll
         for (int d = 0; d < S::kBlocks; ++d) {
-          mma<T>(transposed_operand<T, DP>(g_tile, 32 * b, d, f, lane), w, dv[d]);
-          mma<T>(transposed_operand<T, DP>(q_tile, 32 * b, d, f, lane), dw, dk[d]);
+          mma<T>(transposed_operand<T, S>(g_tile, 32 * b, d, f, lane), w, dv[d]);
+          mma<T>(transposed_operand<T, S>(q_tile, 32 * b, d, f, lane), dw, dk[d]);
         }
       }
     }
@@ -248,19 +255,23 @@ static void attention_sum(const AttentionArgs& a, int64_t n, void* x, void* y, h
 template <typename T, int DP>
 static void attention_backward_launch(AttentionArgs a, int rows, int q_splits, int k_splits,
                                       hipStream_t s) {
-  const dim3 q_grid((unsigned)xcd_blocks(a.n_tiles * a.heads * q_splits));
-  const dim3 k_grid((unsigned)xcd_blocks(a.n_tiles * a.kv_heads * k_splits));
+  const dim3 q_grid((unsigned)(a.n_tiles * a.heads * q_splits));
+  const dim3 k_grid((unsigned)(a.n_tiles * a.kv_heads * k_splits));
   a.splits = q_splits;
-  if (rows == 64)
-    hipLaunchKernelGGL((attention_dq_kernel<T, DP, 2>), q_grid, dim3(128), 0, s, a);
-  else
-    hipLaunchKernelGGL((attention_dq_kernel<T, DP, 4>), q_grid, dim3(256), 0, s, a);
+  if (!a.vec)
+    hipLaunchKernelGGL((attention_dq_kernel<T, DP, 4, 64, false>), q_grid, dim3(256), 0, s, a);
+  else if (rows == 128)
+    hipLaunchKernelGGL((attention_dq_kernel<T, DP, 4, 64, true>), q_grid, dim3(256), 0, s, a);
+  else if constexpr (sizeof(T) * DP <= 128)
+    hipLaunchKernelGGL((attention_dq_kernel<T, DP, 1, 32, true>), q_grid, dim3(64), 0, s, a);
   if (q_splits > 1) attention_sum<T>(a, a.n_tokens * a.heads * a.D, a.dq, nullptr, s);
   a.splits = k_splits;
-  if (rows == 64)
-    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 2>), k_grid, dim3(128), 0, s, a);
-  else
-    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 4>), k_grid, dim3(256), 0, s, a);
+  if (!a.vec)
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 4, 64, false>), k_grid, dim3(256), 0, s, a);
+  else if (rows == 128)
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 4, 64, true>), k_grid, dim3(256), 0, s, a);
+  else if constexpr (sizeof(T) * DP <= 128)
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 1, 32, true>), k_grid, dim3(64), 0, s, a);
   if (k_splits > 1) attention_sum<T>(a, a.n_tokens * a.kv_heads * a.D, a.dk, a.dv, s);
 }
 
@@ -301,8 +312,7 @@ int xnn_attention_backward(int dtype, const xnn_heads* q, const xnn_heads* k, co
                            const void* grad, void* dq, void* dk, void* dv, void* work,
                            size_t work_bytes, xnn_stream_t stream) {
   AttentionArgs a;
-  int rows = 0;
-  const int status = attention_args(a, dtype, q, k, v, n_tokens, head_dim, plan, mask, scale, rows);
+  const int status = attention_args(a, dtype, q, k, v, n_tokens, head_dim, plan, mask, scale);
   if (status != XNN_OK || n_tokens == 0) return status;
   XNN_REQUIRE(out && lse && grad && dq && dk && dv && work, "NULL input, output or work");
   const int q_splits = attention_splits(attention_blocks(plan, a.heads), plan->max_atoms);
@@ -321,6 +331,8 @@ int xnn_attention_backward(int dtype, const xnn_heads* q, const xnn_heads* k, co
   a.part = a.delta + delta_floats(n_tokens, a.heads);
   a.vec_out = head_dim % (16 / storage_bytes(dtype)) == 0 &&
               ((uintptr_t)out | (uintptr_t)grad | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0;
+  a.vec = a.vec && a.vec_out;
+  const int rows = attention_pick(a, plan, dtype);
   hipStream_t s = as_hip(stream);
   XNN_STORAGE_DISPATCH(dtype, T, {
     if (head_dim <= 16)
