@@ -32,7 +32,9 @@ def _close(got, want, bound):
 
 # --------------------------------------------------------------------------- embedding
 @pytest.mark.parametrize("n,V,C", [(1, 1, 1), (0, 5, 16), (21, 119, 128), (33, 3, 65), (4097, 2, 64),
-                                   (700, 70000, 24), (5000, 300, 250), (2500, 1000, 1024)])
+                                   (700, 70000, 24), (5000, 300, 250), (2500, 1000, 1024),
+                                   (16384, 256, 8), (20000, 1000, 8), (40000, 70000, 3),
+                                   (3000, 255, 40), (1100000, 4, 4)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_embedding_and_its_gradient(n, V, C, dtype):
     import xnn_amd as xa

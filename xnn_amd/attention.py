@@ -48,6 +48,23 @@ def _on_gpu(**tensors: Optional[Tensor]) -> torch.device:
     return device
 
 
+_FUNCTIONS: dict = {}
+
+
+def _call(name: str, *args) -> None:
+    """:func:`xnn_amd._lib.call` without its lookups: at these operators' smallest sizes the host's
+    microseconds are the time of a call."""
+    if _lib.timed:
+        return _lib.call(name, *args)
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(_lib.load(), name)
+    _lib.calls[name] = _lib.calls.get(name, 0) + 1
+    code = fn(*args)
+    if code:
+        _lib.check(name, code)
+
+
 def _once_differentiable() -> None:
     if torch.is_grad_enabled():
         raise RuntimeError("the xnn_amd backward is differentiable once; double backward "
@@ -57,7 +74,7 @@ def _once_differentiable() -> None:
 def _stream(t: Tensor) -> int:
     """The current stream of the tensor's device: the handle alone, without the object around it
     (2 us less a call)."""
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _wanted(*tensors: Optional[Tensor]) -> bool:
@@ -79,7 +96,7 @@ def _workspace(name: str, device: torch.device, *sizes: int) -> Tuple[Tensor, in
 # --------------------------------------------------------------------------- embedding
 def _embedding(ids: Tensor, table: Tensor, scale: float) -> Tensor:
     out = table.new_empty((*ids.shape, table.shape[1]))
-    _lib.call("xnn_embedding", _lib.storage_code(table.dtype), ids.data_ptr(), ids.numel(),
+    _call("xnn_embedding", _lib.storage_code(table.dtype), ids.data_ptr(), ids.numel(),
               table.data_ptr(), table.shape[0], table.shape[1], scale, out.data_ptr(),
               _stream(table))
     return out
@@ -104,7 +121,7 @@ def _embedding_grad(ids: Tensor, grad: Tensor, rows: int, scale: float) -> Tenso
     channels = grad.shape[-1]
     out = grad.new_empty((rows, channels))
     work, size = _workspace("xnn_embedding_grad_work_size", grad.device, ids.numel(), rows, channels)
-    _lib.call("xnn_embedding_grad", _lib.storage_code(grad.dtype), ids.data_ptr(), ids.numel(),
+    _call("xnn_embedding_grad", _lib.storage_code(grad.dtype), ids.data_ptr(), ids.numel(),
               grad.data_ptr(), rows, channels, scale, out.data_ptr(), work.data_ptr(), size,
               _stream(grad))
     return out
@@ -131,7 +148,9 @@ def embedding(ids: Tensor, table: Tensor, scale: float = 1.0) -> Tensor:
     ``ids`` of any integer type; one outside the table gives a row of NaN and counts in no
     gradient. The gradient of the table sorts the ids and sums each row's tokens in their order
     (float32, rounded once), the same bits at every call."""
-    _on_gpu(table=table, ids=ids)
+    device = table.get_device()
+    if device < 0 or ids.get_device() != device:
+        _on_gpu(table=table, ids=ids)
     if table.dim() != 2:
         raise ValueError(f"table must be (rows, channels), got {tuple(table.shape)}")
     if ids.dtype.is_floating_point or ids.dtype == torch.bool or ids.dtype.is_complex:
@@ -147,7 +166,7 @@ def embedding(ids: Tensor, table: Tensor, scale: float = 1.0) -> Tensor:
 # --------------------------------------------------------------------------- dropout
 def _dropout(x, residual, drop, seed, offset, counter):
     out = torch.empty_like(x)
-    _lib.call("xnn_dropout_add", _lib.storage_code(x.dtype), x.data_ptr(),
+    _call("xnn_dropout_add", _lib.storage_code(x.dtype), x.data_ptr(),
               None if residual is None else residual.data_ptr(), x.numel(), drop, seed, offset,
               None if counter is None else counter.data_ptr(), out.data_ptr(),
               _stream(x))
@@ -181,7 +200,9 @@ def dropout_add(x: Tensor, residual: Optional[Tensor], p: float, seed: int,
     again. ``seed`` is an integer, ``offset`` an integer or, for a captured graph that advances
     it between replays, an int64 tensor of one element on the device (the backward pass reads it
     again: change it after that)."""
-    _on_gpu(x=x, residual=residual)
+    device = x.get_device()
+    if device < 0 or (residual is not None and residual.get_device() != device):
+        _on_gpu(x=x, residual=residual)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"p must be in [0, 1], got {p}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
@@ -221,7 +242,7 @@ def _norm_args(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
 
 def _norm_rotate(q, k, args):
     q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
-    _lib.call("xnn_head_norm_rotate", *args, q_out.data_ptr(), k_out.data_ptr(), _stream(q))
+    _call("xnn_head_norm_rotate", *args, q_out.data_ptr(), k_out.data_ptr(), _stream(q))
     return q_out, k_out
 
 
@@ -249,7 +270,7 @@ class _NormRotate(torch.autograd.Function):
         if tables:
             d_cos, d_sin = torch.empty_like(cos), torch.empty_like(sin)
         grad_q, grad_k = grad_q.contiguous(), grad_k.contiguous()
-        _lib.call("xnn_head_norm_rotate_backward", *_norm_args(*saved, *ctx.args),
+        _call("xnn_head_norm_rotate_backward", *_norm_args(*saved, *ctx.args),
                   grad_q.data_ptr(), grad_k.data_ptr(), d_q.data_ptr(), d_k.data_ptr(),
                   *(_lib.ptr(t) for t in (d_qw, d_kw, d_cos, d_sin, work)), size,
                   _stream(q))
@@ -268,7 +289,11 @@ def head_norm_rotate(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, c
     Token ``t`` takes row ``positions[t]`` of the tables (one outside gives NaN), or row ``t`` when
     ``positions`` is None; only then do the tables have gradients (phases that depend on the
     geometry lead to forces). Tokens and heads may be strided (views of one projection's output)."""
-    _on_gpu(q=q, k=k, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin, positions=positions)
+    device = q.get_device()
+    if device < 0 or not (device == k.get_device() == q_weight.get_device() == k_weight.get_device()
+                          == cos.get_device() == sin.get_device()) \
+            or (positions is not None and positions.get_device() != device):
+        _on_gpu(q=q, k=k, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin, positions=positions)
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError("q and k must be (tokens, heads, head_dim) of the same tokens and head_dim, "
                          f"got {tuple(q.shape)} and {tuple(k.shape)}")
@@ -353,7 +378,7 @@ def attention_plan(n_atoms: Tensor, n_tokens: Optional[int] = None) -> Attention
     longs = torch.empty(4 * B + 8, dtype=torch.int64, device=device)
     ptr, tile_ptr, order, info = longs.split([B + 1, 2 * (B + 1), B, 5])
     lists = ints.split([3 * c for c in caps])
-    _lib.call("xnn_attention_plan", n_atoms.data_ptr(), B, n_tokens, ptr.data_ptr(),
+    _call("xnn_attention_plan", n_atoms.data_ptr(), B, n_tokens, ptr.data_ptr(),
               tile_ptr.data_ptr(), order.data_ptr(), lists[0].data_ptr(), caps[0], lists[1].data_ptr(), caps[1],
               info.data_ptr(), _stream(n_atoms))
     n32, n128, longest, status, total = info.tolist()
@@ -376,7 +401,7 @@ def _attention(q, plan, args, want_lse):
     size = plan.work_bytes("xnn_attention_work_size", q.shape[1], q.shape[2])
     work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device) if want_lse else None
-    _lib.call("xnn_attention", *args, out.data_ptr(), _lib.ptr(lse),
+    _call("xnn_attention", *args, out.data_ptr(), _lib.ptr(lse),
               _lib.ptr(work), size, _stream(q))
     return out, lse
 
@@ -397,7 +422,7 @@ class _Attention(torch.autograd.Function):
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         size = ctx.plan.work_bytes("xnn_attention_backward_work_size", q.shape[1], k.shape[1], q.shape[2])
         work = torch.empty(size, dtype=torch.uint8, device=q.device)
-        _lib.call("xnn_attention_backward", *_attention_args(q, k, v, ctx.plan, mask, ctx.scale),
+        _call("xnn_attention_backward", *_attention_args(q, k, v, ctx.plan, mask, ctx.scale),
                   out.data_ptr(), lse.data_ptr(), grad.data_ptr(), dq.data_ptr(), dk.data_ptr(),
                   dv.data_ptr(), work.data_ptr(), size, _stream(q))
         need = ctx.needs_input_grad
@@ -415,7 +440,10 @@ def structure_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan,
     key and value gradients; atoms with nothing to attend to get zeros. ``scale``: ``D ** -0.5``
     by default, positive. Returns (T, H, D). Neither scores nor probabilities are stored; the backward
     pass forms them again from the rows' log-sums."""
-    _on_gpu(q=q, k=k, v=v, mask=mask)
+    device = q.get_device()
+    if device < 0 or not device == k.get_device() == v.get_device() == plan.ptr.get_device() \
+            or (mask is not None and mask.get_device() != device):
+        _on_gpu(q=q, k=k, v=v, mask=mask, plan=plan.ptr)
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] \
             or q.shape[2] != k.shape[2]:
         raise ValueError("q must be (tokens, heads, head_dim), k and v (tokens, kv_heads, head_dim), "
@@ -429,8 +457,6 @@ def structure_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan,
         raise TypeError(f"q, k and v must have one dtype, got {q.dtype}, {k.dtype} and {v.dtype}")
     if plan.n_tokens != T:
         raise ValueError(f"the plan is of {plan.n_tokens} tokens, q holds {T}")
-    if plan.ptr.device != q.device:
-        raise ValueError(f"the plan is on {plan.ptr.device}, q on {q.device}")
     if mask is not None:
         if mask.shape != (T,) or mask.dtype != torch.bool:
             raise ValueError(f"mask must be ({T},) bool, got {tuple(mask.shape)} {mask.dtype}")

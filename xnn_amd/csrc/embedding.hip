@@ -4,11 +4,15 @@
 //   out[t]    = scale table[ids[t]]                       (xnn_embedding)
 //   grad[v]   = scale sum_{t: ids[t] = v} g[t]            (xnn_embedding_grad)
 //
-// Both are streams: the rows are moved 16 bytes a lane. The gradient sorts the (id, t) pairs by a
-// stable least-significant-digit radix sort (8 bits a pass, as many passes as the number of rows
-// has bits), sums chunks of kChunk sorted positions a group of lanes each, in the order of t, and
-// joins the runs that cross chunks afterwards in a fixed order: no atomics on floats, the
-// same bits at every call. Sums are held in float32 and rounded once.
+// Both are streams: the rows are moved 16 bytes a lane. The gradient sorts the (id, t) pairs and sums
+// the runs of one id in the order of t, so that no sum is an atomic one and every call gives the same
+// bits; sums are held in float32 and rounded once. Three ways by size:
+//
+//   small tables (at most 255 rows, species): each block sorts its own tokens by counting, sums their
+//     runs and leaves a row for each id it has seen; a block a row of the table adds those in order
+//   up to 16,384 tokens: one block sorts all of them in LDS (8 bits a pass) while the others clear
+//     the table; then runs of the sorted order are summed in chunks, and those that cross chunks joined
+//   beyond: the same with a sort of three launches a pass
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -20,38 +24,55 @@
 
 namespace xnn {
 
-constexpr int kBins = 256;        // digits of a sort pass
-constexpr int kSortTile = 1024;   // ids a block of a sort pass takes, at least
-constexpr int kSortBlocks = 512;  // blocks of a sort pass, at most
-constexpr int kChunk = 32;        // sorted positions a group of lanes sums
+constexpr int kBins = 256;         // digits of a sort pass, ids of a small table
+constexpr int kSortTile = 1024;    // ids a block of a sort pass takes, at least
+constexpr int kSortBlocks = 512;   // blocks of a sort pass, at most
+constexpr int kSortInLds = 16384;  // ids one block sorts in LDS, at most
+constexpr int kChunk = 32;         // sorted positions a group of lanes sums
+constexpr int kOwnTokens = 4096;   // tokens a block sorts for a small table, at most
 
 static int64_t round64(int64_t b) { return (b + 63) / 64 * 64; }
 
 struct EmbeddingWork {
+  bool small, in_lds;
   int passes;
   int64_t blocks, per, chunks;                             // of the sort, of the sums
-  int64_t key[2], perm[2], hist, part, bytes;              // offsets
+  int64_t key[2], perm[2], hist, part, seen, bytes;        // offsets
 };
 
 static EmbeddingWork embedding_work(int64_t n, int64_t n_rows, int64_t C) {
-  EmbeddingWork w;
+  EmbeddingWork w = {};
+  w.small = n_rows < kBins;
+  int64_t o = 0;
+  if (w.small) {
+    // as many blocks as fill the chip, with tokens enough that a block's rows are few beside them
+    w.per = 256;
+    while (w.per < kOwnTokens && n > w.per * 512) w.per *= 2;
+    w.chunks = (n + w.per - 1) / w.per;
+    w.seen = o;
+    o += round64(w.chunks * (kBins / 8));
+    w.part = o;
+    o += 4 * w.chunks * n_rows * C;
+    w.bytes = o;
+    return w;
+  }
   int bits = 1;
   while (bits < 31 && (n_rows >> bits) != 0) ++bits;       // n_rows itself is the invalid id
   w.passes = (bits + 7) / 8;
+  w.in_lds = n <= kSortInLds;
   w.per = std::max<int64_t>(kSortTile,
                             (n + (int64_t)kSortBlocks * kSortTile - 1) / ((int64_t)kSortBlocks * kSortTile) *
                                 kSortTile);
   w.blocks = (n + w.per - 1) / w.per;
   w.chunks = (n + kChunk - 1) / kChunk;
-  int64_t o = 0;
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < (w.in_lds ? 1 : 2); ++i) {
     w.key[i] = o;
     o += round64(4 * n);
     w.perm[i] = o;
     o += round64(4 * n);
   }
   w.hist = o;
-  o += round64(4 * kBins * w.blocks);
+  if (!w.in_lds) o += round64(4 * kBins * w.blocks);
   w.part = o;
   o += 8 * w.chunks * C;
   w.bytes = o;
@@ -176,14 +197,285 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(
   }
 }
 
-// ---------------------------------------------------------------- sums
-template <typename T>
-__global__ __launch_bounds__(256) void fill_zero_kernel(T* __restrict__ out, int64_t n) {
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
-       i += (int64_t)gridDim.x * blockDim.x)
-    out[i] = (T)0.0f;
+// Stable ranks of a block's keys by one digit: wave w holds rounds * 64 consecutive keys, lane l the
+// l-th of each round. count[w][d] (zero before) becomes the wave's keys of digit d; rank[r] the key's
+// place among them.
+template <int ROUNDS>
+__device__ __forceinline__ void wave_ranks(const uint32_t (&digit)[ROUNDS], int rounds, int live_rounds_end,
+                                           uint32_t* count, uint32_t (&rank)[ROUNDS]) {
+  const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    if (r < rounds) {
+      const bool live = r * kWave + lane < live_rounds_end;
+      const uint32_t d = digit[r];
+      uint64_t same = __ballot(live);                      // the lanes with the same digit
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        const uint64_t set = __ballot((d >> b) & 1);
+        same &= ((d >> b) & 1) ? set : ~set;
+      }
+      const uint32_t below = __popcll(same & ((1ull << lane) - 1));
+      const uint32_t before = live ? count[d] : 0;
+      rank[r] = before + below;
+      wave_sync();
+      if (live && below == 0) count[d] = before + __popcll(same);
+      wave_sync();
+    }
+  }
 }
 
+// 16 bytes of zeros a thread and turn
+__device__ __forceinline__ void clear16(char* p, int64_t bytes, int64_t thread, int64_t threads) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const int64_t whole = (uintptr_t)p % 16 == 0 ? bytes / 16 : 0;
+  for (int64_t i = thread; i < whole; i += threads) reinterpret_cast<u32x4*>(p)[i] = u32x4{0, 0, 0, 0};
+  for (int64_t i = whole * 16 + thread; i < bytes; i += threads) p[i] = 0;
+}
+
+__global__ __launch_bounds__(256) void clear_kernel(char* __restrict__ p, int64_t bytes) {
+  clear16(p, bytes, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+}
+
+// Block 0 sorts all (at most 16,384) ids in LDS, sixteen waves of up to sixteen rounds; the others
+// clear the gradient.
+__global__ __launch_bounds__(1024) void sort_all_kernel(const int64_t* __restrict__ ids, int n,
+                                                        int64_t n_rows, int passes,
+                                                        uint32_t* __restrict__ key_out,
+                                                        uint32_t* __restrict__ perm_out,
+                                                        char* __restrict__ grad, int64_t bytes) {
+  if (blockIdx.x > 0) {
+    clear16(grad, bytes, ((int64_t)blockIdx.x - 1) * 1024 + threadIdx.x, ((int64_t)gridDim.x - 1) * 1024);
+    return;
+  }
+  __shared__ uint32_t keys[kSortInLds];
+  __shared__ uint16_t perms[kSortInLds];
+  __shared__ uint32_t count[16][kBins];
+  __shared__ uint32_t sums[4];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = wave_in_block();
+  const int rounds = (n + 1023) / 1024;
+  const int first = wave * rounds * kWave, mine = min(max(n - first, 0), rounds * kWave);
+  uint32_t key[16], perm[16], digit[16], rank[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int i = r * kWave + lane;
+    key[r] = perm[r] = 0;
+    if (r < rounds && i < mine) {
+      key[r] = sort_key(ids, nullptr, first + i, n_rows);
+      perm[r] = first + i;
+    }
+  }
+  for (int p = 0; p < passes; ++p) {
+    for (int i = tid; i < 16 * kBins; i += 1024) (&count[0][0])[i] = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) digit[r] = (key[r] >> (8 * p)) & (kBins - 1);
+    __syncthreads();
+    wave_ranks(digit, rounds, mine, count[wave], rank);
+    __syncthreads();
+    // keys of smaller digits, then those of the same digit in earlier waves
+    uint32_t total = 0, x = 0;
+    if (tid < kBins) {
+#pragma unroll
+      for (int w = 0; w < 16; ++w) total += count[w][tid];
+      x = total;
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) {
+        const uint32_t y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+      }
+      if (lane == kWave - 1) sums[wave] = x;
+    }
+    __syncthreads();
+    if (tid < kBins) {
+      uint32_t at = x - total;
+      for (int w = 0; w < wave; ++w) at += sums[w];
+#pragma unroll
+      for (int w = 0; w < 16; ++w) {
+        const uint32_t c = count[w][tid];
+        count[w][tid] = at;
+        at += c;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (r < rounds && r * kWave + lane < mine) {
+        const uint32_t to = count[wave][digit[r]] + rank[r];
+        keys[to] = key[r];
+        perms[to] = (uint16_t)perm[r];
+      }
+    __syncthreads();
+    if (p + 1 < passes) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (r < rounds && r * kWave + lane < mine) {
+          key[r] = keys[first + r * kWave + lane];
+          perm[r] = perms[first + r * kWave + lane];
+        }
+      __syncthreads();
+    }
+  }
+  for (int i = tid; i < n; i += 1024) {
+    key_out[i] = keys[i];
+    perm_out[i] = perms[i];
+  }
+}
+
+// ---------------------------------------------------------------- small tables
+// A block's `per` tokens sorted by id (counting, at most sixteen rounds of its four waves), then their
+// runs summed by groups of `lanes` lanes over consecutive sorted positions, N channels a lane. A run
+// within one group's positions goes to part[block][id]; of a run that crosses groups each leaves its
+// sum in LDS and the group where it begins adds them in order.
+template <typename T, int N>
+__global__ __launch_bounds__(256) void own_sum_kernel(const int64_t* __restrict__ ids, int64_t n,
+                                                      int n_rows, int64_t C, int64_t per, int lanes,
+                                                      const T* __restrict__ g,
+                                                      uint32_t* __restrict__ seen,
+                                                      float* __restrict__ part) {
+  __shared__ uint32_t count[4][kBins];
+  __shared__ uint32_t sums[4];
+  __shared__ uint16_t order[kOwnTokens];
+  __shared__ uint8_t sorted[kOwnTokens];
+  __shared__ float head[256 * N], tail[256 * N];           // of each group: its first run, its last
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = wave_in_block();
+  const int64_t begin = (int64_t)blockIdx.x * per;
+  const int m = (int)min(per, n - begin), rounds = (int)(per / 256);
+  const int first = wave * rounds * kWave, mine = min(max(m - first, 0), rounds * kWave);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) count[w][tid] = 0;
+  uint32_t digit[16], rank[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    digit[r] = 0;
+    const int i = r * kWave + lane;
+    if (r < rounds && i < mine) digit[r] = sort_key(ids, nullptr, begin + first + i, n_rows);
+  }
+  __syncthreads();
+  wave_ranks(digit, rounds, mine, count[wave], rank);
+  __syncthreads();
+  uint32_t total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) total += count[w][tid];
+  uint32_t x = total;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const uint32_t y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == kWave - 1) sums[wave] = x;
+  const uint64_t present = __ballot(total > 0 && tid < n_rows);
+  if (lane < 2 && blockIdx.y == 0)
+    seen[(int64_t)blockIdx.x * (kBins / 32) + 2 * wave + lane] = (uint32_t)(present >> (32 * lane));
+  __syncthreads();
+  uint32_t at = x - total;
+  for (int w = 0; w < wave; ++w) at += sums[w];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const uint32_t c = count[w][tid];
+    count[w][tid] = at;
+    at += c;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    if (r < rounds && r * kWave + lane < mine) {
+      const uint32_t to = count[wave][digit[r]] + rank[r];
+      order[to] = (uint16_t)(first + r * kWave + lane);
+      sorted[to] = (uint8_t)digit[r];
+    }
+  __syncthreads();
+
+  const int groups = 256 / lanes, group = tid / lanes;
+  const int64_t c = ((int64_t)blockIdx.y * lanes + tid % lanes) * N;
+  const int each = (m + groups - 1) / groups;
+  const int p0 = min(m, group * each), p1 = min(m, p0 + each);
+  float* row = part + (int64_t)blockIdx.x * n_rows * C + c;
+  bool crosses = false;                                    // the last run goes on in the next group
+  if (c < C && p0 < p1) {
+    const bool from_before = p0 > 0 && sorted[p0 - 1] == sorted[p0];
+    crosses = p1 < m && sorted[p1] == sorted[p1 - 1];
+    float sum[N] = {};
+    int began = p0;
+    constexpr int kAhead = 8;                              // rows in flight
+    for (int p = p0; p < p1; p += kAhead) {
+      float v[kAhead][N];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        load_pack<T, N>(g + (begin + order[min(p + j, p1 - 1)]) * C + c, v[j]);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int i = p + j;
+        if (i < p1) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) sum[e] += v[j][e];
+          const int k = sorted[i];
+          if (i + 1 == p1 || sorted[i + 1] != k) {
+            if (began == p0 && from_before)
+              store_pack<float, N>(head + tid * N, sum);
+            else if (i + 1 == p1 && crosses)
+              store_pack<float, N>(tail + tid * N, sum);
+            else if (k < n_rows)
+              store_pack<float, N>(row + (int64_t)k * C, sum);
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum[e] = 0.0f;
+            began = i + 1;
+          }
+        }
+      }
+    }
+    // a run that covers the group from end to end began before and belongs to an earlier group
+    crosses = crosses && !(from_before && sorted[p0] == sorted[p1 - 1]);
+  }
+  __syncthreads();
+  if (crosses && sorted[p1 - 1] < n_rows) {
+    const int k = sorted[p1 - 1];
+    float sum[N];
+    load_pack<float, N>(tail + tid * N, sum);
+    for (int q = group + 1; q < groups && q * each < m && sorted[q * each] == k; ++q) {
+      float v[N];
+      load_pack<float, N>(head + (tid + (q - group) * lanes) * N, v);
+#pragma unroll
+      for (int e = 0; e < N; ++e) sum[e] += v[e];
+    }
+    store_pack<float, N>(row + (int64_t)k * C, sum);
+  }
+}
+
+// A block a row and 64 channels: the sums of the blocks that have seen it, sixteen waves in turn, and
+// theirs in order; zero where none has.
+template <typename T>
+__global__ __launch_bounds__(1024) void own_join_kernel(const uint32_t* __restrict__ seen,
+                                                        const float* __restrict__ part, int64_t chunks,
+                                                        int n_rows, int64_t C, float scale,
+                                                        T* __restrict__ out) {
+  __shared__ float s[16][kWave];
+  const int lane = threadIdx.x & (kWave - 1), wave = wave_in_block(), k = blockIdx.x;
+  const int64_t c = (int64_t)blockIdx.y * kWave + lane;
+  float sum = 0.0f;
+  constexpr int kAhead = 8;
+  for (int64_t q0 = wave; q0 < chunks; q0 += 16 * kAhead) {
+    float v[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int64_t q = q0 + 16 * j;
+      v[j] = 0.0f;
+      if (q < chunks && c < C && (seen[q * (kBins / 32) + k / 32] >> (k % 32)) & 1)
+        v[j] = part[(q * n_rows + k) * C + c];
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) sum += v[j];
+  }
+  s[wave][lane] = sum;
+  __syncthreads();
+  if (wave == 0 && c < C) {
+    float r = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) r += s[w][lane];
+    out[k * C + c] = (T)(r * scale);
+  }
+}
+
+// ---------------------------------------------------------------- sums
 // A group of `lanes` lanes sums chunk positions of the sorted order, N channels a lane. A run that
 // lies within the chunk goes to its row; one that goes on in the next chunk leaves its sum in
 // part[chunk][1], one that came from the chunk before in part[chunk][0].
@@ -198,43 +490,53 @@ __global__ __launch_bounds__(256) void run_sum_kernel(
   if (begin >= n || c >= C) return;
   const bool from_before = begin > 0 && key[begin - 1] == key[begin];
   const bool goes_on = end < n && key[end] == key[end - 1];
-  float sum[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) sum[j] = 0.0f;
+  float sum[N] = {};
   int64_t first = begin;
-  for (int64_t i = begin; i < end; ++i) {
-    const uint32_t k = key[i];
-    float v[N];
-    load_pack<T, N>(g + (int64_t)perm[i] * C + c, v);
+  constexpr int kAhead = 4;                                // rows in flight
+  for (int64_t i0 = begin; i0 < end; i0 += kAhead) {
+    float v[kAhead][N];
+    uint32_t k[kAhead + 1];
 #pragma unroll
-    for (int j = 0; j < N; ++j) sum[j] += v[j];
-    const bool last = i + 1 == end;
-    if (!last && key[i + 1] == k) continue;
-    if (k < n_rows) {
-      if (first == begin && from_before) {
-        store_pack<float, N>(part + 2 * chunk * C + c, sum);
-      } else if (last && goes_on) {
-        store_pack<float, N>(part + (2 * chunk + 1) * C + c, sum);
-      } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) sum[j] *= scale;
-        store_pack<T, N>(out + (int64_t)k * C + c, sum);
-      }
+    for (int j = 0; j < kAhead; ++j) {
+      const int64_t i = min(i0 + j, end - 1);
+      k[j] = key[i];
+      load_pack<T, N>(g + (int64_t)perm[i] * C + c, v[j]);
     }
+    k[kAhead] = i0 + kAhead < end ? key[i0 + kAhead] : 0;
 #pragma unroll
-    for (int j = 0; j < N; ++j) sum[j] = 0.0f;
-    first = i + 1;
+    for (int j = 0; j < kAhead; ++j) {
+      const int64_t i = i0 + j;
+      if (i >= end) break;
+#pragma unroll
+      for (int e = 0; e < N; ++e) sum[e] += v[j][e];
+      const bool last = i + 1 == end;
+      if (!last && k[j + 1] == k[j]) continue;
+      if (k[j] < n_rows) {
+        if (first == begin && from_before) {
+          store_pack<float, N>(part + 2 * chunk * C + c, sum);
+        } else if (last && goes_on) {
+          store_pack<float, N>(part + (2 * chunk + 1) * C + c, sum);
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) sum[e] *= scale;
+          store_pack<T, N>(out + (int64_t)k[j] * C + c, sum);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) sum[e] = 0.0f;
+      first = i + 1;
+    }
   }
 }
 
 // The rows whose runs cross chunks: the block of the chunk where a run begins adds what the
-// following chunks left, sixteen waves in turn, and their sums in order.
-template <typename T>
-__global__ __launch_bounds__(1024) void run_join_kernel(const uint32_t* __restrict__ key, int64_t n,
-                                                        int64_t n_rows, int64_t C, float scale,
-                                                        const float* __restrict__ part,
-                                                        T* __restrict__ out) {
-  __shared__ float s[16][kWave];
+// following chunks left, its four waves in turn, and their sums in order. N channels a lane.
+template <typename T, int N>
+__global__ __launch_bounds__(256) void run_join_kernel(const uint32_t* __restrict__ key, int64_t n,
+                                                       int64_t n_rows, int64_t C, float scale,
+                                                       const float* __restrict__ part,
+                                                       T* __restrict__ out) {
+  __shared__ float s[4][kWave * N];
   const int64_t chunk = blockIdx.x, begin = chunk * kChunk, end = min(n, begin + kChunk);
   if (end >= n) return;
   const uint32_t k = key[end - 1];
@@ -251,20 +553,25 @@ __global__ __launch_bounds__(1024) void run_join_kernel(const uint32_t* __restri
   }
   const int64_t last = (lo - 1) / kChunk;                  // the chunk of its last position
   const int lane = threadIdx.x & (kWave - 1), wave = wave_in_block();
-  const int64_t c = (int64_t)blockIdx.y * kWave + lane;
-  float sum = 0.0f;
+  const int64_t c = ((int64_t)blockIdx.y * kWave + lane) * N;
+  float sum[N] = {};
   if (c < C) {
-    if (wave == 0) sum = part[(2 * chunk + 1) * C + c];
+    if (wave == 0) load_pack<float, N>(part + (2 * chunk + 1) * C + c, sum);
 #pragma unroll 4
-    for (int64_t q = chunk + 1 + wave; q <= last; q += 16) sum += part[2 * q * C + c];
+    for (int64_t q = chunk + 1 + wave; q <= last; q += 4) {
+      float v[N];
+      load_pack<float, N>(part + 2 * q * C + c, v);
+#pragma unroll
+      for (int e = 0; e < N; ++e) sum[e] += v[e];
+    }
   }
-  s[wave][lane] = sum;
+  store_pack<float, N>(&s[wave][lane * N], sum);
   __syncthreads();
   if (wave == 0 && c < C) {
-    float r = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) r += s[w][lane];
-    out[(int64_t)k * C + c] = (T)(r * scale);
+    for (int e = 0; e < N; ++e)
+      sum[e] = (((s[0][lane * N + e] + s[1][lane * N + e]) + s[2][lane * N + e]) + s[3][lane * N + e]) * scale;
+    store_pack<T, N>(out + (int64_t)k * C + c, sum);
   }
 }
 
@@ -285,59 +592,91 @@ static int embedding(const int64_t* ids, int64_t n, const void* table, int64_t n
   return XNN_OK;
 }
 
+// lanes of a group that share a row, N channels each
+static int row_lanes(int64_t C, int N, int most) {
+  int lanes = 1;
+  while (lanes < most && lanes * N < C) lanes *= 2;
+  return lanes;
+}
+
+template <typename T, int N>
+static void own_sums(const int64_t* ids, int64_t n, int64_t n_rows, int64_t C, const EmbeddingWork& w,
+                     const T* g, float scale, uint32_t* seen, float* part, T* out, hipStream_t s) {
+  const int lanes = row_lanes(C, N, 64);
+  hipLaunchKernelGGL((own_sum_kernel<T, N>),
+                     dim3((unsigned)w.chunks, (unsigned)((C + lanes * N - 1) / (lanes * N))), dim3(256),
+                     0, s, ids, n, (int)n_rows, C, w.per, lanes, g, seen, part);
+  hipLaunchKernelGGL(own_join_kernel<T>, dim3((unsigned)n_rows, (unsigned)((C + kWave - 1) / kWave)),
+                     dim3(1024), 0, s, seen, part, w.chunks, (int)n_rows, C, scale, out);
+}
+
 template <typename T, int N>
 static void run_sums(const uint32_t* key, const uint32_t* perm, int64_t n, int64_t n_rows, int64_t C,
                      const EmbeddingWork& w, const T* g, float scale, float* part, T* out,
                      hipStream_t s) {
-  int lanes = 1;
-  while (lanes < 256 && lanes * N < C) lanes *= 2;
+  const int lanes = row_lanes(C, N, 256);
   const int64_t groups = 256 / lanes;
   const dim3 grid((unsigned)((w.chunks + groups - 1) / groups),
                   (unsigned)((C + lanes * N - 1) / (lanes * N)));
   hipLaunchKernelGGL((run_sum_kernel<T, N>), grid, dim3(256), 0, s, key, perm, n, n_rows, C, lanes,
                      g, scale, part, out);
+  constexpr int kJoin = N == 1 ? 1 : 4;
+  hipLaunchKernelGGL((run_join_kernel<T, kJoin>),
+                     dim3((unsigned)w.chunks, (unsigned)((C + kWave * kJoin - 1) / (kWave * kJoin))),
+                     dim3(256), 0, s, key, n, n_rows, C, scale, part, out);
 }
 
 template <typename T>
 static int embedding_grad(const int64_t* ids, int64_t n, const void* g, int64_t n_rows, int64_t C,
                           float scale, void* out, char* work, hipStream_t s) {
   constexpr int kN = 16 / sizeof(T);
+  const T* gt = static_cast<const T*>(g);
   T* o = static_cast<T*>(out);
-  const int64_t cells = n_rows * C;
-  const bool words = (uintptr_t)out % 16 == 0 && cells % kN == 0;
-  const int64_t fill = words ? cells / kN * 4 : cells;
-  const dim3 fill_grid((unsigned)std::min<int64_t>((fill + 255) / 256, 8192));
-  if (words)
-    hipLaunchKernelGGL(fill_zero_kernel<float>, fill_grid, dim3(256), 0, s, (float*)out, fill);
-  else
-    hipLaunchKernelGGL(fill_zero_kernel<T>, fill_grid, dim3(256), 0, s, o, fill);
-  if (n > 0) {
-    const EmbeddingWork w = embedding_work(n, n_rows, C);
+  char* grad = static_cast<char*>(out);
+  const bool vec = ((uintptr_t)g | (uintptr_t)out) % 16 == 0 && C % kN == 0;
+  const int64_t bytes = n_rows * C * (int64_t)sizeof(T);
+  const EmbeddingWork w = embedding_work(n, n_rows, C);
+  float* part = (float*)(work + w.part);
+  if (n == 0) {
+    hipLaunchKernelGGL(clear_kernel, dim3((unsigned)std::min<int64_t>(bytes / 4096 + 1, 4096)),
+                       dim3(256), 0, s, grad, bytes);
+  } else if (w.small) {
+    uint32_t* seen = (uint32_t*)(work + w.seen);
+    if (vec)
+      own_sums<T, kN>(ids, n, n_rows, C, w, gt, scale, seen, part, o, s);
+    else
+      own_sums<T, 1>(ids, n, n_rows, C, w, gt, scale, seen, part, o, s);
+  } else {
     uint32_t *key[2], *perm[2], *hist = (uint32_t*)(work + w.hist);
     for (int i = 0; i < 2; ++i) {
       key[i] = (uint32_t*)(work + w.key[i]);
       perm[i] = (uint32_t*)(work + w.perm[i]);
     }
-    float* part = (float*)(work + w.part);
-    const dim3 grid((unsigned)w.blocks);
-    int from = 1;
-    for (int p = 0; p < w.passes; ++p) {
-      const uint32_t* k = p == 0 ? nullptr : key[from];
-      const uint32_t* q = p == 0 ? nullptr : perm[from];
-      hipLaunchKernelGGL(sort_count_kernel, grid, dim3(256), 0, s, ids, k, n, n_rows, w.per, 8 * p,
-                         hist);
-      hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, s, hist, kBins * w.blocks);
-      hipLaunchKernelGGL(sort_scatter_kernel, grid, dim3(256), 0, s, ids, k, q, n, n_rows, w.per,
-                         8 * p, hist, key[1 - from], perm[1 - from]);
-      from = 1 - from;
+    int from = 0;
+    if (w.in_lds) {
+      const int64_t clear = std::min<int64_t>(bytes / 16384 + 1, 2048);
+      hipLaunchKernelGGL(sort_all_kernel, dim3((unsigned)(1 + clear)), dim3(1024), 0, s, ids, (int)n,
+                         n_rows, w.passes, key[0], perm[0], grad, bytes);
+    } else {
+      hipLaunchKernelGGL(clear_kernel, dim3((unsigned)std::min<int64_t>(bytes / 4096 + 1, 8192)),
+                         dim3(256), 0, s, grad, bytes);
+      const dim3 grid((unsigned)w.blocks);
+      from = 1;
+      for (int p = 0; p < w.passes; ++p) {
+        const uint32_t* k = p == 0 ? nullptr : key[from];
+        const uint32_t* q = p == 0 ? nullptr : perm[from];
+        hipLaunchKernelGGL(sort_count_kernel, grid, dim3(256), 0, s, ids, k, n, n_rows, w.per, 8 * p,
+                           hist);
+        hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, s, hist, kBins * w.blocks);
+        hipLaunchKernelGGL(sort_scatter_kernel, grid, dim3(256), 0, s, ids, k, q, n, n_rows, w.per,
+                           8 * p, hist, key[1 - from], perm[1 - from]);
+        from = 1 - from;
+      }
     }
-    const T* gt = static_cast<const T*>(g);
-    if (((uintptr_t)g | (uintptr_t)out) % 16 == 0 && C % kN == 0)
+    if (vec)
       run_sums<T, kN>(key[from], perm[from], n, n_rows, C, w, gt, scale, part, o, s);
     else
       run_sums<T, 1>(key[from], perm[from], n, n_rows, C, w, gt, scale, part, o, s);
-    hipLaunchKernelGGL(run_join_kernel<T>, dim3((unsigned)w.chunks, (unsigned)((C + 63) / 64)),
-                       dim3(1024), 0, s, key[from], n, n_rows, C, scale, part, o);
   }
   XNN_LAUNCH_CHECK();
   return XNN_OK;
