@@ -274,8 +274,11 @@ struct Stage {
   static constexpr int kStep = THREADS / kChunks;
   static constexpr int kCount = (S::kTile + kStep - 1) / kStep;
   static_assert(THREADS % kChunks == 0, "a thread keeps its place in the rows");
-  Pack<T, kPer> x[kCount];
+  typedef Pack<T, kPer> Piece;
+  Piece x[kCount];
   bool keep[kCount];
+  bool whole;                                              // the tile on its way has no zeros to write
+  bool near;                                               // a tile spans less than 2 GB
   int row, at;                                             // its first row, its element of a row
   int64_t offset;
 
@@ -283,10 +286,20 @@ struct Stage {
     row = threadIdx.x / kChunks;
     at = threadIdx.x % kChunks * kPer;
     offset = row * stride + (at < D ? at : 0);
+    near = VEC && D == S::kWide && stride >= 0 && stride < (int64_t)1 << 22;
   }
   // `tile`: the first of `rows` rows, `mask` its byte
   __device__ __forceinline__ void fetch(const T* tile, int64_t stride, int64_t rows, int D,
                                         const uint8_t* mask) {
+    whole = near && rows >= S::kTile && mask == nullptr;
+    if (whole) {                                           // one address a thread, the rest scalar
+      const uint32_t bytes = (uint32_t)offset * (uint32_t)sizeof(T);
+#pragma unroll
+      for (int n = 0; n < kCount; ++n)
+        x[n] = *reinterpret_cast<const Pack<T, kPer>*>(
+            reinterpret_cast<const char*>(tile + n * kStep * stride) + bytes);
+      return;
+    }
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {
       const int r = row + n * kStep;
@@ -301,15 +314,22 @@ struct Stage {
       }
     }
   }
-  __device__ __forceinline__ void commit(char* tile) const {
+  __device__ __forceinline__ void commit(char* tile) {
+    if (VEC && !whole) {
+#pragma unroll
+      for (int n = 0; n < kCount; ++n) {
+        u32x4 w = __builtin_bit_cast(u32x4, x[n]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = keep[n] ? w[j] : 0u;
+        x[n] = __builtin_bit_cast(Piece, w);
+      }
+    }
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {
       const int r = row + n * kStep;
       if (S::kTile % kStep != 0 && r >= S::kTile) break;
       char* p = tile + r * S::kRow + at * 2;
-      u32x4 w = __builtin_bit_cast(u32x4, x[n]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = keep[n] ? w[j] : 0u;
+      const u32x4 w = __builtin_bit_cast(u32x4, x[n]);
       if constexpr (sizeof(T) == 4) {
         uint32_t a[3], b[3];
         planes_of(__uint_as_float(w[0]), __uint_as_float(w[1]), a);
@@ -408,16 +428,16 @@ constexpr int kCus = 256;
 constexpr int kMostSplits = 16;
 constexpr int kSplitRows = 512;    // walked rows of a part, at least
 
-// Parts of the walked side, for `blocks` blocks without: as few as give every CU two blocks and
-// leave none idle for more than a tenth of the time (blocks of equal length over the chip's 256 CUs).
-// 9,000 rows of 4 heads (284 blocks): 5 parts.
-inline int attention_splits(int64_t blocks, int64_t walked) {
+// Parts of the walked side, for `blocks` blocks of equal length without: as few as give every one of the
+// chip's 256 CUs `each` blocks and leave none idle for more than a tenth of the time.
+inline int attention_splits(int64_t blocks, int64_t walked, int each) {
   const int64_t most = std::min<int64_t>(kMostSplits, walked / kSplitRows);
   int best = 1;
   double best_use = 0.0;
   for (int s = 1; s <= std::max<int64_t>(most, 1); ++s) {
     const int64_t n = blocks * s;
-    const double use = (double)n / ((n + kCus - 1) / kCus * kCus) * (n < 2 * kCus ? 0.6 : 1.0);
+    const double use = (double)n / ((n + kCus - 1) / kCus * kCus) *
+                       (n < each * kCus ? 0.6 + 0.2 * n / (each * kCus) : 1.0);
     if (use > best_use + 0.03) {
       best = s;
       best_use = use;
@@ -426,6 +446,11 @@ inline int attention_splits(int64_t blocks, int64_t walked) {
   }
   return best;
 }
+// Two blocks a CU for the forward pass (24,000 rows of 4 heads, 752 blocks: 752 us undivided, 799 in two
+// parts, with the join); four for the gradients, two of which a CU holds at a time (2,430 us undivided,
+// 2,278 in two parts). 9,000 rows of 4 heads, 284 blocks: five parts for all.
+inline int forward_splits(int64_t blocks, int64_t walked) { return attention_splits(blocks, walked, 2); }
+inline int backward_splits(int64_t blocks, int64_t walked) { return attention_splits(blocks, walked, 4); }
 
 // Rows of a block: 32, one wave, where no structure is longer than 64 (the other waves of a larger
 // block would idle) and one wave's registers hold a tile on its way, otherwise 128.

@@ -337,7 +337,7 @@ int xnn_attention_work_size(int64_t n_tokens, int32_t n_heads, int32_t head_dim,
                             const xnn_attention_tiles* plan, size_t* bytes) {
   XNN_REQUIRE(plan && bytes, "NULL plan or size");
   XNN_REQUIRE(n_tokens >= 0 && n_heads >= 1 && head_dim >= 1, "sizes out of range");
-  const int splits = attention_splits(attention_blocks(plan, n_heads), plan->max_atoms);
+  const int splits = forward_splits(attention_blocks(plan, n_heads), plan->max_atoms);
   *bytes = forward_bytes(n_tokens, n_heads, head_dim, splits);
   return XNN_OK;
 }
@@ -350,7 +350,7 @@ int xnn_attention(int dtype, const xnn_heads* q, const xnn_heads* k, const xnn_h
   const int status = attention_args(a, dtype, q, k, v, n_tokens, head_dim, plan, mask, scale);
   if (status != XNN_OK || n_tokens == 0) return status;
   XNN_REQUIRE(out != nullptr, "NULL output");
-  a.splits = attention_splits(attention_blocks(plan, a.heads), plan->max_atoms);
+  a.splits = forward_splits(attention_blocks(plan, a.heads), plan->max_atoms);
   if (a.splits > 1) {
     XNN_REQUIRE(work && work_bytes >= forward_bytes(n_tokens, a.heads, head_dim, a.splits),
                 "work too small");

@@ -299,8 +299,8 @@ int xnn_attention_backward_work_size(int64_t n_tokens, int32_t n_heads, int32_t 
   XNN_REQUIRE(n_tokens >= 0 && n_heads >= 1 && n_kv_heads >= 1 && n_heads % n_kv_heads == 0 &&
                   head_dim >= 1,
               "sizes out of range");
-  const int q = attention_splits(attention_blocks(plan, n_heads), plan->max_atoms);
-  const int k = attention_splits(attention_blocks(plan, n_kv_heads),
+  const int q = backward_splits(attention_blocks(plan, n_heads), plan->max_atoms);
+  const int k = backward_splits(attention_blocks(plan, n_kv_heads),
                                  plan->max_atoms * (n_heads / n_kv_heads));
   *bytes = backward_bytes(n_tokens, n_heads, n_kv_heads, head_dim, q, k);
   return XNN_OK;
@@ -315,8 +315,8 @@ int xnn_attention_backward(int dtype, const xnn_heads* q, const xnn_heads* k, co
   const int status = attention_args(a, dtype, q, k, v, n_tokens, head_dim, plan, mask, scale);
   if (status != XNN_OK || n_tokens == 0) return status;
   XNN_REQUIRE(out && lse && grad && dq && dk && dv && work, "NULL input, output or work");
-  const int q_splits = attention_splits(attention_blocks(plan, a.heads), plan->max_atoms);
-  const int k_splits = attention_splits(attention_blocks(plan, a.kv_heads),
+  const int q_splits = backward_splits(attention_blocks(plan, a.heads), plan->max_atoms);
+  const int k_splits = backward_splits(attention_blocks(plan, a.kv_heads),
                                         plan->max_atoms * (a.heads / a.kv_heads));
   XNN_REQUIRE(work_bytes >= backward_bytes(n_tokens, a.heads, a.kv_heads, head_dim, q_splits, k_splits),
               "work too small");
