@@ -123,6 +123,13 @@ struct Head {
   // walked rows of a staged tile: 32 also where three planes of 64 would leave a CU one block
   static constexpr int kTile = kPlanes == 3 && DP == 128 ? 32 : TILE;
   static constexpr int kPlane = kTile * kRow;
+  // Planes of the weights (probabilities, score gradients). One in 16 bits: its rounding is of the size of
+  // the output's own, 1.4 times the error of an output that is rounded once (n >= 64; it does not grow
+  // with n). Blocks of one wave take a second plane, the rounding error of the first: in short
+  // structures few terms average it, and the products are not what bounds them (1,024 molecules of 10 to
+  // 60 atoms in bfloat16: the same time).
+  template <int WAVES>
+  static constexpr int kWeights = kPlanes == 3 ? 3 : WAVES == 1 ? 2 : 1;
   // waves of a SIMD: two share its matrix core and vector unit where their registers fit
   static constexpr int kOccupancy = DP <= 32 || (kPlanes == 1 && DP == 64) ? 2 : 1;
   static constexpr int kBytes = kPlanes * kPlane;

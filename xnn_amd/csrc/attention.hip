@@ -228,7 +228,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
     for (int b = 0; b < kParts; ++b)
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        const Operand<T> w = weight_operand<T, Store<T>::kPlanes>(p[b], f);
+        const auto w = weight_operand<T, S::template kWeights<WAVES>>(p[b], f);
 #pragma unroll
         for (int d = 0; d < S::kBlocks; ++d)
           mma<T>(transposed_operand<T, S>(v_tile, 32 * b, d, f, lane), w, o[d]);

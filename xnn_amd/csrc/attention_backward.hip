@@ -98,7 +98,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
       }
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        const Operand<T> w = weight_operand<T, Store<T>::kPlanes>(p, f);
+        const auto w = weight_operand<T, S::template kWeights<WAVES>>(p, f);
 #pragma unroll
         for (int d = 0; d < S::kBlocks; ++d)
           mma<T>(transposed_operand<T, S>(k_tile, 32 * b, d, f, lane), w, dq[d]);
@@ -194,8 +194,8 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
       }
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        const Operand<T> w = weight_operand<T, Store<T>::kPlanes>(p, f);
-        const Operand<T> dw = weight_operand<T, Store<T>::kPlanes>(dp, f);
+        const auto w = weight_operand<T, S::template kWeights<WAVES>>(p, f);
+        const auto dw = weight_operand<T, S::template kWeights<WAVES>>(dp, f);
 #pragma unroll
         for (int d = 0; d < S::kBlocks; ++d) {
           mma<T>(transposed_operand<T, S>(g_tile, 32 * b, d, f, lane), w, dv[d]);
