@@ -425,7 +425,20 @@ def storage_code(dtype: torch.dtype) -> int:
         raise TypeError(f"unsupported dtype {dtype} (float32, bfloat16 or float16)") from None
 
 
-calls: dict = {}
+class CallCounts(dict):
+    """Entry point name -> calls from Python; ``native(name)`` are those from native code."""
+
+    native = None
+
+    def get(self, name, default=None):
+        mine = super().get(name)
+        if self.native is None:
+            return default if mine is None else mine
+        theirs = self.native(name)
+        return theirs + mine if mine is not None else theirs or default
+
+
+calls: dict = CallCounts()
 
 
 def count_call(name: str) -> None:

@@ -22,6 +22,8 @@ SOURCES = ("edge.hip", "segment.hip", "basis_message.hip", "graph.hip", "d4.hip"
            "recip.hip", "radial_mlp.hip", "uvu_conv.hip", "pair.hip", "d4_tiles.hip",
            "embedding.hip", "dropout.hip", "head_norm.hip", "attention.hip",
            "attention_backward.hip")
+# the attention operators' autograd functions: host code over libtorch and the C ABI
+NATIVE_OPS = os.path.join(HERE, "_attention_ops.so")
 ARCH = os.environ.get("XNN_AMD_ARCH", "gfx950")
 
 # packed FP32 instructions stay off (the compiler must not form v_pk_* f32 ops)
@@ -39,8 +41,31 @@ def _hipcc() -> str:
     raise RuntimeError("hipcc not found: the xnn_amd HIP library cannot be built")
 
 
+def build_native_ops() -> str:
+    """Compile ``_attention_ops.so`` against the installed libtorch; returns its path."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    tmp = NATIVE_OPS + ".tmp"
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-DTORCH_EXTENSION_NAME=_attention_ops", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE,
+           "-isystem", os.path.join(root, "include"), "-isystem",
+           os.path.join(root, "include", "torch", "csrc", "api", "include"), "-isystem",
+           "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"],
+           os.path.join(CSRC, "attention_ops.cpp"), "-o", tmp, "-L", os.path.join(root, "lib"),
+           "-ltorch", "-ltorch_cpu", "-ltorch_python", "-ltorch_hip", "-lc10", "-lc10_hip"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on attention_ops.cpp:\n{res.stderr[-6000:]}")
+    os.replace(tmp, NATIVE_OPS)
+    return NATIVE_OPS
+
+
 def build(verbose: bool = False, jobs: int = 4) -> str:
-    """Compile every source and link ``libxnn_amd.so``; returns its path."""
+    """Compile every source and link ``libxnn_amd.so`` (returns its path), and beside it the
+    native autograd functions."""
     hipcc = _hipcc()
     objdir = os.path.join(HERE, "_build")
     os.makedirs(objdir, exist_ok=True)
@@ -56,8 +81,10 @@ def build(verbose: bool = False, jobs: int = 4) -> str:
             raise RuntimeError(f"hipcc failed on {name}:\n{res.stderr[-6000:]}")
         return obj
 
-    with ThreadPoolExecutor(max_workers=max(1, jobs)) as pool:
+    with ThreadPoolExecutor(max_workers=max(1, jobs) + 1) as pool:
+        native = pool.submit(build_native_ops)
         objs = list(pool.map(compile_one, sources))
+        native.result()
     tmp = LIBRARY + ".tmp"
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
     res = subprocess.run(cmd, capture_output=True, text=True)
