@@ -123,13 +123,6 @@ struct Head {
   // walked rows of a staged tile: 32 also where three planes of 64 would leave a CU one block
   static constexpr int kTile = kPlanes == 3 && DP == 128 ? 32 : TILE;
   static constexpr int kPlane = kTile * kRow;
-  // Planes of the weights (probabilities, score gradients). One in 16 bits: its rounding is of the size of
-  // the output's own, 1.4 times the error of an output that is rounded once (n >= 64; it does not grow
-  // with n). Blocks of one wave take a second plane, the rounding error of the first: in short
-  // structures few terms average it, and the products are not what bounds them (1,024 molecules of 10 to
-  // 60 atoms in bfloat16: the same time).
-  template <int WAVES>
-  static constexpr int kWeights = kPlanes == 3 ? 3 : WAVES == 1 ? 2 : 1;
   // waves of a SIMD: two share its matrix core and vector unit where their registers fit
   static constexpr int kOccupancy = DP <= 32 || (kPlanes == 1 && DP == 64) ? 2 : 1;
   static constexpr int kBytes = kPlanes * kPlane;
@@ -216,7 +209,9 @@ __device__ __forceinline__ Pack<T, N> load_row(const T* row, int d, int D) {
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) out.v[i] = d + i < D ? row[d + i] : (T)0.0f;
+    for (int i = 0; i < N; ++i) out.v[i] = row[d + i < D ? d + i : 0];
+#pragma unroll
+    for (int i = 0; i < N; ++i) out.v[i] = d + i < D ? out.v[i] : (T)0.0f;
   }
   return out;
 }
@@ -317,12 +312,17 @@ struct Stage {
         x[n] = *reinterpret_cast<const Pack<T, kPer>*>(p);
       } else {
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) x[n].v[j] = keep[n] && at + j < D ? p[j] : (T)0.0f;
+        for (int j = 0; j < kPer; ++j) x[n].v[j] = p[at + j < D ? j : 0];
       }
     }
   }
-  __device__ __forceinline__ void commit(char* tile) {
-    if (VEC && !whole) {
+  __device__ __forceinline__ void commit(char* tile, int D) {
+    if (!VEC) {
+#pragma unroll
+      for (int n = 0; n < kCount; ++n)
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) x[n].v[j] = keep[n] && at + j < D ? x[n].v[j] : (T)0.0f;
+    } else if (!whole) {
 #pragma unroll
       for (int n = 0; n < kCount; ++n) {
         u32x4 w = __builtin_bit_cast(u32x4, x[n]);
@@ -471,6 +471,16 @@ inline int64_t attention_blocks(const xnn_attention_tiles* plan, int heads) {
   return plan->n_tiles128 * heads;                         // short structures have no parts
 }
 
+// Planes of the weights (probabilities, score gradients). float32 has three. In 16 bits one: its rounding
+// is of the size of the output's own, 1.4 times the error of an output that is rounded once, whatever the
+// length. Where few elements average it a second plane, the rounding error of the first, is taken as
+// well: in blocks of one wave, whose products are not what bounds them (1,024 molecules of 10 to 60 atoms: the
+// same time), and where all scores are some microseconds of work.
+constexpr int64_t kFineScores = (int64_t)1 << 23;
+inline bool fine_weights(const AttentionArgs& a, const xnn_attention_tiles* plan) {
+  return a.n_tokens * plan->max_atoms * a.heads <= kFineScores;
+}
+
 // the tiles of a launch; rows that are not moved 16 bytes at a time are always walked by 128
 inline int attention_pick(AttentionArgs& a, const xnn_attention_tiles* plan, int dtype) {
   const int rows = a.vec ? attention_rows(plan, storage_bytes(dtype), a.D) : 128;
@@ -525,3 +535,20 @@ inline int attention_args(AttentionArgs& a, int dtype, const xnn_heads* q, const
 }
 
 }  // namespace xnn
+
+// One launch of kernel<T, DP, waves, tile, vec, weight planes> for arguments `a` of `rows` rows a block on
+// stream `s`
+#define XNN_ATTENTION_LAUNCH(kernel, grid)                                                          \
+  do {                                                                                              \
+    constexpr int kOne = Store<T>::kPlanes, kFine = kOne == 3 ? 3 : 2;                              \
+    if (!a.vec && fine)                                                                             \
+      hipLaunchKernelGGL((kernel<T, DP, 4, 64, false, kFine>), grid, dim3(256), 0, s, a);           \
+    else if (!a.vec)                                                                                \
+      hipLaunchKernelGGL((kernel<T, DP, 4, 64, false, kOne>), grid, dim3(256), 0, s, a);            \
+    else if (rows == 128 && fine)                                                                   \
+      hipLaunchKernelGGL((kernel<T, DP, 4, 64, true, kFine>), grid, dim3(256), 0, s, a);            \
+    else if (rows == 128)                                                                           \
+      hipLaunchKernelGGL((kernel<T, DP, 4, 64, true, kOne>), grid, dim3(256), 0, s, a);             \
+    else if constexpr (sizeof(T) * DP <= 128)                                                       \
+      hipLaunchKernelGGL((kernel<T, DP, 1, 32, true, kFine>), grid, dim3(64), 0, s, a);             \
+  } while (0)

@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256) void attention_plan_fill_kernel(
 }
 
 // ---------------------------------------------------------------- forward
-template <typename T, int DP, int WAVES, int TILE, bool VEC>
+template <typename T, int DP, int WAVES, int TILE, bool VEC, int WP>
 __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void attention_kernel(AttentionArgs a) {
   typedef Head<T, DP, TILE> S;
   constexpr int kParts = S::kTile / 32;                    // 32-row products of a tile
@@ -180,8 +180,8 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   float top = -INFINITY, sum = 0.0f;                       // the sum over this lane's keys only
   for (int64_t j0 = from; j0 < to; j0 += S::kTile) {
     __syncthreads();
-    next_k.commit(k_tile);
-    next_v.commit(v_tile);
+    next_k.commit(k_tile, a.D);
+    next_v.commit(v_tile, a.D);
     const uint64_t keep = next_keep;
     __syncthreads();
     if (j0 + S::kTile < to) fetch(j0 + S::kTile);
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
     for (int b = 0; b < kParts; ++b)
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        const auto w = weight_operand<T, S::template kWeights<WAVES>>(p[b], f);
+        const auto w = weight_operand<T, WP>(p[b], f);
 #pragma unroll
         for (int d = 0; d < S::kBlocks; ++d)
           mma<T>(transposed_operand<T, S>(v_tile, 32 * b, d, f, lane), w, o[d]);
@@ -281,14 +281,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
 }
 
 template <typename T, int DP>
-static void attention_launch(const AttentionArgs& a, int rows, hipStream_t s) {
+static void attention_launch(const AttentionArgs& a, int rows, bool fine, hipStream_t s) {
   const dim3 grid((unsigned)(a.n_tiles * a.heads * a.splits));
-  if (!a.vec)
-    hipLaunchKernelGGL((attention_kernel<T, DP, 4, 64, false>), grid, dim3(256), 0, s, a);
-  else if (rows == 128)
-    hipLaunchKernelGGL((attention_kernel<T, DP, 4, 64, true>), grid, dim3(256), 0, s, a);
-  else if constexpr (sizeof(T) * DP <= 128)
-    hipLaunchKernelGGL((attention_kernel<T, DP, 1, 32, true>), grid, dim3(64), 0, s, a);
+  XNN_ATTENTION_LAUNCH(attention_kernel, grid);
   if (a.splits == 1) return;
   const int64_t n = a.n_tokens * a.heads;
   if (a.vec_out)
@@ -362,16 +357,17 @@ int xnn_attention(int dtype, const xnn_heads* q, const xnn_heads* k, const xnn_h
   a.part_lse = a.part + (size_t)a.splits * n_tokens * a.heads * head_dim;
   a.vec_out = head_dim % 4 == 0 && (uintptr_t)out % 16 == 0;
   const int rows = attention_pick(a, plan, dtype);
+  const bool fine = fine_weights(a, plan);
   hipStream_t s = as_hip(stream);
   XNN_STORAGE_DISPATCH(dtype, T, {
     if (head_dim <= 16)
-      attention_launch<T, 16>(a, rows, s);
+      attention_launch<T, 16>(a, rows, fine, s);
     else if (head_dim <= 32)
-      attention_launch<T, 32>(a, rows, s);
+      attention_launch<T, 32>(a, rows, fine, s);
     else if (head_dim <= 64)
-      attention_launch<T, 64>(a, rows, s);
+      attention_launch<T, 64>(a, rows, fine, s);
     else
-      attention_launch<T, 128>(a, rows, s);
+      attention_launch<T, 128>(a, rows, fine, s);
   });
   XNN_LAUNCH_CHECK();
   return XNN_OK;

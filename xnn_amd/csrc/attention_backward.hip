@@ -19,7 +19,7 @@
 
 namespace xnn {
 
-template <typename T, int DP, int WAVES, int TILE, bool VEC>
+template <typename T, int DP, int WAVES, int TILE, bool VEC, int WP>
 __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void attention_dq_kernel(AttentionArgs a) {
   typedef Head<T, DP, TILE> S;
   __shared__ __align__(16) char k_tile[S::kBytes];
@@ -75,8 +75,8 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   f32x16 dq[S::kBlocks] = {};
   for (int64_t j0 = from; j0 < to; j0 += S::kTile) {
     __syncthreads();
-    next_k.commit(k_tile);
-    next_v.commit(v_tile);
+    next_k.commit(k_tile, a.D);
+    next_v.commit(v_tile, a.D);
     const uint64_t keep = next_keep;
     __syncthreads();
     if (j0 + S::kTile < to) fetch(j0 + S::kTile);
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
       }
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        const auto w = weight_operand<T, S::template kWeights<WAVES>>(p, f);
+        const auto w = weight_operand<T, WP>(p, f);
 #pragma unroll
         for (int d = 0; d < S::kBlocks; ++d)
           mma<T>(transposed_operand<T, S>(k_tile, 32 * b, d, f, lane), w, dq[d]);
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
     store_own((T*)a.dq + at, dq, a.scale, a.D, a.vec_out, half);
 }
 
-template <typename T, int DP, int WAVES, int TILE, bool VEC>
+template <typename T, int DP, int WAVES, int TILE, bool VEC, int WP>
 __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void attention_dkv_kernel(AttentionArgs a) {
   typedef Head<T, DP, TILE> S;
   __shared__ __align__(16) char q_tile[S::kBytes];
@@ -163,8 +163,8 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   f32x16 dk[S::kBlocks] = {}, dv[S::kBlocks] = {};
   for (int64_t n = from; n < to; ++n) {
     __syncthreads();
-    next_q.commit(q_tile);
-    next_g.commit(g_tile);
+    next_q.commit(q_tile, a.D);
+    next_g.commit(g_tile, a.D);
     if (threadIdx.x < S::kTile) {
       // a row beyond the structure or without keys: every probability is zero
       lse_tile[threadIdx.x] = next_lse == -INFINITY ? INFINITY : next_lse;
@@ -194,8 +194,8 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
       }
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        const auto w = weight_operand<T, S::template kWeights<WAVES>>(p, f);
-        const auto dw = weight_operand<T, S::template kWeights<WAVES>>(dp, f);
+        const auto w = weight_operand<T, WP>(p, f);
+        const auto dw = weight_operand<T, WP>(dp, f);
 #pragma unroll
         for (int d = 0; d < S::kBlocks; ++d) {
           mma<T>(transposed_operand<T, S>(g_tile, 32 * b, d, f, lane), w, dv[d]);
@@ -253,25 +253,15 @@ static void attention_sum(const AttentionArgs& a, int64_t n, void* x, void* y, h
 }
 
 template <typename T, int DP>
-static void attention_backward_launch(AttentionArgs a, int rows, int q_splits, int k_splits,
+static void attention_backward_launch(AttentionArgs a, int rows, bool fine, int q_splits, int k_splits,
                                       hipStream_t s) {
   const dim3 q_grid((unsigned)(a.n_tiles * a.heads * q_splits));
   const dim3 k_grid((unsigned)(a.n_tiles * a.kv_heads * k_splits));
   a.splits = q_splits;
-  if (!a.vec)
-    hipLaunchKernelGGL((attention_dq_kernel<T, DP, 4, 64, false>), q_grid, dim3(256), 0, s, a);
-  else if (rows == 128)
-    hipLaunchKernelGGL((attention_dq_kernel<T, DP, 4, 64, true>), q_grid, dim3(256), 0, s, a);
-  else if constexpr (sizeof(T) * DP <= 128)
-    hipLaunchKernelGGL((attention_dq_kernel<T, DP, 1, 32, true>), q_grid, dim3(64), 0, s, a);
+  XNN_ATTENTION_LAUNCH(attention_dq_kernel, q_grid);
   if (q_splits > 1) attention_sum<T>(a, a.n_tokens * a.heads * a.D, a.dq, nullptr, s);
   a.splits = k_splits;
-  if (!a.vec)
-    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 4, 64, false>), k_grid, dim3(256), 0, s, a);
-  else if (rows == 128)
-    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 4, 64, true>), k_grid, dim3(256), 0, s, a);
-  else if constexpr (sizeof(T) * DP <= 128)
-    hipLaunchKernelGGL((attention_dkv_kernel<T, DP, 1, 32, true>), k_grid, dim3(64), 0, s, a);
+  XNN_ATTENTION_LAUNCH(attention_dkv_kernel, k_grid);
   if (k_splits > 1) attention_sum<T>(a, a.n_tokens * a.kv_heads * a.D, a.dk, a.dv, s);
 }
 
@@ -333,16 +323,17 @@ int xnn_attention_backward(int dtype, const xnn_heads* q, const xnn_heads* k, co
               ((uintptr_t)out | (uintptr_t)grad | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0;
   a.vec = a.vec && a.vec_out;
   const int rows = attention_pick(a, plan, dtype);
+  const bool fine = fine_weights(a, plan);
   hipStream_t s = as_hip(stream);
   XNN_STORAGE_DISPATCH(dtype, T, {
     if (head_dim <= 16)
-      attention_backward_launch<T, 16>(a, rows, q_splits, k_splits, s);
+      attention_backward_launch<T, 16>(a, rows, fine, q_splits, k_splits, s);
     else if (head_dim <= 32)
-      attention_backward_launch<T, 32>(a, rows, q_splits, k_splits, s);
+      attention_backward_launch<T, 32>(a, rows, fine, q_splits, k_splits, s);
     else if (head_dim <= 64)
-      attention_backward_launch<T, 64>(a, rows, q_splits, k_splits, s);
+      attention_backward_launch<T, 64>(a, rows, fine, q_splits, k_splits, s);
     else
-      attention_backward_launch<T, 128>(a, rows, q_splits, k_splits, s);
+      attention_backward_launch<T, 128>(a, rows, fine, q_splits, k_splits, s);
   });
   XNN_LAUNCH_CHECK();
   return XNN_OK;

@@ -10,9 +10,10 @@
 //
 //   small tables (at most 255 rows, species): each block sorts its own tokens by counting, sums their
 //     runs and leaves a row for each id it has seen; a block a row of the table adds those in order
-//   up to 16,384 tokens: one block sorts all of them in LDS (8 bits a pass) while the others clear
-//     the table; then runs of the sorted order are summed in chunks, and those that cross chunks joined
-//   beyond: the same with a sort of three launches a pass
+//   up to 65,536 tokens: chunks of 1,024 sorted in LDS while other blocks clear the table, merged by
+//     rank (16,384 ids: 10 us in place of 30 in the LDS of one block and 26 by the passes below); then
+//     runs of the sorted order are summed in chunks, and those that cross chunks joined
+//   beyond: the same with a radix sort of three launches a pass
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -27,14 +28,14 @@ namespace xnn {
 constexpr int kBins = 256;         // digits of a sort pass, ids of a small table
 constexpr int kSortTile = 1024;    // ids a block of a sort pass takes, at least
 constexpr int kSortBlocks = 512;   // blocks of a sort pass, at most
-constexpr int kSortInLds = 16384;  // ids one block sorts in LDS, at most
+constexpr int kSortMerge = 65536;  // ids sorted in chunks of 1,024 that are merged, at most
 constexpr int kChunk = 32;         // sorted positions a group of lanes sums
 constexpr int kOwnTokens = 4096;   // tokens a block sorts for a small table, at most
 
 static int64_t round64(int64_t b) { return (b + 63) / 64 * 64; }
 
 struct EmbeddingWork {
-  bool small, in_lds;
+  bool small, merge;
   int passes;
   int64_t blocks, per, chunks;                             // of the sort, of the sums
   int64_t key[2], perm[2], hist, part, seen, bytes;        // offsets
@@ -59,20 +60,20 @@ static EmbeddingWork embedding_work(int64_t n, int64_t n_rows, int64_t C) {
   int bits = 1;
   while (bits < 31 && (n_rows >> bits) != 0) ++bits;       // n_rows itself is the invalid id
   w.passes = (bits + 7) / 8;
-  w.in_lds = n <= kSortInLds;
+  w.merge = n <= kSortMerge;
   w.per = std::max<int64_t>(kSortTile,
                             (n + (int64_t)kSortBlocks * kSortTile - 1) / ((int64_t)kSortBlocks * kSortTile) *
                                 kSortTile);
   w.blocks = (n + w.per - 1) / w.per;
   w.chunks = (n + kChunk - 1) / kChunk;
-  for (int i = 0; i < (w.in_lds ? 1 : 2); ++i) {
+  for (int i = 0; i < 2; ++i) {
     w.key[i] = o;
     o += round64(4 * n);
     w.perm[i] = o;
     o += round64(4 * n);
   }
   w.hist = o;
-  if (!w.in_lds) o += round64(4 * kBins * w.blocks);
+  if (!w.merge) o += round64(4 * kBins * w.blocks);
   w.part = o;
   o += 8 * w.chunks * C;
   w.bytes = o;
@@ -237,40 +238,32 @@ __global__ __launch_bounds__(256) void clear_kernel(char* __restrict__ p, int64_
   clear16(p, bytes, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
 }
 
-// Block 0 sorts all (at most 16,384) ids in LDS, sixteen waves of up to sixteen rounds; the others
-// clear the gradient.
-__global__ __launch_bounds__(1024) void sort_all_kernel(const int64_t* __restrict__ ids, int n,
-                                                        int64_t n_rows, int passes,
-                                                        uint32_t* __restrict__ key_out,
-                                                        uint32_t* __restrict__ perm_out,
-                                                        char* __restrict__ grad, int64_t bytes) {
-  if (blockIdx.x > 0) {
-    clear16(grad, bytes, ((int64_t)blockIdx.x - 1) * 1024 + threadIdx.x, ((int64_t)gridDim.x - 1) * 1024);
+// Blocks below `chunks` sort 1,024 ids each in LDS, one a thread; the others clear the gradient.
+__global__ __launch_bounds__(1024) void sort_chunk_kernel(const int64_t* __restrict__ ids, int n,
+                                                          int64_t n_rows, int passes, int chunks,
+                                                          uint32_t* __restrict__ key_out,
+                                                          uint32_t* __restrict__ perm_out,
+                                                          char* __restrict__ grad, int64_t bytes) {
+  if ((int)blockIdx.x >= chunks) {
+    clear16(grad, bytes, ((int64_t)blockIdx.x - chunks) * 1024 + threadIdx.x,
+            ((int64_t)gridDim.x - chunks) * 1024);
     return;
   }
-  __shared__ uint32_t keys[kSortInLds];
-  __shared__ uint16_t perms[kSortInLds];
+  __shared__ uint32_t keys[1024];
+  __shared__ uint16_t perms[1024];
   __shared__ uint32_t count[16][kBins];
   __shared__ uint32_t sums[4];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = wave_in_block();
-  const int rounds = (n + 1023) / 1024;
-  const int first = wave * rounds * kWave, mine = min(max(n - first, 0), rounds * kWave);
-  uint32_t key[16], perm[16], digit[16], rank[16];
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int i = r * kWave + lane;
-    key[r] = perm[r] = 0;
-    if (r < rounds && i < mine) {
-      key[r] = sort_key(ids, nullptr, first + i, n_rows);
-      perm[r] = first + i;
-    }
-  }
+  const int begin = blockIdx.x * 1024, m = min(1024, n - begin);
+  const int mine = min(max(m - wave * kWave, 0), kWave);
+  const bool live = tid < m;
+  uint32_t key = live ? sort_key(ids, nullptr, begin + tid, n_rows) : 0u;
+  uint32_t perm = tid, digit[1], rank[1];
   for (int p = 0; p < passes; ++p) {
     for (int i = tid; i < 16 * kBins; i += 1024) (&count[0][0])[i] = 0;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) digit[r] = (key[r] >> (8 * p)) & (kBins - 1);
+    digit[0] = (key >> (8 * p)) & (kBins - 1);
     __syncthreads();
-    wave_ranks(digit, rounds, mine, count[wave], rank);
+    wave_ranks(digit, 1, mine, count[wave], rank);
     __syncthreads();
     // keys of smaller digits, then those of the same digit in earlier waves
     uint32_t total = 0, x = 0;
@@ -297,27 +290,54 @@ __global__ __launch_bounds__(1024) void sort_all_kernel(const int64_t* __restric
       }
     }
     __syncthreads();
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-      if (r < rounds && r * kWave + lane < mine) {
-        const uint32_t to = count[wave][digit[r]] + rank[r];
-        keys[to] = key[r];
-        perms[to] = (uint16_t)perm[r];
-      }
-    __syncthreads();
-    if (p + 1 < passes) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (r < rounds && r * kWave + lane < mine) {
-          key[r] = keys[first + r * kWave + lane];
-          perm[r] = perms[first + r * kWave + lane];
-        }
-      __syncthreads();
+    if (live) {
+      const uint32_t to = count[wave][digit[0]] + rank[0];
+      keys[to] = key;
+      perms[to] = (uint16_t)perm;
     }
+    __syncthreads();
+    if (live) {
+      key = keys[tid];
+      perm = perms[tid];
+    }
+    __syncthreads();
   }
-  for (int i = tid; i < n; i += 1024) {
-    key_out[i] = keys[i];
-    perm_out[i] = perms[i];
+  if (live) {
+    key_out[begin + tid] = key;
+    perm_out[begin + tid] = begin + perm;
+  }
+}
+
+// The place of every element of the sorted chunks among all: in its own chunk, plus the elements of each
+// other chunk that come before it (equal ones of earlier chunks do), by bisection, `lanes` lanes an
+// element.
+__global__ __launch_bounds__(256) void sort_merge_kernel(const uint32_t* __restrict__ key,
+                                                         const uint32_t* __restrict__ perm, int n,
+                                                         int chunks, int lanes,
+                                                         uint32_t* __restrict__ key_out,
+                                                         uint32_t* __restrict__ perm_out) {
+  const int i = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes);
+  const bool live = i < n;
+  const uint32_t k = live ? key[i] : 0u;
+  const int own = i / 1024;
+  int before = 0;
+  for (int c = threadIdx.x % lanes; live && c < chunks; c += lanes) {
+    if (c == own) continue;
+    const uint32_t* a = key + c * 1024;
+    int lo = 0, hi = min(1024, n - c * 1024);
+    while (lo < hi) {                                      // the first element not before this one
+      const int mid = (lo + hi) / 2;
+      const bool earlier = c < own ? a[mid] <= k : a[mid] < k;
+      lo = earlier ? mid + 1 : lo;
+      hi = earlier ? hi : mid;
+    }
+    before += lo;
+  }
+  for (int o = 1; o < lanes; o <<= 1) before += __shfl_xor(before, o);
+  if (live && threadIdx.x % lanes == 0) {
+    const int to = i % 1024 + before;
+    key_out[to] = k;
+    perm_out[to] = perm[i];
   }
 }
 
@@ -492,7 +512,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(
   const bool goes_on = end < n && key[end] == key[end - 1];
   float sum[N] = {};
   int64_t first = begin;
-  constexpr int kAhead = 4;                                // rows in flight
+  constexpr int kAhead = 8;                                // rows in flight
   for (int64_t i0 = begin; i0 < end; i0 += kAhead) {
     float v[kAhead][N];
     uint32_t k[kAhead + 1];
@@ -653,10 +673,17 @@ static int embedding_grad(const int64_t* ids, int64_t n, const void* g, int64_t 
       perm[i] = (uint32_t*)(work + w.perm[i]);
     }
     int from = 0;
-    if (w.in_lds) {
+    if (w.merge) {
+      const int chunks = (int)((n + 1023) / 1024);
       const int64_t clear = std::min<int64_t>(bytes / 16384 + 1, 2048);
-      hipLaunchKernelGGL(sort_all_kernel, dim3((unsigned)(1 + clear)), dim3(1024), 0, s, ids, (int)n,
-                         n_rows, w.passes, key[0], perm[0], grad, bytes);
+      from = chunks > 1 ? 1 : 0;
+      hipLaunchKernelGGL(sort_chunk_kernel, dim3((unsigned)(chunks + clear)), dim3(1024), 0, s, ids, (int)n,
+                         n_rows, w.passes, chunks, key[0], perm[0], grad, bytes);
+      if (chunks > 1) {
+        const int lanes = row_lanes(chunks, 1, 64);
+        hipLaunchKernelGGL(sort_merge_kernel, dim3((unsigned)((n * lanes + 255) / 256)), dim3(256), 0, s,
+                           key[0], perm[0], (int)n, chunks, lanes, key[1], perm[1]);
+      }
     } else {
       hipLaunchKernelGGL(clear_kernel, dim3((unsigned)std::min<int64_t>(bytes / 4096 + 1, 8192)),
                          dim3(256), 0, s, grad, bytes);
