@@ -243,6 +243,34 @@ def test_structure_attention(counts, H, K, D, dtype, masked, packed):
         assert torch.equal(xa.structure_attention(*dev, plan, mask=m), out)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [16, 64])
+def test_a_long_structure_loses_no_more_than_short_ones(dtype, D):
+    """20,000 atoms: the average probability is below float16's least normal number. The norm of the
+    errors is at most that of two roundings, of the output and of the weights, each of half a unit at
+    most."""
+    import xnn_amd as xa
+    n = 20000
+    gen = torch.Generator(device=DEV).manual_seed(D)
+    q, k, v, g = (torch.randn(n, 1, D, generator=gen, device=DEV).to(dtype) for _ in range(4))
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = xa.structure_attention(*leaves, xa.attention_plan(torch.tensor([n], device=DEV)))
+    got = (out, *torch.autograd.grad(out, leaves, g))
+    a, b, c, e = (t[:, 0].double() for t in (q, k, v, g))
+    want = [torch.zeros_like(a) for _ in range(4)]
+    for i in range(0, n, 2500):
+        r = slice(i, i + 2500)
+        p = torch.softmax(a[r] @ b.T * D ** -0.5, 1)
+        o, dp = p @ c, e[r] @ c.T
+        ds = p * (dp - (e[r] * o).sum(1, keepdim=True)) * D ** -0.5
+        want[0][r], want[1][r] = o, ds @ b
+        want[2] += ds.T @ a[r]
+        want[3] += p.T @ e[r]
+    for name, x, y in zip(("out", "dq", "dk", "dv"), got, want):
+        off = float((x[:, 0].double() - y).norm() / y.norm())
+        assert off <= 2 * UNIT[dtype] / 2, (name, off)
+
+
 def test_attention_gradients_against_differences():
     """Central differences of the float64 definition along a direction and the kernels' gradients."""
     import xnn_amd as xa

@@ -475,10 +475,25 @@ inline int64_t attention_blocks(const xnn_attention_tiles* plan, int heads) {
 // is of the size of the output's own, 1.4 times the error of an output that is rounded once, whatever the
 // length. Where few elements average it a second plane, the rounding error of the first, is taken as
 // well: in blocks of one wave, whose products are not what bounds them (1,024 molecules of 10 to 60 atoms: the
-// same time), and where all scores are some microseconds of work.
+// same time), and where all scores are some microseconds of work. So it is for the queries' gradient in
+// heads of at most 32 elements: the row's weights sum to zero, so that what is left of a sum over few
+// elements is smaller than its parts (1.45 to 1.67 times the output's rounding with one plane).
 constexpr int64_t kFineScores = (int64_t)1 << 23;
 inline bool fine_weights(const AttentionArgs& a, const xnn_attention_tiles* plan) {
   return a.n_tokens * plan->max_atoms * a.heads <= kFineScores;
+}
+inline bool fine_query_gradient(const AttentionArgs& a, const xnn_attention_tiles* plan) {
+  return a.D <= 32 || fine_weights(a, plan);
+}
+
+// Probabilities of a long structure are small beside float16's least normal number, 2^-14: the gradients
+// carry them, and what is formed from them, 2^this times larger (half the average 1 / n at most, and no
+// more than 2^5, which leaves score gradients up to 2,047) and take the factor back at the end. Exact;
+// the other types have the exponents.
+template <typename T>
+__device__ __forceinline__ int carried(int64_t n) {
+  if constexpr (Store<T>::kPlanes == 3 || __is_same(T, bf16_t)) return 0;
+  return max(0, min(5, 63 - __clzll((long long)n) - 9));
 }
 
 // the tiles of a launch; rows that are not moved 16 bytes at a time are always walked by 128
@@ -538,7 +553,7 @@ inline int attention_args(AttentionArgs& a, int dtype, const xnn_heads* q, const
 
 // One launch of kernel<T, DP, waves, tile, vec, weight planes> for arguments `a` of `rows` rows a block on
 // stream `s`
-#define XNN_ATTENTION_LAUNCH(kernel, grid)                                                          \
+#define XNN_ATTENTION_LAUNCH(kernel, grid, fine)                                                    \
   do {                                                                                              \
     constexpr int kOne = Store<T>::kPlanes, kFine = kOne == 3 ? 3 : 2;                              \
     if (!a.vec && fine)                                                                             \

@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
 template <typename T, int DP>
 static void attention_launch(const AttentionArgs& a, int rows, bool fine, hipStream_t s) {
   const dim3 grid((unsigned)(a.n_tiles * a.heads * a.splits));
-  XNN_ATTENTION_LAUNCH(attention_kernel, grid);
+  XNN_ATTENTION_LAUNCH(attention_kernel, grid, fine);
   if (a.splits == 1) return;
   const int64_t n = a.n_tokens * a.heads;
   if (a.vec_out)

@@ -70,6 +70,9 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   }
   float lse = live ? a.lse[(int64_t)t.head * a.n_tokens + row] : -INFINITY;
   const bool empty = lse == -INFINITY;
+  const int carry = carried<T>(t.end - t.begin);
+  const float factor = ldexpf(a.scale, -carry);
+  lse -= (float)carry;
   if (empty) lse = INFINITY;                               // every probability of the row is zero
   if (live && half == 0 && t.split == 0) a.delta[(int64_t)t.head * a.n_tokens + row] = delta;
   f32x16 dq[S::kBlocks] = {};
@@ -114,10 +117,10 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   }
   const int64_t at = (row * a.heads + t.head) * a.D;
   if (a.splits > 1)
-    store_own(a.part + (int64_t)t.split * a.n_tokens * a.heads * a.D + at, dq, a.scale, a.D,
+    store_own(a.part + (int64_t)t.split * a.n_tokens * a.heads * a.D + at, dq, factor, a.D,
               a.D % 4 == 0, half);
   else
-    store_own((T*)a.dq + at, dq, a.scale, a.D, a.vec_out, half);
+    store_own((T*)a.dq + at, dq, factor, a.D, a.vec_out, half);
 }
 
 template <typename T, int DP, int WAVES, int TILE, bool VEC, int WP>
@@ -136,6 +139,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   const float scale = a.scale * kLog2e;
   const int group = a.heads / a.kv_heads;
   const int64_t out_stride = (int64_t)a.heads * a.D;
+  const int carry = carried<T>(t.end - t.begin);
   // the walk: the rows of every head that shares these keys
   const int64_t per = (t.end - t.begin + S::kTile - 1) / S::kTile;
   int64_t from, to;
@@ -167,7 +171,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
     next_g.commit(g_tile, a.D);
     if (threadIdx.x < S::kTile) {
       // a row beyond the structure or without keys: every probability is zero
-      lse_tile[threadIdx.x] = next_lse == -INFINITY ? INFINITY : next_lse;
+      lse_tile[threadIdx.x] = next_lse == -INFINITY ? INFINITY : next_lse - (float)carry;
       delta_tile[threadIdx.x] = next_delta;
     }
     __syncthreads();
@@ -212,13 +216,14 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
       for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.0f;
   }
   const int64_t at = (key * a.kv_heads + t.head) * a.D;
+  const float k_factor = ldexpf(a.scale, -carry), v_factor = ldexpf(1.0f, -carry);
   if (a.splits > 1) {
     const int64_t one = a.n_tokens * a.kv_heads * a.D;
-    store_own(a.part + t.split * one + at, dk, a.scale, a.D, a.D % 4 == 0, half);
-    store_own(a.part + (a.splits + t.split) * one + at, dv, 1.0f, a.D, a.D % 4 == 0, half);
+    store_own(a.part + t.split * one + at, dk, k_factor, a.D, a.D % 4 == 0, half);
+    store_own(a.part + (a.splits + t.split) * one + at, dv, v_factor, a.D, a.D % 4 == 0, half);
   } else {
-    store_own((T*)a.dk + at, dk, a.scale, a.D, a.vec_out, half);
-    store_own((T*)a.dv + at, dv, 1.0f, a.D, a.vec_out, half);
+    store_own((T*)a.dk + at, dk, k_factor, a.D, a.vec_out, half);
+    store_own((T*)a.dv + at, dv, v_factor, a.D, a.vec_out, half);
   }
 }
 
@@ -253,15 +258,15 @@ static void attention_sum(const AttentionArgs& a, int64_t n, void* x, void* y, h
 }
 
 template <typename T, int DP>
-static void attention_backward_launch(AttentionArgs a, int rows, bool fine, int q_splits, int k_splits,
-                                      hipStream_t s) {
+static void attention_backward_launch(AttentionArgs a, int rows, bool fine_query, bool fine, int q_splits,
+                                      int k_splits, hipStream_t s) {
   const dim3 q_grid((unsigned)(a.n_tiles * a.heads * q_splits));
   const dim3 k_grid((unsigned)(a.n_tiles * a.kv_heads * k_splits));
   a.splits = q_splits;
-  XNN_ATTENTION_LAUNCH(attention_dq_kernel, q_grid);
+  XNN_ATTENTION_LAUNCH(attention_dq_kernel, q_grid, fine_query);
   if (q_splits > 1) attention_sum<T>(a, a.n_tokens * a.heads * a.D, a.dq, nullptr, s);
   a.splits = k_splits;
-  XNN_ATTENTION_LAUNCH(attention_dkv_kernel, k_grid);
+  XNN_ATTENTION_LAUNCH(attention_dkv_kernel, k_grid, fine);
   if (k_splits > 1) attention_sum<T>(a, a.n_tokens * a.kv_heads * a.D, a.dk, a.dv, s);
 }
 
@@ -323,17 +328,17 @@ int xnn_attention_backward(int dtype, const xnn_heads* q, const xnn_heads* k, co
               ((uintptr_t)out | (uintptr_t)grad | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0;
   a.vec = a.vec && a.vec_out;
   const int rows = attention_pick(a, plan, dtype);
-  const bool fine = fine_weights(a, plan);
+  const bool fine = fine_weights(a, plan), fine_query = fine_query_gradient(a, plan);
   hipStream_t s = as_hip(stream);
   XNN_STORAGE_DISPATCH(dtype, T, {
     if (head_dim <= 16)
-      attention_backward_launch<T, 16>(a, rows, fine, q_splits, k_splits, s);
+      attention_backward_launch<T, 16>(a, rows, fine_query, fine, q_splits, k_splits, s);
     else if (head_dim <= 32)
-      attention_backward_launch<T, 32>(a, rows, fine, q_splits, k_splits, s);
+      attention_backward_launch<T, 32>(a, rows, fine_query, fine, q_splits, k_splits, s);
     else if (head_dim <= 64)
-      attention_backward_launch<T, 64>(a, rows, fine, q_splits, k_splits, s);
+      attention_backward_launch<T, 64>(a, rows, fine_query, fine, q_splits, k_splits, s);
     else
-      attention_backward_launch<T, 128>(a, rows, fine, q_splits, k_splits, s);
+      attention_backward_launch<T, 128>(a, rows, fine_query, fine, q_splits, k_splits, s);
   });
   XNN_LAUNCH_CHECK();
   return XNN_OK;
