@@ -1230,7 +1230,7 @@ int xnn_attention_plan(const int64_t* n_atoms, int64_t n_structures, int64_t n_t
 
 /* Bytes of the workspace of xnn_attention (0 where it needs none: only long structures of few
  * tiles are walked in parts that are joined). */
-int xnn_attention_work_size(int64_t n_tokens, int32_t n_heads, int32_t head_dim,
+int xnn_attention_work_size(int dtype, int64_t n_tokens, int32_t n_heads, int32_t head_dim,
                             const xnn_attention_tiles* plan, size_t* bytes);
 
 /* Attention of every token to the tokens of its structure that `mask` (n_tokens bytes, zero
@@ -1244,8 +1244,8 @@ int xnn_attention(int dtype, const xnn_heads* q, const xnn_heads* k, const xnn_h
                   size_t work_bytes, xnn_stream_t stream);
 
 /* Bytes of the workspace of xnn_attention_backward. */
-int xnn_attention_backward_work_size(int64_t n_tokens, int32_t n_heads, int32_t n_kv_heads,
-                                     int32_t head_dim, const xnn_attention_tiles* plan,
+int xnn_attention_backward_work_size(int dtype, int64_t n_tokens, int32_t n_heads,
+                                     int32_t n_kv_heads, int32_t head_dim, const xnn_attention_tiles* plan,
                                      size_t* bytes);
 
 /* Gradients of xnn_attention for the cotangent `grad`, from its inputs and its outputs out and

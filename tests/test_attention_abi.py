@@ -99,10 +99,10 @@ def test_attention_arguments(lib):
     assert call(T=0, p=plan(tokens=0, tiles=False), out=None) == 0
     _refused(lib, lib.xnn_attention_plan(BUF, 2, 100, BUF, BUF, BUF, BUF, 2, BUF, 2, BUF, None), b"too small")
     _refused(lib, lib.xnn_attention_plan(BUF, 2, 1 << 31, BUF, BUF, BUF, BUF, 2, BUF, 2, BUF, None), b"too many")
-    assert lib.xnn_attention_backward_work_size(10, 4, 2, 16, plan(), ctypes.byref(SIZE)) == 0
+    assert lib.xnn_attention_backward_work_size(0, 10, 4, 2, 16, plan(), ctypes.byref(SIZE)) == 0
     long = ctypes.byref(_lib.AttentionTiles(9000, 9000, 141, 71, None, None))
-    assert lib.xnn_attention_work_size(9000, 4, 32, long, ctypes.byref(SPLIT)) == 0 and SPLIT.value > 0
-    assert lib.xnn_attention_work_size(10, 4, 16, plan(), ctypes.byref(SPLIT)) == 0 and SPLIT.value == 0
+    assert lib.xnn_attention_work_size(0, 9000, 4, 32, long, ctypes.byref(SPLIT)) == 0 and SPLIT.value > 0
+    assert lib.xnn_attention_work_size(0, 10, 4, 16, plan(), ctypes.byref(SPLIT)) == 0 and SPLIT.value == 0
     _refused(lib, lib.xnn_attention_backward(0, _heads(4), _heads(2), _heads(2), 10, 16, plan(), None,
                                              0.25, BUF, BUF, BUF, BUF, BUF, BUF, BUF, SIZE.value - 1,
                                              None), b"too small")

@@ -283,9 +283,9 @@ _SIGNATURES = {
     "xnn_head_norm_rotate_backward": [c_int, _heads, _heads, i64, i32, i32, vp, vp, vp, vp, i64, vp,
                                       f32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp],
     "xnn_attention_plan": [vp, i64, i64, vp, vp, vp, vp, i64, vp, i64, vp, vp],
-    "xnn_attention_work_size": [i64, i32, i32, _tiles, vp],
+    "xnn_attention_work_size": [c_int, i64, i32, i32, _tiles, vp],
     "xnn_attention": [c_int, _heads, _heads, _heads, i64, i32, _tiles, vp, f32, vp, vp, vp, sz, vp],
-    "xnn_attention_backward_work_size": [i64, i32, i32, i32, _tiles, vp],
+    "xnn_attention_backward_work_size": [c_int, i64, i32, i32, i32, _tiles, vp],
     "xnn_attention_backward": [c_int, _heads, _heads, _heads, i64, i32, _tiles, vp, f32, vp, vp, vp,
                                vp, vp, vp, vp, sz, vp],
 }

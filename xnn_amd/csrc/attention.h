@@ -125,6 +125,7 @@ struct Head {
   static constexpr int kPlane = kTile * kRow;
   // waves of a SIMD: two share its matrix core and vector unit where their registers fit
   static constexpr int kOccupancy = DP <= 32 || (kPlanes == 1 && DP == 64) ? 2 : 1;
+  static constexpr int kForward = DP <= 64 || kPlanes == 1 ? 2 : 1;
   static constexpr int kBytes = kPlanes * kPlane;
 };
 
@@ -433,19 +434,24 @@ __device__ __forceinline__ void walk_part(int64_t n, const AttentionArgs& a, int
 
 constexpr int kCus = 256;
 constexpr int kMostSplits = 16;
-constexpr int kSplitRows = 512;    // walked rows of a part, at least
+
+// Walked rows of a part, at least: some ten microseconds of walking, beside which a join is small (512 rows
+// of 64 elements in 16 bits; fewer of wider heads, and a sixth in float32, which has six products for one).
+inline int64_t split_rows(int dtype, int D) {
+  return std::max<int64_t>(64, 512 * 64 / (std::max(D, 32) * (dtype == XNN_F32 ? 6 : 1)));
+}
 
 // Parts of the walked side, for `blocks` blocks of equal length without: as few as give every one of the
 // chip's 256 CUs `each` blocks and leave none idle for more than a tenth of the time.
-inline int attention_splits(int64_t blocks, int64_t walked, int each) {
-  const int64_t most = std::min<int64_t>(kMostSplits, walked / kSplitRows);
+inline int attention_splits(int64_t blocks, int64_t walked, int64_t rows, int each) {
+  const int64_t most = std::min<int64_t>(kMostSplits, walked / rows);
   int best = 1;
   double best_use = 0.0;
   for (int s = 1; s <= std::max<int64_t>(most, 1); ++s) {
     const int64_t n = blocks * s;
     const double use = (double)n / ((n + kCus - 1) / kCus * kCus) *
                        (n < each * kCus ? 0.6 + 0.2 * n / (each * kCus) : 1.0);
-    if (use > best_use + 0.03) {
+    if (use > best_use * 1.03) {
       best = s;
       best_use = use;
     }
@@ -456,8 +462,12 @@ inline int attention_splits(int64_t blocks, int64_t walked, int each) {
 // Two blocks a CU for the forward pass (24,000 rows of 4 heads, 752 blocks: 752 us undivided, 799 in two
 // parts, with the join); four for the gradients, two of which a CU holds at a time (2,430 us undivided,
 // 2,278 in two parts). 9,000 rows of 4 heads, 284 blocks: five parts for all.
-inline int forward_splits(int64_t blocks, int64_t walked) { return attention_splits(blocks, walked, 2); }
-inline int backward_splits(int64_t blocks, int64_t walked) { return attention_splits(blocks, walked, 4); }
+inline int forward_splits(int64_t blocks, int64_t walked, int64_t rows) {
+  return attention_splits(blocks, walked, rows, 2);
+}
+inline int backward_splits(int64_t blocks, int64_t walked, int64_t rows) {
+  return attention_splits(blocks, walked, rows, 4);
+}
 
 // Rows of a block: 32, one wave, where no structure is longer than 64 (the other waves of a larger
 // block would idle) and one wave's registers hold a tile on its way, otherwise 128.
@@ -468,7 +478,7 @@ inline int attention_rows(const xnn_attention_tiles* plan, int bytes, int D) {
 
 // blocks of a launch without parts
 inline int64_t attention_blocks(const xnn_attention_tiles* plan, int heads) {
-  return plan->n_tiles128 * heads;                         // short structures have no parts
+  return plan->n_tiles128 * heads;
 }
 
 // Planes of the weights (probabilities, score gradients). float32 has three. In 16 bits one: its rounding

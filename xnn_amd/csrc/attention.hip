@@ -144,7 +144,7 @@ __global__ __launch_bounds__(256) void attention_plan_fill_kernel(
 
 // ---------------------------------------------------------------- forward
 template <typename T, int DP, int WAVES, int TILE, bool VEC, int WP>
-__global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void attention_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kForward)) void attention_kernel(AttentionArgs a) {
   typedef Head<T, DP, TILE> S;
   constexpr int kParts = S::kTile / 32;                    // 32-row products of a tile
   __shared__ __align__(16) char k_tile[S::kBytes];
@@ -294,6 +294,13 @@ static void attention_launch(const AttentionArgs& a, int rows, bool fine, hipStr
                        dim3(256), 0, s, a);
 }
 
+// parts of a launch: short structures, whose blocks are of one wave, are walked whole
+static int part_count(const xnn_attention_tiles* plan, int heads, int dtype, int D) {
+  return attention_rows(plan, storage_bytes(dtype), D) == 32
+             ? 1
+             : forward_splits(attention_blocks(plan, heads), plan->max_atoms, split_rows(dtype, D));
+}
+
 static size_t forward_bytes(int64_t n_tokens, int heads, int D, int splits) {
   return splits == 1 ? 0 : sizeof(float) * (size_t)splits * n_tokens * heads * (D + 1);
 }
@@ -328,11 +335,12 @@ int xnn_attention_plan(const int64_t* n_atoms, int64_t n_structures, int64_t n_t
   return XNN_OK;
 }
 
-int xnn_attention_work_size(int64_t n_tokens, int32_t n_heads, int32_t head_dim,
+int xnn_attention_work_size(int dtype, int64_t n_tokens, int32_t n_heads, int32_t head_dim,
                             const xnn_attention_tiles* plan, size_t* bytes) {
+  XNN_REQUIRE(is_storage(dtype), "dtype must be XNN_F32, XNN_BF16 or XNN_F16");
   XNN_REQUIRE(plan && bytes, "NULL plan or size");
   XNN_REQUIRE(n_tokens >= 0 && n_heads >= 1 && head_dim >= 1, "sizes out of range");
-  const int splits = forward_splits(attention_blocks(plan, n_heads), plan->max_atoms);
+  const int splits = part_count(plan, n_heads, dtype, head_dim);
   *bytes = forward_bytes(n_tokens, n_heads, head_dim, splits);
   return XNN_OK;
 }
@@ -345,7 +353,7 @@ int xnn_attention(int dtype, const xnn_heads* q, const xnn_heads* k, const xnn_h
   const int status = attention_args(a, dtype, q, k, v, n_tokens, head_dim, plan, mask, scale);
   if (status != XNN_OK || n_tokens == 0) return status;
   XNN_REQUIRE(out != nullptr, "NULL output");
-  a.splits = forward_splits(attention_blocks(plan, a.heads), plan->max_atoms);
+  a.splits = part_count(plan, a.heads, dtype, head_dim);
   if (a.splits > 1) {
     XNN_REQUIRE(work && work_bytes >= forward_bytes(n_tokens, a.heads, head_dim, a.splits),
                 "work too small");

@@ -74,7 +74,9 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   const float factor = ldexpf(a.scale, -carry);
   lse -= (float)carry;
   if (empty) lse = INFINITY;                               // every probability of the row is zero
-  if (live && half == 0 && t.split == 0) a.delta[(int64_t)t.head * a.n_tokens + row] = delta;
+  // Where the row's keys are one product, d_i = sum_j p_ij g_i . v_j from the registers: what the stored out
+  // lost in its rounding, much beside the differences of two or three keys, is not in it.
+  const bool single = t.end - t.begin <= 32;
   f32x16 dq[S::kBlocks] = {};
   for (int64_t j0 = from; j0 < to; j0 += S::kTile) {
     __syncthreads();
@@ -93,12 +95,20 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
         mma<T>(natural_operand<T, S>(v_tile, 32 * b + lane % 32, c, half), g[c], dp);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] = weight<T>(p[r], scale, lse) * (dp[r] - delta);
-      if (keep != (~0ull >> (64 - S::kTile))) {
+      for (int r = 0; r < 16; ++r) p[r] = weight<T>(p[r], scale, lse);
+      if (keep != (~0ull >> (64 - S::kTile))) {            // the left out keys' g . v is zero
         const uint64_t mine = keep >> (32 * b + 4 * half);
 #pragma unroll
         for (int r = 0; r < 16; ++r) p[r] = (mine >> tile_row(r, 0)) & 1 ? p[r] : 0.0f;
       }
+      if (single && b == 0) {
+        delta = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) delta = fmaf(p[r], dp[r], delta);
+        delta = add_xor32(delta);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[r] *= dp[r] - delta;
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
         const auto w = weight_operand<T, WP>(p, f);
@@ -109,6 +119,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
     }
   }
   if (!live) return;
+  if (half == 0 && (single ? from < to : t.split == 0)) a.delta[(int64_t)t.head * a.n_tokens + row] = delta;
   if (empty) {
 #pragma unroll
     for (int d = 0; d < S::kBlocks; ++d)
@@ -270,6 +281,17 @@ static void attention_backward_launch(AttentionArgs a, int rows, bool fine_query
   if (k_splits > 1) attention_sum<T>(a, a.n_tokens * a.kv_heads * a.D, a.dk, a.dv, s);
 }
 
+// parts of the queries' gradient, which walks keys, and of the keys' and values', which walks the rows of
+// every head that shares them; short structures, whose blocks are of one wave, are walked whole
+static void part_counts(const xnn_attention_tiles* plan, int heads, int kv_heads, int dtype, int D, int& q,
+                        int& k) {
+  q = k = 1;
+  if (attention_rows(plan, storage_bytes(dtype), D) == 32) return;
+  const int64_t rows = split_rows(dtype, D);
+  q = backward_splits(attention_blocks(plan, heads), plan->max_atoms, rows);
+  k = backward_splits(attention_blocks(plan, kv_heads), plan->max_atoms * (heads / kv_heads), rows);
+}
+
 // the rows' dot products, then the parts of the queries' gradients and after those the parts of the
 // keys' and values' (one after the other in the same place)
 static int64_t delta_floats(int64_t n_tokens, int heads) { return (n_tokens * heads + 3) / 4 * 4; }
@@ -287,16 +309,16 @@ using namespace xnn;
 
 extern "C" {
 
-int xnn_attention_backward_work_size(int64_t n_tokens, int32_t n_heads, int32_t n_kv_heads,
-                                     int32_t head_dim, const xnn_attention_tiles* plan,
+int xnn_attention_backward_work_size(int dtype, int64_t n_tokens, int32_t n_heads,
+                                     int32_t n_kv_heads, int32_t head_dim, const xnn_attention_tiles* plan,
                                      size_t* bytes) {
+  XNN_REQUIRE(is_storage(dtype), "dtype must be XNN_F32, XNN_BF16 or XNN_F16");
   XNN_REQUIRE(plan && bytes, "NULL plan or size");
   XNN_REQUIRE(n_tokens >= 0 && n_heads >= 1 && n_kv_heads >= 1 && n_heads % n_kv_heads == 0 &&
                   head_dim >= 1,
               "sizes out of range");
-  const int q = backward_splits(attention_blocks(plan, n_heads), plan->max_atoms);
-  const int k = backward_splits(attention_blocks(plan, n_kv_heads),
-                                 plan->max_atoms * (n_heads / n_kv_heads));
+  int q, k;
+  part_counts(plan, n_heads, n_kv_heads, dtype, head_dim, q, k);
   *bytes = backward_bytes(n_tokens, n_heads, n_kv_heads, head_dim, q, k);
   return XNN_OK;
 }
@@ -310,9 +332,8 @@ int xnn_attention_backward(int dtype, const xnn_heads* q, const xnn_heads* k, co
   const int status = attention_args(a, dtype, q, k, v, n_tokens, head_dim, plan, mask, scale);
   if (status != XNN_OK || n_tokens == 0) return status;
   XNN_REQUIRE(out && lse && grad && dq && dk && dv && work, "NULL input, output or work");
-  const int q_splits = backward_splits(attention_blocks(plan, a.heads), plan->max_atoms);
-  const int k_splits = backward_splits(attention_blocks(plan, a.kv_heads),
-                                        plan->max_atoms * (a.heads / a.kv_heads));
+  int q_splits, k_splits;
+  part_counts(plan, a.heads, a.kv_heads, dtype, head_dim, q_splits, k_splits);
   XNN_REQUIRE(work_bytes >= backward_bytes(n_tokens, a.heads, a.kv_heads, head_dim, q_splits, k_splits),
               "work too small");
   XNN_REQUIRE((uintptr_t)work % 16 == 0, "work must be aligned to 16 bytes");

@@ -412,7 +412,7 @@ struct AttentionBackward : Node {
                  dv = at::empty(v.sizes(), v.options());
     size_t need = 0;
     check("xnn_attention_backward_work_size",
-          api.xnn_attention_backward_work_size(q.size(0), (int32_t)q.size(1), (int32_t)k.size(1),
+          api.xnn_attention_backward_work_size(storage_code(q), q.size(0), (int32_t)q.size(1), (int32_t)k.size(1),
                                                (int32_t)q.size(2), &plan->tiles, &need));
     const Tensor work = bytes(q, need);
     const xnn_heads qh = heads_of(q), kh = heads_of(k), vh = heads_of(v);
@@ -464,7 +464,7 @@ Tensor structure_attention(Tensor q, Tensor k, Tensor v, const std::shared_ptr<P
   if (train) lse = at::empty({H, T}, q.options().dtype(at::kFloat));
   size_t need = 0;
   check("xnn_attention_work_size",
-        api.xnn_attention_work_size(T, (int32_t)H, (int32_t)D, &plan->tiles, &need));
+        api.xnn_attention_work_size(code, T, (int32_t)H, (int32_t)D, &plan->tiles, &need));
   if (need > 0) work = bytes(q, need);
   const xnn_heads qh = heads_of(q), kh = heads_of(k), vh = heads_of(v);
   XNN_CALL(xnn_attention, code, &qh, &kh, &vh, T, (int32_t)D, &plan->tiles, (const uint8_t*)data(mask),
