@@ -40,7 +40,7 @@ def test_pytorch_forms_equal_the_definitions():
 
 
 def test_philox_known_answers():
-    """The published test vectors of Philox4x32-10 (Salmon et al., Random123's known answers)."""
+    """The test vectors published with Philox4x32-10 (Salmon, Moraes, Dror and Shaw, SC 2011)."""
     m = 0xFFFFFFFF
     assert R.philox((0,) * 4, (0, 0)) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
     assert R.philox((m,) * 4, (m, m)) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]

@@ -33,7 +33,7 @@ def _close(got, want, bound):
 # --------------------------------------------------------------------------- embedding
 @pytest.mark.parametrize("n,V,C", [(1, 1, 1), (0, 5, 16), (21, 119, 128), (33, 3, 65), (4097, 2, 64),
                                    (700, 70000, 24), (5000, 300, 250), (2500, 1000, 1024),
-                                   (16384, 256, 8), (20000, 1000, 8), (40000, 70000, 3),
+                                   (16384, 256, 8), (20000, 1000, 8), (70000, 300, 4), (40000, 70000, 3),
                                    (3000, 255, 40), (1100000, 4, 4)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_embedding_and_its_gradient(n, V, C, dtype):
@@ -350,6 +350,59 @@ def test_attention_of_far_apart_scores():
     out = xa.structure_attention(q, k, v, plan)
     assert torch.equal(out.detach(), v[-1:].expand_as(v))
     assert (torch.autograd.grad(out.sum(), q)[0] == 0).all()
+
+
+@pytest.mark.parametrize("counts", [[], [0, 0]])
+def test_batches_without_atoms(counts):
+    import xnn_amd as xa
+    plan = xa.attention_plan(torch.tensor(counts, dtype=torch.int64, device=DEV))
+    assert (plan.n_tokens, plan.max_atoms) == (0, 0)
+    q = torch.randn(0, 2, 8, device=DEV, requires_grad=True)
+    out = xa.structure_attention(q, q, q, plan, mask=torch.ones(0, dtype=torch.bool, device=DEV))
+    assert out.shape == (0, 2, 8) and torch.autograd.grad(out.sum(), q)[0].shape == q.shape
+
+
+def test_only_wanted_gradients_are_formed():
+    """Gradients asked for one at a time are those asked for together; an output without a cotangent
+    counts as zeros."""
+    import xnn_amd as xa
+    gen = torch.Generator().manual_seed(8)
+    leaves = [_normal(gen, *s).to(DEV).requires_grad_(True)
+              for s in ((40, 2, 16), (40, 1, 16), (16,), (16,), (40, 8), (40, 8))]
+    grads = [_normal(gen, 40, h, 16).to(DEV) for h in (2, 1)]
+    outs = xa.head_norm_rotate(*leaves)
+    together = torch.autograd.grad(outs, leaves, grads, retain_graph=True)
+    for x, g in zip(leaves, together):
+        assert torch.equal(torch.autograd.grad(outs, x, grads, retain_graph=True)[0], g)
+    alone = torch.autograd.grad(outs[0], leaves[:2], grads[0], retain_graph=True)
+    assert torch.equal(alone[0], together[0]) and (alone[1] == 0).all()
+    v = _normal(gen, 40, 1, 16).to(DEV).requires_grad_(True)
+    out = xa.structure_attention(leaves[0], leaves[1], v, xa.attention_plan(torch.tensor([40], device=DEV)))
+    g = torch.randn_like(out)
+    together = torch.autograd.grad(out, (leaves[0], leaves[1], v), g, retain_graph=True)
+    for x, a in zip((leaves[0], leaves[1], v), together):
+        assert torch.equal(torch.autograd.grad(out, x, g, retain_graph=True)[0], a)
+
+
+def test_dropout_is_differentiable_twice():
+    import xnn_amd as xa
+    x = torch.randn(50, 9, device=DEV, requires_grad=True)
+    y = xa.dropout_add(x, None, 0.4, 11, 3)
+    (g,) = torch.autograd.grad((y ** 2).sum(), x, create_graph=True)
+    (h,) = torch.autograd.grad(g.sum(), x)
+    factor = torch.where(y.detach() != 0, 65536 / (65536 - round(0.4 * 65536)), 0.0)
+    torch.testing.assert_close(h, 2 * factor ** 2, rtol=1e-5, atol=1e-6)
+
+
+def test_forward_mode_and_batched_transforms_are_refused():
+    import torch.autograd.forward_ad as fa
+    import xnn_amd as xa
+    x = torch.randn(4, 8, device=DEV)
+    with fa.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            xa.dropout_add(fa.make_dual(x, torch.ones_like(x)), None, 0.5, 1)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: xa.dropout_add(t, None, 0.5, 1))(x)
 
 
 def test_attention_with_strides_beyond_32_bits():

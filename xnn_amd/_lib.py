@@ -414,17 +414,6 @@ def dtype_code(dtype: torch.dtype) -> int:
     raise TypeError(f"unsupported dtype {dtype} (float32 or float64)")
 
 
-STORAGE = {torch.float32: XNN_F32, torch.bfloat16: XNN_BF16, torch.float16: XNN_F16}
-
-
-def storage_code(dtype: torch.dtype) -> int:
-    """The dtype code of an attention operator's tensors."""
-    try:
-        return STORAGE[dtype]
-    except KeyError:
-        raise TypeError(f"unsupported dtype {dtype} (float32, bfloat16 or float16)") from None
-
-
 class CallCounts(dict):
     """Entry point name -> calls from Python; ``native(name)`` are those from native code."""
 
