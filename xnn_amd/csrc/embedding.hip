@@ -81,6 +81,9 @@ static EmbeddingWork embedding_work(int64_t n, int64_t n_rows, int64_t C) {
 }
 
 // ---------------------------------------------------------------- lookup
+// A thread 16 bytes of a row. Bounded by the rows written where the table stays in the caches: 72,000 rows
+// of 128 in float32 10.8 us, 3.4 TB/s; 16,384 rows of 1,024 in bfloat16 from 50,000 10.6 us, 6.3 TB/s
+// read and written (part of it in the last-level cache).
 template <typename T, int N>
 __global__ __launch_bounds__(256) void embedding_kernel(const int64_t* __restrict__ ids, int64_t n,
                                                         const T* __restrict__ table,
@@ -238,7 +241,9 @@ __global__ __launch_bounds__(256) void clear_kernel(char* __restrict__ p, int64_
   clear16(p, bytes, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
 }
 
-// Blocks below `chunks` sort 1,024 ids each in LDS, one a thread; the others clear the gradient.
+// Blocks below `chunks` sort 1,024 ids each in LDS, one a thread; the others clear the gradient, whose
+// writes bound it where the table is large (50,000 rows of 1,024 in bfloat16: 15.6 us, 6.6 TB/s with the
+// last-level cache; the sort of 16,384 ids alone 7).
 __global__ __launch_bounds__(1024) void sort_chunk_kernel(const int64_t* __restrict__ ids, int n,
                                                           int64_t n_rows, int passes, int chunks,
                                                           uint32_t* __restrict__ key_out,
@@ -310,7 +315,7 @@ __global__ __launch_bounds__(1024) void sort_chunk_kernel(const int64_t* __restr
 
 // The place of every element of the sorted chunks among all: in its own chunk, plus the elements of each
 // other chunk that come before it (equal ones of earlier chunks do), by bisection, `lanes` lanes an
-// element.
+// element. 6.3 us for 16,384 ids: sixteen bisections of ten dependent loads, in parallel lanes.
 __global__ __launch_bounds__(256) void sort_merge_kernel(const uint32_t* __restrict__ key,
                                                          const uint32_t* __restrict__ perm, int n,
                                                          int chunks, int lanes,
@@ -345,7 +350,8 @@ __global__ __launch_bounds__(256) void sort_merge_kernel(const uint32_t* __restr
 // A block's `per` tokens sorted by id (counting, at most sixteen rounds of its four waves), then their
 // runs summed by groups of `lanes` lanes over consecutive sorted positions, N channels a lane. A run
 // within one group's positions goes to part[block][id]; of a run that crosses groups each leaves its
-// sum in LDS and the group where it begins adds them in order.
+// sum in LDS and the group where it begins adds them in order. Bounded by the cotangents it reads, behind
+// the sort of its ids: 72,000 rows of 128 in float32, two ids, 13.8 us, 2.7 TB/s.
 template <typename T, int N>
 __global__ __launch_bounds__(256) void own_sum_kernel(const int64_t* __restrict__ ids, int64_t n,
                                                       int n_rows, int64_t C, int64_t per, int lanes,
@@ -462,7 +468,8 @@ __global__ __launch_bounds__(256) void own_sum_kernel(const int64_t* __restrict_
 }
 
 // A block a row and 64 channels: the sums of the blocks that have seen it, sixteen waves in turn, and
-// theirs in order; zero where none has.
+// theirs in order; zero where none has. 7.6 us for 119 rows of 128 from 282 blocks, bound by the latency
+// of those loads one after the other.
 template <typename T>
 __global__ __launch_bounds__(1024) void own_join_kernel(const uint32_t* __restrict__ seen,
                                                         const float* __restrict__ part, int64_t chunks,
@@ -498,7 +505,8 @@ __global__ __launch_bounds__(1024) void own_join_kernel(const uint32_t* __restri
 // ---------------------------------------------------------------- sums
 // A group of `lanes` lanes sums chunk positions of the sorted order, N channels a lane. A run that
 // lies within the chunk goes to its row; one that goes on in the next chunk leaves its sum in
-// part[chunk][1], one that came from the chunk before in part[chunk][0].
+// part[chunk][1], one that came from the chunk before in part[chunk][0]. Bounded by rows gathered in
+// sorted order: 16,384 rows of 1,024 in bfloat16 13.6 us, 2.5 TB/s read.
 template <typename T, int N>
 __global__ __launch_bounds__(256) void run_sum_kernel(
     const uint32_t* __restrict__ key, const uint32_t* __restrict__ perm, int64_t n, int64_t n_rows,
@@ -550,7 +558,8 @@ __global__ __launch_bounds__(256) void run_sum_kernel(
 }
 
 // The rows whose runs cross chunks: the block of the chunk where a run begins adds what the
-// following chunks left, its four waves in turn, and their sums in order. N channels a lane.
+// following chunks left, its four waves in turn, and their sums in order. N channels a lane. 7.6 us for
+// 512 chunks of 1,024 channels, the longest run 18 % of the tokens; bound by that run.
 template <typename T, int N>
 __global__ __launch_bounds__(256) void run_join_kernel(const uint32_t* __restrict__ key, int64_t n,
                                                        int64_t n_rows, int64_t C, float scale,
