@@ -176,14 +176,13 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kForward)) void attenti
   from = t.begin + from * S::kTile;
   to = min(t.end, t.begin + to * S::kTile);
   Stage<T, S, WAVES * kWave, VEC> next_k, next_v;
-  uint64_t next_keep = 0;
+  uint8_t next_keep = 0;
   next_k.init(a.k_token, a.D);
   next_v.init(a.v_token, a.D);
   const auto fetch = [&](int64_t j0) {
-    const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + j0;
-    next_k.fetch(k + j0 * a.k_token, a.k_token, to - j0, a.D, mask);
-    next_v.fetch(v + j0 * a.v_token, a.v_token, to - j0, a.D, mask);
-    next_keep = live_rows<S::kTile>(j0, to, a.mask, lane);
+    next_keep = row_byte<S::kTile>(j0, to, a.mask, lane);
+    next_k.fetch(k + j0 * a.k_token, a.k_token, to - j0, a.D);
+    next_v.fetch(v + j0 * a.v_token, a.v_token, to - j0, a.D);
   };
   if (from < to) fetch(from);
   Operand<T> q[S::kSteps];
@@ -192,12 +191,12 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kForward)) void attenti
   float top = -INFINITY, sum = 0.0f;                       // the sum over this lane's keys only
   for (int64_t j0 = from; j0 < to; j0 += S::kTile) {
     __syncthreads();
-    next_k.commit(k_tile, a.D);
-    next_v.commit(v_tile, a.D);
-    const uint64_t keep = next_keep;
+    const uint64_t keep = __ballot(next_keep != 0);
+    next_k.commit(k_tile, a.D, keep);
+    next_v.commit(v_tile, a.D, keep);
     __syncthreads();
     if (j0 + S::kTile < to) fetch(j0 + S::kTile);
-    if (!busy) continue;
+    if (!busy || keep == 0) continue;
     f32x16 p[kParts] = {};
 #pragma unroll
     for (int c = 0; c < S::kSteps; ++c)

@@ -44,14 +44,13 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   from = t.begin + from * S::kTile;
   to = min(t.end, t.begin + to * S::kTile);
   Stage<T, S, WAVES * kWave, VEC> next_k, next_v;
-  uint64_t next_keep = 0;
+  uint8_t next_keep = 0;
   next_k.init(a.k_token, a.D);
   next_v.init(a.v_token, a.D);
   const auto fetch = [&](int64_t j0) {
-    const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + j0;
-    next_k.fetch(k + j0 * a.k_token, a.k_token, to - j0, a.D, mask);
-    next_v.fetch(v + j0 * a.v_token, a.v_token, to - j0, a.D, mask);
-    next_keep = live_rows<S::kTile>(j0, to, a.mask, lane);
+    next_keep = row_byte<S::kTile>(j0, to, a.mask, lane);
+    next_k.fetch(k + j0 * a.k_token, a.k_token, to - j0, a.D);
+    next_v.fetch(v + j0 * a.v_token, a.v_token, to - j0, a.D);
   };
   if (from < to) fetch(from);
   Operand<T> q[S::kSteps], g[S::kSteps];
@@ -85,9 +84,9 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   f32x16 dq[S::kBlocks] = {};
   for (int64_t j0 = from; j0 < to; j0 += S::kTile) {
     __syncthreads();
-    next_k.commit(k_tile, a.D);
-    next_v.commit(v_tile, a.D);
-    const uint64_t keep = next_keep;
+    const uint64_t keep = __ballot(next_keep != 0);
+    next_k.commit(k_tile, a.D, keep);
+    next_v.commit(v_tile, a.D, keep);
     __syncthreads();
     if (j0 + S::kTile < to) fetch(j0 + S::kTile);
     if (!busy) continue;
@@ -168,14 +167,15 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   walk_part(per * group, a, t.split, from, to);
   Stage<T, S, WAVES * kWave, VEC> next_q, next_g;
   float next_lse = 0.0f, next_delta = 0.0f;
+  uint64_t next_keep = 0;
   next_q.init(a.q_token, a.D);
   next_g.init(out_stride, a.D);
   const auto fetch = [&](int64_t n) {
     const int h = t.head * group + (int)(n / per);
     const int64_t i0 = t.begin + n % per * S::kTile;
-    next_q.fetch((const T*)a.q + h * a.q_head + i0 * a.q_token, a.q_token, t.end - i0, a.D, nullptr);
-    next_g.fetch((const T*)a.grad + (int64_t)h * a.D + i0 * out_stride, out_stride, t.end - i0, a.D,
-                 nullptr);
+    next_keep = rows_before<S::kTile>(t.end - i0);
+    next_q.fetch((const T*)a.q + h * a.q_head + i0 * a.q_token, a.q_token, t.end - i0, a.D);
+    next_g.fetch((const T*)a.grad + (int64_t)h * a.D + i0 * out_stride, out_stride, t.end - i0, a.D);
     const int64_t i = i0 + threadIdx.x;
     if (threadIdx.x < S::kTile) {
       next_lse = i < t.end ? a.lse[(int64_t)h * a.n_tokens + i] : -INFINITY;
@@ -189,8 +189,8 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   f32x16 dk[S::kBlocks] = {}, dv[S::kBlocks] = {};
   for (int64_t n = from; n < to; ++n) {
     __syncthreads();
-    next_q.commit(q_tile, a.D);
-    next_g.commit(g_tile, a.D);
+    next_q.commit(q_tile, a.D, next_keep);
+    next_g.commit(g_tile, a.D, next_keep);
     if (threadIdx.x < S::kTile) {
       // a row beyond the structure or without keys: every probability is zero
       lse_tile[threadIdx.x] = next_lse == -INFINITY ? INFINITY : next_lse - (float)carry;
