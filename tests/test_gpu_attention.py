@@ -243,6 +243,28 @@ def test_structure_attention(counts, H, K, D, dtype, masked, packed):
         assert torch.equal(xa.structure_attention(*dev, plan, mask=m), out)
 
 
+@pytest.mark.parametrize("runs", [[(0, 64)], [(64, 128), (192, 448)], [(10, 447)], [(0, 447)]])
+@pytest.mark.parametrize("D", [16, 32])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_whole_tiles_that_the_mask_leaves_out(runs, D, dtype):
+    import xnn_amd as xa
+    counts, H, K = [448, 20], 2, 1
+    parts, dev, grad, _ = _attention_inputs(counts, H, K, D, dtype, False, True)
+    mask = torch.ones(sum(counts), dtype=torch.bool)
+    for a, b in runs:
+        mask[a:b] = False
+    *want, bounds = R.attention(*(t.double() for t in parts), counts, mask, None, grad.double())
+    plan = xa.attention_plan(torch.tensor(counts, device=DEV), sum(counts))
+    with torch.no_grad():
+        for t in dev[1:]:                                           # what they hold reaches nothing
+            t[~mask.to(DEV)] = float("nan")
+    out = xa.structure_attention(*dev, plan, mask=mask.to(DEV))
+    got = (out, *torch.autograd.grad(out, dev, grad.to(DEV)))
+    u = UNIT[dtype]
+    for a, b, e in zip(got, want, bounds(EPS, u, 0.0 if dtype == torch.float32 else u)):
+        _close(a, b, e + 1e-30)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("D", [16, 64])
 def test_a_long_structure_loses_no_more_than_short_ones(dtype, D):

@@ -362,6 +362,14 @@ __device__ __forceinline__ uint8_t row_byte(int64_t first, int64_t end, const ui
   return mask == nullptr ? 1 : mask[row];
 }
 
+// Whether the walked row of this lane in register r is among `rows` (a bit a row of a 32-row product): a
+// mask of lanes from two scalar bits, so that the choice costs one vector instruction
+__device__ __forceinline__ bool has_row(uint32_t rows, int r) {
+  const uint32_t low = (uint32_t)((int32_t)(rows << (31 - tile_row(r, 0))) >> 31);
+  const uint32_t high = (uint32_t)((int32_t)(rows << (31 - tile_row(r, 1))) >> 31);
+  return __builtin_amdgcn_inverse_ballot_w64(low | (uint64_t)high << 32);
+}
+
 // a bit a row of a tile with `rows` (at least one) before its end
 template <int ROWS>
 __device__ __forceinline__ uint64_t rows_before(int64_t rows) {

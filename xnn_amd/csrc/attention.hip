@@ -204,12 +204,11 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kForward)) void attenti
       for (int b = 0; b < kParts; ++b)
         mma<T>(natural_operand<T, S>(k_tile, 32 * b + lane % 32, c, half), q[c], p[b]);
     if (keep != (~0ull >> (64 - S::kTile))) {
-      const uint64_t mine = keep >> (4 * half);
 #pragma unroll
       for (int b = 0; b < kParts; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          p[b][r] = (mine >> (32 * b + tile_row(r, 0))) & 1 ? p[b][r] : -INFINITY;
+          p[b][r] = has_row((uint32_t)(keep >> (32 * b)), r) ? p[b][r] : -INFINITY;
     }
     float m = p[0][0];
 #pragma unroll

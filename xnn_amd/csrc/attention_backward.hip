@@ -89,7 +89,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
     next_v.commit(v_tile, a.D, keep);
     __syncthreads();
     if (j0 + S::kTile < to) fetch(j0 + S::kTile);
-    if (!busy) continue;
+    if (!busy || keep == 0) continue;
 #pragma unroll
     for (int b = 0; b < S::kTile / 32; ++b) {
       f32x16 p = {}, dp = {};
@@ -101,9 +101,8 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
 #pragma unroll
       for (int r = 0; r < 16; ++r) p[r] = weight<T>(p[r], scale, lse);
       if (keep != (~0ull >> (64 - S::kTile))) {            // the left out keys' g . v is zero
-        const uint64_t mine = keep >> (32 * b + 4 * half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] = (mine >> tile_row(r, 0)) & 1 ? p[r] : 0.0f;
+        for (int r = 0; r < 16; ++r) p[r] = has_row((uint32_t)(keep >> (32 * b)), r) ? p[r] : 0.0f;
       }
       if (single && b == 0) {
         delta = 0.0f;
