@@ -18,8 +18,8 @@
 // Measured, 24,000 tokens of 16 + 4 heads of 128 in bfloat16: forward 44 us for the
 // 246 MB it reads and writes, the rate of a large copy, which bounds it; backward 80 us for 369 MB, 4.6 TB/s,
 // where loads wait on the two sums of a head before the next head's are issued (asking for the next head's
-// loads first: 196 us against 100, for the registers). 9,000 tokens of 4 + 4 heads of 32 in float32: 6.0
-// and 14 us, the launch and two loads in a row, the tables' and the heads'.
+// loads first: 196 us against 100, for the registers). 9,000 tokens of 4 + 4 heads of 32 in float32: 5.9
+// and 10.4 us, the launch and two loads in a row, the tables' and the heads'.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -86,6 +86,23 @@ __device__ __forceinline__ float lanes_sum(float x, int lanes) {
   if (lanes > 16) x = add_xor16(x);
   if (lanes > 32) x = add_xor32(x);
   return x;
+}
+
+// x[j] += x[j] of lane ^ o for o = from, 2 from, ... below `to` (powers of two), in the vector unit:
+// the backward pass of 9,000 tokens 10.4 us, by shuffles through the LDS unit 12.3
+template <int N>
+__device__ __forceinline__ void add_lanes(float (&x)[N], int from, int to) {
+#define XNN_ADD_LANES(O, SUM)                   \
+  if (from <= O && O < to) {                    \
+    _Pragma("unroll") for (int j = 0; j < N; ++j) x[j] = SUM; \
+  }
+  XNN_ADD_LANES(1, x[j] + dpp_move<0xB1>(x[j]))
+  XNN_ADD_LANES(2, x[j] + dpp_move<0x4E>(x[j]))
+  XNN_ADD_LANES(4, x[j] + dpp_move<0x1B>(dpp_move<0x141>(x[j])))   // the half row mirrored, its quads turned back
+  XNN_ADD_LANES(8, x[j] + dpp_move<0x128>(x[j]))                   // the row turned by half
+  XNN_ADD_LANES(16, add_xor16(x[j]))
+  XNN_ADD_LANES(32, add_xor32(x[j]))
+#undef XNN_ADD_LANES
 }
 
 template <typename T, int N, bool INTER, bool BACK>
@@ -204,13 +221,8 @@ __global__ __launch_bounds__(256, BACK ? 5 : 4) void head_norm_kernel(HeadArgs h
       if (on) store_unit<T, N>((T*)(is_q ? h.q_out : h.k_out) + at, o0, o1, D, x);
     }
     if (BACK && h.d_cos != nullptr) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        for (int o = h.lanes; o < per_token; o <<= 1) {
-          dc[j] += __shfl_xor(dc[j], o);
-          ds[j] += __shfl_xor(ds[j], o);
-        }
-      }
+      add_lanes(dc, h.lanes, per_token);
+      add_lanes(ds, h.lanes, per_token);
       if (live && turned && slot == 0) {
         store_pack<float, N>(h.d_cos + t * (h.R / 2) + u * N, dc);
         store_pack<float, N>(h.d_sin + t * (h.R / 2) + u * N, ds);
@@ -220,14 +232,12 @@ __global__ __launch_bounds__(256, BACK ? 5 : 4) void head_norm_kernel(HeadArgs h
   if (BACK && h.part != nullptr) {
     // the block's sums over tokens and heads: across the lanes of a wave, then its waves in order
     __shared__ float sums[4][2][128];
+    add_lanes(dwq.a, h.lanes, kWave);
+    add_lanes(dwq.b, h.lanes, kWave);
+    add_lanes(dwk.a, h.lanes, kWave);
+    add_lanes(dwk.b, h.lanes, kWave);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      for (int o = h.lanes; o < kWave; o <<= 1) {
-        dwq.a[j] += __shfl_xor(dwq.a[j], o);
-        dwq.b[j] += __shfl_xor(dwq.b[j], o);
-        dwk.a[j] += __shfl_xor(dwk.a[j], o);
-        dwk.b[j] += __shfl_xor(dwk.b[j], o);
-      }
       if (mine && lane < h.lanes) {
         sums[wave][0][o0 + j] = dwq.a[j];
         sums[wave][1][o0 + j] = dwk.a[j];
