@@ -154,7 +154,8 @@ __global__ __launch_bounds__(256) void attention_plan_fill_kernel(
 //     has one or two tiles to walk
 // The next tile is asked for before this one is used and waits in registers. No gain came from two LDS
 // buffers and one barrier a tile, from raised wave priority around the products, or from products of the
-// next tile between the exponentials of this one (float32, 9,000 rows: within 2 %).
+// next tile between the exponentials of this one (24,000 rows in bfloat16, both passes:
+// 3,020-3,117 us against 3,040).
 template <typename T, int DP, int WAVES, int TILE, bool VEC, int WP>
 __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kForward)) void attention_kernel(AttentionArgs a) {
   typedef Head<T, DP, TILE> S;
