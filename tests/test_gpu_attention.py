@@ -243,6 +243,15 @@ def test_structure_attention(counts, H, K, D, dtype, masked, packed):
         assert torch.equal(xa.structure_attention(*dev, plan, mask=m), out)
 
 
+@pytest.mark.parametrize("counts,H,K,D", [
+    ([65], 2, 2, 65), ([33, 129], 2, 1, 72), ([64, 1, 200], 4, 4, 80), ([700], 4, 1, 95),
+    ([31, 60], 1, 1, 96), ([1500, 3], 2, 2, 96), ([129, 300], 2, 2, 97)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("masked,packed", [(False, True), (True, True), (True, False)])
+def test_structure_attention_around_heads_of_96(counts, H, K, D, dtype, masked, packed):
+    test_structure_attention(counts, H, K, D, dtype, masked, packed)
+
+
 @pytest.mark.parametrize("runs", [[(0, 64)], [(64, 128), (192, 448)], [(10, 447)], [(0, 447)]])
 @pytest.mark.parametrize("D", [16, 32])
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -112,16 +112,20 @@ __device__ __forceinline__ void planes_of(float a, float b, uint32_t (&out)[3]) 
   out[2] = upper_halves(a, b);
 }
 
-// Sizes of a head padded to DP elements (16, 32, 64 or 128; zeros beyond the head)
+// Sizes of a head padded to DP elements (16, 32, 64, 96 or 128; zeros beyond the head). Heads of 65 to 96
+// have rows of 128 in LDS, which the threads of a block divide evenly, and products of 96: what stands in a
+// row beyond them is in no product (8,000 rows, 2 heads of 96, both passes: 1,549 us in float32 and 509 in
+// bfloat16, padded to 128 2,252 and 684, the keys' gradients in float32 with spilled registers)
 template <typename T, int DP, int TILE = 64>
 struct Head {
   static constexpr int kPlanes = Store<T>::kPlanes;
   static constexpr int kSteps = DP / 16;                 // operands along the head
   static constexpr int kBlocks = (DP + 31) / 32;         // 32-element blocks of an output
-  static constexpr int kWide = DP;                       // elements of a staged row
+  static constexpr int kHead = DP;
+  static constexpr int kWide = DP == 96 ? 128 : DP;      // elements of a staged row
   static constexpr int kRow = kWide * 2 + 16;            // its bytes in a plane: 16 more spread the banks
   // walked rows of a staged tile: 32 also where three planes of 64 would leave a CU one block
-  static constexpr int kTile = kPlanes == 3 && DP == 128 ? 32 : TILE;
+  static constexpr int kTile = kPlanes == 3 && DP > 64 ? 32 : TILE;
   static constexpr int kPlane = kTile * kRow;
   // waves of a SIMD: two share its matrix core and vector unit where their registers fit
   static constexpr int kOccupancy = DP <= 32 || (kPlanes == 1 && DP == 64) ? 2 : 1;
@@ -282,7 +286,7 @@ struct Stage {
   typedef Pack<T, kPer> Piece;
   static constexpr uint64_t kAll = ~0ull >> (64 - S::kTile);
   Piece x[kCount];
-  bool full;                                               // no elements beyond the head
+  bool full;                                               // no elements beyond the head in its products
   bool near;                                               // full, and a tile spans less than 2 GB
   int row, at;                                             // its first row, its element of a row
   int64_t offset;
@@ -291,7 +295,7 @@ struct Stage {
     row = threadIdx.x / kChunks;
     at = threadIdx.x % kChunks * kPer;
     offset = (row < S::kTile ? row : 0) * stride + (at < D ? at : 0);   // heads of 16: more threads than pieces
-    full = VEC && D == S::kWide;
+    full = VEC && D == S::kHead;
     near = full && stride >= 0 && stride < (int64_t)1 << 22;
   }
   // `tile`: the first of `rows` rows

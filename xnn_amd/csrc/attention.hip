@@ -385,6 +385,8 @@ int xnn_attention(int dtype, const xnn_heads* q, const xnn_heads* k, const xnn_h
       attention_launch<T, 32>(a, rows, fine, s);
     else if (head_dim <= 64)
       attention_launch<T, 64>(a, rows, fine, s);
+    else if (head_dim <= 96)
+      attention_launch<T, 96>(a, rows, fine, s);
     else
       attention_launch<T, 128>(a, rows, fine, s);
   });

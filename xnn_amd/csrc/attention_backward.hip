@@ -138,7 +138,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
 }
 
 // Keys' and values' gradients: four products, with k, v, dk and dv of the wave's rows in registers.
-// Bounded as the forward pass is; float32 heads of 65 to 128 also by 260 bytes a lane that do not fit
+// Bounded as the forward pass is; float32 heads of 97 to 128 also by 260 bytes a lane that do not fit
 // the registers of one wave a SIMD.
 //   24,000 rows, 4 heads of 64, bfloat16: 1,283 us, 920 TFLOP/s, and 18 us of the sums over two parts
 //   9,000 rows, 4 heads of 32, float32: 464 us and 10, 179 TFLOP/s
@@ -369,6 +369,8 @@ int xnn_attention_backward(int dtype, const xnn_heads* q, const xnn_heads* k, co
       attention_backward_launch<T, 32>(a, rows, fine_query, fine, q_splits, k_splits, s);
     else if (head_dim <= 64)
       attention_backward_launch<T, 64>(a, rows, fine_query, fine, q_splits, k_splits, s);
+    else if (head_dim <= 96)
+      attention_backward_launch<T, 96>(a, rows, fine_query, fine, q_splits, k_splits, s);
     else
       attention_backward_launch<T, 128>(a, rows, fine_query, fine, q_splits, k_splits, s);
   });
