@@ -114,7 +114,7 @@ __device__ __forceinline__ void planes_of(float a, float b, uint32_t (&out)[3]) 
 
 // Sizes of a head padded to DP elements (16, 32, 64, 96 or 128; zeros beyond the head). Heads of 65 to 96
 // have rows of 128 in LDS, which the threads of a block divide evenly, and products of 96: what stands in a
-// row beyond them is in no product (8,000 rows, 2 heads of 96, both passes: 1,549 us in float32 and 509 in
+// row beyond them is in no product (8,000 rows, 2 heads of 96, both passes: 1,543 us in float32 and 509 in
 // bfloat16, padded to 128 2,252 and 684, the keys' gradients in float32 with spilled registers)
 template <typename T, int DP, int TILE = 64>
 struct Head {
@@ -274,7 +274,8 @@ __device__ __forceinline__ float max_xor32(float x) {
 // 16 bytes of every kStep-th row. Rows beyond the structure, elements beyond the head and rows that
 // the mask leaves out become zeros as they are written, so that what they hold reaches no sum: no
 // address waits for the mask (24,000 rows of 4 heads with a tenth masked,
-// both passes 4.01 ms where they did, 3.24 so). Loads beyond the structure go to the tile's first row,
+// both passes 4.01 ms where they did, 3.24 so). A thread whose piece is beyond the head reads its row's
+// first one (8,000 rows, 2 heads of 80 in float32, both passes: 1,553 us, with an address a row 1,742). Loads beyond the structure go to the tile's first row,
 // which exists.
 template <typename T, typename S, int THREADS, bool VEC>
 struct Stage {
@@ -287,7 +288,7 @@ struct Stage {
   static constexpr uint64_t kAll = ~0ull >> (64 - S::kTile);
   Piece x[kCount];
   bool full;                                               // no elements beyond the head in its products
-  bool near;                                               // full, and a tile spans less than 2 GB
+  bool near;                                               // 16-byte pieces, and a tile spans less than 2 GB
   int row, at;                                             // its first row, its element of a row
   int64_t offset;
 
@@ -296,7 +297,7 @@ struct Stage {
     at = threadIdx.x % kChunks * kPer;
     offset = (row < S::kTile ? row : 0) * stride + (at < D ? at : 0);   // heads of 16: more threads than pieces
     full = VEC && D == S::kHead;
-    near = full && stride >= 0 && stride < (int64_t)1 << 22;
+    near = VEC && stride >= 0 && stride < (int64_t)1 << 22;
   }
   // `tile`: the first of `rows` rows
   __device__ __forceinline__ void fetch(const T* tile, int64_t stride, int64_t rows, int D) {
@@ -323,7 +324,7 @@ struct Stage {
   // `keep`: a bit a row of the tile
   __device__ __forceinline__ void commit(char* tile, int D, uint64_t keep) {
     if (!full || keep != kAll) {
-      const uint64_t mine = row < S::kTile ? keep >> row : 0;
+      const uint64_t mine = row < S::kTile && at < D ? keep >> row : 0;
 #pragma unroll
       for (int n = 0; n < kCount; ++n) {
         const bool kept = (mine >> (n * kStep)) & 1;
@@ -334,7 +335,7 @@ struct Stage {
         }
         u32x4 w = __builtin_bit_cast(u32x4, x[n]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = kept && at < D ? w[j] : 0u;
+        for (int j = 0; j < 4; ++j) w[j] = kept ? w[j] : 0u;
         x[n] = __builtin_bit_cast(Piece, w);
       }
     }
