@@ -477,6 +477,28 @@ def test_results_do_not_depend_on_the_alignment(shift):
         torch.testing.assert_close(a, b, rtol=2e-5, atol=2e-5)
 
 
+@pytest.mark.parametrize("D", [1, 5, 17, 33, 50, 66, 97, 127])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_what_lies_between_the_heads_reaches_nothing(D, dtype):
+    """Heads of odd sizes and strides with NaN after each: the same bits as without gaps."""
+    import xnn_amd as xa
+    counts = [130, 1, 64, 65]
+    parts, dev, grad, _ = _attention_inputs(counts, 2, 1, D, dtype, False, False)
+    plan = xa.attention_plan(torch.tensor(counts, device=DEV))
+    gaps = []
+    for x in parts:
+        wide = torch.full((*x.shape[:2], D + 9), float("nan"), dtype=dtype, device=DEV)
+        wide[..., :D] = x.to(DEV)
+        gaps.append(wide[..., :D].detach().requires_grad_(True))
+    for mask in (None, torch.arange(sum(counts), device=DEV) % 3 != 0):
+        got = []
+        for qkv in (dev, gaps):
+            out = xa.structure_attention(*qkv, plan, mask=mask)
+            got.append((out, *torch.autograd.grad(out, qkv, grad.to(DEV))))
+        for a, b in zip(*got):
+            assert a.isfinite().all() and torch.equal(a, b)
+
+
 def test_the_operators_repeat_bit_for_bit_on_any_stream():
     import xnn_amd as xa
     gen = torch.Generator().manual_seed(6)

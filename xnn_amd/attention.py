@@ -149,8 +149,10 @@ def structure_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan,
     ``q`` (T, H, D); ``k`` and ``v`` (T, K, D) with ``H`` a multiple of ``K`` (query heads ``h`` read
     head ``h // (H / K)``); ``D <= 128``; tokens and heads may be strided (views of one projection's
     output). ``plan`` from :func:`attention_plan`. ``mask`` (T,), bool: atoms that may be attended
-    to (None: all); an atom that is masked out reaches no other, whatever its values, and gets zero
-    key and value gradients; atoms with nothing to attend to get zeros. ``scale``: ``D ** -0.5``
-    by default, positive. Returns (T, H, D). Neither scores nor probabilities are stored; the backward
+    to (None: all); an atom that is masked out reaches no other through its key and value, whatever they
+    hold, and gets zero gradients of them; atoms with nothing to attend to get zeros. ``scale``: ``D ** -0.5``
+    by default, positive. A masked atom's own row is computed as any other: where its query is not
+    finite, neither are its output and, through its row's gradient, those of its structure's keys.
+    Returns (T, H, D). Neither scores nor probabilities are stored; the backward
     pass forms them again from the rows' log-sums."""
     return (_native or _ops()).structure_attention(q, k, v, plan.native, mask, scale)
