@@ -61,8 +61,13 @@ def split_dispersion(model: nn.Module) -> Tuple[Optional[nn.Module], List[nn.Mod
 
 
 def _sh_pair_supported(core: nn.Module) -> bool:
-    from .models import ShEdgePotential
-    return (isinstance(core, ShEdgePotential)
+    """Whether the fused call evaluates ``core``: the edge potential's own energy, not that of a model
+    that builds on it, with the (C, (l_max+1)^2) readout that the kernel indexes."""
+    from .models import ShEdgePotential as Edge
+    cls = type(core)
+    return (isinstance(core, Edge) and cls.forward is Edge.forward and cls.messages is Edge.messages
+            and cls.aggregate_energy is Edge.aggregate_energy
+            and tuple(core.U.shape) == (core.W.shape[1], (core.l_max + 1) ** 2)
             and linear_message_supported(core.W.shape[0], core.W.shape[1], core.l_max)
             and not getattr(core.edge_feat, "radial_trainable", False))
 
