@@ -329,6 +329,10 @@ def load() -> ctypes.CDLL:
             fn.restype = _RESTYPES.get(name, ctypes.c_int)
         if lib.xnn_abi_version() != ABI_VERSION:
             raise RuntimeError(f"{LIBRARY} has ABI {lib.xnn_abi_version()}, expected {ABI_VERSION}")
+        # Its thread-local message, read once: until a thread reads the thread-local data of the library
+        # loaded last, glibc before 2.39 looks up every other library's the slow way (torch's included:
+        # 0.25 us more an allocation, 0.5 a launch)
+        lib.xnn_last_error()
         _lib = lib
         return lib
 

@@ -15,7 +15,9 @@ They take GPU tensors of float32, bfloat16 or float16 (arithmetic and sums in fl
 output rounded once) and raise on any other; there is no fallback. They run on the
 current stream without host reads (:func:`attention_plan` makes one), every sum has a fixed
 order, and the kernels may be captured in a HIP graph. Checks, autograd and launches are native code
-(``csrc/attention_ops.cpp``). :func:`embedding` and :func:`dropout_add`
+(``csrc/attention_ops.cpp``), registered as operators (``torch.ops.xnn_amd``) with a form for shapes
+alone, so that tracers, fake tensors and compilers record them. They have no forward-mode derivative and
+no batching rule (``vmap``), and raise there. :func:`embedding` and :func:`dropout_add`
 are differentiable to any order, the other two once. The per-edge reference path has no
 counterpart.
 """
@@ -27,29 +29,39 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.compiler import is_compiling
 
 from . import _lib
 
-_native = None
+_native, _failure = None, None
+try:
+    # registers the operators (torch.ops.xnn_amd) with their shapes and derivatives
+    from . import _attention_ops as _built
+    _built.set_library(os.path.abspath(_lib.LIBRARY))
+    _lib.calls.native = _built.calls
+except (ImportError, AttributeError) as err:     # not built, or from other sources: the first call says so
+    _built, _failure = None, err
 
 
 def _ops():
-    """The native autograd functions, opened on first use (raises when they are not built)."""
+    """The native operators, checked on first use (raises when they are not built)."""
     global _native
     if _native is None:
         _lib.load()
-        try:
-            from . import _attention_ops as ops
-        except ImportError as err:
-            raise RuntimeError("xnn_amd/_attention_ops.so is missing or does not load: build it with "
-                               "`python -m xnn_amd.build` (the kernels have no fallback)") from err
-        ops.load(os.path.abspath(_lib.LIBRARY))
-        _lib.calls.native = ops.calls
-        _native = ops
+        if _built is None:
+            raise RuntimeError("xnn_amd/_attention_ops.so is missing, old or does not load: build it with "
+                               "`python -m xnn_amd.build` (the kernels have no fallback)") from _failure
+        _native = _built
     return _native
 
 
 _U64 = (1 << 64) - 1
+
+
+def _signed(x: int) -> int:
+    """The low 64 bits of ``x`` as a signed integer."""
+    x = int(x) & _U64
+    return x - (1 << 64) if x >> 63 else x
 
 
 def embedding(ids: Tensor, table: Tensor, scale: float = 1.0) -> Tensor:
@@ -58,6 +70,8 @@ def embedding(ids: Tensor, table: Tensor, scale: float = 1.0) -> Tensor:
     ``ids`` of any integer type; one outside the table gives a row of NaN and counts in no
     gradient. The gradient of the table sorts the ids and sums each row's tokens in their order
     (float32, rounded once), the same bits at every call."""
+    if is_compiling():               # a compiler cannot look into the native entry: the same operator by name
+        return torch.ops.xnn_amd.embedding_rows(ids, table, scale)
     return (_native or _ops()).embedding(ids, table, scale)
 
 
@@ -75,6 +89,8 @@ def dropout_add(x: Tensor, residual: Optional[Tensor], p: float, seed: int,
     counter = None
     if isinstance(offset, Tensor):
         counter, offset = offset, 0
+    if is_compiling():
+        return torch.ops.xnn_amd.dropout_add(x, residual, p, _signed(seed), _signed(offset), counter)
     return (_native or _ops()).dropout_add(x, residual, p, int(seed) & _U64, int(offset) & _U64, counter)
 
 
@@ -89,6 +105,9 @@ def head_norm_rotate(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, c
     Token ``t`` takes row ``positions[t]`` of the tables (one outside gives NaN), or row ``t`` when
     ``positions`` is None; only then do the tables have gradients (phases that depend on the
     geometry lead to forces). Tokens and heads may be strided (views of one projection's output)."""
+    if is_compiling():
+        return torch.ops.xnn_amd.head_norm_rotate(q, k, q_weight, k_weight, cos, sin, positions, eps,
+                                                  interleaved)
     return (_native or _ops()).head_norm_rotate(q, k, q_weight, k_weight, cos, sin, positions, eps,
                                                 interleaved)
 
@@ -155,4 +174,7 @@ def structure_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan,
     finite, neither are its output and, through its row's gradient, those of its structure's keys.
     Returns (T, H, D). Neither scores nor probabilities are stored; the backward
     pass forms them again from the rows' log-sums."""
+    if is_compiling():
+        return torch.ops.xnn_amd.structure_attention(q, k, v, plan.tiles32, plan.tiles128, mask,
+                                                     plan.n_tokens, plan.max_atoms, scale)
     return (_native or _ops()).structure_attention(q, k, v, plan.native, mask, scale)
