@@ -8,7 +8,7 @@ to any order (``use_fast=False``, a CPU, float64, or a training step on forces).
 from __future__ import annotations
 
 import math
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Union
 
 import torch
 from torch import Tensor, nn
@@ -24,11 +24,14 @@ def _takes(device: torch.device, dtype: torch.dtype) -> bool:
 
 
 # --------------------------------------------------------------------------- PyTorch forms
-def dropout_keep(shape, p: float, seed: int, offset: int, device) -> Tensor:
+def dropout_keep(shape, p: float, seed: int, offset: Union[int, Tensor], device) -> Tensor:
     """The mask of :func:`~xnn_amd.attention.dropout_add`, bool of ``shape``."""
     m, n = 0xFFFFFFFF, math.prod(shape)
     i = torch.arange((n + 7) // 8, device=device)
-    c = [i & m, i >> 32, torch.full_like(i, offset & m), torch.full_like(i, (offset >> 32) & m)]
+
+    def words(x):
+        return x.to(device).reshape(1).expand_as(i) if isinstance(x, Tensor) else torch.full_like(i, x)
+    c = [i & m, i >> 32, words(offset & m), words((offset >> 32) & m)]
     k = [seed & m, (seed >> 32) & m]
     for _ in range(10):
         # 64-bit products in int64: the shifts' sign bits are masked away
@@ -40,7 +43,8 @@ def dropout_keep(shape, p: float, seed: int, offset: int, device) -> Tensor:
     return (draws >= int(round(65536 * p))).view(shape)
 
 
-def dropout_add_torch(x: Tensor, residual: Tensor, p: float, seed: int, offset: int) -> Tensor:
+def dropout_add_torch(x: Tensor, residual: Tensor, p: float, seed: int,
+                      offset: Union[int, Tensor]) -> Tensor:
     drop = int(round(65536 * p))
     keep = dropout_keep(x.shape, p, seed, offset, x.device)
     factor = 65536.0 / (65536 - drop) if drop < 65536 else 0.0
@@ -103,8 +107,11 @@ class AtomAttention(nn.Module, FastPathModule):
     """``x + dropout(W_o attention(rotate(norm(q)), rotate(norm(k)), v))`` with ``q, k, v = W x``.
 
     The heads of queries and keys are normalized and rotated by each atom's phases; an atom attends to
-    the atoms of its structure. In training mode the dropout of call ``n`` draws with counter
-    ``n`` (:attr:`calls`) and the module's ``seed``."""
+    the atoms of its structure. In training mode the dropout of call ``n`` draws with counter ``n``
+    (:attr:`calls`, kept in the state dict: a resumed run goes on with the next one) and the module's
+    ``seed``. A call that is given its ``offset`` draws with that one and leaves the counter alone:
+    what is computed again in the backward pass (``torch.utils.checkpoint``) needs it, since the
+    counter is by then another call's, and raises without."""
 
     def __init__(self, channels: int, heads: int, kv_heads: Optional[int] = None,
                  dropout: float = 0.0, seed: int = 0, eps: float = 1e-6,
@@ -128,10 +135,34 @@ class AtomAttention(nn.Module, FastPathModule):
     def fast_supported(self, device: torch.device, dtype: torch.dtype) -> bool:
         return _takes(device, dtype) and self.head_dim <= 128
 
+    def get_extra_state(self) -> Tensor:
+        return torch.tensor(self.calls)
+
+    def set_extra_state(self, state: Tensor) -> None:
+        self.calls = int(state)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys,
+                              unexpected_keys, error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys,
+                                      unexpected_keys, error_msgs)
+        # a state that was saved without the counter leaves it as it is
+        key = prefix + "_extra_state"
+        if key in missing_keys:
+            missing_keys.remove(key)
+
+    def _next_offset(self) -> int:
+        if torch._C._current_graph_task_id() != -1:
+            raise RuntimeError("the dropout of a block that is computed again in a backward pass (activation "
+                               "checkpointing) would draw another mask: call it with its offset")
+        self.calls += 1
+        return self.calls
+
     def forward(self, x: Tensor, cos: Tensor, sin: Tensor, n_atoms: Tensor,
-                plan: Optional[AttentionPlan] = None, param_grads: bool = True) -> Tensor:
+                plan: Optional[AttentionPlan] = None, param_grads: bool = True,
+                offset: Union[None, int, Tensor] = None) -> Tensor:
         """``x`` (N, channels), the phases' cosines and sines (N, R/2), ``n_atoms`` (B,); ``plan``
-        of ``n_atoms`` for the kernels (made here when None)."""
+        of ``n_atoms`` for the kernels (made here when None); ``offset`` of the dropout's draws, an
+        integer or an int64 tensor of one element (None: the next of :attr:`calls`)."""
         n, H, K, D = x.shape[0], self.heads, self.kv_heads, self.head_dim
         q_weight, k_weight = self.q_weight.to(x.dtype), self.k_weight.to(x.dtype)
         if not param_grads:
@@ -149,9 +180,9 @@ class AtomAttention(nn.Module, FastPathModule):
         y = y.reshape(n, H * D) @ self.out.to(x.dtype)
         if not self.training or self.dropout == 0.0:
             return x + y
-        self.calls += 1
+        offset = self._next_offset() if offset is None else offset
         add = dropout_add if self.fast_active else dropout_add_torch
-        return add(y, x, self.dropout, self.seed, self.calls)
+        return add(y, x, self.dropout, self.seed, offset)
 
 
 @register_model("atom_attention")
@@ -165,19 +196,27 @@ class AtomAttentionPotential(ShEdgePotential):
     ``E_i = <U, x_i> + atom_ref[Z_i]``. All geometry enters through the edge vectors: forces and
     stress come from the edge backward. ``use_fast=False``, a CPU or a training step on forces
     (``create_graph=True``) takes the PyTorch formulation.
+
+    Block ``i`` draws its dropout with key ``(i, dropout_seed)``; ``dropout_seed`` is ``seed`` by default
+    (of no ``seed``, that of torch's generator). Data-parallel ranks that are to draw different
+    masks from the same weights take different ones.
     """
 
     def __init__(self, species: Sequence[int] = (1, 6, 7, 8), n_rbf: int = 8, l_max: int = 3,
                  channels: int = 128, cutoff: float = 5.0, heads: int = 4,
                  kv_heads: Optional[int] = None, layers: int = 2, dropout: float = 0.0,
-                 embedding_scale: float = 1.0, seed: Optional[int] = 0, **kwargs):
+                 embedding_scale: float = 1.0, seed: Optional[int] = 0,
+                 dropout_seed: Optional[int] = None, **kwargs):
         super().__init__(species=species, n_rbf=n_rbf, l_max=l_max, channels=channels,
                          cutoff=cutoff, seed=seed, **kwargs)
         gen = torch.Generator().manual_seed(seed + 1) if seed is not None else None
         n_inv = channels * (l_max + 1)
         self.embed = SpeciesEmbedding(max(species) + 1, channels, embedding_scale, gen)
+        if dropout_seed is None:
+            dropout_seed = torch.initial_seed() if seed is None else seed
         self.blocks = nn.ModuleList(
-            AtomAttention(channels, heads, kv_heads, dropout, seed=i, generator=gen)
+            AtomAttention(channels, heads, kv_heads, dropout, seed=(int(dropout_seed) & 0xFFFFFFFF) << 32 | i,
+                          generator=gen)
             for i in range(layers))
         self.mix = nn.Parameter(torch.randn(n_inv, channels, generator=gen) / n_inv ** 0.5)
         half = self.blocks[0].head_dim // 2 if layers else 0
@@ -186,7 +225,8 @@ class AtomAttentionPotential(ShEdgePotential):
         orders = torch.cat([torch.full((2 * l + 1,), l) for l in range(l_max + 1)])
         self.register_buffer("per_order", torch.nn.functional.one_hot(orders).float())
 
-    def forward(self, data) -> dict:
+    def forward(self, data, offset: Union[None, int, Tensor] = None) -> dict:
+        """``offset``: of the blocks' dropout (:class:`AtomAttention`)."""
         dtype = data.model_dtype
         select(fast_modules(self), self.use_fast, MI355X_POLICY, data.pos.device, dtype,
                data.num_edges, double_backward=self.double_backward)
@@ -201,7 +241,7 @@ class AtomAttentionPotential(ShEdgePotential):
         if self.blocks and self.blocks[0].fast_active:
             plan = attention_plan(data.n_atoms, data.num_nodes)
         for block in self.blocks:
-            x = block(x, cos, sin, data.n_atoms, plan, self.param_grads)
+            x = block(x, cos, sin, data.n_atoms, plan, self.param_grads, offset)
         ref = self.atom_ref.to(x.dtype)
         if x.is_cuda and self.embed.fast_active:
             from .ops import node_readout_op
