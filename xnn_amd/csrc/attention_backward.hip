@@ -82,6 +82,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   // lost in its rounding, much beside the differences of two or three keys, is not in it.
   const bool single = t.end - t.begin <= 32;
   f32x16 dq[S::kBlocks] = {};
+  GradientRange<T> range;
   for (int64_t j0 = from; j0 < to; j0 += S::kTile) {
     __syncthreads();
     const uint64_t keep = __ballot(next_keep != 0);
@@ -112,6 +113,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) p[r] *= dp[r] - delta;
+      range.hold(p, dq);
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
         const auto w = weight_operand<T, WP>(p, f);
@@ -131,10 +133,10 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   }
   const int64_t at = (row * a.heads + t.head) * a.D;
   if (a.splits > 1)
-    store_own(a.part + (int64_t)t.split * a.n_tokens * a.heads * a.D + at, dq, factor, a.D,
+    store_own(a.part + (int64_t)t.split * a.n_tokens * a.heads * a.D + at, dq, factor * range.back(), a.D,
               a.D % 4 == 0, half);
   else
-    store_own((T*)a.dq + at, dq, factor, a.D, a.vec_out, half);
+    store_own((T*)a.dq + at, dq, factor * range.back(), a.D, a.vec_out, half);
 }
 
 // Keys' and values' gradients: four products, with k, v, dk and dv of the wave's rows in registers.
@@ -186,6 +188,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
   load_own<T, DP, VEC>((const T*)a.k + t.head * a.k_head, a.k_token, key, kept, a.D, half, scale, k);
   load_own<T, DP, VEC>((const T*)a.v + t.head * a.v_head, a.v_token, key, kept, a.D, half, 1.0f, v);
   f32x16 dk[S::kBlocks] = {}, dv[S::kBlocks] = {};
+  GradientRange<T> range;
   for (int64_t n = from; n < to; ++n) {
     __syncthreads();
     next_q.commit(q_tile, a.D, next_keep);
@@ -217,6 +220,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
           dp[r] = p[r] * (dp[r] - d[j]);
         }
       }
+      range.hold(dp, dk);
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
         const auto w = weight_operand<T, WP>(p, f);
@@ -237,7 +241,7 @@ __global__ __launch_bounds__(WAVES* kWave, (Head<T, DP>::kOccupancy)) void atten
       for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.0f;
   }
   const int64_t at = (key * a.kv_heads + t.head) * a.D;
-  const float k_factor = ldexpf(a.scale, -carry), v_factor = ldexpf(1.0f, -carry);
+  const float k_factor = ldexpf(a.scale, -carry) * range.back(), v_factor = ldexpf(1.0f, -carry);
   if (a.splits > 1) {
     const int64_t one = a.n_tokens * a.kv_heads * a.D;
     store_own(a.part + t.split * one + at, dk, k_factor, a.D, a.D % 4 == 0, half);
