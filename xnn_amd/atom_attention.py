@@ -164,20 +164,21 @@ class AtomAttention(nn.Module, FastPathModule):
         of ``n_atoms`` for the kernels (made here when None); ``offset`` of the dropout's draws, an
         integer or an int64 tensor of one element (None: the next of :attr:`calls`)."""
         n, H, K, D = x.shape[0], self.heads, self.kv_heads, self.head_dim
-        q_weight, k_weight = self.q_weight.to(x.dtype), self.k_weight.to(x.dtype)
+        # under autocast the projections are of its type, in which the heads go on; x keeps its own
+        q, k, v = (x @ self.qkv.to(x.dtype)).view(n, H + 2 * K, D).split([H, K, K], 1)
+        q_weight, k_weight = self.q_weight.to(q.dtype), self.k_weight.to(q.dtype)
         if not param_grads:
             q_weight, k_weight = q_weight.detach(), k_weight.detach()
-        q, k, v = (x @ self.qkv.to(x.dtype)).view(n, H + 2 * K, D).split([H, K, K], 1)
         if self.fast_active:
             q, k = head_norm_rotate(q, k, q_weight, k_weight, cos.float(), sin.float(),
                                     eps=self.eps)
             plan = attention_plan(n_atoms, n) if plan is None else plan
             y = structure_attention(q, k, v, plan)
         else:
-            q, k = (head_norm_rotate_torch(t, w, cos.to(x.dtype), sin.to(x.dtype), self.eps)
+            q, k = (head_norm_rotate_torch(t, w, cos.to(t.dtype), sin.to(t.dtype), self.eps)
                     for t, w in ((q, q_weight), (k, k_weight)))
             y = structure_attention_torch(q, k, v, n_atoms)
-        y = y.reshape(n, H * D) @ self.out.to(x.dtype)
+        y = (y.reshape(n, H * D) @ self.out.to(y.dtype)).to(x.dtype)
         if not self.training or self.dropout == 0.0:
             return x + y
         offset = self._next_offset() if offset is None else offset
