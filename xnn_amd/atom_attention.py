@@ -240,7 +240,7 @@ class AtomAttentionPotential(ShEdgePotential):
         cos, sin = torch.cos(angle), torch.sin(angle)
         plan = None
         if self.blocks and self.blocks[0].fast_active:
-            plan = attention_plan(data.n_atoms, data.num_nodes)
+            plan = data.attention_plan()                   # one host read a graph, not a step
         for block in self.blocks:
             x = block(x, cos, sin, data.n_atoms, plan, self.param_grads, offset)
         ref = self.atom_ref.to(x.dtype)

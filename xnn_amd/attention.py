@@ -161,6 +161,20 @@ def attention_plan(n_atoms: Tensor, n_tokens: Optional[int] = None) -> Attention
                          lists[1][:3 * n128].view(-1, 3), ptr)
 
 
+def plan_for(graph) -> AttentionPlan:
+    """The cached plan of an :class:`~xnn_amd.data.AtomicGraph` (made again when ``n_atoms`` is another tensor
+    or was written to, or the number of atoms changes)."""
+    n_atoms = graph.n_atoms
+    version = None if n_atoms.is_inference() else n_atoms._version
+    key = (version, graph.num_nodes)
+    cached = getattr(graph, "_xnn_attention_plan", None)
+    if cached is not None and cached[0] is n_atoms and cached[1] == key:
+        return cached[2]
+    plan = attention_plan(n_atoms, graph.num_nodes)
+    object.__setattr__(graph, "_xnn_attention_plan", (n_atoms, key, plan))
+    return plan
+
+
 def structure_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan,
                         mask: Optional[Tensor] = None, scale: Optional[float] = None) -> Tensor:
     """``softmax(scale q k^T) v`` of every atom over the atoms of its structure.

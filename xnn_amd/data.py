@@ -139,6 +139,11 @@ class AtomicGraph:
         from .plan import plan_for
         return plan_for(self)
 
+    def attention_plan(self):
+        """The cached :class:`~xnn_amd.attention.AttentionPlan` of this graph (GPU only)."""
+        from .attention import plan_for
+        return plan_for(self)
+
     def edge_vectors(self) -> Tensor:
         """``pos[dst] - pos[src] + cell_shift @ cell`` per edge, in :attr:`model_dtype`,
         differentiable with respect to ``pos`` and ``cell`` (atomic_data.py:371-418)."""
