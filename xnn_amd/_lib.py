@@ -8,7 +8,8 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
-from typing import Optional
+from collections.abc import MutableMapping
+from typing import Callable, Dict, Optional, Tuple
 
 import torch
 
@@ -418,25 +419,53 @@ def dtype_code(dtype: torch.dtype) -> int:
     raise TypeError(f"unsupported dtype {dtype} (float32 or float64)")
 
 
-class CallCounts(dict):
-    """Entry point name -> calls from Python; ``native(name)`` are those from native code."""
+class CallCounts(MutableMapping):
+    """Entry point name -> its calls, from Python and from native code (:meth:`join`) together; names that were
+    not called are not in it."""
 
-    native = None
+    def __init__(self):
+        self.python: Dict[str, int] = {}
+        self._names: Tuple[str, ...] = ()
+        self._native: Callable[[str], int] = lambda name: 0
 
-    def get(self, name, default=None):
-        mine = super().get(name)
-        if self.native is None:
-            return default if mine is None else mine
-        theirs = self.native(name)
-        return theirs + mine if mine is not None else theirs or default
+    def join(self, names, native) -> None:
+        """``native(name)`` are the calls of each of ``names`` that native code counts."""
+        self._names, self._native = tuple(names), native
+
+    def __getitem__(self, name: str) -> int:
+        n = self.python.get(name, 0) + self._native(name)
+        if n == 0:
+            raise KeyError(name)
+        return n
+
+    def __setitem__(self, name: str, n: int) -> None:
+        self.python[name] = n - self._native(name)
+
+    def __delitem__(self, name: str) -> None:
+        self[name]
+        self[name] = 0
+
+    def __iter__(self):
+        return iter([n for n in {**self.python, **dict.fromkeys(self._names)} if n in self])
+
+    def __len__(self) -> int:
+        return sum(1 for _ in self)
+
+    def clear(self) -> None:
+        self.python.clear()
+        for name in self._names:
+            self[name] = 0
+
+    def __repr__(self) -> str:
+        return repr(dict(self))
 
 
-calls: dict = CallCounts()
+calls = CallCounts()
 
 
 def count_call(name: str) -> None:
     """Record that a HIP entry point ran (tests assert the native path was taken)."""
-    calls[name] = calls.get(name, 0) + 1
+    calls.python[name] = calls.python.get(name, 0) + 1
 
 
 def virial_reduce(partial: torch.Tensor, n_rows: int, seg_ptr: torch.Tensor, n_graphs: int,

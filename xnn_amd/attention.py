@@ -38,7 +38,7 @@ try:
     # registers the operators (torch.ops.xnn_amd) with their shapes and derivatives
     from . import _attention_ops as _built
     _built.set_library(os.path.abspath(_lib.LIBRARY))
-    _lib.calls.native = _built.calls
+    _lib.calls.join(_built.entries(), _built.calls)
 except (ImportError, AttributeError) as err:     # not built, or from other sources: the first call says so
     _built, _failure = None, err
 

@@ -73,6 +73,11 @@ int64_t calls(const std::string& name) {
   return 0;
 }
 
+std::vector<std::string> entries() {
+#define XNN_NAME(entry) #entry,
+  return {XNN_ENTRIES(XNN_NAME)};
+}
+
 void check(const char* name, int status) {
   if (status == XNN_OK) return;
   TORCH_CHECK_VALUE(status != XNN_EINVAL, name, ": ", api.xnn_last_error());
@@ -886,6 +891,7 @@ Tensor structure_attention_entry(const Tensor& q, const Tensor& k, const Tensor&
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   namespace py = pybind11;
   m.def("set_library", [](const std::string& path) { library = path; });
+  m.def("entries", &entries);
   m.def("calls", &calls);
   m.def("embedding", &embedding_entry);
   m.def("dropout_add", &dropout_entry);
