@@ -40,6 +40,18 @@ def test_a_graph_has_one_plan_until_its_structures_change():
         g.attention_plan()
 
 
+def test_a_graph_is_copied_and_pickled_with_its_plan():
+    import pickle
+    g = _graph()
+    plan = g.attention_plan()
+    q = torch.randn(g.num_nodes, 2, 16, device=DEV)
+    want = xa.structure_attention(q, q, q, plan)
+    for other in (copy.deepcopy(g), pickle.loads(pickle.dumps(g))):
+        again = other.attention_plan()
+        assert again is not plan and torch.equal(again.tiles32, plan.tiles32)
+        assert torch.equal(xa.structure_attention(q, q, q, again), want)
+
+
 def test_a_step_of_the_model_reads_nothing_on_the_host():
     g = _graph()
     wrapped = xa.ForceStressOutput(xa.AtomAttentionPotential(channels=32, heads=4, cutoff=4.0).to(DEV)).eval()

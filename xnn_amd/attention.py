@@ -125,6 +125,14 @@ class AttentionPlan:
     def __post_init__(self):
         self.native = _ops().Plan(self.n_tokens, self.max_atoms, self.tiles32, self.tiles128)
 
+    # a graph that keeps its plan is copied and pickled with it
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "native"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self.__post_init__()
+
 
 def attention_plan(n_atoms: Tensor, n_tokens: Optional[int] = None) -> AttentionPlan:
     """The plan of structures with ``n_atoms`` (B,) consecutive atoms each (a graph's
