@@ -120,7 +120,7 @@ class AttentionPlan:
     max_atoms: int
     tiles32: Tensor                  # (tiles, 3) int32: first row, end and begin of its structure
     tiles128: Tensor
-    ptr: Tensor                      # (B + 1,) int64
+    ptr: Tensor                      # (B + 1,) int64: where each structure's atoms begin
 
     def __post_init__(self):
         self.native = _ops().Plan(self.n_tokens, self.max_atoms, self.tiles32, self.tiles128)
@@ -135,9 +135,10 @@ class AttentionPlan:
 
 
 def attention_plan(n_atoms: Tensor, n_tokens: Optional[int] = None) -> AttentionPlan:
-    """The plan of structures with ``n_atoms`` (B,) consecutive atoms each (a graph's
-    ``n_atoms``), kept as long as the batch: two launches and one host read (of the checks and
-    sizes). ``n_tokens``: the atoms of the batch, read from the sum where it is not given.
+    """The plan of structures with ``n_atoms`` (B,) consecutive atoms each, kept as long as the
+    batch (:meth:`~xnn_amd.data.AtomicGraph.attention_plan` keeps it with the graph): two launches and
+    one host read, of the checks and sizes. ``n_tokens``: the atoms of the batch; where it is not
+    given their sum is read as well.
 
     Raises ``ValueError`` for negative counts or counts that do not sum to ``n_tokens``."""
     device = n_atoms.device
@@ -195,7 +196,14 @@ def structure_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan,
     by default, positive. A masked atom's own row is computed as any other: where its query is not
     finite, neither are its output and, through its row's gradient, those of its structure's keys.
     Returns (T, H, D). Neither scores nor probabilities are stored; the backward
-    pass forms them again from the rows' log-sums."""
+    pass forms them again from the rows' log-sums.
+
+    Scores, softmax statistics and all sums are float32. float32 operands enter the products as three
+    planes of 8 bits: a key or value that is not finite and not masked makes its structure's rows NaN,
+    also where its weight would be zero. In 16 bits probabilities and score gradients are rounded to the
+    type between the two products, with their rounding errors as a second term where the batch has few
+    scores (``T * H * max_atoms`` up to 2^23), and the backward pass takes the rows' ``g . out``
+    from the stored output in structures of more than 32 atoms."""
     if is_compiling():
         return torch.ops.xnn_amd.structure_attention(q, k, v, plan.tiles32, plan.tiles128, mask,
                                                      plan.n_tokens, plan.max_atoms, scale)

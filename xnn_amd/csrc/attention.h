@@ -628,10 +628,10 @@ inline int attention_args(AttentionArgs& a, int dtype, const xnn_heads* q, const
           (a.q_token | a.q_head | a.k_token | a.k_head | a.v_token | a.v_head) % per == 0 &&
           head_dim % per == 0;
   // Keys and values of all heads of a structure within half an XCD's 4 MB of L2: its heads side by side,
-  // which share the lines of packed projections and spread the longest structures (64 of 10 to 1,000 atoms,
-  // 8 heads of 64 in 16 bits: 33 us forward, one head after the other 42). Otherwise one head after the
-  // other (24,000 atoms, 16 heads of 64 on 4, both passes: 11.25 ms, side by side 11.2 to 11.7; 3 heads 2.28
-  // and 2.30).
+  // which spreads the longest structures over the chip (64 of 10 to 1,000 atoms, 8 heads of 64 in 16 bits: 33 us
+  // forward, one head after the other 42; neighbouring blocks are on different XCDs, so that each fetches the
+  // lines of packed projections for itself, 40.6 MB for 20.2). Otherwise one head after the other (24,000 atoms, 16
+  // heads of 64 on 4, both passes: 11.25 ms, side by side 11.2 to 11.7; 3 heads 2.28 and 2.30).
   a.head_major = plan->max_atoms * a.kv_heads * head_dim * storage_bytes(dtype) * 2 > (2 << 20);
   return XNN_OK;
 }
