@@ -449,9 +449,10 @@ __device__ __forceinline__ void block_tile(const AttentionArgs& a, int heads, Ti
     t.split = (int)(slot % a.splits);
     tile = slot / a.splits;
   }
-  t.first = a.tiles[3 * tile];
-  t.end = a.tiles[3 * tile + 1];
-  t.begin = a.tiles[3 * tile + 2];
+  // a tile that is not of these tokens reads and writes none outside them
+  t.first = max(a.tiles[3 * tile], 0);
+  t.end = min((int64_t)a.tiles[3 * tile + 1], a.n_tokens);
+  t.begin = max(a.tiles[3 * tile + 2], 0);
 }
 
 // part `split` of `n` walked tiles: [from, to)
