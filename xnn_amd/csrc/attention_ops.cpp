@@ -167,28 +167,6 @@ Tensor as_int64(const Tensor& t) {
   return (t.scalar_type() == at::kLong ? t : t.to(at::kLong)).contiguous();
 }
 
-// Whether an operator below its derivative is its kernel alone: tensors of GPU memory, and no tracer, mode, wrapper
-// or transform that would take part. A step of the dispatcher costs 0.3 to 0.5 us of a call of 5.3 to 5.8.
-bool kernel_alone(std::initializer_list<const Tensor*> ts) {
-  if (c10::impl::tls_local_dispatch_key_set().included_ != c10::default_included_set) return false;
-  const c10::DispatchKeySet memory = c10::DispatchKeySet(c10::DispatchKey::CUDA) |
-                                     c10::getAutocastRelatedKeySetFromBackend(c10::BackendComponent::CUDABit) |
-                                     c10::getAutogradRelatedKeySetFromBackend(c10::BackendComponent::CUDABit);
-  for (const Tensor* t : ts)
-    if (t->defined() && t->key_set() != memory) return false;
-  return true;
-}
-
-// the same where nothing is to be differentiated either
-bool call_alone(std::initializer_list<const Tensor*> ts) {
-  if (!kernel_alone(ts) || wanted(ts) ||
-      c10::impl::tls_local_dispatch_key_set().excluded_ != c10::default_excluded_set)
-    return false;
-  for (const Tensor* t : ts)
-    if (torch::autograd::isFwGradDefined(*t)) return false;
-  return true;
-}
-
 template <typename N, typename... Ts>
 std::shared_ptr<N> node_of(const Ts&... inputs) {
   std::shared_ptr<N> node(new N(), deleteNode);
@@ -286,7 +264,7 @@ Tensor embedding_autograd(const Tensor& ids_, const Tensor& table, double scale)
   Tensor out;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    out = (kernel_alone({&ids, &table}) ? embedding_kernel : embedding)(ids, table, scale);
+    out = embedding(ids, table, scale);
   }
   if (train) {
     auto node = node_of<EmbeddingBackward>(table);
@@ -303,7 +281,7 @@ Tensor embedding_grad_autograd(const Tensor& ids, const Tensor& grad, c10::SymIn
   Tensor out;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    out = (kernel_alone({&ids, &grad}) ? embedding_grad_kernel : embedding_grad)(ids, grad, rows, scale);
+    out = embedding_grad(ids, grad, rows, scale);
   }
   if (wanted({&grad})) {
     auto node = node_of<EmbeddingGradBackward>(grad);
@@ -375,7 +353,7 @@ Tensor dropout_autograd(const Tensor& x, const MaybeTensor& residual_, double p,
   Tensor out;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    out = (kernel_alone({&x, &residual, &c}) ? dropout_kernel : dropout)(x, residual_, p, seed, offset, counter);
+    out = dropout(x, residual_, p, seed, offset, counter);
   }
   if (wanted({&x, &residual})) {
     auto node = node_of<DropoutBackward>(x, residual);
@@ -409,11 +387,10 @@ Two head_norm_rotate(const Tensor& q, const Tensor& k, const Tensor& q_weight, c
 // the gradients of q, k, their weights, cos and sin; without `weights` or `tables` theirs are empty
 typedef std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> Six;
 
-Six head_norm_rotate_backward(const Tensor& grad_q, const Tensor& grad_k, const Tensor& q,
-                                              const Tensor& k, const Tensor& q_weight, const Tensor& k_weight,
-                                              const Tensor& cos, const Tensor& sin,
-                                              const MaybeTensor& positions, double eps, bool interleaved,
-                                              bool weights, bool tables) {
+Six head_norm_rotate_backward(const Tensor& grad_q, const Tensor& grad_k, const Tensor& q, const Tensor& k,
+                              const Tensor& q_weight, const Tensor& k_weight, const Tensor& cos,
+                              const Tensor& sin, const MaybeTensor& positions, double eps, bool interleaved,
+                              bool weights, bool tables) {
   XNN_OPERATOR("head_norm_rotate_backward",
                Six(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
                    const Tensor&, const Tensor&, const MaybeTensor&, double, bool, bool, bool));
@@ -474,12 +451,10 @@ Two head_norm_rotate_shape(const Tensor& q, const Tensor& k, const Tensor&, cons
   return {at::empty_symint(q.sym_sizes(), q.options()), at::empty_symint(k.sym_sizes(), k.options())};
 }
 
-Six head_norm_rotate_backward_kernel(const Tensor& grad_q, const Tensor& grad_k,
-                                                     const Tensor& q_, const Tensor& k_,
-                                                     const Tensor& q_weight_, const Tensor& k_weight_,
-                                                     const Tensor& cos_, const Tensor& sin_,
-                                                     const MaybeTensor& positions_, double eps,
-                                                     bool interleaved, bool weights, bool tables) {
+Six head_norm_rotate_backward_kernel(const Tensor& grad_q, const Tensor& grad_k, const Tensor& q_,
+                                     const Tensor& k_, const Tensor& q_weight_, const Tensor& k_weight_,
+                                     const Tensor& cos_, const Tensor& sin_, const MaybeTensor& positions_,
+                                     double eps, bool interleaved, bool weights, bool tables) {
   check_heads(q_, k_, q_weight_, k_weight_, cos_, sin_, or_none(positions_));
   check_tensors({&q_, &grad_q, &grad_k});
   TORCH_CHECK_VALUE(grad_q.sizes() == q_.sizes() && grad_k.sizes() == k_.sizes() &&
@@ -511,11 +486,10 @@ Six head_norm_rotate_backward_kernel(const Tensor& grad_q, const Tensor& grad_k,
   return {dq, dk, dqw, dkw, dc, ds};
 }
 
-Six head_norm_rotate_backward_shape(const Tensor&, const Tensor&, const Tensor& q,
-                                                    const Tensor& k, const Tensor& q_weight,
-                                                    const Tensor& k_weight, const Tensor& cos,
-                                                    const Tensor& sin, const MaybeTensor&, double, bool,
-                                                    bool weights, bool tables) {
+Six head_norm_rotate_backward_shape(const Tensor&, const Tensor&, const Tensor& q, const Tensor& k,
+                                    const Tensor& q_weight, const Tensor& k_weight, const Tensor& cos,
+                                    const Tensor& sin, const MaybeTensor&, double, bool, bool weights,
+                                    bool tables) {
   const auto like = [](const Tensor& t, bool wanted) {
     return wanted ? at::empty_symint(t.sym_sizes(), t.options()) : at::empty({0}, t.options());
   };
@@ -539,9 +513,8 @@ struct NormRotateBackward : Node {
     at::AutoDispatchBelowADInplaceOrView below;            // no derivative of its own
     const Tensor gq = grads[0].defined() ? grads[0] : at::zeros_symint(q.sym_sizes(), q.options());
     const Tensor gk = grads[1].defined() ? grads[1] : at::zeros_symint(k.sym_sizes(), k.options());
-    const auto f = kernel_alone({&gq, &gk, &q, &k, &qw, &kw, &c, &s, &pos}) ? head_norm_rotate_backward_kernel
-                                                                            : head_norm_rotate_backward;
-    const Six all = f(gq, gk, q, k, qw, kw, c, s, maybe(pos), eps, interleaved, weights, tables);
+    const Six all = head_norm_rotate_backward(gq, gk, q, k, qw, kw, c, s, maybe(pos), eps, interleaved, weights,
+                                              tables);
     const auto& [dq, dk, dqw, dkw, dc, ds] = all;
     const Tensor* each[] = {&dq, &dk, &dqw, &dkw, &dc, &ds};
     for (int i = 0; i < 6; ++i)
@@ -572,9 +545,7 @@ Two head_norm_rotate_autograd(const Tensor& q_, const Tensor& k_, const Tensor& 
   Two out;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    const auto f = kernel_alone({&q, &k, &q_weight, &k_weight, &cos, &sin, &positions}) ? head_norm_rotate_kernel
-                                                                                        : head_norm_rotate;
-    out = f(q, k, q_weight, k_weight, cos, sin, maybe(positions), eps, interleaved);
+    out = head_norm_rotate(q, k, q_weight, k_weight, cos, sin, maybe(positions), eps, interleaved);
   }
   auto node = node_of<NormRotateBackward>(q, k, q_weight, k_weight, cos, sin);
   node->q = SavedVariable(q, false);
@@ -742,13 +713,9 @@ struct AttentionBackward : Node {
     variable_list result(3);
     if (!grads[0].defined()) return result;
     at::AutoDispatchBelowADInplaceOrView below;            // no derivative of its own
-    const Tensor q = this->q.unpack(), k = this->k.unpack(), v = this->v.unpack(),
-                 o = out.unpack(shared_from_this()), l = lse.unpack(), t32 = tiles32.unpack(),
-                 t128 = tiles128.unpack(), m = mask.unpack();
-    const auto f = kernel_alone({&grads[0], &o, &l, &q, &k, &v, &t32, &t128, &m})
-                       ? structure_attention_backward_kernel
-                       : structure_attention_backward;
-    const Three all = f(grads[0], o, l, q, k, v, t32, t128, maybe(m), n_tokens, max_atoms, scale);
+    const Three all = structure_attention_backward(
+        grads[0], out.unpack(shared_from_this()), lse.unpack(), q.unpack(), k.unpack(), v.unpack(),
+        tiles32.unpack(), tiles128.unpack(), maybe(mask.unpack()), n_tokens, max_atoms, scale);
     if (task_should_compute_output(0)) result[0] = std::get<0>(all);
     if (task_should_compute_output(1)) result[1] = std::get<1>(all);
     if (task_should_compute_output(2)) result[2] = std::get<2>(all);
@@ -773,9 +740,8 @@ Tensor structure_attention_autograd(const Tensor& q_, const Tensor& k_, const Te
   if (mask.defined()) mask = mask.contiguous();
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    const auto f = kernel_alone({&q, &k, &v, &tiles32, &tiles128, &mask}) ? structure_attention_lse_kernel
-                                                                          : structure_attention_lse;
-    std::tie(out, lse) = f(q, k, v, tiles32, tiles128, maybe(mask), n_tokens, max_atoms, scale);
+    std::tie(out, lse) =
+        structure_attention_lse(q, k, v, tiles32, tiles128, maybe(mask), n_tokens, max_atoms, scale);
   }
   auto node = node_of<AttentionBackward>(q, k, v);
   node->q = SavedVariable(q, false);
@@ -852,24 +818,9 @@ TORCH_LIBRARY_IMPL(xnn_amd, Autograd, m) {
 
 namespace {
 
-Tensor embedding_entry(const Tensor& ids, const Tensor& table, double scale) {
-  return call_alone({&ids, &table}) ? embedding_kernel(ids, table, scale) : embedding(ids, table, scale);
-}
-
 Tensor dropout_entry(const Tensor& x, const MaybeTensor& residual, double p, uint64_t seed, uint64_t offset,
                      const MaybeTensor& counter) {
-  const Tensor r = or_none(residual), c = or_none(counter);
-  const auto f = call_alone({&x, &r, &c}) ? dropout_kernel : dropout;
-  return f(x, residual, p, (int64_t)seed, (int64_t)offset, counter);
-}
-
-Two head_norm_rotate_entry(const Tensor& q, const Tensor& k, const Tensor& q_weight, const Tensor& k_weight,
-                           const Tensor& cos, const Tensor& sin, const MaybeTensor& positions, double eps,
-                           bool interleaved) {
-  const Tensor p = or_none(positions);
-  const auto f = call_alone({&q, &k, &q_weight, &k_weight, &cos, &sin, &p}) ? head_norm_rotate_kernel
-                                                                              : head_norm_rotate;
-  return f(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved);
+  return dropout(x, residual, p, (int64_t)seed, (int64_t)offset, counter);
 }
 
 struct Plan {
@@ -879,10 +830,6 @@ struct Plan {
 
 Tensor structure_attention_entry(const Tensor& q, const Tensor& k, const Tensor& v, const Plan& plan,
                                  const MaybeTensor& mask, const std::optional<double>& scale) {
-  const Tensor m = or_none(mask);
-  if (call_alone({&q, &k, &v, &plan.tiles32, &plan.tiles128, &m}))
-    return structure_attention_kernel(q, k, v, plan.tiles32, plan.tiles128, mask, plan.n_tokens, plan.max_atoms,
-                                      scale);
   return structure_attention(q, k, v, plan.tiles32, plan.tiles128, mask, plan.n_tokens, plan.max_atoms, scale);
 }
 
@@ -893,9 +840,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("set_library", [](const std::string& path) { library = path; });
   m.def("entries", &entries);
   m.def("calls", &calls);
-  m.def("embedding", &embedding_entry);
+  m.def("embedding", &embedding);
   m.def("dropout_add", &dropout_entry);
-  m.def("head_norm_rotate", &head_norm_rotate_entry);
+  m.def("head_norm_rotate", &head_norm_rotate);
   m.def("structure_attention", &structure_attention_entry);
   py::class_<Plan>(m, "Plan").def(py::init([](int64_t n_tokens, int64_t max_atoms, const Tensor& tiles32,
                                               const Tensor& tiles128) {
