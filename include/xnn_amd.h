@@ -1256,6 +1256,64 @@ int xnn_attention_backward(int dtype, const xnn_heads* q, const xnn_heads* k, co
                            const void* grad, void* dq, void* dk, void* dv, void* work,
                            size_t work_bytes, xnn_stream_t stream);
 
+/* ---- the feed-forward layer over atoms ------------------------------------------------
+ * Norm and dense layers, with one weight or with that of each row's group (its species, its
+ * expert); no counterpart on the reference's per-edge path. Types and sums as for the attention
+ * operators above. */
+#define XNN_NO_ACTIVATION 0
+#define XNN_SILU 1
+#define XNN_GELU 2 /* z Phi(z), by erf */
+#define XNN_TANH 3
+
+/* out = (x - mean) / sqrt(mean (x - mean)^2 + eps) * weight + bias over the `width` elements (at
+ * most 16,384) of each row; row r of x at x + r * x_stride elements (x_stride >= width), out
+ * contiguous. weight and bias (width) may be NULL. stats (n_rows, 2) for the backward pass: mean
+ * and reciprocal deviation (NULL: not wanted). */
+int xnn_layer_norm(int dtype, const void* x, int64_t x_stride, int64_t n_rows, int32_t width,
+                   const void* weight, const void* bias, float eps, void* out, float* stats,
+                   xnn_stream_t stream);
+
+/* Bytes of the workspace of xnn_layer_norm_backward. */
+int xnn_layer_norm_backward_work_size(int32_t width, size_t* bytes);
+
+/* Gradients for the cotangent `grad` (contiguous): dx (contiguous), dweight, dbias, each of which
+ * may be NULL; without the last two no work is needed. */
+int xnn_layer_norm_backward(int dtype, const void* grad, const void* x, int64_t x_stride, int64_t n_rows,
+                            int32_t width, const void* weight, const float* stats, void* dx, void* dweight,
+                            void* dbias, void* work, size_t work_bytes, xnn_stream_t stream);
+
+/* Bytes of the plan and of the workspace of xnn_group_plan. */
+int xnn_group_plan_size(int64_t n, int32_t n_groups, size_t* plan_bytes, size_t* work_bytes);
+
+/* The rows of each group 0 ... n_groups - 1 (at most 4,096) for ids (n): the sorted rows (stable;
+ * those of no group last), where the groups begin, and their tiles, in int32. Nothing is read on
+ * the host. */
+int xnn_group_plan(const int64_t* ids, int64_t n, int32_t n_groups, int32_t* plan, void* work,
+                   size_t work_bytes, xnn_stream_t stream);
+
+/* out (n_rows, n_out) = residual + activation(x weight + bias), weight (n_in, n_out), bias (n_out)
+ * and residual (n_rows, n_out) contiguous, bias and residual may be NULL; row r of x at
+ * x + r * x_stride. With a plan (xnn_group_plan of these rows) weight (n_groups, n_in, n_out) and
+ * bias (n_groups, n_out) are those of each row's group, and a row of no group is NaN; without
+ * (NULL) n_groups is 1. slope (n_rows, n_out), for the backward pass: the activation's derivative
+ * (NULL: not wanted, and where there is no activation). */
+int xnn_linear(int dtype, const void* x, int64_t x_stride, int64_t n_rows, int32_t n_in, int32_t n_out,
+               const void* weight, const void* bias, int32_t activation, const void* residual,
+               const int32_t* plan, int32_t n_groups, void* out, void* slope, xnn_stream_t stream);
+
+/* Bytes of the workspace of xnn_linear_backward; grouped: with a plan. */
+int xnn_linear_backward_work_size(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, int32_t n_groups,
+                                  int32_t grouped, size_t* bytes);
+
+/* Gradients for the cotangent `grad` (n_rows, n_out), contiguous: dx (n_rows, n_in; zero in rows of no
+ * group), dweight and dbias as weight and bias (zero for a group without rows), each of which may be
+ * NULL (dbias with dweight only; without dweight no work is needed). slope: the forward pass's, NULL
+ * where there is no activation. The residual's gradient is `grad`. `work` is aligned to 16 bytes. */
+int xnn_linear_backward(int dtype, const void* grad, const void* slope, const void* x, int64_t x_stride,
+                        int64_t n_rows, int32_t n_in, int32_t n_out, const void* weight,
+                        const int32_t* plan, int32_t n_groups, void* dx, void* dweight, void* dbias,
+                        void* work, size_t work_bytes, xnn_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,7 @@ from .radial import FullyConnectedNet, RadialNet, set_recompute_radial
 from .conv import ConvTensorProduct
 from .attention import (AttentionPlan, attention_plan, dropout_add, embedding, head_norm_rotate,
                         structure_attention)
+from .feed_forward import GroupPlan, group_plan, grouped_linear, layer_norm, linear
 from .atom_attention import AtomAttention, AtomAttentionPotential, SpeciesEmbedding
 from .irreps import Irrep, Irreps, tp_out_irreps_with_instructions, wigner_3j
 
@@ -37,5 +38,6 @@ __all__ = [
     "FullyConnectedNet", "RadialNet", "set_recompute_radial", "ConvTensorProduct",
     "AttentionPlan", "attention_plan", "dropout_add", "embedding", "head_norm_rotate",
     "structure_attention", "AtomAttention", "AtomAttentionPotential", "SpeciesEmbedding",
+    "GroupPlan", "group_plan", "grouped_linear", "layer_norm", "linear",
     "Irrep", "Irreps", "tp_out_irreps_with_instructions", "wigner_3j",
 ]

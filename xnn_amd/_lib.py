@@ -289,6 +289,14 @@ _SIGNATURES = {
     "xnn_attention_backward_work_size": [c_int, i64, i32, i32, i32, _tiles, vp],
     "xnn_attention_backward": [c_int, _heads, _heads, _heads, i64, i32, _tiles, vp, f32, vp, vp, vp,
                                vp, vp, vp, vp, sz, vp],
+    "xnn_layer_norm": [c_int, vp, i64, i64, i32, vp, vp, f32, vp, vp, vp],
+    "xnn_layer_norm_backward_work_size": [i32, vp],
+    "xnn_layer_norm_backward": [c_int, vp, vp, i64, i64, i32, vp, vp, vp, vp, vp, vp, sz, vp],
+    "xnn_group_plan_size": [i64, i32, vp, vp],
+    "xnn_group_plan": [vp, i64, i32, vp, vp, sz, vp],
+    "xnn_linear": [c_int, vp, i64, i64, i32, i32, vp, vp, i32, vp, vp, i32, vp, vp, vp],
+    "xnn_linear_backward_work_size": [c_int, i64, i32, i32, i32, i32, vp],
+    "xnn_linear_backward": [c_int, vp, vp, vp, i64, i64, i32, i32, vp, vp, i32, vp, vp, vp, vp, sz, vp],
 }
 _RESTYPES = {"xnn_last_error": ctypes.c_char_p, "xnn_scan_workspace_bytes": sz,
              "xnn_edge_plan_workspace_bytes": sz, "xnn_graph_plan_workspace_bytes": sz,
@@ -426,11 +434,14 @@ class CallCounts(MutableMapping):
     def __init__(self):
         self.python: Dict[str, int] = {}
         self._names: Tuple[str, ...] = ()
-        self._native: Callable[[str], int] = lambda name: 0
+        self._modules: Tuple[Callable[[str], int], ...] = ()
 
     def join(self, names, native) -> None:
-        """``native(name)`` are the calls of each of ``names`` that native code counts."""
-        self._names, self._native = tuple(names), native
+        """``native(name)`` are the calls of each of ``names`` that one more native module counts."""
+        self._names, self._modules = (*self._names, *names), (*self._modules, native)
+
+    def _native(self, name: str) -> int:
+        return sum(native(name) for native in self._modules)
 
     def __getitem__(self, name: str) -> int:
         n = self.python.get(name, 0) + self._native(name)

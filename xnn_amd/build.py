@@ -21,9 +21,9 @@ SOURCES = ("edge.hip", "segment.hip", "basis_message.hip", "graph.hip", "d4.hip"
            "atm.hip", "eeq.hip", "eeq_cg.hip",
            "recip.hip", "radial_mlp.hip", "uvu_conv.hip", "pair.hip", "d4_tiles.hip",
            "embedding.hip", "dropout.hip", "head_norm.hip", "attention.hip",
-           "attention_backward.hip")
-# the attention operators' autograd functions: host code over libtorch and the C ABI
-NATIVE_OPS = os.path.join(HERE, "_attention_ops.so")
+           "attention_backward.hip", "layer_norm.hip", "group_plan.hip", "dense.hip", "dense_backward.hip")
+# the registered operators with their autograd functions: host code over libtorch and the C ABI, source -> module
+NATIVE_OPS = {"attention_ops.cpp": "_attention_ops", "feed_forward_ops.cpp": "_feed_forward_ops"}
 ARCH = os.environ.get("XNN_AMD_ARCH", "gfx950")
 
 # packed FP32 instructions stay off (the compiler must not form v_pk_* f32 ops)
@@ -41,26 +41,27 @@ def _hipcc() -> str:
     raise RuntimeError("hipcc not found: the xnn_amd HIP library cannot be built")
 
 
-def build_native_ops() -> str:
-    """Compile ``_attention_ops.so`` against the installed libtorch; returns its path."""
+def build_native_ops(source: str) -> str:
+    """Compile one of :data:`NATIVE_OPS` against the installed libtorch; returns its path."""
     import sysconfig
 
     import torch
     root = os.path.dirname(torch.__file__)
-    tmp = NATIVE_OPS + ".tmp"
+    path = os.path.join(HERE, NATIVE_OPS[source] + ".so")
+    tmp = path + ".tmp"
     cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           "-DTORCH_EXTENSION_NAME=_attention_ops", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-DTORCH_EXTENSION_NAME={NATIVE_OPS[source]}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE,
            "-isystem", os.path.join(root, "include"), "-isystem",
            os.path.join(root, "include", "torch", "csrc", "api", "include"), "-isystem",
            "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"],
-           os.path.join(CSRC, "attention_ops.cpp"), "-o", tmp, "-L", os.path.join(root, "lib"),
+           os.path.join(CSRC, source), "-o", tmp, "-L", os.path.join(root, "lib"),
            "-ltorch", "-ltorch_cpu", "-ltorch_python", "-ltorch_hip", "-lc10", "-lc10_hip"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"g++ failed on attention_ops.cpp:\n{res.stderr[-6000:]}")
-    os.replace(tmp, NATIVE_OPS)
-    return NATIVE_OPS
+        raise RuntimeError(f"g++ failed on {source}:\n{res.stderr[-6000:]}")
+    os.replace(tmp, path)
+    return path
 
 
 def build(verbose: bool = False, jobs: int = 4) -> str:
@@ -81,10 +82,11 @@ def build(verbose: bool = False, jobs: int = 4) -> str:
             raise RuntimeError(f"hipcc failed on {name}:\n{res.stderr[-6000:]}")
         return obj
 
-    with ThreadPoolExecutor(max_workers=max(1, jobs) + 1) as pool:
-        native = pool.submit(build_native_ops)
+    with ThreadPoolExecutor(max_workers=max(1, jobs) + len(NATIVE_OPS)) as pool:
+        native = [pool.submit(build_native_ops, source) for source in NATIVE_OPS]
         objs = list(pool.map(compile_one, sources))
-        native.result()
+        for n in native:
+            n.result()
     tmp = LIBRARY + ".tmp"
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
     res = subprocess.run(cmd, capture_output=True, text=True)

@@ -144,6 +144,11 @@ class AtomicGraph:
         from .attention import plan_for
         return plan_for(self)
 
+    def species_plan(self, n_groups: int):
+        """The cached :class:`~xnn_amd.feed_forward.GroupPlan` of this graph's atomic numbers (GPU only)."""
+        from .feed_forward import species_plan_for
+        return species_plan_for(self, n_groups)
+
     def edge_vectors(self) -> Tensor:
         """``pos[dst] - pos[src] + cell_shift @ cell`` per edge, in :attr:`model_dtype`,
         differentiable with respect to ``pos`` and ``cell`` (atomic_data.py:371-418)."""

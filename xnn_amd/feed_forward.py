@@ -1,0 +1,142 @@
+"""The feed-forward half of an attention block over atoms, its operators as HIP kernels.
+
+=======================  ============================================================
+:func:`layer_norm`       norm of rows; the backward pass sums the weight's and the bias's
+                         gradients over the rows
+:func:`linear`           product with a weight; bias, activation and residual in its
+                         epilogue
+:func:`grouped_linear`   the same with the weight of each row's group (the species of an
+                         atom, the expert that it is routed to)
+:func:`group_plan`       the rows of each group, for :func:`grouped_linear`
+=======================  ============================================================
+
+As the operators of :mod:`xnn_amd.attention` (whose manner they share: types, streams, errors,
+registration with the dispatcher) they take GPU tensors of float32, bfloat16 or float16, do
+arithmetic and sums in float32 and round every output once, raise on any other tensor, run on
+the current stream without host reads, sum in a fixed order and may be captured in a HIP graph.
+They are differentiable once. The per-edge reference path has no counterpart.
+"""
+from __future__ import annotations
+
+import os
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+from torch import Tensor
+from torch.compiler import is_compiling
+
+from . import _lib
+
+_native, _failure = None, None
+try:
+    # registers the operators (torch.ops.xnn_amd) with their shapes and derivatives
+    from . import _feed_forward_ops as _built
+    _built.set_library(os.path.abspath(_lib.LIBRARY))
+    _lib.calls.join(_built.entries(), _built.calls)
+except (ImportError, AttributeError) as err:     # not built, or from other sources: the first call says so
+    _built, _failure = None, err
+
+#: activations by name, with their codes in the C ABI
+ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "tanh": 3}
+
+
+def _ops():
+    """The native operators, checked on first use (raises when they are not built)."""
+    global _native
+    if _native is None:
+        _lib.load()
+        if _built is None:
+            raise RuntimeError("xnn_amd/_feed_forward_ops.so is missing, old or does not load: build it with "
+                               "`python -m xnn_amd.build` (the kernels have no fallback)") from _failure
+        _native = _built
+    return _native
+
+
+def _activation(name: Optional[str]) -> int:
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"unknown activation {name!r} (None, 'silu', 'gelu' or 'tanh')") from None
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
+               eps: float = 1e-5) -> Tensor:
+    """``(x - mean) / sqrt(mean (x - mean)^2 + eps) * weight + bias`` over the last dimension of ``x``
+    (..., C), ``C <= 16384``; ``weight`` and ``bias`` (C,), each of which may be left out. Rows may
+    be strided (a part of wider ones).
+
+    The squares are those of the centered values. Each gradient is summed over the rows in a fixed
+    order, float32 within a block of rows and float64 over the blocks."""
+    if is_compiling():               # a compiler cannot look into the native entry: the same operator by name
+        return torch.ops.xnn_amd.layer_norm(x, weight, bias, eps)
+    return (_native or _ops()).layer_norm(x, weight, bias, eps)
+
+
+def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None,
+           residual: Optional[Tensor] = None) -> Tensor:
+    """``residual + f(x @ weight + bias)`` for ``x`` (..., K), ``weight`` (K, N), ``bias`` (N,) and
+    ``residual`` (..., N), the last two where they are given; ``activation`` ``f``: None, ``"silu"``,
+    ``"gelu"`` (``z Phi(z)``, by the error function) or ``"tanh"``. Rows of ``x`` may be strided.
+
+    Where a gradient is wanted the forward pass keeps ``f'(z)`` in ``x``'s type, and the backward pass
+    rounds ``d = grad f'(z)`` to that type between the two products, as ``f'(z)`` before it: two roundings of
+    independent sign in each term of the gradients' sums. float32 operands enter the products as three
+    planes of 8 bits: one that is not finite makes the outputs it reaches NaN."""
+    code = _activation(activation)
+    if is_compiling():
+        return torch.ops.xnn_amd.dense(x, weight, bias, code, residual, None)
+    return (_native or _ops()).dense(x, weight, bias, code, residual, None)
+
+
+@dataclass
+class GroupPlan:
+    """The rows of each group (:func:`group_plan`)."""
+    n_rows: int
+    n_groups: int
+    rows: Tensor                     # int32: the sorted rows, where the groups begin, their tiles
+
+
+def group_plan(ids: Tensor, n_groups: int) -> GroupPlan:
+    """The plan of rows whose groups are ``ids`` (T,), integers; kept as long as they are
+    (:meth:`~xnn_amd.data.AtomicGraph.species_plan` keeps that of the species with the graph). A row with
+    an id outside ``[0, n_groups)`` is of no group. At most 4,096 groups. Three launches and no host
+    read: a plan of ids that are made on the device may be captured with what uses it."""
+    if is_compiling():
+        rows = torch.ops.xnn_amd.group_plan(ids, n_groups)
+    else:
+        rows = (_native or _ops()).group_plan(ids, n_groups)
+    return GroupPlan(ids.shape[0], int(n_groups), rows)
+
+
+def species_plan_for(graph, n_groups: int) -> GroupPlan:
+    """The cached plan of an :class:`~xnn_amd.data.AtomicGraph`'s species (made again when its
+    ``atomic_numbers`` are another tensor or were written to, or for another number of groups)."""
+    ids = graph.atomic_numbers
+    version = None if ids.is_inference() else ids._version
+    key = (version, int(n_groups))
+    cached = getattr(graph, "_xnn_species_plan", None)
+    if cached is not None and cached[0] is ids and cached[1] == key:
+        return cached[2]
+    plan = group_plan(ids, n_groups)
+    object.__setattr__(graph, "_xnn_species_plan", (ids, key, plan))
+    return plan
+
+
+def grouped_linear(x: Tensor, weight: Tensor, plan: GroupPlan, bias: Optional[Tensor] = None,
+                   activation: Optional[str] = None, residual: Optional[Tensor] = None) -> Tensor:
+    """:func:`linear` with the weight of each row's group: row ``t`` of ``x`` (T, K) is multiplied by
+    ``weight[ids[t]]``, with ``weight`` (G, K, N), ``bias`` (G, N) and ``plan`` =
+    :func:`group_plan` ``(ids, G)``. Rows are read and written where they stand, in any order of groups.
+
+    A row of no group gives a row of NaN, counts in no weight's gradient and gets zero gradients of
+    its own; the weights of a group without rows get zero gradients."""
+    code = _activation(activation)
+    if not isinstance(plan, GroupPlan):
+        raise TypeError(f"plan must be a GroupPlan (group_plan), got {type(plan).__name__}")
+    if weight.dim() == 3 and weight.shape[0] != plan.n_groups:
+        raise ValueError(f"the plan is of {plan.n_groups} groups, weight {tuple(weight.shape)} has "
+                         f"{weight.shape[0]}")
+    if is_compiling():
+        return torch.ops.xnn_amd.dense(x, weight, bias, code, residual, plan.rows)
+    return (_native or _ops()).dense(x, weight, bias, code, residual, plan.rows)
