@@ -1295,19 +1295,21 @@ int xnn_group_plan(const int64_t* ids, int64_t n, int32_t n_groups, int32_t* pla
  * and residual (n_rows, n_out) contiguous, bias and residual may be NULL; row r of x at
  * x + r * x_stride. With a plan (xnn_group_plan of these rows) weight (n_groups, n_in, n_out) and
  * bias (n_groups, n_out) are those of each row's group, and a row of no group is NaN; without
- * (NULL) n_groups is 1. slope (n_rows, n_out), for the backward pass: the activation's derivative
- * (NULL: not wanted, and where there is no activation). */
+ * (NULL) n_groups is 1. slope (n_rows, n_out), for the backward pass: the activation's derivative, of
+ * 4 bytes an element for XNN_F32 and 2 for the others, in a form of its own (NULL: not wanted, and
+ * where there is no activation). */
 int xnn_linear(int dtype, const void* x, int64_t x_stride, int64_t n_rows, int32_t n_in, int32_t n_out,
                const void* weight, const void* bias, int32_t activation, const void* residual,
                const int32_t* plan, int32_t n_groups, void* out, void* slope, xnn_stream_t stream);
 
-/* Bytes of the workspace of xnn_linear_backward; grouped: with a plan. */
+/* Bytes of the workspace of xnn_linear_backward; grouped: with a plan; slope, weight, bias: with a
+ * slope, with dweight, with dbias. */
 int xnn_linear_backward_work_size(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, int32_t n_groups,
-                                  int32_t grouped, size_t* bytes);
+                                  int32_t grouped, int32_t slope, int32_t weight, int32_t bias, size_t* bytes);
 
 /* Gradients for the cotangent `grad` (n_rows, n_out), contiguous: dx (n_rows, n_in; zero in rows of no
  * group), dweight and dbias as weight and bias (zero for a group without rows), each of which may be
- * NULL (dbias with dweight only; without dweight no work is needed). slope: the forward pass's, NULL
+ * NULL. slope: the forward pass's, NULL
  * where there is no activation. The residual's gradient is `grad`. `work` is aligned to 16 bytes. */
 int xnn_linear_backward(int dtype, const void* grad, const void* slope, const void* x, int64_t x_stride,
                         int64_t n_rows, int32_t n_in, int32_t n_out, const void* weight,

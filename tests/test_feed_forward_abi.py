@@ -94,25 +94,33 @@ def test_linear_arguments(lib):
 
 
 def test_linear_backward_arguments(lib):
-    assert lib.xnn_linear_backward_work_size(0, 100000, 64, 64, 1, 0, ctypes.byref(SIZE)) == 0
+    def size(dtype, rows, groups, grouped=0, slope=0, weight=1, bias=0, out=None):
+        return lib.xnn_linear_backward_work_size(dtype, rows, 64, 64, groups, grouped, slope, weight, bias,
+                                                 ctypes.byref(SIZE) if out is None else out)
+    assert size(0, 20, 1) == 0 and SIZE.value == 0
+    assert size(2, 1000, 1, slope=1, weight=0) == 0 and SIZE.value == 1000 * 64 * 2
+    assert size(0, 100000, 1) == 0
     need = SIZE.value
     assert need > 0
-    assert lib.xnn_linear_backward_work_size(0, 20, 64, 64, 1, 0, ctypes.byref(MORE)) == 0 and MORE.value == 0
-    _refused(lib, lib.xnn_linear_backward_work_size(0, 20, 64, 64, 5000, 1, ctypes.byref(MORE)), b"n_groups")
-    _refused(lib, lib.xnn_linear_backward_work_size(0, 20, 64, 64, 1, 0, None), b"NULL size")
+    _refused(lib, size(0, 20, 5000, 1), b"n_groups")
+    _refused(lib, size(1, 20, 1), b"dtype")
+    _refused(lib, lib.xnn_linear_backward_work_size(0, 20, 64, 64, 1, 0, 0, 1, 0, None), b"NULL size")
     f = lib.xnn_linear_backward
 
-    def call(grad=BUF, x=BUF, stride=64, rows=100000, w=BUF, dx=None, dw=BUF, db=None, work=BUF, size=need):
-        return f(0, grad, None, x, stride, rows, 64, 64, w, None, 1, dx, dw, db, work, size, None)
+    def call(grad=BUF, slope=None, x=BUF, stride=64, rows=100000, w=BUF, dx=None, dw=BUF, db=None, work=BUF,
+             size=need):
+        return f(0, grad, slope, x, stride, rows, 64, 64, w, None, 1, dx, dw, db, work, size, None)
     _refused(lib, call(grad=None), b"NULL cotangent")
     _refused(lib, call(w=None, dx=BUF), b"NULL weight")
     _refused(lib, call(x=None), b"NULL input")
-    _refused(lib, call(dw=None, db=BUF), b"goes with")
     _refused(lib, call(stride=63), b"overlap")
     _refused(lib, call(size=need - 1), b"work too small")
+    _refused(lib, call(db=BUF), b"work too small")
+    _refused(lib, call(slope=BUF), b"work too small")
     _refused(lib, call(work=None), b"work too small")
     _refused(lib, call(work=ctypes.addressof(BUF) + 4), b"aligned")
-    assert f(0, None, None, None, 0, 0, 64, 64, None, None, 1, None, None, None, None, 0, None) == 0
+    assert call(dw=None) == 0
+    assert f(0, None, None, None, 0, 0, 64, 64, None, None, 1, BUF, None, None, None, 0, None) == 0
 
 
 def test_functions_refuse_cpu_tensors():

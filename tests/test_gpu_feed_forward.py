@@ -1,8 +1,8 @@
 """The feed-forward operators over atoms on the GPU against the same operations in float64.
 
 A result is off by its own rounding (half a step of the type, u) and by what the operator documents: float32
-sums, the products of float32 operands left out of the planes (2^-23 of each product) and the two roundings
-of d = grad f'(z) in 16 bits. The bounds below add these up over each output's own terms."""
+sums, the products of float32 operands left out of the planes (2^-23 of each product) and, in 16 bits, the
+form in which f'(z) is kept and the rounding of d = grad f'(z). The bounds below add these up over each output's own terms."""
 import math
 
 import numpy as np
@@ -189,9 +189,11 @@ def _check_dense(dtype, case, activation):
         _close(out[rows], want, bound, f"output of {group}")
         gd = g[rows].double()
         d = gd * slope
-        # f' changes by at most |f''| <= 1; kept in the type, and d rounded to it
-        dd = gd.abs() * (dz + f32 * (1 + z.abs()) + (0 if activation is None else 2.1 * u * slope.abs() + 2 * tiny))
-        dd = dd + (0 if activation is None else tiny)
+        # f' changes by at most |f''| <= 1; its root is kept in units of 1 / 30,000 (16-bit types), so it is off by
+        # 2 root(f') e + e^2 with e half a unit; d is rounded to the type
+        e = 0.0 if activation is None or exact else 1.01 / 60000
+        dd = gd.abs() * (dz + f32 * (1 + z.abs()) + 2 * e * slope.abs().sqrt() + e * e)
+        dd = dd + (0 if activation is None else u * d.abs() + tiny)
         dx = d @ wd.t()
         _close(grads[0][rows], dx, _term(dtype, N) * (d.abs() @ wd.abs().t()) + dd @ wd.abs().t() + u * dx.abs() + tiny,
                f"dx of {group}")

@@ -1,7 +1,7 @@
 // Matrix products of a dense layer on tiles, shared by its forward and backward kernels (gfx950, wave64).
 //
 //   forward   out = residual + f(x W + b)    rows of x (reduction along them)    x  W read across its rows
-//   input     dx  = d W^T,  d = g f'(z)      rows of g                           x  rows of W
+//   input     dx  = d W^T,  d = g f'(z)      rows of d                           x  rows of W
 //   weight    dW  = x^T d                    x read across its rows              x  d read across its rows
 //
 // A block owns a tile of the output and walks the reduction in steps that all its threads stage in LDS,
@@ -109,7 +109,7 @@ __device__ __forceinline__ void fill_rows(const GroupView& v, const RowTile& t, 
 // ---------------------------------------------------------------- activations
 enum Activation : int { kNone = 0, kSilu = 1, kGelu = 2, kTanh = 3 };
 
-// f(z) and f'(z)
+// f(z) and f'(z), to a few float32 steps of the larger of 1 and |z|
 __device__ __forceinline__ void activate(int kind, float z, float& y, float& slope) {
   if (kind == kSilu) {
     // the exponential's error is |z| 2^-24 of it, p (1 - p) |z| < 1/4 of that in p
@@ -117,16 +117,61 @@ __device__ __forceinline__ void activate(int kind, float z, float& y, float& slo
     y = z * p;
     slope = p * fmaf(z, 1.0f - p, 1.0f);
   } else if (kind == kGelu) {
-    const float c = fmaf(0.5f, erff(0.70710678118654752f * z), 0.5f);
+    // erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + 0.3275911 x), x >= 0, to 1.5e-7 (Abramowitz and Stegun,
+    // Handbook of Mathematical Functions, 7.1.26): the exponential is that of the slope
+    const float e = __builtin_amdgcn_exp2f(-0.5f * kLog2e * z * z);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.0f));
+    float q = fmaf(t, 1.061405429f, -1.453152027f);
+    q = fmaf(t, q, 1.421413741f);
+    q = fmaf(t, q, -0.284496736f);
+    q = fmaf(t, q, 0.254829592f);
+    q *= 0.5f * t * e;
+    const float c = z < 0.0f ? q : 1.0f - q;
     y = z * c;
-    slope = fmaf(z * 0.39894228040143268f, __builtin_amdgcn_exp2f(-0.5f * kLog2e * z * z), c);
+    slope = fmaf(z * 0.39894228040143268f, e, c);
   } else if (kind == kTanh) {
-    y = tanhf(z);
+    // by the exponential; near zero, where that loses it, the series
+    const float a = fabsf(z), e = __builtin_amdgcn_exp2f(-2.0f * kLog2e * a), w = z * z;
+    const float far = copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), z);
+    float q = fmaf(w, 62.0f / 2835.0f, -17.0f / 315.0f);
+    q = fmaf(w, q, 2.0f / 15.0f);
+    q = fmaf(w, q, -1.0f / 3.0f);
+    const float near = fmaf(z * w, q, z);
+    y = a < 0.25f ? near : far;
     slope = fmaf(-y, y, 1.0f);
   } else {
     y = z;
     slope = 1.0f;
   }
+}
+
+// f'(z) as the backward pass gets it: float32 as it is; for the 16-bit types its root with its sign in 15 bits of
+// fixed point (f' is below 1.13), off by 2^-15 of it at most near 1 and by less below, so that d = g f'(z) is
+// rounded once and not twice (the gradients' error in bfloat16 1.4 times an output's rounding, 1.7 with f' in it).
+// The number below -32,767 stands for NaN.
+template <typename T>
+struct Slope {
+  typedef int16_t type;
+};
+template <>
+struct Slope<float> {
+  typedef float type;
+};
+constexpr float kSlopeUnit = 30000.0f;
+template <typename T>
+__device__ __forceinline__ typename Slope<T>::type slope_stored(float s) {
+  if constexpr (sizeof(T) == 4)
+    return s;
+  else
+    return s == s ? (int16_t)__float2int_rn(copysignf(kSlopeUnit * __builtin_amdgcn_sqrtf(fabsf(s)), s))
+                  : (int16_t)-32768;
+}
+template <typename T>
+__device__ __forceinline__ float slope_value(typename Slope<T>::type s) {
+  if constexpr (sizeof(T) == 4)
+    return s;
+  else
+    return s == -32768 ? __builtin_nanf("") : (float)s * fabsf((float)s) * (1.0f / (kSlopeUnit * kSlopeUnit));
 }
 
 // ---------------------------------------------------------------- sizes
@@ -170,135 +215,153 @@ __device__ __forceinline__ void rounded_planes(float a, float b, uint32_t (&out)
   }
 }
 
-// One 16-byte piece to LDS: as it is, or in three planes of half the bytes
-template <typename T, int N>
-__device__ __forceinline__ void put_piece(char* at, int plane, const Pack<T, N>& x) {
-  if constexpr (sizeof(T) == 4) {
-    uint32_t a[3], b[3];
-    rounded_planes(x.v[0], x.v[1], a);
-    rounded_planes(x.v[2], x.v[3], b);
+// the first `left` elements of a piece, zeros for the others
+template <typename T>
+__device__ __forceinline__ u32x4 piece_head(u32x4 x, int left) {
+  constexpr int kWord = 4 / sizeof(T);
 #pragma unroll
-    for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x2*>(at + n * plane) = u32x2{a[n], b[n]};
-  } else {
-    *reinterpret_cast<Pack<T, N>*>(at) = x;
+  for (int i = 0; i < 4; ++i) {
+    const int n = left - i * kWord;
+    x[i] = n >= kWord ? x[i] : n == 1 && kWord == 2 ? x[i] & 0xFFFFu : 0u;
   }
+  return x;
 }
 
-// Pieces need no alignment (the loads are unaligned ones, at full rate where the address happens to be aligned).
-// One that reaches beyond its row's `width` elements is within the tensor where another row follows; the last
-// row's is taken element by element.
-template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> load_piece(const T* p) {
-  Pack<T, N> x;
+// A piece from any address (the loads are unaligned ones, at full rate where the address happens to be aligned).
+// One that reaches beyond its row's `left` elements is within the tensor where another row follows; in the last
+// row it is taken element by element.
+__device__ __forceinline__ u32x4 load_raw(const char* p) {
+  u32x4 x;
   __builtin_memcpy(&x, p, sizeof(x));
   return x;
 }
-template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> load_piece(const T* row, int at, int width, bool last) {
-  if (at + N <= width || (at < width && !last)) return load_piece<T, N>(row + at);
+template <typename T>
+__device__ __forceinline__ u32x4 load_raw(const char* p, int left, bool last) {
+  constexpr int N = 16 / sizeof(T);
+  if (left >= N || (left > 0 && !last)) return load_raw(p);
   Pack<T, N> x;
 #pragma unroll
-  for (int i = 0; i < N; ++i) x.v[i] = at + i < width ? row[at + i] : (T)0.0f;
-  return x;
+  for (int i = 0; i < N; ++i) x.v[i] = i < left ? reinterpret_cast<const T*>(p)[i] : (T)0.0f;
+  return __builtin_bit_cast(u32x4, x);
 }
 
-// One operand on its way: a matrix of `tensor_rows` rows of `width` elements, row r at data + r stride (and
-// the factor of d beside it, of the same layout), of which LEN rows or columns are this tile's. ALONG: the
-// tile's rows, along which the reduction runs; else its columns, and the reduction runs over the rows. Row r of
-// the tile, or of the reduction, is order[first + r], or first + r without an order.
-template <typename T, int LEN, bool ALONG, bool TIMES>
+// One piece to LDS: as it is, or in three planes of half the bytes
+template <typename T>
+__device__ __forceinline__ void put_piece(char* at, int plane, u32x4 x) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t a[3], b[3];
+    rounded_planes(__uint_as_float(x[0]), __uint_as_float(x[1]), a);
+    rounded_planes(__uint_as_float(x[2]), __uint_as_float(x[3]), b);
+#pragma unroll
+    for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x2*>(at + n * plane) = u32x2{a[n], b[n]};
+  } else {
+    *reinterpret_cast<u32x4*>(at) = x;
+  }
+}
+
+// One operand on its way: a matrix of rows of `width` elements, row r at data + r stride, of which LEN rows or
+// columns are this tile's. ALONG: the tile's rows, along which the reduction runs; else its columns, and the
+// reduction runs over the rows. Row r of the tile, or of the reduction, is order[first + r], or first + r
+// without an order.
+//
+// Steps that begin before `fast` are of whole pieces, one address each that the step before has left: along the rows
+// those that end within them; across them all but the last one where a piece may reach beyond its row (the
+// tensor's last row is the last of its group).
+template <typename T, int LEN, bool ALONG>
 struct Operator {
   static constexpr int BK = 128 / sizeof(T), kPer = 16 / sizeof(T);
   static constexpr int kRows = ALONG ? LEN : BK, kCols = ALONG ? BK : LEN;   // of a staged step
   static constexpr int kChunks = kCols / kPer;
   static constexpr int kStep = kDenseThreads / kChunks;
   static constexpr int kCount = kRows / kStep;
-  static_assert(kDenseThreads % kChunks == 0 && kRows % kStep == 0, "");
-  typedef Pack<T, kPer> Piece;
+  static_assert(kDenseThreads % kChunks == 0 && kRows % kStep == 0 && kCount <= 32, "");
   typedef Place<T, LEN, ALONG> At;
 
-  const T *data, *factor;
-  const int32_t* order;
-  int64_t stride;
-  int width, row, at, first, end, last;   // last: the tensor's last row
-  bool whole;                      // no piece reaches beyond its row
-  int32_t index[kCount];           // rows of the next step (ALONG: of all)
-  Piece x[kCount], y[TIMES ? kCount : 1];
+  const char *data, *column;       // the tensor, and the thread's first piece of its row 0
+  const int32_t* order;            // from `first` on
+  int64_t stride;                  // bytes of a row
+  int width, row, at, first, end, last, fast;   // last: the tensor's last row
+  int most;                        // the last row that a whole piece may begin in
+  uint32_t edges;                  // ALONG: pieces of the tensor's last row
+  const char* p[kCount];           // pieces of the next step; across rows in an order
+  int32_t index[ALONG ? 1 : kCount];   // those rows, whose loads have a step's time
+  u32x4 x[kCount];
 
   // rows [first_row, end_row), columns from first_col on
-  __device__ __forceinline__ void init(const void* data_, const void* factor_, const int32_t* order_,
-                                       int64_t stride_, int tensor_rows, int width_, int first_row,
-                                       int end_row, int first_col) {
-    data = (const T*)data_;
-    factor = (const T*)factor_;
-    order = order_;
-    stride = stride_;
+  __device__ __forceinline__ void init(const void* data_, const int32_t* order_, int64_t stride_,
+                                       int tensor_rows, int width_, int first_row, int end_row,
+                                       int first_col) {
+    data = (const char*)data_;
+    order = order_ == nullptr ? nullptr : order_ + first_row;
+    stride = stride_ * (int)sizeof(T);
     last = tensor_rows - 1;
     width = width_;
     row = threadIdx.x / kChunks;
     at = first_col + threadIdx.x % kChunks * kPer;
     if (!ALONG && at >= width) at = 0;                     // columns beyond the edge: any that exist
+    column = data + at * (int)sizeof(T);
     first = first_row;
     end = end_row - first_row;
-    whole = width % kPer == 0;
-    look(0);
-  }
-  // the rows that the step from reduction index k0 on reads
-  __device__ __forceinline__ void look(int k0) {
+    const bool whole = width % kPer == 0;
+    most = ALONG || whole ? last : max(last - 1, 0);
+    fast = stride_ < kPer ? 0 : ALONG ? width / BK * BK : (whole ? end : end - 1) / BK * BK;
+    edges = 0;
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {
-      const int r = first + min((ALONG ? 0 : k0) + row + n * kStep, end - 1);
-      index[n] = order == nullptr ? r : min(max(order[r], 0), last);
+      const int i = row_of(row + n * kStep);
+      if (ALONG && i == last) edges |= 1u << n;
+      if constexpr (!ALONG) index[n] = i;
+      p[n] = column + i * stride;
     }
   }
-  // the step from reduction index k0 on (across the rows: that of the last look)
+  __device__ __forceinline__ int row_of(int r) const {
+    r = min(r, end - 1);
+    return order == nullptr ? first + r : min(max(order[r], 0), last);
+  }
+  // the step from reduction index k0 < fast on
+  __device__ __forceinline__ void fetch_fast(int k0) {
+    if constexpr (!ALONG)
+      if (order != nullptr) {
+#pragma unroll
+        for (int n = 0; n < kCount; ++n) p[n] = column + min(index[n], most) * stride;
+      }
+    const int64_t step = ALONG ? 128 : BK * stride;
+#pragma unroll
+    for (int n = 0; n < kCount; ++n) {
+      x[n] = load_raw(p[n]);
+      p[n] += step;
+    }
+    if constexpr (!ALONG)
+      if (order != nullptr) {
+#pragma unroll
+        for (int n = 0; n < kCount; ++n) index[n] = row_of(k0 + BK + row + n * kStep);
+      }
+  }
+  // any step
   __device__ __forceinline__ void fetch(int k0) {
-    const int col = ALONG ? at + k0 : at;
-    if (whole && (!ALONG || k0 + BK <= width)) {
-#pragma unroll
-      for (int n = 0; n < kCount; ++n) {
-        const int64_t i = index[n] * stride + col;
-        x[n] = load_piece<T, kPer>(data + i);
-        if constexpr (TIMES) y[n] = load_piece<T, kPer>(factor + i);
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < kCount; ++n) {
-        const int64_t i = index[n] * stride;
-        const bool edge = index[n] == last || stride < kPer;
-        x[n] = load_piece<T, kPer>(data + i, col, width, edge);
-        if constexpr (TIMES) y[n] = load_piece<T, kPer>(factor + i, col, width, edge);
-      }
+    if (k0 < fast) {
+      fetch_fast(k0);
+      return;
     }
-    if (!ALONG) look(k0 + BK);
+#pragma unroll
+    for (int n = 0; n < kCount; ++n) {
+      const int i = ALONG ? 0 : row_of(k0 + row + n * kStep);
+      const char* q = ALONG ? p[n] : column + i * stride;
+      const int left = width - at - (ALONG ? k0 : 0);
+      const bool edge = (ALONG ? (edges >> n & 1) != 0 : i == last) || stride < 16;
+      x[n] = load_raw<T>(q, left, edge);
+      if (ALONG) p[n] += 128;
+    }
   }
-  // to LDS, zeros beyond the reduction's `length`; sums: of each of the thread's columns, added to
-  template <bool SUMS = false>
-  __device__ __forceinline__ void commit(char* lds, int k0, int length, float* sums = nullptr) {
-    const bool tail = k0 + BK > length;
+  // to LDS, TAIL: zeros beyond the reduction's `length`
+  template <bool TAIL>
+  __device__ __forceinline__ void commit(char* lds, int k0, int length) {
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {
       const int r = row + n * kStep, c = threadIdx.x % kChunks * kPer;
-      float v[kPer];
-      Piece out;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        out.v[i] = x[n].v[i];
-        if constexpr (TIMES) out.v[i] = (T)(v[i] = (float)x[n].v[i] * (float)y[n].v[i]);
-      }
-      if (tail) {
-        const int left = ALONG ? length - k0 - c : k0 + r < length ? kPer : 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (i >= left) {
-            out.v[i] = (T)0.0f;
-            v[i] = 0.0f;
-          }
-      }
-      if constexpr (SUMS)
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) sums[i] += TIMES ? v[i] : (float)out.v[i];
-      put_piece<T, kPer>(lds + r * At::kRow + c * 2, At::kPlane, out);
+      u32x4 out = x[n];
+      if constexpr (TAIL) out = piece_head<T>(out, ALONG ? length - k0 - c : k0 + r < length ? kPer : 0);
+      put_piece<T>(lds + r * At::kRow + c * 2, At::kPlane, out);
     }
   }
 };
@@ -330,6 +393,22 @@ __device__ __forceinline__ Operand<T> dense_operand(const char* lds, int outer, 
   return out;
 }
 
+// N elements from any address, and from column `at` on of a row of `width` (as load_raw)
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_piece(const T* p) {
+  Pack<T, N> x;
+  __builtin_memcpy(&x, p, sizeof(x));
+  return x;
+}
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_piece(const T* row, int at, int width, bool last) {
+  if (at + N <= width || (at < width && !last)) return load_piece<T, N>(row + at);
+  Pack<T, N> x;
+#pragma unroll
+  for (int i = 0; i < N; ++i) x.v[i] = at + i < width ? row[at + i] : (T)0.0f;
+  return x;
+}
+
 // ---------------------------------------------------------------- the product
 // LDS of a block: one stage of both operands, and the waves' rows on their way out
 template <typename L, typename T, bool ALONG_A, bool ALONG_B>
@@ -337,14 +416,31 @@ struct DenseLds {
   static constexpr int kA = Place<T, L::BM, ALONG_A>::kBytes, kB = Place<T, L::BN, ALONG_B>::kBytes;
   static constexpr int kOutRow = L::NT * 32 + 4;                         // floats
   static constexpr int kOut = kDenseWaves * 32 * kOutRow * 4;
+  static constexpr int kPlanes = Store<T>::kPlanes;
   static constexpr int kStages = 2 * (kA + kB) <= 150 * 1024 && sizeof(T) == 2 ? 2 : 1;
   static constexpr int kBytes = kStages * (kA + kB) > kOut ? kStages * (kA + kB) : kOut;
 };
 
-// acc = the reduction over [k_begin, k_end) of `length` indices; SUMS: b's columns added up in `sums`
-template <typename T, typename L, bool ALONG_A, bool ALONG_B, bool SUMS, typename A, typename B>
-__device__ __forceinline__ void dense_product(A& a, B& b, int k_begin, int k_end, int length, char* lds,
-                                              f32x16 (&acc)[L::MT][L::NT], float* sums = nullptr) {
+// The order of a region's instructions: among M products, READS reads of LDS in the first three quarters, WRITES writes
+// to it and LOADS global loads evenly. Without it the compiler puts each kind in a row and the matrix cores wait.
+template <int M, int READS, int WRITES, int LOADS, int I = 0>
+__device__ __forceinline__ void interleave() {
+  if constexpr (I < M) {
+    constexpr auto reads = [](int i) { return i * READS * 4 / (3 * M) < READS ? i * READS * 4 / (3 * M) : READS; };
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if constexpr (reads(I + 1) > reads(I)) __builtin_amdgcn_sched_group_barrier(0x100, reads(I + 1) - reads(I), 0);
+    if constexpr ((I + 1) * WRITES / M > I * WRITES / M)
+      __builtin_amdgcn_sched_group_barrier(0x200, (I + 1) * WRITES / M - I * WRITES / M, 0);
+    if constexpr ((I + 1) * LOADS / M > I * LOADS / M)
+      __builtin_amdgcn_sched_group_barrier(0x020, (I + 1) * LOADS / M - I * LOADS / M, 0);
+    interleave<M, READS, WRITES, LOADS, I + 1>();
+  }
+}
+
+// The tile's sums over `length` reduction indices. The rows of a 32 x 32 product are the output's columns, so that
+// a lane holds four of them in a row.
+template <typename T, typename L, bool ALONG_A, bool ALONG_B, typename A, typename B>
+__device__ __forceinline__ void dense_product(A& a, B& b, int length, char* lds, f32x16 (&acc)[L::MT][L::NT]) {
   typedef DenseLds<L, T, ALONG_A, ALONG_B> S;
   constexpr int BK = L::BK;
   const int wave = wave_in_block();
@@ -353,74 +449,135 @@ __device__ __forceinline__ void dense_product(A& a, B& b, int k_begin, int k_end
   for (int i = 0; i < L::MT; ++i)
 #pragma unroll
     for (int j = 0; j < L::NT; ++j) acc[i][j] = f32x16{};
-  if (k_begin >= k_end) return;
-  const auto compute = [&](const char* s) {
+  // operands `step` of a stage, two steps' in registers: a step's are read while the products of the one before run
+  constexpr int kSteps = BK / 16;
+  static_assert(kSteps % 2 == 0, "");
+  Operand<T> fa[2][L::MT], fb[2][L::NT];
+  const auto read = [&](const char* s, int step) {
 #pragma unroll
-    for (int step = 0; step < BK / 16; ++step) {
-      Operand<T> fa[L::MT], fb[L::NT];
+    for (int i = 0; i < L::MT; ++i) fa[step & 1][i] = dense_operand<T, L::BM, ALONG_A>(s, m0 + 32 * i, step);
 #pragma unroll
-      for (int i = 0; i < L::MT; ++i) fa[i] = dense_operand<T, L::BM, ALONG_A>(s, m0 + 32 * i, step);
+    for (int j = 0; j < L::NT; ++j)
+      fb[step & 1][j] = dense_operand<T, L::BN, ALONG_B>(s + S::kA, n0 + 32 * j, step);
+  };
+  const auto multiply = [&](int step) {
 #pragma unroll
-      for (int j = 0; j < L::NT; ++j) fb[j] = dense_operand<T, L::BN, ALONG_B>(s + S::kA, n0 + 32 * j, step);
+    for (int i = 0; i < L::MT; ++i)
 #pragma unroll
-      for (int i = 0; i < L::MT; ++i)
-#pragma unroll
-        for (int j = 0; j < L::NT; ++j) mma<T>(fa[i], fb[j], acc[i][j]);
-    }
+      for (int j = 0; j < L::NT; ++j) mma<T>(fb[step & 1][j], fa[step & 1][i], acc[i][j]);
+  };
+  constexpr int kProducts = L::MT * L::NT * (S::kPlanes == 3 ? 6 : 1);          // of a step
+  constexpr int kReads = (L::MT * (ALONG_A ? 1 : 2) + L::NT * (ALONG_B ? 1 : 2)) * S::kPlanes;
+  constexpr int kMoves = A::kCount + B::kCount;
+  const auto commit_fast = [&](char* s, int k) {
+    a.template commit<false>(s, k, length);
+    b.template commit<false>(s + S::kA, k, length);
   };
   const auto commit = [&](char* s, int k) {
-    a.commit(s, k, length);
-    b.template commit<SUMS>(s + S::kA, k, length, sums);
+    if (k + BK <= length) {
+      commit_fast(s, k);
+    } else {
+      a.template commit<true>(s, k, length);
+      b.template commit<true>(s + S::kA, k, length);
+    }
   };
   const auto fetch = [&](int k) {
     a.fetch(k);
     b.fetch(k);
   };
-  fetch(k_begin);
+  const auto fetch_fast = [&](int k) {
+    a.fetch_fast(k);
+    b.fetch_fast(k);
+  };
+  const int fast = min(a.fast, b.fast);
+  int k = 0;
+  fetch(k);
   if constexpr (S::kStages == 2) {
-    commit(lds, k_begin);
-    if (k_begin + BK < k_end) fetch(k_begin + BK);
+    constexpr int kStage = S::kA + S::kB;
+    commit(lds, k);
+    if (k + BK < length) fetch(k + BK);
     __syncthreads();
     int stage = 0;
-    for (int k = k_begin; k < k_end; k += BK, stage ^= 1) {
-      if (k + BK < k_end) commit(lds + (stage ^ 1) * (S::kA + S::kB), k + BK);
-      if (k + 2 * BK < k_end) fetch(k + 2 * BK);
-      compute(lds + stage * (S::kA + S::kB));
+    read(lds, 0);
+    for (; k + 2 * BK < fast; k += BK, stage ^= 1) {
+      commit_fast(lds + (stage ^ 1) * kStage, k + BK);
+      fetch_fast(k + 2 * BK);
+#pragma unroll
+      for (int step = 0; step + 1 < kSteps; ++step) {
+        read(lds + stage * kStage, step + 1);
+        multiply(step);
+      }
+      interleave<kProducts * (kSteps - 1), kReads * (kSteps - 1), kMoves, kMoves>();
+      __syncthreads();
+      read(lds + (stage ^ 1) * kStage, 0);
+      multiply(kSteps - 1);
+      interleave<kProducts, kReads, 0, 0>();
+    }
+    for (; k < length; k += BK, stage ^= 1) {
+      if (k + BK < length) commit(lds + (stage ^ 1) * kStage, k + BK);
+      if (k + 2 * BK < length) fetch(k + 2 * BK);
+#pragma unroll
+      for (int step = 0; step + 1 < kSteps; ++step) {
+        read(lds + stage * kStage, step + 1);
+        multiply(step);
+      }
+      __syncthreads();
+      if (k + BK < length) read(lds + (stage ^ 1) * kStage, 0);
+      multiply(kSteps - 1);
+    }
+    __syncthreads();
+  } else {
+    const auto compute = [&]() {
+      read(lds, 0);
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step) {
+        if (step + 1 < kSteps) read(lds, step + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(step);
+      }
+    };
+    for (; k + BK < fast; k += BK) {
+      commit_fast(lds, k);
+      __syncthreads();
+      fetch_fast(k + BK);
+      compute();
       __syncthreads();
     }
-  } else {
-    for (int k = k_begin; k < k_end; k += BK) {
+    for (; k < length; k += BK) {
       commit(lds, k);
       __syncthreads();
-      if (k + BK < k_end) fetch(k + BK);
-      compute(lds);
+      if (k + BK < length) fetch(k + BK);
+      compute();
       __syncthreads();
     }
   }
 }
 
-// The wave's sums by rows of the output: 8 columns a lane at a time, through its own part of the LDS.
-// put(row of the tile, column of the tile, its 8 sums)
-template <typename L, typename F>
-__device__ __forceinline__ void dense_rows(char* lds, const f32x16 (&acc)[L::MT][L::NT], F&& put) {
+// The wave's sums by rows of the output, through its own part of the LDS: a lane has eight columns, the same in
+// every row. put(row of the tile, its 8 sums) for each of them, begin(column of the tile) before
+template <typename L, typename G, typename F>
+__device__ __forceinline__ void dense_rows(char* lds, const f32x16 (&acc)[L::MT][L::NT], G&& begin, F&& put) {
   constexpr int kRow = L::NT * 32 + 4, kLanes = L::NT * 4, kRows = kWave / kLanes;
   const int wave = wave_in_block(), lane = threadIdx.x % kWave;
   const int m0 = wave / L::kWavesN * L::MT * 32, n0 = wave % L::kWavesN * L::NT * 32;
   float* s = reinterpret_cast<float*>(lds) + wave * 32 * kRow;
+  begin(n0 + lane % kLanes * 8);
 #pragma unroll
   for (int i = 0; i < L::MT; ++i) {
 #pragma unroll
     for (int j = 0; j < L::NT; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[tile_row(r, lane / 32) * kRow + 32 * j + lane % 32] = acc[i][j][r];
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(s + lane % 32 * kRow + 32 * j + tile_row(4 * q, lane / 32)) =
+            f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
     wave_sync();
 #pragma unroll 4
     for (int r = lane / kLanes; r < 32; r += kRows) {
-      const int c = lane % kLanes * 8;
+      const float* p = s + r * kRow + lane % kLanes * 8;
       float v[8];
-      load_pack<float, 4>(s + r * kRow + c, v);
-      load_pack<float, 4>(s + r * kRow + c + 4, v + 4);
-      put(m0 + 32 * i + r, n0 + c, v);
+      load_pack<float, 4>(p, v);
+      load_pack<float, 4>(p + 4, v + 4);
+      put(m0 + 32 * i + r, v);
     }
     wave_sync();
   }
@@ -438,8 +595,8 @@ __device__ __forceinline__ void load_row_part(const T* row, int at, int width, f
     for (int i = 0; i < N; ++i) out[i] = at + i < width ? (float)row[at + i] : 0.0f;
   }
 }
-template <typename T, int N>
-__device__ __forceinline__ void store_row_part(T* row, int at, int width, const float* in) {
+template <typename T, int N, typename V>
+__device__ __forceinline__ void store_row_part(T* row, int at, int width, const V* in) {
   if (at + N <= width) {
     Pack<T, N> x;
 #pragma unroll
@@ -453,19 +610,30 @@ __device__ __forceinline__ void store_row_part(T* row, int at, int width, const 
 }
 
 // ---------------------------------------------------------------- host side
-template <typename T>
-using Small = Shape<T, 64, 64, 2, 2>;
-template <typename T>
-using Middle = Shape<T, 128, 128, 2, 2>;
-template <typename T>
-using Large = Shape<T, sizeof(T) == 4 ? 128 : 256, 256, 2, 2>;
+template <typename T, int SIZE>
+using Square = Shape<T, SIZE, SIZE, 2, 2>;
 
-// the tile of an output of m x n: 0, 1, 2
+// the side of the tiles of an output of m x n
 inline int dense_tile(size_t size, int64_t m, int64_t n) {
-  const auto tiles = [&](int64_t bm, int64_t bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
-  if (n >= 256 && tiles(size == 4 ? 128 : 256, 256) >= 256) return 2;
-  return tiles(128, 128) >= 256 ? 1 : 0;
+  const auto tiles = [&](int64_t b) { return ((m + b - 1) / b) * ((n + b - 1) / b); };
+  if (size == 2 && n >= 192 && tiles(256) >= 192) return 256;
+  return n > 64 && tiles(128) >= 256 ? 128 : 64;
 }
+
+// call(Square<T, side>) for the side
+#define XNN_TILE_DISPATCH(side, T, L, ...)       \
+  do {                                           \
+    if ((side) == 64) {                          \
+      typedef ::xnn::Square<T, 64> L;            \
+      __VA_ARGS__;                               \
+    } else if ((side) == 128) {                  \
+      typedef ::xnn::Square<T, 128> L;           \
+      __VA_ARGS__;                               \
+    } else if constexpr (sizeof(T) == 2) {       \
+      typedef ::xnn::Square<T, 256> L;           \
+      __VA_ARGS__;                               \
+    }                                            \
+  } while (0)
 
 inline int group_level(int64_t rows) {
   int s = 0;

@@ -32,37 +32,49 @@ __global__ __launch_bounds__(kDenseThreads) void dense_forward_kernel(ForwardArg
     fill_rows<T, L::BN>(p.groups, t, p.n_rows, (T*)p.out, n0, p.n_out, (T)__builtin_nanf(""));
     return;
   }
-  Operator<T, L::BM, true, false> a;
-  Operator<T, L::BN, false, false> b;
-  a.init(p.x, nullptr, p.groups.order, p.x_stride, p.n_rows, p.n_in, t.begin, t.end, 0);
-  b.init((const T*)p.w + (int64_t)t.group * p.n_in * p.n_out, nullptr, nullptr, p.n_out, p.n_in, p.n_out, 0,
-         p.n_in, n0);
+  Operator<T, L::BM, true> a;
+  Operator<T, L::BN, false> b;
+  a.init(p.x, p.groups.order, p.x_stride, p.n_rows, p.n_in, t.begin, t.end, 0);
+  b.init((const T*)p.w + (int64_t)t.group * p.n_in * p.n_out, nullptr, p.n_out, p.n_in, p.n_out, 0, p.n_in, n0);
   f32x16 acc[L::MT][L::NT];
-  dense_product<T, L, true, false, false>(a, b, 0, p.n_in, p.n_in, lds, acc);
-  const T* bias = p.bias == nullptr ? nullptr : (const T*)p.bias + (int64_t)t.group * p.n_out;
-  dense_rows<L>(lds, acc, [&](int m, int n, float (&v)[8]) {
-    const int r = t.begin + m, c = n0 + n;
-    if (r >= t.end || c >= p.n_out) return;
-    const int64_t row = group_row(p.groups, r);
-    if (row < 0 || row >= p.n_rows) return;
-    float z[8], s[8];
-    if (bias != nullptr) {
-      load_row_part<T, 8>(bias, c, p.n_out, z);
+  dense_product<T, L, true, false>(a, b, p.n_in, lds, acc);
+  typedef typename Slope<T>::type S1;
+  int c;
+  float bias[8];
+  dense_rows<L>(
+      lds, acc,
+      [&](int n) {
+        c = n0 + n;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += z[i];
-    }
-    if (p.activation != kNone) {
+        for (int i = 0; i < 8; ++i) bias[i] = 0.0f;
+        if (p.bias != nullptr && c < p.n_out)
+          load_row_part<T, 8>((const T*)p.bias + (int64_t)t.group * p.n_out, c, p.n_out, bias);
+      },
+      [&](int m, float(&v)[8]) {
+        const int r = t.begin + m;
+        if (r >= t.end || c >= p.n_out) return;
+        const int64_t row = group_row(p.groups, r);
+        if (row < 0 || row >= p.n_rows) return;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) activate(p.activation, v[i], v[i], s[i]);
-      if (p.slope != nullptr) store_row_part<T, 8>((T*)p.slope + row * p.n_out, c, p.n_out, s);
-    }
-    if (p.residual != nullptr) {
-      load_row_part<T, 8>((const T*)p.residual + row * p.n_out, c, p.n_out, z);
+        for (int i = 0; i < 8; ++i) v[i] += bias[i];
+        if (p.activation != kNone) {
+          S1 slope[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += z[i];
-    }
-    store_row_part<T, 8>((T*)p.out + row * p.n_out, c, p.n_out, v);
-  });
+          for (int i = 0; i < 8; ++i) {
+            float s;
+            activate(p.activation, v[i], v[i], s);
+            slope[i] = slope_stored<T>(s);
+          }
+          if (p.slope != nullptr) store_row_part<S1, 8>((S1*)p.slope + row * p.n_out, c, p.n_out, slope);
+        }
+        if (p.residual != nullptr) {
+          float z[8];
+          load_row_part<T, 8>((const T*)p.residual + row * p.n_out, c, p.n_out, z);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] += z[i];
+        }
+        store_row_part<T, 8>((T*)p.out + row * p.n_out, c, p.n_out, v);
+      });
 }
 
 template <typename T, typename L>
@@ -103,13 +115,8 @@ int xnn_linear(int dtype, const void* x, int64_t x_stride, int64_t n_rows, int32
   p.n_out = n_out;
   p.activation = activation;
   hipStream_t s = as_hip(stream);
-  XNN_STORAGE_DISPATCH(dtype, T, {
-    switch (dense_tile(sizeof(T), n_rows, n_out)) {
-      case 0: forward_launch<T, Small<T>>(p, plan, n_groups, s); break;
-      case 1: forward_launch<T, Middle<T>>(p, plan, n_groups, s); break;
-      default: forward_launch<T, Large<T>>(p, plan, n_groups, s);
-    }
-  });
+  const int side = dense_tile(storage_bytes(dtype), n_rows, n_out);
+  XNN_STORAGE_DISPATCH(dtype, T, XNN_TILE_DISPATCH(side, T, L, forward_launch<T, L>(p, plan, n_groups, s)));
   XNN_LAUNCH_CHECK();
   return XNN_OK;
 }

@@ -236,6 +236,9 @@ Three dense_backward(const Tensor& grad, const MaybeTensor& slope, const Tensor&
   return op.call(grad, slope, x, weight, plan, input, weights, biases);
 }
 
+// the slope's own form: two bytes an element beside the 16-bit types
+at::ScalarType slope_type(const Tensor& x) { return x.scalar_type() == at::kFloat ? at::kFloat : at::kShort; }
+
 // the sizes of an operation's operands
 struct Dense {
   int64_t rows, n_in, n_out, groups;
@@ -284,7 +287,9 @@ Two dense_forward(XNN_DENSE_ARGUMENTS, bool keep) {
   const c10::DeviceGuard guard(x.device());
   const Tensor rows = as_rows(x), w = weight.contiguous();
   Tensor out = at::empty(d.out, x.options()), slope;
-  if (keep) slope = empty_if(activation != XNN_NO_ACTIVATION, d.out, x);
+  if (keep)
+    slope = at::empty(activation != XNN_NO_ACTIVATION ? at::IntArrayRef(d.out) : at::IntArrayRef({0}),
+                      x.options().dtype(slope_type(x)));
   XNN_CALL(xnn_linear, storage_code(x), data(rows), row_stride(rows), d.rows, (int32_t)d.n_in, (int32_t)d.n_out,
            data(w), data(b), (int32_t)activation, data(r), (const int32_t*)data(p), (int32_t)d.groups, data(out),
            data_if(keep && activation != XNN_NO_ACTIVATION, slope), stream_of(x));
@@ -305,7 +310,8 @@ Tensor dense_shape(XNN_DENSE_ARGUMENTS) {
 }
 Two dense_slope_shape(XNN_DENSE_ARGUMENTS) {
   const Tensor out = dense_shape(x, weight, bias, activation, residual, plan);
-  return {out, empty_shape(activation != XNN_NO_ACTIVATION, out)};
+  const auto options = x.options().dtype(slope_type(x));
+  return {out, activation != XNN_NO_ACTIVATION ? at::empty_symint(out.sym_sizes(), options) : at::empty({0}, options)};
 }
 
 Three dense_backward_kernel(const Tensor& grad_, const MaybeTensor& slope_, const Tensor& x, const Tensor& weight,
@@ -314,20 +320,18 @@ Three dense_backward_kernel(const Tensor& grad_, const MaybeTensor& slope_, cons
   check_tensors({&x, &grad_, &slope, &weight, &p});
   const Dense d = check_dense(x, weight, p);
   check_like(grad_, x, d.out, "the cotangent");
-  check_like(slope, x, d.out, "the slope");
-  weights = weights || biases;                             // the weight's product has the bias's sums
+  TORCH_CHECK_VALUE(!slope.defined() || (slope.sizes() == d.out && slope.scalar_type() == slope_type(x)),
+                    "the slope is not that of the forward pass");
   const c10::DeviceGuard guard(x.device());
   const Tensor rows = as_rows(x), w = weight.contiguous(), grad = grad_.contiguous();
   const Tensor dx = empty_if(input, x.sizes(), x), dw = empty_if(weights, weight.sizes(), x),
                db = empty_if(biases, d.bias, x);
   Tensor work;
   size_t need = 0;
-  if (weights) {
-    check("xnn_linear_backward_work_size",
-          api.xnn_linear_backward_work_size(storage_code(x), d.rows, (int32_t)d.n_in, (int32_t)d.n_out,
-                                            (int32_t)d.groups, p.defined(), &need));
-    if (need > 0) work = bytes(x, need);
-  }
+  check("xnn_linear_backward_work_size",
+        api.xnn_linear_backward_work_size(storage_code(x), d.rows, (int32_t)d.n_in, (int32_t)d.n_out,
+                                          (int32_t)d.groups, p.defined(), slope.defined(), weights, biases, &need));
+  if (need > 0) work = bytes(x, need);
   XNN_CALL(xnn_linear_backward, storage_code(x), data(grad), data(slope), data(rows), row_stride(rows), d.rows,
            (int32_t)d.n_in, (int32_t)d.n_out, data(w), (const int32_t*)data(p), (int32_t)d.groups,
            data_if(input, dx), data_if(weights, dw), data_if(biases, db), data(work), need, stream_of(x));
@@ -339,7 +343,7 @@ Three dense_backward_shape(const Tensor&, const MaybeTensor&, const Tensor& x, c
   std::vector<c10::SymInt> bias;
   if (or_none(plan).defined()) bias.push_back(weight.sym_size(0));
   bias.push_back(weight.sym_size(-1));
-  return {empty_shape(input, x), empty_shape(weights || biases, weight),
+  return {empty_shape(input, x), empty_shape(weights, weight),
           biases ? at::empty_symint(bias, x.options()) : at::empty({0}, x.options())};
 }
 
