@@ -169,7 +169,6 @@ def _check_dense(dtype, case, activation):
     grads = list(torch.autograd.grad(out, [t for t in leaves if t is not None], g))
     out = out.detach()
     K, N, u = x.shape[1], w.shape[-1], _u(dtype)
-    exact = dtype == "f32"
     tiny = TINY[dtype]
     seen = torch.zeros(len(x), dtype=torch.bool, device=DEV)
     for group in range(1 if ids is None else w.shape[0]):
@@ -189,10 +188,13 @@ def _check_dense(dtype, case, activation):
         _close(out[rows], want, bound, f"output of {group}")
         gd = g[rows].double()
         d = gd * slope
-        # f' changes by at most |f''| <= 1; its root is kept in units of 1 / 30,000 (16-bit types), so it is off by
-        # 2 root(f') e + e^2 with e half a unit; d is rounded to the type
-        e = 0.0 if activation is None or exact else 1.01 / 60000
-        dd = gd.abs() * (dz + f32 * (1 + z.abs()) + 2 * e * slope.abs().sqrt() + e * e)
+        # f' changes by at most |f''| <= 1. It is kept in float16 beside bfloat16; beside float16 its root is, in units
+        # of 1 / 30,000, so it is off by 2 root(f') e + e^2 with e half a unit. d is rounded to the type
+        e = 0.0 if activation is None or dtype != "f16" else 1.01 / 60000
+        kept = 2 * e * slope.abs().sqrt() + e * e
+        if dtype == "bf16" and activation is not None:
+            kept = 2.0 ** -11 * slope.abs() + 2.0 ** -24
+        dd = gd.abs() * (dz + f32 * (1 + z.abs()) + kept)
         dd = dd + (0 if activation is None else u * d.abs() + tiny)
         dx = d @ wd.t()
         _close(grads[0][rows], dx, _term(dtype, N) * (d.abs() @ wd.abs().t()) + dd @ wd.abs().t() + u * dx.abs() + tiny,

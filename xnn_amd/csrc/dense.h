@@ -145,59 +145,59 @@ __device__ __forceinline__ void activate(int kind, float z, float& y, float& slo
   }
 }
 
-// f'(z) as the backward pass gets it: float32 as it is; for the 16-bit types its root with its sign in 15 bits of
-// fixed point (f' is below 1.13), off by 2^-15 of it at most near 1 and by less below, so that d = g f'(z) is
-// rounded once and not twice (the gradients' error in bfloat16 1.4 times an output's rounding, 1.7 with f' in it).
-// The number below -32,767 stands for NaN.
+// f'(z) as the backward pass gets it, so that d = g f'(z) is rounded once and not twice (the gradients' error is 1.4
+// times an output's rounding, 1.7 with f' in the type): float32 as it is, for bfloat16 a float16; for float16 its
+// root with its sign in 15 bits of fixed point (f' is below 1.13), off by 2^-15 near 1, the number below -32,767
+// standing for NaN
 template <typename T>
 struct Slope {
-  typedef int16_t type;
+  typedef T type;
 };
 template <>
-struct Slope<float> {
-  typedef float type;
+struct Slope<bf16_t> {
+  typedef f16_t type;
+};
+template <>
+struct Slope<f16_t> {
+  typedef int16_t type;
 };
 constexpr float kSlopeUnit = 30000.0f;
 template <typename T>
 __device__ __forceinline__ typename Slope<T>::type slope_stored(float s) {
-  if constexpr (sizeof(T) == 4)
-    return s;
+  if constexpr (!__is_same(T, f16_t))
+    return (typename Slope<T>::type)s;
   else
     return s == s ? (int16_t)__float2int_rn(copysignf(kSlopeUnit * __builtin_amdgcn_sqrtf(fabsf(s)), s))
                   : (int16_t)-32768;
 }
 template <typename T>
 __device__ __forceinline__ float slope_value(typename Slope<T>::type s) {
-  if constexpr (sizeof(T) == 4)
-    return s;
+  if constexpr (!__is_same(T, f16_t))
+    return (float)s;
   else
     return s == -32768 ? __builtin_nanf("") : (float)s * fabsf((float)s) * (1.0f / (kSlopeUnit * kSlopeUnit));
 }
 
 // ---------------------------------------------------------------- sizes
-// BK: 64 elements of the reduction a step in 16 bits, 32 in float32 (eight 16-byte pieces of a row each)
-template <typename T, int BM_, int BN_, int WM_, int WN_>
+// BK: elements of the reduction a step
+template <typename T, int BM_, int BN_, int WM_, int WN_, int BK_>
 struct Shape {
   static constexpr int BM = BM_, BN = BN_, kWavesM = WM_, kWavesN = WN_;
   static constexpr int MT = BM / WM_ / 32, NT = BN / WN_ / 32;   // 32 x 32 products of a wave
-  static constexpr int BK = 128 / sizeof(T);
-  static constexpr int kPer = 16 / sizeof(T);
-  static constexpr int kPlanes = Store<T>::kPlanes;
+  static constexpr int BK = BK_;
   static_assert(WM_ * WN_ == kDenseWaves, "");
 };
 
 // an operand in LDS: ROWS outer indices
-template <typename T, int ROWS, bool ALONG>
+template <typename T, int ROWS, int BK, bool ALONG>
 struct Place;
-template <typename T, int ROWS>
-struct Place<T, ROWS, true> {      // rows along the reduction; 16 bytes more spread the banks
-  static constexpr int BK = 128 / sizeof(T);
+template <typename T, int ROWS, int BK>
+struct Place<T, ROWS, BK, true> {  // rows along the reduction; 16 bytes more spread the banks
   static constexpr int kRow = BK * 2 + 16, kPlane = ROWS * kRow;
   static constexpr int kBytes = kPlane * Store<T>::kPlanes;
 };
-template <typename T, int ROWS>
-struct Place<T, ROWS, false> {     // rows across it; 64 more: four rows of a transposing read on other banks
-  static constexpr int BK = 128 / sizeof(T);
+template <typename T, int ROWS, int BK>
+struct Place<T, ROWS, BK, false> { // rows across it; 64 more: four rows of a transposing read on other banks
   static constexpr int kRow = ROWS * 2 + 64, kPlane = BK * kRow;
   static constexpr int kBytes = kPlane * Store<T>::kPlanes;
 };
@@ -267,15 +267,15 @@ __device__ __forceinline__ void put_piece(char* at, int plane, u32x4 x) {
 // Steps that begin before `fast` are of whole pieces, one address each that the step before has left: along the rows
 // those that end within them; across them all but the last one where a piece may reach beyond its row (the
 // tensor's last row is the last of its group).
-template <typename T, int LEN, bool ALONG>
+template <typename T, int LEN, int BK, bool ALONG>
 struct Operator {
-  static constexpr int BK = 128 / sizeof(T), kPer = 16 / sizeof(T);
+  static constexpr int kPer = 16 / sizeof(T);
   static constexpr int kRows = ALONG ? LEN : BK, kCols = ALONG ? BK : LEN;   // of a staged step
   static constexpr int kChunks = kCols / kPer;
   static constexpr int kStep = kDenseThreads / kChunks;
   static constexpr int kCount = kRows / kStep;
   static_assert(kDenseThreads % kChunks == 0 && kRows % kStep == 0 && kCount <= 32, "");
-  typedef Place<T, LEN, ALONG> At;
+  typedef Place<T, LEN, BK, ALONG> At;
 
   const char *data, *column;       // the tensor, and the thread's first piece of its row 0
   const int32_t* order;            // from `first` on
@@ -325,7 +325,7 @@ struct Operator {
 #pragma unroll
         for (int n = 0; n < kCount; ++n) p[n] = column + min(index[n], most) * stride;
       }
-    const int64_t step = ALONG ? 128 : BK * stride;
+    const int64_t step = ALONG ? BK * (int)sizeof(T) : BK * stride;
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {
       x[n] = load_raw(p[n]);
@@ -350,7 +350,7 @@ struct Operator {
       const int left = width - at - (ALONG ? k0 : 0);
       const bool edge = (ALONG ? (edges >> n & 1) != 0 : i == last) || stride < 16;
       x[n] = load_raw<T>(q, left, edge);
-      if (ALONG) p[n] += 128;
+      if (ALONG) p[n] += BK * (int)sizeof(T);
     }
   }
   // to LDS, TAIL: zeros beyond the reduction's `length`
@@ -367,9 +367,9 @@ struct Operator {
 };
 
 // operand `step` of 16 reduction indices for the 32 outer indices from `outer` on
-template <typename T, int LEN, bool ALONG>
+template <typename T, int LEN, int BK, bool ALONG>
 __device__ __forceinline__ Operand<T> dense_operand(const char* lds, int outer, int step) {
-  typedef Place<T, LEN, ALONG> At;
+  typedef Place<T, LEN, BK, ALONG> At;
   const int lane = threadIdx.x % kWave, half = lane / 32;
   Operand<T> out;
   if constexpr (ALONG) {
@@ -413,7 +413,8 @@ __device__ __forceinline__ Pack<T, N> load_piece(const T* row, int at, int width
 // LDS of a block: one stage of both operands, and the waves' rows on their way out
 template <typename L, typename T, bool ALONG_A, bool ALONG_B>
 struct DenseLds {
-  static constexpr int kA = Place<T, L::BM, ALONG_A>::kBytes, kB = Place<T, L::BN, ALONG_B>::kBytes;
+  static constexpr int kA = Place<T, L::BM, L::BK, ALONG_A>::kBytes,
+                       kB = Place<T, L::BN, L::BK, ALONG_B>::kBytes;
   static constexpr int kOutRow = L::NT * 32 + 4;                         // floats
   static constexpr int kOut = kDenseWaves * 32 * kOutRow * 4;
   static constexpr int kPlanes = Store<T>::kPlanes;
@@ -455,10 +456,10 @@ __device__ __forceinline__ void dense_product(A& a, B& b, int length, char* lds,
   Operand<T> fa[2][L::MT], fb[2][L::NT];
   const auto read = [&](const char* s, int step) {
 #pragma unroll
-    for (int i = 0; i < L::MT; ++i) fa[step & 1][i] = dense_operand<T, L::BM, ALONG_A>(s, m0 + 32 * i, step);
+    for (int i = 0; i < L::MT; ++i) fa[step & 1][i] = dense_operand<T, L::BM, BK, ALONG_A>(s, m0 + 32 * i, step);
 #pragma unroll
     for (int j = 0; j < L::NT; ++j)
-      fb[step & 1][j] = dense_operand<T, L::BN, ALONG_B>(s + S::kA, n0 + 32 * j, step);
+      fb[step & 1][j] = dense_operand<T, L::BN, BK, ALONG_B>(s + S::kA, n0 + 32 * j, step);
   };
   const auto multiply = [&](int step) {
 #pragma unroll
@@ -553,15 +554,15 @@ __device__ __forceinline__ void dense_product(A& a, B& b, int length, char* lds,
   }
 }
 
-// The wave's sums by rows of the output, through its own part of the LDS: a lane has eight columns, the same in
-// every row. put(row of the tile, its 8 sums) for each of them, begin(column of the tile) before
-template <typename L, typename G, typename F>
+// The wave's sums by rows of the output, through its own part of the LDS: a lane has the N columns of a 16-byte store,
+// the same in every row. put(row of the tile, its N sums) for each of them, begin(column of the tile) before
+template <typename L, int N, typename G, typename F>
 __device__ __forceinline__ void dense_rows(char* lds, const f32x16 (&acc)[L::MT][L::NT], G&& begin, F&& put) {
-  constexpr int kRow = L::NT * 32 + 4, kLanes = L::NT * 4, kRows = kWave / kLanes;
+  constexpr int kRow = L::NT * 32 + 4, kLanes = L::NT * 32 / N, kRows = kWave / kLanes;
   const int wave = wave_in_block(), lane = threadIdx.x % kWave;
   const int m0 = wave / L::kWavesN * L::MT * 32, n0 = wave % L::kWavesN * L::NT * 32;
   float* s = reinterpret_cast<float*>(lds) + wave * 32 * kRow;
-  begin(n0 + lane % kLanes * 8);
+  begin(n0 + lane % kLanes * N);
 #pragma unroll
   for (int i = 0; i < L::MT; ++i) {
 #pragma unroll
@@ -573,10 +574,10 @@ __device__ __forceinline__ void dense_rows(char* lds, const f32x16 (&acc)[L::MT]
     wave_sync();
 #pragma unroll 4
     for (int r = lane / kLanes; r < 32; r += kRows) {
-      const float* p = s + r * kRow + lane % kLanes * 8;
-      float v[8];
-      load_pack<float, 4>(p, v);
-      load_pack<float, 4>(p + 4, v + 4);
+      const float* p = s + r * kRow + lane % kLanes * N;
+      float v[N];
+#pragma unroll
+      for (int q = 0; q < N; q += 4) load_pack<float, 4>(p + q, v + q);
       put(m0 + 32 * i + r, v);
     }
     wave_sync();
@@ -610,29 +611,42 @@ __device__ __forceinline__ void store_row_part(T* row, int at, int width, const 
 }
 
 // ---------------------------------------------------------------- host side
-template <typename T, int SIZE>
-using Square = Shape<T, SIZE, SIZE, 2, 2>;
+// Tiles: 64 x 64; 128 x 128; in 16 bits 256 x 128, whose steps of 32 leave LDS and registers for two blocks a CU, one
+// in its products while the other loads or stores (24,000 x 1,024 x 4,096 in bfloat16 with gelu: 256 x 256, one
+// block a CU, 495 us; 256 x 128 423; 128 x 128 in steps of 64 470).
+enum TileKind : int { kTile64 = 0, kTile128 = 1, kTile256 = 2 };
+template <typename T>
+using Tile64 = Shape<T, 64, 64, 2, 2, 128 / sizeof(T)>;
+template <typename T>
+using Tile128 = Shape<T, 128, 128, 2, 2, 128 / sizeof(T)>;
+template <typename T>
+using Tile256 = Shape<T, 256, 128, 2, 2, 32>;
 
-// the side of the tiles of an output of m x n
-inline int dense_tile(size_t size, int64_t m, int64_t n) {
-  const auto tiles = [&](int64_t b) { return ((m + b - 1) / b) * ((n + b - 1) / b); };
-  if (size == 2 && n >= 192 && tiles(256) >= 192) return 256;
-  return n > 64 && tiles(128) >= 256 ? 128 : 64;
+// The kind for an output of m x n, in `groups` of rows where they are grouped (then a group's last tile is half empty).
+// 256 x 128 tiles pay where they come in full rounds of two a CU (9,000 x 512 x 2,048 with silu, 1.1 rounds: 78 us,
+// 128 x 128 57; 24,000 x 1,024 x 4,096, 5.9: 423 and 470), 64 x 64 where 128 x 128 are not one a CU
+// (1,000^3: 10 us, 128 x 128 21).
+inline int dense_tile(size_t size, int64_t m, int64_t n, int64_t groups) {
+  const auto rounds = [&](int64_t bm, int64_t bn) {
+    return (double)(m / bm + (groups + 1) / 2 + 1) * (double)((n + bn - 1) / bn) / 512;
+  };
+  if (n <= 64 || rounds(128, 128) < 0.5) return kTile64;
+  return size == 2 && 1.8 * std::ceil(rounds(256, 128)) <= std::ceil(rounds(128, 128)) ? kTile256 : kTile128;
 }
 
-// call(Square<T, side>) for the side
-#define XNN_TILE_DISPATCH(side, T, L, ...)       \
-  do {                                           \
-    if ((side) == 64) {                          \
-      typedef ::xnn::Square<T, 64> L;            \
-      __VA_ARGS__;                               \
-    } else if ((side) == 128) {                  \
-      typedef ::xnn::Square<T, 128> L;           \
-      __VA_ARGS__;                               \
-    } else if constexpr (sizeof(T) == 2) {       \
-      typedef ::xnn::Square<T, 256> L;           \
-      __VA_ARGS__;                               \
-    }                                            \
+// call(Shape) for the kind
+#define XNN_TILE_DISPATCH(kind, T, L, ...)           \
+  do {                                               \
+    if ((kind) == kTile64) {                         \
+      typedef ::xnn::Tile64<T> L;                    \
+      __VA_ARGS__;                                   \
+    } else if (sizeof(T) == 4 || (kind) == kTile128) { \
+      typedef ::xnn::Tile128<T> L;                   \
+      __VA_ARGS__;                                   \
+    } else if constexpr (sizeof(T) == 2) {           \
+      typedef ::xnn::Tile256<T> L;                   \
+      __VA_ARGS__;                                   \
+    }                                                \
   } while (0)
 
 inline int group_level(int64_t rows) {

@@ -32,48 +32,50 @@ __global__ __launch_bounds__(kDenseThreads) void dense_forward_kernel(ForwardArg
     fill_rows<T, L::BN>(p.groups, t, p.n_rows, (T*)p.out, n0, p.n_out, (T)__builtin_nanf(""));
     return;
   }
-  Operator<T, L::BM, true> a;
-  Operator<T, L::BN, false> b;
+  Operator<T, L::BM, L::BK, true> a;
+  Operator<T, L::BN, L::BK, false> b;
   a.init(p.x, p.groups.order, p.x_stride, p.n_rows, p.n_in, t.begin, t.end, 0);
   b.init((const T*)p.w + (int64_t)t.group * p.n_in * p.n_out, nullptr, p.n_out, p.n_in, p.n_out, 0, p.n_in, n0);
   f32x16 acc[L::MT][L::NT];
   dense_product<T, L, true, false>(a, b, p.n_in, lds, acc);
-  typedef typename Slope<T>::type S1;
+  typedef typename Slope<T>::type SlopeType;
+  constexpr int N = 16 / sizeof(T);
   int c;
-  float bias[8];
-  dense_rows<L>(
+  float bias[N];
+  dense_rows<L, N>(
       lds, acc,
       [&](int n) {
         c = n0 + n;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) bias[i] = 0.0f;
+        for (int i = 0; i < N; ++i) bias[i] = 0.0f;
         if (p.bias != nullptr && c < p.n_out)
-          load_row_part<T, 8>((const T*)p.bias + (int64_t)t.group * p.n_out, c, p.n_out, bias);
+          load_row_part<T, N>((const T*)p.bias + (int64_t)t.group * p.n_out, c, p.n_out, bias);
       },
-      [&](int m, float(&v)[8]) {
+      [&](int m, float(&v)[N]) {
         const int r = t.begin + m;
         if (r >= t.end || c >= p.n_out) return;
         const int64_t row = group_row(p.groups, r);
         if (row < 0 || row >= p.n_rows) return;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += bias[i];
+        for (int i = 0; i < N; ++i) v[i] += bias[i];
         if (p.activation != kNone) {
-          S1 slope[8];
+          SlopeType slope[N];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < N; ++i) {
             float s;
             activate(p.activation, v[i], v[i], s);
             slope[i] = slope_stored<T>(s);
           }
-          if (p.slope != nullptr) store_row_part<S1, 8>((S1*)p.slope + row * p.n_out, c, p.n_out, slope);
+          if (p.slope != nullptr)
+            store_row_part<SlopeType, N>((SlopeType*)p.slope + row * p.n_out, c, p.n_out, slope);
         }
         if (p.residual != nullptr) {
-          float z[8];
-          load_row_part<T, 8>((const T*)p.residual + row * p.n_out, c, p.n_out, z);
+          float z[N];
+          load_row_part<T, N>((const T*)p.residual + row * p.n_out, c, p.n_out, z);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] += z[i];
+          for (int i = 0; i < N; ++i) v[i] += z[i];
         }
-        store_row_part<T, 8>((T*)p.out + row * p.n_out, c, p.n_out, v);
+        store_row_part<T, N>((T*)p.out + row * p.n_out, c, p.n_out, v);
       });
 }
 
@@ -115,8 +117,8 @@ int xnn_linear(int dtype, const void* x, int64_t x_stride, int64_t n_rows, int32
   p.n_out = n_out;
   p.activation = activation;
   hipStream_t s = as_hip(stream);
-  const int side = dense_tile(storage_bytes(dtype), n_rows, n_out);
-  XNN_STORAGE_DISPATCH(dtype, T, XNN_TILE_DISPATCH(side, T, L, forward_launch<T, L>(p, plan, n_groups, s)));
+  const int kind = dense_tile(storage_bytes(dtype), n_rows, n_out, plan != nullptr ? n_groups : 0);
+  XNN_STORAGE_DISPATCH(dtype, T, XNN_TILE_DISPATCH(kind, T, L, forward_launch<T, L>(p, plan, n_groups, s)));
   XNN_LAUNCH_CHECK();
   return XNN_OK;
 }

@@ -20,10 +20,11 @@ struct BackwardArgs {
   const void *g, *slope, *x, *w;   // g: d where there is a slope (the products')
   void *d, *dx, *dw, *db;
   float *part, *part_bias;         // the parts' sums
-  int64_t x_stride, tiles;
+  int64_t x_stride, tiles, parts;  // parts: of the weight's sums, at most
   GroupView groups, bias_groups;
   int n_rows, n_in, n_out, tiles_m, tiles_n;
   int rows, bias_rows;             // of a part of the weight's sums, of the bias's
+  int spread;                      // parts of different lengths: to the XCDs in turn
 };
 
 // Where the sums of the part of sorted rows from `begin` on stand: parts of one weight follow each other; among
@@ -53,7 +54,7 @@ __global__ __launch_bounds__(256) void dense_cotangent_kernel(BackwardArgs p, in
 #pragma unroll
   for (int i = 0; i < N; ++i) sum[i] = 0.0f;
   if (c < p.n_out)
-#pragma unroll 2
+#pragma unroll 4
     for (int r = t.begin + slot; r < t.end; r += slots) {
       const int64_t row = group_row(p.bias_groups, r);
       if (row < 0 || row >= p.n_rows) continue;
@@ -102,23 +103,31 @@ __global__ __launch_bounds__(kDenseThreads) void dense_input_kernel(BackwardArgs
     fill_rows<T, L::BN>(p.groups, t, p.n_rows, (T*)p.dx, n0, p.n_in, (T)0.0f);
     return;
   }
-  Operator<T, L::BM, true> a;
-  Operator<T, L::BN, true> b;
+  Operator<T, L::BM, L::BK, true> a;
+  Operator<T, L::BN, L::BK, true> b;
   a.init(p.g, p.groups.order, p.n_out, p.n_rows, p.n_out, t.begin, t.end, 0);
   b.init((const T*)p.w + (int64_t)t.group * p.n_in * p.n_out, nullptr, p.n_out, p.n_in, p.n_out, n0,
          min(n0 + L::BN, p.n_in), 0);
   f32x16 acc[L::MT][L::NT];
   dense_product<T, L, true, true>(a, b, p.n_out, lds, acc);
+  constexpr int N = 16 / sizeof(T);
   int c;
-  dense_rows<L>(
+  dense_rows<L, N>(
       lds, acc, [&](int n) { c = n0 + n; },
-      [&](int m, float(&v)[8]) {
+      [&](int m, float(&v)[N]) {
         const int r = t.begin + m;
         if (r >= t.end || c >= p.n_in) return;
         const int64_t row = group_row(p.groups, r);
         if (row < 0 || row >= p.n_rows) return;
-        store_row_part<T, 8>((T*)p.dx + row * p.n_in, c, p.n_in, v);
+        store_row_part<T, N>((T*)p.dx + row * p.n_in, c, p.n_in, v);
       });
+}
+
+// the parts go to the XCDs in turn, a part's tiles to one
+__device__ __forceinline__ int64_t slot_of_xcd(int64_t tiles, int64_t& tile) {
+  const int64_t i = blockIdx.x / kXcds;
+  tile = i % tiles;
+  return i / tiles * kXcds + blockIdx.x % kXcds;
 }
 
 template <typename T, typename L>
@@ -126,14 +135,19 @@ __global__ __launch_bounds__(kDenseThreads) void dense_weight_kernel(BackwardArg
   typedef DenseLds<L, T, false, false> S;
   __shared__ __align__(16) char lds[S::kBytes];
   const int64_t slot = xcd_slot();
-  if (slot >= p.tiles) return;
-  const int tile = (int)(slot % (p.tiles_m * p.tiles_n));
-  const int m0 = tile / p.tiles_n * L::BM, n0 = tile % p.tiles_n * L::BN;
-  const int part = (int)(slot / (p.tiles_m * p.tiles_n));
-  const RowTile t = row_tile(p.groups, p.groups.n_groups, p.n_rows, part, p.rows);
+  int64_t part, tile;
+  if (p.spread) {
+    part = slot_of_xcd(p.tiles_m * p.tiles_n, tile);
+  } else {
+    part = slot / (p.tiles_m * p.tiles_n);
+    tile = slot % (p.tiles_m * p.tiles_n);
+  }
+  if (part >= p.parts) return;
+  const int m0 = (int)(tile / p.tiles_n) * L::BM, n0 = (int)(tile % p.tiles_n) * L::BN;
+  const RowTile t = row_tile(p.groups, p.groups.n_groups, p.n_rows, (int)part, p.rows);
   if (t.group < 0) return;
-  Operator<T, L::BM, false> a;
-  Operator<T, L::BN, false> b;
+  Operator<T, L::BM, L::BK, false> a;
+  Operator<T, L::BN, L::BK, false> b;
   a.init(p.x, p.groups.order, p.x_stride, p.n_rows, p.n_in, t.begin, t.end, m0);
   b.init(p.g, p.groups.order, p.n_out, p.n_rows, p.n_out, t.begin, t.end, n0);
   f32x16 acc[L::MT][L::NT];
@@ -144,71 +158,77 @@ __global__ __launch_bounds__(kDenseThreads) void dense_weight_kernel(BackwardArg
   T* dw = (T*)p.dw + (int64_t)t.group * p.n_in * p.n_out;
   float* sum = p.part + at * p.n_in * p.n_out;
   int c;
-  dense_rows<L>(
-      lds, acc, [&](int n) { c = n0 + n; },
-      [&](int m, float(&v)[8]) {
-        const int r = m0 + m;
-        if (r >= p.n_in || c >= p.n_out) return;
-        if (only)
-          store_row_part<T, 8>(dw + (int64_t)r * p.n_out, c, p.n_out, v);
-        else
-          store_row_part<float, 8>(sum + (int64_t)r * p.n_out, c, p.n_out, v);
-      });
+  if (only) {
+    constexpr int N = 16 / sizeof(T);
+    dense_rows<L, N>(
+        lds, acc, [&](int n) { c = n0 + n; },
+        [&](int m, float(&v)[N]) {
+          if (m0 + m < p.n_in && c < p.n_out)
+            store_row_part<T, N>(dw + (int64_t)(m0 + m) * p.n_out, c, p.n_out, v);
+        });
+  } else {
+    dense_rows<L, 4>(
+        lds, acc, [&](int n) { c = n0 + n; },
+        [&](int m, float(&v)[4]) {
+          if (m0 + m < p.n_in && c < p.n_out)
+            store_row_part<float, 4>(sum + (int64_t)(m0 + m) * p.n_out, c, p.n_out, v);
+        });
+  }
 }
 
 // ---------------------------------------------------------------- the parts
-// the sum over the parts of a group of element k of `size` (4 of them in a row), in the parts' order; false where the
-// group's only part has written it
-template <int N>
-__device__ __forceinline__ bool part_sum(const GroupView& v, int n_rows, int rows, int group, const float* part,
-                                         int64_t size, int64_t k, float (&out)[N]) {
-  int begin = 0, parts = (n_rows + rows - 1) / rows;
-  if (v.n_groups > 0) {
-    begin = min(max(v.row_ptr[group], 0), n_rows);
-    parts = min(v.tile_ptr[group + 1] - v.tile_ptr[group], (n_rows - begin + rows - 1) / rows);
-  }
-  if (parts == 1) return false;
-#pragma unroll
-  for (int i = 0; i < N; ++i) out[i] = 0.0f;
-#pragma unroll 4
-  for (int n = 0; n < parts; ++n) {
-    const float* p = part + part_slot(v, begin + n * rows, rows, n == 0) * size + k;
-    float x[N];
-    if constexpr (N == 1)
-      x[0] = *p;
-    else
-      load_row_part<float, N>(p, 0, N, x);
-#pragma unroll
-    for (int i = 0; i < N; ++i) out[i] += x[i];
-  }
-  return true;
+// the parts of a group, and where its sorted rows begin
+__device__ __forceinline__ int group_parts(const GroupView& v, int n_rows, int rows, int group, int& begin) {
+  begin = 0;
+  if (v.n_groups == 0) return (n_rows + rows - 1) / rows;
+  begin = min(max(v.row_ptr[group], 0), n_rows);
+  return min(v.tile_ptr[group + 1] - v.tile_ptr[group], (n_rows - begin + rows - 1) / rows);
 }
 
-// The parts of a weight and of its bias added in their order, zeros where there is none
+// the parts of a weight added in their order, zeros where there is none; a group's only part is done
 template <typename T>
 __global__ __launch_bounds__(256) void dense_join_kernel(BackwardArgs p, int blocks) {
-  const int g = blockIdx.x / blocks, block = blockIdx.x % blocks;
+  const int g = blockIdx.x / blocks;
   const int64_t size = (int64_t)p.n_in * p.n_out;
+  int begin;
+  const int parts = group_parts(p.groups, p.n_rows, p.rows, g, begin);
+  if (parts == 1) return;
   T* dw = (T*)p.dw + g * size;
-  for (int64_t k = ((int64_t)block * 256 + threadIdx.x) * 4; p.dw != nullptr && k < size; k += (int64_t)blocks * 1024) {
-    float v[4];
-    if (k + 4 <= size) {
-      if (!part_sum<4>(p.groups, p.n_rows, p.rows, g, p.part, size, k, v)) break;
-      store_row_part<T, 4>(dw + k, 0, 4, v);
-    } else {
-      for (int64_t e = k; e < size; ++e) {
-        float one[1];
-        if (!part_sum<1>(p.groups, p.n_rows, p.rows, g, p.part, size, e, one)) break;
-        dw[e] = (T)one[0];
-      }
+  for (int64_t k = ((int64_t)(blockIdx.x % blocks) * 256 + threadIdx.x) * 4; k < size; k += (int64_t)blocks * 1024) {
+    const int count = (int)min((int64_t)4, size - k);
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int n = 0; n < parts; ++n) {
+      float x[4];
+      load_row_part<float, 4>(p.part + part_slot(p.groups, begin + n * p.rows, p.rows, n == 0) * size + k, 0, count, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += x[i];
     }
+    store_row_part<T, 4>(dw + k, 0, count, v);
   }
-  if (p.db == nullptr) return;
-  for (int c = block * 256 + threadIdx.x; c < p.n_out; c += blocks * 256) {
-    float one[1];
-    if (!part_sum<1>(p.bias_groups, p.n_rows, p.bias_rows, g, p.part_bias, p.n_out, c, one)) break;
-    ((T*)p.db)[(int64_t)g * p.n_out + c] = (T)one[0];
-  }
+}
+
+// the same of a bias: its many parts sixty-four at a time, then those sums in order
+template <typename T>
+__global__ __launch_bounds__(1024) void dense_bias_join_kernel(BackwardArgs p, int blocks) {
+  __shared__ float s[64][17];
+  const int g = blockIdx.x / blocks, x = threadIdx.x % 16, y = threadIdx.x / 16;
+  const int c = blockIdx.x % blocks * 16 + x;
+  int begin;
+  const int parts = group_parts(p.bias_groups, p.n_rows, p.bias_rows, g, begin);
+  if (parts == 1) return;
+  float v = 0.0f;
+  if (c < p.n_out)
+#pragma unroll 4
+    for (int n = y; n < parts; n += 64)
+      v += p.part_bias[part_slot(p.bias_groups, begin + n * p.bias_rows, p.bias_rows, n == 0) * p.n_out + c];
+  s[y][x] = v;
+  __syncthreads();
+  if (y != 0 || c >= p.n_out) return;
+  v = 0.0f;
+#pragma unroll
+  for (int q = 0; q < 64; ++q) v += s[q][x];
+  ((T*)p.db)[(int64_t)g * p.n_out + c] = (T)v;
 }
 
 // ---------------------------------------------------------------- host side
@@ -232,22 +252,45 @@ static Parts parts_of(int64_t n_rows, bool grouped, int64_t want, int64_t least)
 }
 
 struct BackwardPlan {
-  int side;                        // of the weight's tiles
+  int kind;                        // of the weight's tiles
   Parts weight, bias;
   size_t d, bytes;                 // of d, of all: the weight's parts, the bias's, d
   size_t bias_at, d_at;
 };
-static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, bool grouped, bool slope,
-                                  bool weight, bool bias) {
+static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, int64_t n_groups,
+                                  bool grouped, bool slope, bool weight, bool bias) {
   BackwardPlan b{};
   const int64_t size = storage_bytes(dtype);
-  const auto tiles = [&](int64_t s) { return ((n_in + s - 1) / s) * ((n_out + s - 1) / s); };
-  // parts times tiles: two blocks a CU of 128 x 128 tiles and smaller, one of the larger
-  b.side = n_in > 64 && n_out > 64 ? 128 : 64;
-  if (size == 2 && n_in >= 192 && n_out >= 192 && n_rows * tiles(256) >= 256 * 512) b.side = 256;
-  if (weight)
-    b.weight = parts_of(n_rows, grouped, std::max<int64_t>(1, (b.side == 256 ? 256 : 512) / tiles(b.side)), 256);
-  if (bias || slope) b.bias = parts_of(n_rows, grouped, 512, 64);
+  const auto tiles = [&](int64_t bm, int64_t bn) { return ((n_in + bm - 1) / bm) * ((n_out + bn - 1) / bn); };
+  if (weight) {
+    // The tiles and the number of parts with the least time, estimated from the rates of large products
+    // (kinds 0, 1, 2: microseconds of 64 rows of a tile with all of a CU's blocks at work, and those blocks) and
+    // the parts' sums, written and read at 4 TB/s
+    static const double step16[] = {0.9, 1.5, 2.4}, step32[] = {2.9, 5.4, 0.0};
+    static const int per_cu[] = {3, 2, 2}, bm[] = {64, 128, 256}, bn[] = {64, 128, 128};
+    const double sums = (double)n_in * n_out * 8 / 4e6;
+    double best = 0.0;
+    for (int kind = 0; kind < (size == 2 ? 3 : 2); ++kind) {
+      const int64_t t = tiles(bm[kind], bn[kind]);
+      for (int64_t want = 1; want <= 1024; want *= 2) {
+        const Parts parts = parts_of(n_rows, grouped, want, 256);
+        const int64_t n = row_tiles(n_rows, n_groups, false, parts.rows) + (grouped ? n_groups / 2 : 0);
+        const double rounds = std::max(1.0, std::ceil((double)(n * t) / (256 * per_cu[kind])));
+        const double steps = (double)std::min<int64_t>(parts.rows, n_rows) / 64 + 2;   // and two for what is around
+        const double time = rounds * steps * (size == 2 ? step16[kind] : step32[kind]) +
+                            (parts.slots > 0 ? 5.0 + sums * (double)row_tiles(n_rows, 0, false, parts.rows) : 0.0);
+        if (best == 0.0 || time < best) {
+          best = time;
+          b.kind = kind;
+          b.weight = parts;
+        }
+        if (parts.slots > 0 && parts.rows <= 256) break;
+      }
+    }
+  }
+  // eight blocks a CU of 512 bytes of the columns each
+  if (bias || slope)
+    b.bias = parts_of(n_rows, grouped, std::max<int64_t>(1, 2048 / ((n_out * size + 511) / 512)), 64);
   const auto room = [](size_t n) { return (n + 255) / 256 * 256; };
   b.d = slope ? (size_t)n_rows * n_out * size : 0;
   b.bias_at = room((size_t)b.weight.slots * n_in * n_out * sizeof(float));
@@ -274,12 +317,17 @@ static void input_launch(BackwardArgs p, const int32_t* plan, int n_groups, hipS
   hipLaunchKernelGGL((dense_input_kernel<T, L>), dim3((unsigned)xcd_blocks(p.tiles)), dim3(kDenseThreads), 0, s, p);
 }
 
+// Groups of different sizes have parts of different lengths, the long ones next to each other: spread over the XCDs
+// where there are enough of them (16,384 rows in 64 groups, 1,024 x 1,024 in bfloat16: MEASURED)
 template <typename T, typename L>
 static void weight_launch(BackwardArgs p, const int32_t* plan, int n_groups, hipStream_t s) {
   p.tiles_m = (p.n_in + L::BM - 1) / L::BM;
   p.tiles_n = (p.n_out + L::BN - 1) / L::BN;
-  p.tiles = row_tiles(p.n_rows, n_groups, plan != nullptr, p.rows) * p.tiles_m * p.tiles_n;
-  hipLaunchKernelGGL((dense_weight_kernel<T, L>), dim3((unsigned)xcd_blocks(p.tiles)), dim3(kDenseThreads), 0, s, p);
+  p.parts = row_tiles(p.n_rows, n_groups, plan != nullptr, p.rows);
+  p.spread = plan != nullptr && p.parts >= 4 * kXcds;
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  const int64_t blocks = p.spread ? xcd_blocks(p.parts) * tiles : xcd_blocks(p.parts * tiles);
+  hipLaunchKernelGGL((dense_weight_kernel<T, L>), dim3((unsigned)blocks), dim3(kDenseThreads), 0, s, p);
 }
 
 }  // namespace xnn
@@ -294,7 +342,7 @@ int xnn_linear_backward_work_size(int dtype, int64_t n_rows, int32_t n_in, int32
   const int status = dense_sizes(dtype, n_rows, n_in, n_out, &some, n_groups);
   if (status != XNN_OK) return status;
   XNN_REQUIRE(bytes != nullptr, "NULL size");
-  *bytes = backward_plan(dtype, n_rows, n_in, n_out, grouped != 0, slope != 0, weight != 0, bias != 0).bytes;
+  *bytes = backward_plan(dtype, n_rows, n_in, n_out, n_groups, grouped != 0, slope != 0, weight != 0, bias != 0).bytes;
   return XNN_OK;
 }
 
@@ -311,7 +359,7 @@ int xnn_linear_backward(int dtype, const void* grad, const void* slope, const vo
   if (dx == nullptr && dweight == nullptr && dbias == nullptr) return XNN_OK;
   if (n_rows == 0 && dweight == nullptr && dbias == nullptr) return XNN_OK;
   const bool grouped = plan != nullptr && n_rows > 0;
-  const BackwardPlan b = backward_plan(dtype, n_rows, n_in, n_out, grouped, slope != nullptr, dweight != nullptr,
+  const BackwardPlan b = backward_plan(dtype, n_rows, n_in, n_out, n_groups, grouped, slope != nullptr, dweight != nullptr,
                                        dbias != nullptr);
   XNN_REQUIRE(b.bytes == 0 || (work && work_bytes >= b.bytes), "work too small");
   XNN_REQUIRE((uintptr_t)work % 16 == 0, "work must be aligned to 16 bytes");
@@ -336,19 +384,23 @@ int xnn_linear_backward(int dtype, const void* grad, const void* slope, const vo
   p.groups = group_view(order, n_rows, n_groups, grouped ? group_level(p.rows) : 0);
   p.bias_groups = group_view(order, n_rows, n_groups, grouped ? group_level(p.bias_rows) : 0);
   hipStream_t s = as_hip(stream);
-  const int side = dense_tile(storage_bytes(dtype), n_rows, n_in);
+  const int kind = dense_tile(storage_bytes(dtype), n_rows, n_in, grouped ? n_groups : 0);
   XNN_STORAGE_DISPATCH(dtype, T, {
     if (n_rows > 0 && (slope != nullptr || dbias != nullptr)) cotangent_launch<T>(p, order, n_groups, s);
     if (slope != nullptr) p.g = p.d;
-    if (n_rows > 0 && dx != nullptr) XNN_TILE_DISPATCH(side, T, L, input_launch<T, L>(p, order, n_groups, s));
+    if (n_rows > 0 && dx != nullptr) XNN_TILE_DISPATCH(kind, T, L, input_launch<T, L>(p, order, n_groups, s));
     if (n_rows > 0 && dweight != nullptr)
-      XNN_TILE_DISPATCH(b.side, T, L, weight_launch<T, L>(p, order, n_groups, s));
+      XNN_TILE_DISPATCH(b.kind, T, L, weight_launch<T, L>(p, order, n_groups, s));
     // groups without rows have zeros, parts have sums
-    if ((dweight != nullptr && (grouped || b.weight.slots > 0 || n_rows == 0)) ||
-        (dbias != nullptr && (grouped || b.bias.slots > 0 || n_rows == 0))) {
-      const int64_t all = dweight != nullptr ? (int64_t)n_in * n_out : n_out;
-      const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>((all + 1023) / 1024, 65536 / n_groups));
+    if (dweight != nullptr && (grouped || b.weight.slots > 0 || n_rows == 0)) {
+      const int64_t all = ((int64_t)n_in * n_out + 1023) / 1024;
+      const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(all, 65536 / n_groups));
       hipLaunchKernelGGL(dense_join_kernel<T>, dim3((unsigned)(blocks * n_groups)), dim3(256), 0, s, p, blocks);
+    }
+    if (dbias != nullptr && (grouped || b.bias.slots > 0 || n_rows == 0)) {
+      const int blocks = (n_out + 15) / 16;
+      hipLaunchKernelGGL(dense_bias_join_kernel<T>, dim3((unsigned)blocks * (unsigned)n_groups), dim3(1024), 0, s, p,
+                         blocks);
     }
   });
   XNN_LAUNCH_CHECK();

@@ -80,7 +80,7 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     ``"gelu"`` (``z Phi(z)``, by the error function) or ``"tanh"``. Rows of ``x`` may be strided.
 
     Where a gradient is wanted the forward pass keeps ``f'(z)`` (beside the 16-bit types in 16 bits of its own
-    form, to ``2^-15`` of it near one), and the backward pass rounds ``d = grad f'(z)`` to ``x``'s type once, between
+    form, finer than theirs), and the backward pass rounds ``d = grad f'(z)`` to ``x``'s type once, between
     ``f'`` and the two products. float32 operands enter the products as three
     planes of 8 bits: one that is not finite makes the outputs it reaches NaN."""
     code = _activation(activation)
