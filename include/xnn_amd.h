@@ -1309,7 +1309,7 @@ int xnn_linear_backward_work_size(int dtype, int64_t n_rows, int32_t n_in, int32
 
 /* Gradients for the cotangent `grad` (n_rows, n_out), contiguous: dx (n_rows, n_in; zero in rows of no
  * group), dweight and dbias as weight and bias (zero for a group without rows), each of which may be
- * NULL. slope: the forward pass's, NULL
+ * NULL (dbias with dweight only). slope: the forward pass's, NULL
  * where there is no activation. The residual's gradient is `grad`. `work` is aligned to 16 bytes. */
 int xnn_linear_backward(int dtype, const void* grad, const void* slope, const void* x, int64_t x_stride,
                         int64_t n_rows, int32_t n_in, int32_t n_out, const void* weight,

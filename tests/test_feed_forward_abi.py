@@ -98,7 +98,9 @@ def test_linear_backward_arguments(lib):
         return lib.xnn_linear_backward_work_size(dtype, rows, 64, 64, groups, grouped, slope, weight, bias,
                                                  ctypes.byref(SIZE) if out is None else out)
     assert size(0, 20, 1) == 0 and SIZE.value == 0
-    assert size(2, 1000, 1, slope=1, weight=0) == 0 and SIZE.value == 1000 * 64 * 2
+    assert size(2, 1000, 1, slope=1, weight=0) == 0 and SIZE.value == 0
+    assert lib.xnn_linear_backward_work_size(2, 1000, 200, 64, 1, 0, 1, 0, 0, ctypes.byref(SIZE)) == 0
+    assert SIZE.value == 1000 * 64 * 2                      # d
     assert size(0, 100000, 1) == 0
     need = SIZE.value
     assert need > 0
@@ -116,7 +118,7 @@ def test_linear_backward_arguments(lib):
     _refused(lib, call(stride=63), b"overlap")
     _refused(lib, call(size=need - 1), b"work too small")
     _refused(lib, call(db=BUF), b"work too small")
-    _refused(lib, call(slope=BUF), b"work too small")
+    _refused(lib, call(dw=None, db=BUF), b"goes with")
     _refused(lib, call(work=None), b"work too small")
     _refused(lib, call(work=ctypes.addressof(BUF) + 4), b"aligned")
     assert call(dw=None) == 0

@@ -259,15 +259,28 @@ __device__ __forceinline__ void put_piece(char* at, int plane, u32x4 x) {
   }
 }
 
-// One operand on its way: a matrix of rows of `width` elements, row r at data + r stride, of which LEN rows or
-// columns are this tile's. ALONG: the tile's rows, along which the reduction runs; else its columns, and the
+// d = g f'(z) of a piece
+template <typename T>
+__device__ __forceinline__ u32x4 times_slope(u32x4 g, u32x4 slope) {
+  constexpr int N = 16 / sizeof(T);
+  typedef typename Slope<T>::type S;
+  const Pack<T, N> x = __builtin_bit_cast(Pack<T, N>, g);
+  const Pack<S, N> y = __builtin_bit_cast(Pack<S, N>, slope);
+  Pack<T, N> out;
+#pragma unroll
+  for (int i = 0; i < N; ++i) out.v[i] = (T)((float)x.v[i] * slope_value<T>(y.v[i]));
+  return __builtin_bit_cast(u32x4, out);
+}
+
+// One operand on its way: a matrix of rows of `width` elements, row r at data + r stride (TIMES: times the slope's,
+// of the same layout), of which LEN rows or columns are this tile's. ALONG: the tile's rows, along which the reduction runs; else its columns, and the
 // reduction runs over the rows. Row r of the tile, or of the reduction, is order[first + r], or first + r
 // without an order.
 //
 // Steps that begin before `fast` are of whole pieces, one address each that the step before has left: along the rows
 // those that end within them; across them all but the last one where a piece may reach beyond its row (the
 // tensor's last row is the last of its group).
-template <typename T, int LEN, int BK, bool ALONG>
+template <typename T, int LEN, int BK, bool ALONG, bool TIMES = false>
 struct Operator {
   static constexpr int kPer = 16 / sizeof(T);
   static constexpr int kRows = ALONG ? LEN : BK, kCols = ALONG ? BK : LEN;   // of a staged step
@@ -279,19 +292,20 @@ struct Operator {
 
   const char *data, *column;       // the tensor, and the thread's first piece of its row 0
   const int32_t* order;            // from `first` on
-  int64_t stride;                  // bytes of a row
+  int64_t stride, slope;           // bytes of a row, bytes from data to the slope
   int width, row, at, first, end, last, fast;   // last: the tensor's last row
   int most;                        // the last row that a whole piece may begin in
   uint32_t edges;                  // ALONG: pieces of the tensor's last row
   const char* p[kCount];           // pieces of the next step; across rows in an order
   int32_t index[ALONG ? 1 : kCount];   // those rows, whose loads have a step's time
-  u32x4 x[kCount];
+  u32x4 x[kCount], y[TIMES ? kCount : 1];
 
   // rows [first_row, end_row), columns from first_col on
   __device__ __forceinline__ void init(const void* data_, const int32_t* order_, int64_t stride_,
                                        int tensor_rows, int width_, int first_row, int end_row,
-                                       int first_col) {
+                                       int first_col, const void* slope_ = nullptr) {
     data = (const char*)data_;
+    slope = TIMES ? (const char*)slope_ - data : 0;
     order = order_ == nullptr ? nullptr : order_ + first_row;
     stride = stride_ * (int)sizeof(T);
     last = tensor_rows - 1;
@@ -329,6 +343,7 @@ struct Operator {
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {
       x[n] = load_raw(p[n]);
+      if constexpr (TIMES) y[n] = load_raw(p[n] + slope);
       p[n] += step;
     }
     if constexpr (!ALONG)
@@ -350,6 +365,7 @@ struct Operator {
       const int left = width - at - (ALONG ? k0 : 0);
       const bool edge = (ALONG ? (edges >> n & 1) != 0 : i == last) || stride < 16;
       x[n] = load_raw<T>(q, left, edge);
+      if constexpr (TIMES) y[n] = load_raw<T>(q + slope, left, edge);
       if (ALONG) p[n] += BK * (int)sizeof(T);
     }
   }
@@ -359,9 +375,20 @@ struct Operator {
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {
       const int r = row + n * kStep, c = threadIdx.x % kChunks * kPer;
+      if constexpr (TIMES) x[n] = times_slope<T>(x[n], y[n]);
       u32x4 out = x[n];
       if constexpr (TAIL) out = piece_head<T>(out, ALONG ? length - k0 - c : k0 + r < length ? kPer : 0);
       put_piece<T>(lds + r * At::kRow + c * 2, At::kPlane, out);
+    }
+  }
+  // the step's rows before `length`, added to each of the thread's columns (after commit, before the next fetch)
+  __device__ __forceinline__ void add_rows(int k0, int length, float (&sums)[kPer]) const {
+#pragma unroll
+    for (int n = 0; n < kCount; ++n) {
+      const Pack<T, kPer> v = __builtin_bit_cast(Pack<T, kPer>, x[n]);
+      const bool in = k0 + row + n * kStep < length;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) sums[i] += in ? (float)v.v[i] : 0.0f;
     }
   }
 };
@@ -438,10 +465,11 @@ __device__ __forceinline__ void interleave() {
   }
 }
 
-// The tile's sums over `length` reduction indices. The rows of a 32 x 32 product are the output's columns, so that
-// a lane holds four of them in a row.
-template <typename T, typename L, bool ALONG_A, bool ALONG_B, typename A, typename B>
-__device__ __forceinline__ void dense_product(A& a, B& b, int length, char* lds, f32x16 (&acc)[L::MT][L::NT]) {
+// The tile's sums over `length` reduction indices; seen(k) after each step that starts at k is in LDS. The rows of
+// a 32 x 32 product are the output's columns, so that a lane holds four of them in a row.
+template <typename T, typename L, bool ALONG_A, bool ALONG_B, typename A, typename B, typename F>
+__device__ __forceinline__ void dense_product(A& a, B& b, int length, char* lds, f32x16 (&acc)[L::MT][L::NT],
+                                              F&& seen) {
   typedef DenseLds<L, T, ALONG_A, ALONG_B> S;
   constexpr int BK = L::BK;
   const int wave = wave_in_block();
@@ -473,6 +501,7 @@ __device__ __forceinline__ void dense_product(A& a, B& b, int length, char* lds,
   const auto commit_fast = [&](char* s, int k) {
     a.template commit<false>(s, k, length);
     b.template commit<false>(s + S::kA, k, length);
+    seen(k);
   };
   const auto commit = [&](char* s, int k) {
     if (k + BK <= length) {
@@ -480,6 +509,7 @@ __device__ __forceinline__ void dense_product(A& a, B& b, int length, char* lds,
     } else {
       a.template commit<true>(s, k, length);
       b.template commit<true>(s + S::kA, k, length);
+      seen(k);
     }
   };
   const auto fetch = [&](int k) {
@@ -622,16 +652,19 @@ using Tile128 = Shape<T, 128, 128, 2, 2, 128 / sizeof(T)>;
 template <typename T>
 using Tile256 = Shape<T, 256, 128, 2, 2, 32>;
 
-// The kind for an output of m x n, in `groups` of rows where they are grouped (then a group's last tile is half empty).
+// The kind for an output of m x n, in `groups` of rows where they are grouped (then a group's last tile is half empty;
+// how many groups have rows is not known here, and that any has does not speak for smaller tiles).
 // 256 x 128 tiles pay where they come in full rounds of two a CU (9,000 x 512 x 2,048 with silu, 1.1 rounds: 78 us,
 // 128 x 128 57; 24,000 x 1,024 x 4,096, 5.9: 423 and 470), 64 x 64 where 128 x 128 are not one a CU
 // (1,000^3: 10 us, 128 x 128 21).
 inline int dense_tile(size_t size, int64_t m, int64_t n, int64_t groups) {
-  const auto rounds = [&](int64_t bm, int64_t bn) {
-    return (double)(m / bm + (groups + 1) / 2 + 1) * (double)((n + bn - 1) / bn) / 512;
+  const auto rounds = [&](int64_t bm, int64_t bn, int64_t more) {
+    return (double)((m + bm - 1) / bm + more) * (double)((n + bn - 1) / bn) / 512;
   };
-  if (n <= 64 || rounds(128, 128) < 0.5) return kTile64;
-  return size == 2 && 1.8 * std::ceil(rounds(256, 128)) <= std::ceil(rounds(128, 128)) ? kTile256 : kTile128;
+  if (n <= 64 || rounds(128, 128, 0) < 0.5) return kTile64;
+  const int64_t more = groups / 2;
+  return size == 2 && 1.8 * std::ceil(rounds(256, 128, more)) <= std::ceil(rounds(128, 128, more)) ? kTile256
+                                                                                                 : kTile128;
 }
 
 // call(Shape) for the kind

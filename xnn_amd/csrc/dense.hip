@@ -37,7 +37,7 @@ __global__ __launch_bounds__(kDenseThreads) void dense_forward_kernel(ForwardArg
   a.init(p.x, p.groups.order, p.x_stride, p.n_rows, p.n_in, t.begin, t.end, 0);
   b.init((const T*)p.w + (int64_t)t.group * p.n_in * p.n_out, nullptr, p.n_out, p.n_in, p.n_out, 0, p.n_in, n0);
   f32x16 acc[L::MT][L::NT];
-  dense_product<T, L, true, false>(a, b, p.n_in, lds, acc);
+  dense_product<T, L, true, false>(a, b, p.n_in, lds, acc, [](int) {});
   typedef typename Slope<T>::type SlopeType;
   constexpr int N = 16 / sizeof(T);
   int c;

@@ -2,11 +2,12 @@
 //
 //   dx = d W^T,   dW = x^T d,   db = sum of d over the rows
 //
-// of one weight or of each row's group. d is formed once, with db's sums, by a pass that reads g and the slope;
-// without an activation d is g, which that pass reads for db alone. A weight's reduction runs over all rows of
-// its group: it is cut into parts, one a block, which are added in their order where there is more than one.
-// (d formed where each product stages it: 24,000 rows of 1,024 -> 4,096 in bfloat16, both products 843 us, for the
-// registers, against 529 and 110 for the pass.)
+// of one weight or of each row's group. Where both products need d once (a width of 128 at most in x), they form it as
+// they stage it; else a pass over g and the slope does, with db's sums. (Formed in the staging of 24,000 rows of
+// 1,024 -> 4,096 in bfloat16, both products 843 us, for the registers, against 529 and 110 for the pass; 72,000
+// rows of 128 -> 512 in float32: MEASURED.) A weight's reduction runs over all rows of its group: it is cut into
+// parts, one a block, which are added in their order where there is more than one. Without the pass db's sums
+// are the weight's product's, taken from what it stages.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -25,6 +26,7 @@ struct BackwardArgs {
   int n_rows, n_in, n_out, tiles_m, tiles_n;
   int rows, bias_rows;             // of a part of the weight's sums, of the bias's
   int spread;                      // parts of different lengths: to the XCDs in turn
+  int sums;                        // the weight's product adds up db
 };
 
 // Where the sums of the part of sorted rows from `begin` on stand: parts of one weight follow each other; among
@@ -90,7 +92,7 @@ __global__ __launch_bounds__(256) void dense_cotangent_kernel(BackwardArgs p, in
 }
 
 // ---------------------------------------------------------------- the products
-template <typename T, typename L>
+template <typename T, typename L, bool TIMES>
 __global__ __launch_bounds__(kDenseThreads) void dense_input_kernel(BackwardArgs p) {
   typedef DenseLds<L, T, true, true> S;
   __shared__ __align__(16) char lds[S::kBytes];
@@ -103,13 +105,13 @@ __global__ __launch_bounds__(kDenseThreads) void dense_input_kernel(BackwardArgs
     fill_rows<T, L::BN>(p.groups, t, p.n_rows, (T*)p.dx, n0, p.n_in, (T)0.0f);
     return;
   }
-  Operator<T, L::BM, L::BK, true> a;
+  Operator<T, L::BM, L::BK, true, TIMES> a;
   Operator<T, L::BN, L::BK, true> b;
-  a.init(p.g, p.groups.order, p.n_out, p.n_rows, p.n_out, t.begin, t.end, 0);
+  a.init(p.g, p.groups.order, p.n_out, p.n_rows, p.n_out, t.begin, t.end, 0, p.slope);
   b.init((const T*)p.w + (int64_t)t.group * p.n_in * p.n_out, nullptr, p.n_out, p.n_in, p.n_out, n0,
          min(n0 + L::BN, p.n_in), 0);
   f32x16 acc[L::MT][L::NT];
-  dense_product<T, L, true, true>(a, b, p.n_out, lds, acc);
+  dense_product<T, L, true, true>(a, b, p.n_out, lds, acc, [](int) {});
   constexpr int N = 16 / sizeof(T);
   int c;
   dense_rows<L, N>(
@@ -130,7 +132,7 @@ __device__ __forceinline__ int64_t slot_of_xcd(int64_t tiles, int64_t& tile) {
   return i / tiles * kXcds + blockIdx.x % kXcds;
 }
 
-template <typename T, typename L>
+template <typename T, typename L, bool TIMES>
 __global__ __launch_bounds__(kDenseThreads) void dense_weight_kernel(BackwardArgs p) {
   typedef DenseLds<L, T, false, false> S;
   __shared__ __align__(16) char lds[S::kBytes];
@@ -146,15 +148,38 @@ __global__ __launch_bounds__(kDenseThreads) void dense_weight_kernel(BackwardArg
   const int m0 = (int)(tile / p.tiles_n) * L::BM, n0 = (int)(tile % p.tiles_n) * L::BN;
   const RowTile t = row_tile(p.groups, p.groups.n_groups, p.n_rows, (int)part, p.rows);
   if (t.group < 0) return;
+  typedef Operator<T, L::BN, L::BK, false, TIMES> B;
   Operator<T, L::BM, L::BK, false> a;
-  Operator<T, L::BN, L::BK, false> b;
+  B b;
   a.init(p.x, p.groups.order, p.x_stride, p.n_rows, p.n_in, t.begin, t.end, m0);
-  b.init(p.g, p.groups.order, p.n_out, p.n_rows, p.n_out, t.begin, t.end, n0);
+  b.init(p.g, p.groups.order, p.n_out, p.n_rows, p.n_out, t.begin, t.end, n0, p.slope);
   f32x16 acc[L::MT][L::NT];
-  dense_product<T, L, false, false>(a, b, t.end - t.begin, lds, acc);
+  const bool bias = p.sums && m0 == 0;
+  const int length = t.end - t.begin;
+  float sums[B::kPer];
+#pragma unroll
+  for (int i = 0; i < B::kPer; ++i) sums[i] = 0.0f;
+  dense_product<T, L, false, false>(a, b, length, lds, acc, [&](int k) {
+    if (bias) b.add_rows(k, length, sums);
+  });
   const bool only = part_alone(p.groups, p.n_rows, p.rows, t.group);
   const int64_t at =
       part_slot(p.groups, t.begin, p.rows, p.groups.n_groups > 0 && part == p.groups.tile_ptr[t.group]);
+  if (bias) {
+    float* s = reinterpret_cast<float*>(lds);                // (kStep, BN)
+    store_pack<float, B::kPer>(s + b.row * L::BN + threadIdx.x % B::kChunks * B::kPer, sums);
+    __syncthreads();
+    for (int i = threadIdx.x; i < L::BN && n0 + i < p.n_out; i += kDenseThreads) {
+      float v = 0.0f;
+#pragma unroll
+      for (int r = 0; r < B::kStep; ++r) v += s[r * L::BN + i];
+      if (only)
+        ((T*)p.db)[(int64_t)t.group * p.n_out + n0 + i] = (T)v;
+      else
+        p.part_bias[at * p.n_out + n0 + i] = v;
+    }
+    __syncthreads();
+  }
   T* dw = (T*)p.dw + (int64_t)t.group * p.n_in * p.n_out;
   float* sum = p.part + at * p.n_in * p.n_out;
   int c;
@@ -185,16 +210,37 @@ __device__ __forceinline__ int group_parts(const GroupView& v, int n_rows, int r
   return min(v.tile_ptr[group + 1] - v.tile_ptr[group], (n_rows - begin + rows - 1) / rows);
 }
 
-// the parts of a weight added in their order, zeros where there is none; a group's only part is done
+// The parts of a weight and of its bias added in their order, zeros where there is none; a group's only part is done.
+// Of a group's blocks the last `bias_blocks` have sixteen columns of the bias each, whose parts may be many:
+// sixteen of them at a time, then those sums in order
 template <typename T>
-__global__ __launch_bounds__(256) void dense_join_kernel(BackwardArgs p, int blocks) {
-  const int g = blockIdx.x / blocks;
+__global__ __launch_bounds__(256) void dense_join_kernel(BackwardArgs p, int weight_blocks, int bias_blocks) {
+  const int g = blockIdx.x / (weight_blocks + bias_blocks);
+  int block = blockIdx.x % (weight_blocks + bias_blocks), begin;
+  if (block >= weight_blocks) {
+    __shared__ float s[16][17];
+    const int x = threadIdx.x % 16, y = threadIdx.x / 16, c = (block - weight_blocks) * 16 + x;
+    const int parts = group_parts(p.bias_groups, p.n_rows, p.bias_rows, g, begin);
+    if (parts == 1) return;
+    float v = 0.0f;
+    if (c < p.n_out)
+#pragma unroll 4
+      for (int n = y; n < parts; n += 16)
+        v += p.part_bias[part_slot(p.bias_groups, begin + n * p.bias_rows, p.bias_rows, n == 0) * p.n_out + c];
+    s[y][x] = v;
+    __syncthreads();
+    if (y != 0 || c >= p.n_out) return;
+    v = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) v += s[q][x];
+    ((T*)p.db)[(int64_t)g * p.n_out + c] = (T)v;
+    return;
+  }
   const int64_t size = (int64_t)p.n_in * p.n_out;
-  int begin;
   const int parts = group_parts(p.groups, p.n_rows, p.rows, g, begin);
   if (parts == 1) return;
   T* dw = (T*)p.dw + g * size;
-  for (int64_t k = ((int64_t)(blockIdx.x % blocks) * 256 + threadIdx.x) * 4; k < size; k += (int64_t)blocks * 1024) {
+  for (int64_t k = ((int64_t)block * 256 + threadIdx.x) * 4; k < size; k += (int64_t)weight_blocks * 1024) {
     const int count = (int)min((int64_t)4, size - k);
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
@@ -206,29 +252,6 @@ __global__ __launch_bounds__(256) void dense_join_kernel(BackwardArgs p, int blo
     }
     store_row_part<T, 4>(dw + k, 0, count, v);
   }
-}
-
-// the same of a bias: its many parts sixty-four at a time, then those sums in order
-template <typename T>
-__global__ __launch_bounds__(1024) void dense_bias_join_kernel(BackwardArgs p, int blocks) {
-  __shared__ float s[64][17];
-  const int g = blockIdx.x / blocks, x = threadIdx.x % 16, y = threadIdx.x / 16;
-  const int c = blockIdx.x % blocks * 16 + x;
-  int begin;
-  const int parts = group_parts(p.bias_groups, p.n_rows, p.bias_rows, g, begin);
-  if (parts == 1) return;
-  float v = 0.0f;
-  if (c < p.n_out)
-#pragma unroll 4
-    for (int n = y; n < parts; n += 64)
-      v += p.part_bias[part_slot(p.bias_groups, begin + n * p.bias_rows, p.bias_rows, n == 0) * p.n_out + c];
-  s[y][x] = v;
-  __syncthreads();
-  if (y != 0 || c >= p.n_out) return;
-  v = 0.0f;
-#pragma unroll
-  for (int q = 0; q < 64; ++q) v += s[q][x];
-  ((T*)p.db)[(int64_t)g * p.n_out + c] = (T)v;
 }
 
 // ---------------------------------------------------------------- host side
@@ -251,10 +274,14 @@ static Parts parts_of(int64_t n_rows, bool grouped, int64_t want, int64_t least)
   return w;
 }
 
+// the width of x up to which the products form d themselves: a tile of both
+constexpr int kFormInProducts = 128;
+
 struct BackwardPlan {
   int kind;                        // of the weight's tiles
   Parts weight, bias;
-  size_t d, bytes;                 // of d, of all: the weight's parts, the bias's, d
+  bool pass;                       // forms d
+  size_t bytes;                    // of the weight's parts, the bias's, d
   size_t bias_at, d_at;
 };
 static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, int64_t n_groups,
@@ -270,7 +297,7 @@ static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32
     static const int per_cu[] = {3, 2, 2}, bm[] = {64, 128, 256}, bn[] = {64, 128, 128};
     const double sums = (double)n_in * n_out * 8 / 4e6;
     double best = 0.0;
-    for (int kind = 0; kind < (size == 2 ? 3 : 2); ++kind) {
+    for (int kind = 0; kind < (size == 2 && !(slope && n_in <= kFormInProducts) ? 3 : 2); ++kind) {
       const int64_t t = tiles(bm[kind], bn[kind]);
       for (int64_t want = 1; want <= 1024; want *= 2) {
         const Parts parts = parts_of(n_rows, grouped, want, 256);
@@ -288,14 +315,14 @@ static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32
       }
     }
   }
+  b.pass = slope && n_in > kFormInProducts;
+  b.bias = b.weight;
   // eight blocks a CU of 512 bytes of the columns each
-  if (bias || slope)
-    b.bias = parts_of(n_rows, grouped, std::max<int64_t>(1, 2048 / ((n_out * size + 511) / 512)), 64);
+  if (b.pass) b.bias = parts_of(n_rows, grouped, std::max<int64_t>(1, 2048 / ((n_out * size + 511) / 512)), 64);
   const auto room = [](size_t n) { return (n + 255) / 256 * 256; };
-  b.d = slope ? (size_t)n_rows * n_out * size : 0;
   b.bias_at = room((size_t)b.weight.slots * n_in * n_out * sizeof(float));
   b.d_at = b.bias_at + (bias ? room((size_t)b.bias.slots * n_out * sizeof(float)) : 0);
-  b.bytes = b.d_at + b.d;
+  b.bytes = b.d_at + (b.pass ? (size_t)n_rows * n_out * size : 0);
   return b;
 }
 
@@ -314,7 +341,14 @@ static void input_launch(BackwardArgs p, const int32_t* plan, int n_groups, hipS
   p.groups = group_view(plan, p.n_rows, n_groups, group_level(L::BM));
   p.tiles_n = (p.n_in + L::BN - 1) / L::BN;
   p.tiles = row_tiles(p.n_rows, n_groups, plan != nullptr, L::BM) * p.tiles_n;
-  hipLaunchKernelGGL((dense_input_kernel<T, L>), dim3((unsigned)xcd_blocks(p.tiles)), dim3(kDenseThreads), 0, s, p);
+  const dim3 grid((unsigned)xcd_blocks(p.tiles));
+  if constexpr (L::BM <= 128) {
+    if (p.slope != nullptr) {
+      hipLaunchKernelGGL((dense_input_kernel<T, L, true>), grid, dim3(kDenseThreads), 0, s, p);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((dense_input_kernel<T, L, false>), grid, dim3(kDenseThreads), 0, s, p);
 }
 
 // Groups of different sizes have parts of different lengths, the long ones next to each other: spread over the XCDs
@@ -327,7 +361,13 @@ static void weight_launch(BackwardArgs p, const int32_t* plan, int n_groups, hip
   p.spread = plan != nullptr && p.parts >= 4 * kXcds;
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   const int64_t blocks = p.spread ? xcd_blocks(p.parts) * tiles : xcd_blocks(p.parts * tiles);
-  hipLaunchKernelGGL((dense_weight_kernel<T, L>), dim3((unsigned)blocks), dim3(kDenseThreads), 0, s, p);
+  if constexpr (L::BM <= 128) {
+    if (p.slope != nullptr) {
+      hipLaunchKernelGGL((dense_weight_kernel<T, L, true>), dim3((unsigned)blocks), dim3(kDenseThreads), 0, s, p);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((dense_weight_kernel<T, L, false>), dim3((unsigned)blocks), dim3(kDenseThreads), 0, s, p);
 }
 
 }  // namespace xnn
@@ -356,8 +396,8 @@ int xnn_linear_backward(int dtype, const void* grad, const void* slope, const vo
   XNN_REQUIRE(n_rows == 0 || dx == nullptr || weight, "NULL weight");
   XNN_REQUIRE(dweight == nullptr || n_rows == 0 || x, "NULL input");
   XNN_REQUIRE(dweight == nullptr || n_rows == 0 || x_stride >= n_in, "rows of x overlap");
-  if (dx == nullptr && dweight == nullptr && dbias == nullptr) return XNN_OK;
-  if (n_rows == 0 && dweight == nullptr && dbias == nullptr) return XNN_OK;
+  XNN_REQUIRE(dbias == nullptr || dweight != nullptr, "the bias's gradient goes with the weight's");
+  if (dweight == nullptr && (dx == nullptr || n_rows == 0)) return XNN_OK;
   const bool grouped = plan != nullptr && n_rows > 0;
   const BackwardPlan b = backward_plan(dtype, n_rows, n_in, n_out, n_groups, grouped, slope != nullptr, dweight != nullptr,
                                        dbias != nullptr);
@@ -384,23 +424,26 @@ int xnn_linear_backward(int dtype, const void* grad, const void* slope, const vo
   p.groups = group_view(order, n_rows, n_groups, grouped ? group_level(p.rows) : 0);
   p.bias_groups = group_view(order, n_rows, n_groups, grouped ? group_level(p.bias_rows) : 0);
   hipStream_t s = as_hip(stream);
-  const int kind = dense_tile(storage_bytes(dtype), n_rows, n_in, grouped ? n_groups : 0);
+  int kind = dense_tile(storage_bytes(dtype), n_rows, n_in, grouped ? n_groups : 0);
+  if (slope != nullptr && !b.pass) kind = std::min<int>(kind, kTile128);
+  p.sums = dbias != nullptr && !b.pass;
   XNN_STORAGE_DISPATCH(dtype, T, {
-    if (n_rows > 0 && (slope != nullptr || dbias != nullptr)) cotangent_launch<T>(p, order, n_groups, s);
-    if (slope != nullptr) p.g = p.d;
+    if (b.pass && n_rows > 0) {
+      cotangent_launch<T>(p, order, n_groups, s);
+      p.g = p.d;
+      p.slope = nullptr;
+    }
     if (n_rows > 0 && dx != nullptr) XNN_TILE_DISPATCH(kind, T, L, input_launch<T, L>(p, order, n_groups, s));
     if (n_rows > 0 && dweight != nullptr)
       XNN_TILE_DISPATCH(b.kind, T, L, weight_launch<T, L>(p, order, n_groups, s));
     // groups without rows have zeros, parts have sums
-    if (dweight != nullptr && (grouped || b.weight.slots > 0 || n_rows == 0)) {
+    if (dweight != nullptr &&
+        (grouped || b.weight.slots > 0 || n_rows == 0 || (dbias != nullptr && b.bias.slots > 0))) {
       const int64_t all = ((int64_t)n_in * n_out + 1023) / 1024;
       const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(all, 65536 / n_groups));
-      hipLaunchKernelGGL(dense_join_kernel<T>, dim3((unsigned)(blocks * n_groups)), dim3(256), 0, s, p, blocks);
-    }
-    if (dbias != nullptr && (grouped || b.bias.slots > 0 || n_rows == 0)) {
-      const int blocks = (n_out + 15) / 16;
-      hipLaunchKernelGGL(dense_bias_join_kernel<T>, dim3((unsigned)blocks * (unsigned)n_groups), dim3(1024), 0, s, p,
-                         blocks);
+      const int bias_blocks = dbias != nullptr ? (n_out + 15) / 16 : 0;
+      hipLaunchKernelGGL(dense_join_kernel<T>, dim3((unsigned)(blocks + bias_blocks) * (unsigned)n_groups), dim3(256),
+                         0, s, p, blocks, bias_blocks);
     }
   });
   XNN_LAUNCH_CHECK();

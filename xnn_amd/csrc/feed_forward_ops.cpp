@@ -324,6 +324,7 @@ Three dense_backward_kernel(const Tensor& grad_, const MaybeTensor& slope_, cons
   check_like(grad_, x, d.out, "the cotangent");
   TORCH_CHECK_VALUE(!slope.defined() || (slope.sizes() == d.out && slope.scalar_type() == slope_type(x)),
                     "the slope is not that of the forward pass");
+  weights = weights || biases;                             // the weight's product has the bias's sums
   const c10::DeviceGuard guard(x.device());
   const Tensor rows = as_rows(x), w = weight.contiguous(), grad = grad_.contiguous();
   const Tensor dx = empty_if(input, x.sizes(), x), dw = empty_if(weights, weight.sizes(), x),
@@ -345,7 +346,7 @@ Three dense_backward_shape(const Tensor&, const MaybeTensor&, const Tensor& x, c
   std::vector<c10::SymInt> bias;
   if (or_none(plan).defined()) bias.push_back(weight.sym_size(0));
   bias.push_back(weight.sym_size(-1));
-  return {empty_shape(input, x), empty_shape(weights, weight),
+  return {empty_shape(input, x), empty_shape(weights || biases, weight),
           biases ? at::empty_symint(bias, x.options()) : at::empty({0}, x.options())};
 }
 

@@ -5,9 +5,11 @@
 //   dx = r (g w - mean(g w) - n mean(g w n)),   dw = sum_rows g n,   db = sum_rows g
 //
 // A stream: a row lies in the registers of 2^k threads, U pieces of 16 bytes a thread, so that the
-// squares are of the centered values and nothing is read twice. Sums over a row are exchanges within a wave and,
-// for rows of more than a wave, through LDS. A thread keeps its columns from row to row and adds up
-// their gradients in registers; the blocks' sums are added in their order. Arithmetic is float32.
+// squares are of the centered values and nothing is read twice. A wave has a row of its own up to four pieces a
+// lane: its sums are exchanges in the vector unit and wait for no other wave (24,000 rows of 2,048 in bfloat16, a
+// piece a thread and four waves a row: forward 81 us, so 38, the rate of a large copy). Longer rows add their waves' sums through LDS. A
+// thread keeps its columns from row to row and adds up their gradients in registers; the blocks' sums are
+// added in their order. Arithmetic is float32.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -17,8 +19,6 @@
 
 namespace xnn {
 
-constexpr int kNormThreads = 1024;
-constexpr int kNormWaves = kNormThreads / kWave;
 constexpr int kNormParts = 512;    // blocks of the backward pass, at most: two a CU
 constexpr int kMaxNormWidth = 16384;
 
@@ -35,8 +35,8 @@ struct LayerNormArgs {
 
 // The sums of N values over the `lanes` threads of each row, every thread getting them; `s` (two in turn) for rows
 // of more than a wave, where all threads of the block call it.
-template <int N>
-__device__ __forceinline__ void row_sums(float (&v)[N], int lanes, float (*s)[kNormWaves][2], int& turn) {
+template <int N, int WAVES>
+__device__ __forceinline__ void row_sums(float (&v)[N], int lanes, float (*s)[WAVES][2], int& turn) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     if (lanes > 1) v[i] += dpp_move<0xB1>(v[i]);
@@ -60,62 +60,78 @@ __device__ __forceinline__ void row_sums(float (&v)[N], int lanes, float (*s)[kN
   turn ^= 1;
 }
 
-// piece `at` of a row: zeros beyond its width
-template <typename T, int N>
-__device__ __forceinline__ void norm_piece(const T* row, int at, int width, bool edge, float (&out)[N]) {
-  const Pack<T, N> x = load_piece<T, N>(row, at, width, edge);
+// piece `at` of a row as it is in memory, zeros beyond its width
+template <typename T>
+__device__ __forceinline__ u32x4 norm_piece(const T* row, int at, int width, bool last) {
+  const int left = width - at;
+  u32x4 x = load_raw<T>(reinterpret_cast<const char*>(row + at), left, last);
+  if (left < (int)(16 / sizeof(T))) x = piece_head<T>(x, left);
+  return x;
+}
+template <typename T>
+__device__ __forceinline__ void piece_values(u32x4 x, float (&v)[16 / sizeof(T)]) {
+  constexpr int N = 16 / sizeof(T);
+  const Pack<T, N> p = __builtin_bit_cast(Pack<T, N>, x);
 #pragma unroll
-  for (int i = 0; i < N; ++i) out[i] = at + i < width ? (float)x.v[i] : 0.0f;
+  for (int i = 0; i < N; ++i) v[i] = (float)p.v[i];
 }
 
-template <typename T, int U, bool BACK>
-__global__ __launch_bounds__(kNormThreads) void layer_norm_kernel(LayerNormArgs p) {
-  constexpr int N = 16 / sizeof(T);
-  __shared__ float sums[2][kNormWaves][2];
-  __shared__ __align__(16) float columns[BACK ? kNormThreads * N : 4];
+template <typename T, int THREADS, int U, bool BACK>
+__global__ __launch_bounds__(THREADS) void layer_norm_kernel(LayerNormArgs p) {
+  constexpr int N = 16 / sizeof(T), WAVES = THREADS / kWave;
+  __shared__ float sums[2][WAVES][2];
+  __shared__ __align__(16) float columns[BACK ? THREADS * N : 4];
   int turn = 0;
-  const int rows = kNormThreads / p.lanes, slot = threadIdx.x / p.lanes, lane = threadIdx.x % p.lanes;
-  float w[U][N], b[U][N], dw[BACK ? U : 1][N], db[BACK ? U : 1][N];
+  const int rows = THREADS / p.lanes, slot = threadIdx.x / p.lanes, lane = threadIdx.x % p.lanes;
+  // values stay as they are in memory, two to a register in 16 bits, and are taken apart where they are used: the
+  // backward pass of rows of 2,048 in bfloat16 has three waves a SIMD so, one (and 178 us) with them apart
+  const auto place = [&](int u) { return (u * p.lanes + lane) * N; };
+  u32x4 w[U], b[U];
+  float dw[BACK ? U : 1][N], db[BACK ? U : 1][N];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int at = (u * p.lanes + lane) * N;
+    if (p.w != nullptr) w[u] = norm_piece<T>((const T*)p.w, place(u), p.width, true);
+    if (!BACK && p.b != nullptr) b[u] = norm_piece<T>((const T*)p.b, place(u), p.width, true);
+    if constexpr (BACK)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      w[u][i] = 1.0f;
-      b[u][i] = 0.0f;
-      if constexpr (BACK) dw[u][i] = db[u][i] = 0.0f;
-    }
-    if (p.w != nullptr) norm_piece<T, N>((const T*)p.w, at, p.width, true, w[u]);
-    if (!BACK && p.b != nullptr) norm_piece<T, N>((const T*)p.b, at, p.width, true, b[u]);
+      for (int i = 0; i < N; ++i) dw[u][i] = db[u][i] = 0.0f;
   }
   const bool small = p.x_stride < N;
   for (int64_t r0 = (int64_t)blockIdx.x * rows; r0 < p.n_rows; r0 += (int64_t)gridDim.x * rows) {
     // threads without a row go through the sums with the last one's
     const bool live = r0 + slot < p.n_rows;
     const int64_t r = live ? r0 + slot : p.n_rows - 1;
-    const bool edge = r == p.n_rows - 1;
+    const bool last = r == p.n_rows - 1;
     const T* row = (const T*)p.x + r * p.x_stride;
-    float x[U][N];
+    T* out = (T*)p.out + r * p.width;
+    u32x4 x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      norm_piece<T, N>(row, (u * p.lanes + lane) * N, p.width, edge || small, x[u]);
+    for (int u = 0; u < U; ++u) x[u] = norm_piece<T>(row, place(u), p.width, last || small);
     if constexpr (!BACK) {
       float s[1] = {0.0f};
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        float v[N];
+        piece_values<T>(x[u], v);
 #pragma unroll
-        for (int i = 0; i < N; ++i) s[0] += x[u][i];
-      row_sums<1>(s, p.lanes, sums, turn);
+        for (int i = 0; i < N; ++i) s[0] += v[i];
+      }
+      row_sums<1, WAVES>(s, p.lanes, sums, turn);
       const float mean = s[0] * p.inv;
       s[0] = 0.0f;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        float v[N];
+        piece_values<T>(x[u], v);
+        if (place(u) + N <= p.width) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          x[u][i] = (u * p.lanes + lane) * N + i < p.width ? x[u][i] - mean : 0.0f;
-          s[0] = fmaf(x[u][i], x[u][i], s[0]);
+          for (int i = 0; i < N; ++i) s[0] = fmaf(v[i] - mean, v[i] - mean, s[0]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) s[0] = place(u) + i < p.width ? fmaf(v[i] - mean, v[i] - mean, s[0]) : s[0];
         }
-      row_sums<1>(s, p.lanes, sums, turn);
+      }
+      row_sums<1, WAVES>(s, p.lanes, sums, turn);
       const float rstd = rsqrtf(fmaf(s[0], p.inv, p.eps));
       if (!live) continue;
       if (p.stats != nullptr && lane == 0) {
@@ -124,44 +140,65 @@ __global__ __launch_bounds__(kNormThreads) void layer_norm_kernel(LayerNormArgs 
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int at = (u * p.lanes + lane) * N;
-        if (at >= p.width) break;
-        float y[N];
+        if (place(u) >= p.width) break;
+        float v[N], f[N];
+        piece_values<T>(x[u], v);
 #pragma unroll
-        for (int i = 0; i < N; ++i) y[i] = fmaf(x[u][i] * rstd, w[u][i], b[u][i]);
-        store_row_part<T, N>((T*)p.out + r * p.width, at, p.width, y);
+        for (int i = 0; i < N; ++i) v[i] = (v[i] - mean) * rstd;
+        if (p.w != nullptr) {
+          piece_values<T>(w[u], f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) v[i] *= f[i];
+        }
+        if (p.b != nullptr) {
+          piece_values<T>(b[u], f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) v[i] += f[i];
+        }
+        store_row_part<T, N>(out, place(u), p.width, v);
       }
     } else {
-      const bool g_edge = edge || p.width < N;
+      const T* cotangent = (const T*)p.g + r * p.width;
       const float mean = p.stats[2 * r], rstd = p.stats[2 * r + 1];
-      float g[U][N], s[2] = {0.0f, 0.0f};
+      u32x4 g[U];
+      float s[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int u = 0; u < U; ++u) g[u] = norm_piece<T>(cotangent, place(u), p.width, last || p.width < N);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int at = (u * p.lanes + lane) * N;
-        norm_piece<T, N>((const T*)p.g + r * p.width, at, p.width, g_edge, g[u]);
+        float n[N], v[N], f[N];
+        piece_values<T>(x[u], n);
+        piece_values<T>(g[u], v);
+        if (p.w != nullptr) piece_values<T>(w[u], f);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          x[u][i] = at + i < p.width ? (x[u][i] - mean) * rstd : 0.0f;
+          n[i] = (n[i] - mean) * rstd;                     // beyond the width g is zero
           if (live) {
-            dw[u][i] = fmaf(g[u][i], x[u][i], dw[u][i]);
-            db[u][i] += g[u][i];
+            dw[u][i] = fmaf(v[i], n[i], dw[u][i]);
+            db[u][i] += v[i];
           }
-          g[u][i] *= w[u][i];
-          s[0] += g[u][i];
-          s[1] = fmaf(g[u][i], x[u][i], s[1]);
+          if (p.w != nullptr) v[i] *= f[i];
+          s[0] += v[i];
+          s[1] = fmaf(v[i], n[i], s[1]);
         }
       }
-      row_sums<2>(s, p.lanes, sums, turn);
+      row_sums<2, WAVES>(s, p.lanes, sums, turn);
       if (!live || p.out == nullptr) continue;
       const float mg = s[0] * p.inv, mgn = s[1] * p.inv;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int at = (u * p.lanes + lane) * N;
-        if (at >= p.width) break;
-        float y[N];
+        if (place(u) >= p.width) break;
+        float n[N], v[N], f[N];
+        piece_values<T>(x[u], n);
+        piece_values<T>(g[u], v);
+        if (p.w != nullptr) {
+          piece_values<T>(w[u], f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) y[i] = rstd * (g[u][i] - fmaf(x[u][i], mgn, mg));
-        store_row_part<T, N>((T*)p.out + r * p.width, at, p.width, y);
+          for (int i = 0; i < N; ++i) v[i] *= f[i];
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = rstd * (v[i] - fmaf((n[i] - mean) * rstd, mgn, mg));
+        store_row_part<T, N>(out, place(u), p.width, v);
       }
     }
   }
@@ -176,7 +213,7 @@ __global__ __launch_bounds__(kNormThreads) void layer_norm_kernel(LayerNormArgs 
         __syncthreads();
         store_pack<float, N>(columns + (size_t)threadIdx.x * N, m == 0 ? dw[u] : db[u]);
         __syncthreads();
-        for (int i = threadIdx.x; i < span; i += kNormThreads) {
+        for (int i = threadIdx.x; i < span; i += THREADS) {
           const int c = u * span + i;
           if (c >= p.width) continue;
           float v = 0.0f;
@@ -212,26 +249,44 @@ __global__ __launch_bounds__(1024) void layer_norm_join_kernel(const float* __re
   }
 }
 
-// pieces a thread; fills in the threads of a row
+// Threads of a block, pieces a thread; fills in the threads of a row: a wave at most where four pieces a lane do
+struct NormShape {
+  int threads, pieces;
+  int64_t rows;                    // of a block
+};
 template <typename T>
-static int norm_pieces(LayerNormArgs& p) {
+static NormShape norm_shape(LayerNormArgs& p) {
   constexpr int N = 16 / sizeof(T);
   const int pieces = (p.width + N - 1) / N;
-  int u = 1;
-  while (u * kNormThreads < pieces) u *= 2;
+  NormShape n{pieces > 4 * 256 ? 1024 : 256, 1, 0};
+  const int most = n.threads == 1024 ? 1024 : kWave;
+  while (n.pieces < 4 && n.pieces * most < pieces) n.pieces *= 2;
   p.lanes = 1;
-  while (u * p.lanes < pieces) p.lanes *= 2;
-  return u;
+  while (n.pieces * p.lanes < pieces) p.lanes *= 2;
+  n.rows = n.threads / p.lanes;
+  return n;
 }
 
 template <typename T, bool BACK>
-static void layer_norm_launch(LayerNormArgs p, int blocks, int u, hipStream_t s) {
-  if (u == 1)
-    hipLaunchKernelGGL((layer_norm_kernel<T, 1, BACK>), dim3(blocks), dim3(kNormThreads), 0, s, p);
-  else if (u == 2)
-    hipLaunchKernelGGL((layer_norm_kernel<T, 2, BACK>), dim3(blocks), dim3(kNormThreads), 0, s, p);
-  else if constexpr (sizeof(T) == 4)
-    hipLaunchKernelGGL((layer_norm_kernel<T, 4, BACK>), dim3(blocks), dim3(kNormThreads), 0, s, p);
+static void layer_norm_launch(LayerNormArgs p, int blocks, const NormShape& n, hipStream_t s) {
+#define XNN_NORM_LAUNCH(THREADS, U)                                                                        \
+  hipLaunchKernelGGL((layer_norm_kernel<T, THREADS, U, BACK>), dim3(blocks), dim3(THREADS), 0, s, p)
+  if (n.threads == 1024) {
+    if constexpr (sizeof(T) == 4) {
+      if (n.pieces == 4) {
+        XNN_NORM_LAUNCH(1024, 4);
+        return;
+      }
+    }
+    XNN_NORM_LAUNCH(1024, 2);
+  } else if (n.pieces == 1) {
+    XNN_NORM_LAUNCH(256, 1);
+  } else if (n.pieces == 2) {
+    XNN_NORM_LAUNCH(256, 2);
+  } else {
+    XNN_NORM_LAUNCH(256, 4);
+  }
+#undef XNN_NORM_LAUNCH
 }
 
 static int layer_norm_sizes(int dtype, int64_t n_rows, int32_t width) {
@@ -267,10 +322,9 @@ int xnn_layer_norm(int dtype, const void* x, int64_t x_stride, int64_t n_rows, i
   p.eps = eps;
   p.inv = 1.0f / (float)width;
   XNN_STORAGE_DISPATCH(dtype, T, {
-    const int u = norm_pieces<T>(p);
-    const int64_t rows = kNormThreads / p.lanes;
-    layer_norm_launch<T, false>(p, (int)std::min<int64_t>((n_rows + rows - 1) / rows, 1 << 20), u,
-                                as_hip(stream));
+    const NormShape n = norm_shape<T>(p);
+    // eight blocks a CU go over the rows: their weights are read once
+    layer_norm_launch<T, false>(p, (int)std::min<int64_t>((n_rows + n.rows - 1) / n.rows, 2048), n, as_hip(stream));
   });
   XNN_LAUNCH_CHECK();
   return XNN_OK;
@@ -310,10 +364,9 @@ int xnn_layer_norm_backward(int dtype, const void* grad, const void* x, int64_t 
   XNN_STORAGE_DISPATCH(dtype, T, {
     int blocks = 0;
     if (n_rows > 0) {
-      const int u = norm_pieces<T>(p);
-      const int64_t rows = kNormThreads / p.lanes;
-      blocks = (int)std::min<int64_t>((n_rows + rows - 1) / rows, kNormParts);
-      layer_norm_launch<T, true>(p, blocks, u, s);
+      const NormShape n = norm_shape<T>(p);
+      blocks = (int)std::min<int64_t>((n_rows + n.rows - 1) / n.rows, kNormParts);
+      layer_norm_launch<T, true>(p, blocks, n, s);
     }
     if (weights && blocks != 1)
       hipLaunchKernelGGL(layer_norm_join_kernel<T>, dim3((2 * width + 15) / 16), dim3(1024), 0, s,
