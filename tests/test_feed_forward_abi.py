@@ -56,7 +56,7 @@ def test_group_plan_arguments(lib):
     size, f = lib.xnn_group_plan_size, lib.xnn_group_plan
     two = (ctypes.byref(SIZE), ctypes.byref(MORE))
     assert size(1000, 9, *two) == 0
-    assert SIZE.value == 4 * (1000 + 17 * 11) and MORE.value > 0
+    assert SIZE.value == 4 * (1000 + 53 * 11) and MORE.value > 0
     _refused(lib, size(-1, 9, *two), b"n must")
     _refused(lib, size(1 << 30, 9, *two), b"n must")
     _refused(lib, size(10, 0, *two), b"n_groups")
@@ -130,7 +130,7 @@ def test_functions_refuse_cpu_tensors():
     x, w = torch.zeros(4, 8), torch.zeros(8, 8)
     for call in (lambda: xa.layer_norm(x), lambda: xa.linear(x, w),
                  lambda: xa.group_plan(torch.zeros(4, dtype=torch.int64), 3),
-                 lambda: xa.grouped_linear(x, w[None], xa.GroupPlan(4, 1, torch.zeros(55, dtype=torch.int32)))):
+                 lambda: xa.grouped_linear(x, w[None], xa.GroupPlan(4, 1, torch.zeros(163, dtype=torch.int32)))):
         with pytest.raises(RuntimeError, match="GPU only"):
             call()
 
@@ -145,4 +145,4 @@ def test_refused_names_and_plans():
     with pytest.raises(TypeError, match="GroupPlan"):
         xa.grouped_linear(x, w[None], torch.zeros(4))
     with pytest.raises(ValueError, match="groups"):
-        xa.grouped_linear(x, torch.zeros(3, 8, 8), xa.GroupPlan(4, 2, torch.zeros(72, dtype=torch.int32)))
+        xa.grouped_linear(x, torch.zeros(3, 8, 8), xa.GroupPlan(4, 2, torch.zeros(216, dtype=torch.int32)))

@@ -360,10 +360,11 @@ def test_group_plan(rows, groups):
         assert (plan.n_rows, plan.n_groups) == (rows, groups)
         assert np.array_equal(got[:rows], np.argsort(bucket, kind="stable"))
         counts = np.bincount(bucket, minlength=groups + 1)
-        lists = got[rows:].reshape(17, groups + 2)
+        lists = got[rows:].reshape(53, groups + 2)
         assert np.array_equal(lists[0], np.concatenate([[0], np.cumsum(counts)]))
-        for level in range(16):
-            tiles = -(-counts // (32 << level))
+        sizes = [32, 64, 128, 256] + [(256 << o) // 4 * q for o in range(12) for q in (5, 6, 7, 8)]
+        for level, size in enumerate(sizes):
+            tiles = -(-counts // size)
             assert np.array_equal(lists[1 + level], np.concatenate([[0], np.cumsum(tiles)])), level
 
 

@@ -37,10 +37,16 @@ constexpr int kDenseWaves = kDenseThreads / kWave;
 
 // ---------------------------------------------------------------- groups
 // What xnn_group_plan leaves, in int32: `order`, the rows by group (stable); row_ptr (n_groups + 2), where a
-// group's rows begin, the last bucket holding the rows of no group; for each level s the prefix sums of the
-// groups' tiles of 32 << s rows.
-constexpr int kGroupLevels = 16;
+// group's rows begin, the last bucket holding the rows of no group; for each level the prefix sums of the groups'
+// tiles of its rows: 32, 64, 128, 256, then four levels an octave, so that a weight's parts fill whole rounds of
+// blocks nearly as well as parts of any size do.
+constexpr int kGroupLevels = 52;
 constexpr int kMaxGroups = 4096;
+
+__host__ __device__ constexpr int level_rows(int level) {
+  return level < 4 ? 32 << level : (256 << ((level - 4) / 4)) / 4 * (5 + (level - 4) % 4);
+}
+static_assert(level_rows(4) == 320 && level_rows(7) == 512 && level_rows(kGroupLevels - 1) == 1 << 20, "");
 
 struct GroupView {
   const int32_t *order, *row_ptr, *tile_ptr;   // tile_ptr of the level in use
@@ -84,15 +90,39 @@ __device__ __forceinline__ RowTile row_tile(const GroupView& v, int n_buckets, i
     const int begin = t * size;
     return RowTile{begin, min(n_rows, begin + size), 0};
   }
-  if (t >= v.tile_ptr[n_buckets]) return RowTile{0, 0, -1};
-  const int g = find_group(v.tile_ptr, n_buckets, t);
-  const int begin = max(0, v.row_ptr[g] + (t - v.tile_ptr[g]) * size);
-  const int end = min(min(v.row_ptr[g + 1], n_rows), begin + size);
+  int g, before, from, to;         // tiles before the group's, its rows
+  if (n_buckets < kWave) {         // both lists in one load each
+    const int lane = min((int)(threadIdx.x % kWave), n_buckets);
+    const int tiles = v.tile_ptr[lane], rows = v.row_ptr[lane];
+    if (t >= __builtin_amdgcn_readlane(tiles, n_buckets)) return RowTile{0, 0, -1};
+    g = __builtin_amdgcn_readfirstlane(__popcll(__ballot(threadIdx.x % kWave < n_buckets && tiles <= t)) - 1);
+    g = max(g, 0);
+    before = __builtin_amdgcn_readlane(tiles, g);
+    from = __builtin_amdgcn_readlane(rows, g);
+    to = __builtin_amdgcn_readlane(rows, g + 1);
+  } else {
+    if (t >= v.tile_ptr[n_buckets]) return RowTile{0, 0, -1};
+    g = find_group(v.tile_ptr, n_buckets, t);
+    before = v.tile_ptr[g];
+    from = v.row_ptr[g];
+    to = v.row_ptr[g + 1];
+  }
+  const int begin = max(0, from + (t - before) * size);
+  const int end = min(min(to, n_rows), begin + size);
   return RowTile{begin, end, begin < end ? g : -1};
 }
 
 __device__ __forceinline__ int64_t group_row(const GroupView& v, int r) {
   return v.order == nullptr ? r : v.order[r];
+}
+
+// the tile's rows for its way out, -1 where it has none; the product's barriers are between this and their use
+template <int BM>
+__device__ __forceinline__ void note_rows(const GroupView& v, const RowTile& t, int n_rows, int32_t (&rows)[BM]) {
+  for (int i = threadIdx.x; i < BM; i += blockDim.x) {
+    const int64_t row = t.begin + i < t.end ? group_row(v, t.begin + i) : -1;
+    rows[i] = row >= 0 && row < n_rows ? (int32_t)row : -1;
+  }
 }
 
 // the tile's columns [n0, n0 + BN) of the tile's rows, all of one value
@@ -682,9 +712,10 @@ inline int dense_tile(size_t size, int64_t m, int64_t n, int64_t groups) {
     }                                                \
   } while (0)
 
+// the first level of at least so many rows
 inline int group_level(int64_t rows) {
   int s = 0;
-  while ((32 << s) < rows) ++s;
+  while (s < kGroupLevels - 1 && level_rows(s) < rows) ++s;
   return s;
 }
 

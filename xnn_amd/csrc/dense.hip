@@ -22,6 +22,7 @@ template <typename T, typename L>
 __global__ __launch_bounds__(kDenseThreads) void dense_forward_kernel(ForwardArgs p) {
   typedef DenseLds<L, T, true, false> S;
   __shared__ __align__(16) char lds[S::kBytes];
+  __shared__ int32_t rows[L::BM];
   const int64_t slot = xcd_slot();
   if (slot >= p.tiles) return;
   const int tn = (int)(slot % p.tiles_n);
@@ -32,6 +33,7 @@ __global__ __launch_bounds__(kDenseThreads) void dense_forward_kernel(ForwardArg
     fill_rows<T, L::BN>(p.groups, t, p.n_rows, (T*)p.out, n0, p.n_out, (T)__builtin_nanf(""));
     return;
   }
+  note_rows(p.groups, t, p.n_rows, rows);
   Operator<T, L::BM, L::BK, true> a;
   Operator<T, L::BN, L::BK, false> b;
   a.init(p.x, p.groups.order, p.x_stride, p.n_rows, p.n_in, t.begin, t.end, 0);
@@ -52,10 +54,8 @@ __global__ __launch_bounds__(kDenseThreads) void dense_forward_kernel(ForwardArg
           load_row_part<T, N>((const T*)p.bias + (int64_t)t.group * p.n_out, c, p.n_out, bias);
       },
       [&](int m, float(&v)[N]) {
-        const int r = t.begin + m;
-        if (r >= t.end || c >= p.n_out) return;
-        const int64_t row = group_row(p.groups, r);
-        if (row < 0 || row >= p.n_rows) return;
+        const int64_t row = rows[m];
+        if (row < 0 || c >= p.n_out) return;
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] += bias[i];
         if (p.activation != kNone) {

@@ -96,6 +96,7 @@ template <typename T, typename L, bool TIMES>
 __global__ __launch_bounds__(kDenseThreads) void dense_input_kernel(BackwardArgs p) {
   typedef DenseLds<L, T, true, true> S;
   __shared__ __align__(16) char lds[S::kBytes];
+  __shared__ int32_t rows[L::BM];
   const int64_t slot = xcd_slot();
   if (slot >= p.tiles) return;
   const int n0 = (int)(slot % p.tiles_n) * L::BN;
@@ -105,6 +106,7 @@ __global__ __launch_bounds__(kDenseThreads) void dense_input_kernel(BackwardArgs
     fill_rows<T, L::BN>(p.groups, t, p.n_rows, (T*)p.dx, n0, p.n_in, (T)0.0f);
     return;
   }
+  note_rows(p.groups, t, p.n_rows, rows);
   Operator<T, L::BM, L::BK, true, TIMES> a;
   Operator<T, L::BN, L::BK, true> b;
   a.init(p.g, p.groups.order, p.n_out, p.n_rows, p.n_out, t.begin, t.end, 0, p.slope);
@@ -117,10 +119,8 @@ __global__ __launch_bounds__(kDenseThreads) void dense_input_kernel(BackwardArgs
   dense_rows<L, N>(
       lds, acc, [&](int n) { c = n0 + n; },
       [&](int m, float(&v)[N]) {
-        const int r = t.begin + m;
-        if (r >= t.end || c >= p.n_in) return;
-        const int64_t row = group_row(p.groups, r);
-        if (row < 0 || row >= p.n_rows) return;
+        const int64_t row = rows[m];
+        if (row < 0 || c >= p.n_in) return;
         store_row_part<T, N>((T*)p.dx + row * p.n_in, c, p.n_in, v);
       });
 }
@@ -259,12 +259,12 @@ struct Parts {
   int rows;
   int64_t slots;                   // parts that have sums of their own
 };
-// Parts of at least `least` rows, about `want` of them; in groups of a power of two rows (the plan has their tiles)
+// Parts of at least `least` rows, about `want` of them; in groups of a level's rows (the plan has their tiles)
 static Parts parts_of(int64_t n_rows, bool grouped, int64_t want, int64_t least) {
   int64_t rows = std::max<int64_t>(least, (n_rows + want - 1) / std::max<int64_t>(want, 1));
   Parts w;
   if (grouped) {
-    rows = (int64_t)32 << std::min(group_level(rows), kGroupLevels - 1);
+    rows = level_rows(group_level(rows));
     w.slots = n_rows <= rows ? 0 : 2 * (n_rows / rows + 1);
   } else {
     rows = (rows + 63) / 64 * 64;
@@ -299,7 +299,7 @@ static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32
     double best = 0.0;
     for (int kind = 0; kind < (size == 2 && !(slope && n_in <= kFormInProducts) ? 3 : 2); ++kind) {
       const int64_t t = tiles(bm[kind], bn[kind]);
-      for (int64_t want = 1; want <= 1024; want *= 2) {
+      for (int64_t want = 1; want <= 1024; want += std::max<int64_t>(1, want / 4)) {
         const Parts parts = parts_of(n_rows, grouped, want, 256);
         const int64_t n = row_tiles(n_rows, n_groups, false, parts.rows) + (grouped ? n_groups / 2 : 0);
         const double rounds = std::max(1.0, std::ceil((double)(n * t) / (256 * per_cu[kind])));

@@ -205,9 +205,9 @@ Tensor group_plan_kernel(const Tensor& ids_, int64_t n_groups) {
   return plan;
 }
 
-// as xnn_group_plan_size: the rows, where the groups begin, and sixteen lists of their tiles
+// as xnn_group_plan_size: the rows, where the groups begin, and fifty-two lists of their tiles
 Tensor group_plan_shape(const Tensor& ids, int64_t n_groups) {
-  return at::empty_symint({ids.sym_numel() + 17 * (n_groups + 2)}, ids.options().dtype(at::kInt));
+  return at::empty_symint({ids.sym_numel() + 53 * (n_groups + 2)}, ids.options().dtype(at::kInt));
 }
 
 // ---------------------------------------------------------------- dense layers

@@ -34,54 +34,53 @@ __global__ __launch_bounds__(kWave) void group_count_kernel(const int64_t* __res
     counts[(int64_t)blockIdx.x * (n_groups + 1) + b] = c[b];
 }
 
-// counts become the place of each run's first row of the bucket; row_ptr and the levels' tile_ptr
+// Counts become the place of each run's first row of the bucket; row_ptr and the levels' tile_ptr. A bucket's counts go
+// to 2^k threads, each a stretch of the runs; then a wave a list adds up the buckets, 64 at a time.
 __global__ __launch_bounds__(1024) void group_place_kernel(int32_t* __restrict__ counts, int runs, int n_groups,
-                                                           int32_t* __restrict__ row_ptr) {
-  __shared__ int32_t total[kMaxGroups + 2];
-  __shared__ int32_t waves[16];
+                                                           int lanes, int32_t* __restrict__ row_ptr) {
+  __shared__ int32_t total[kMaxGroups + 1];
+  __shared__ int32_t part[1024];
   const int tid = threadIdx.x, buckets = n_groups + 1;
-  for (int b = tid; b < buckets; b += 1024) {
+  const int per = 1024 / lanes, lane = tid / per, each = (runs + lanes - 1) / lanes;
+  const int r0 = min(runs, lane * each), r1 = min(runs, r0 + each);
+  for (int b0 = 0; b0 < buckets; b0 += per) {
+    const int b = b0 + tid % per;
     int32_t s = 0;
-    for (int r = 0; r < runs; ++r) {
-      int32_t* p = counts + (int64_t)r * buckets + b;
-      const int32_t v = *p;
-      *p = s;
-      s += v;
-    }
-    total[b] = s;
-  }
-  __syncthreads();
-  // prefix sums of the rows (level -1) and of each level's tiles: five buckets a thread in turn
-  constexpr int kEach = (kMaxGroups + 1 + 1023) / 1024;
-  for (int level = -1; level < kGroupLevels; ++level) {
-    const auto tiles = [&](int32_t rows) {
-      return level < 0 ? rows : (int32_t)(((int64_t)rows + (32 << level) - 1) >> (5 + level));
-    };
-    int32_t own = 0;
-    for (int i = 0; i < kEach; ++i) {
-      const int b = tid * kEach + i;
-      if (b < buckets) own += tiles(total[b]);
-    }
-    int32_t sum = own;                                     // inclusive within the wave
-#pragma unroll
-    for (int o = 1; o < kWave; o *= 2) {
-      const int32_t v = __shfl_up(sum, o, kWave);
-      if (tid % kWave >= o) sum += v;
-    }
-    if (tid % kWave == kWave - 1) waves[tid / kWave] = sum;
+    if (b < buckets)
+#pragma unroll 8
+      for (int r = r0; r < r1; ++r) s += counts[(int64_t)r * buckets + b];
+    part[tid] = s;
     __syncthreads();
-    int32_t at = sum - own;
-    for (int w = 0; w < tid / kWave; ++w) at += waves[w];
-    int32_t* out = row_ptr + (int64_t)(level + 1) * (n_groups + 2);
-    for (int i = 0; i < kEach; ++i) {
-      const int b = tid * kEach + i;
-      if (b < buckets) {
-        out[b] = at;
-        at += tiles(total[b]);
-        if (b == buckets - 1) out[buckets] = at;
+    if (b < buckets) {
+      int32_t at = 0;
+      for (int l = 0; l < lane; ++l) at += part[l * per + tid % per];
+      if (lane == lanes - 1) total[b] = at + s;
+      for (int r = r0; r < r1; ++r) {
+        int32_t* p = counts + (int64_t)r * buckets + b;
+        const int32_t v = *p;
+        *p = at;
+        at += v;
       }
     }
     __syncthreads();
+  }
+  for (int list = tid / kWave; list <= kGroupLevels; list += 1024 / kWave) {
+    int32_t* out = row_ptr + (int64_t)list * (n_groups + 2);
+    const int size = list == 0 ? 1 : level_rows(list - 1);
+    int32_t before = 0;
+    for (int b0 = 0; b0 < buckets; b0 += kWave) {
+      const int b = b0 + tid % kWave;
+      const int32_t own = b < buckets ? (int32_t)(((int64_t)total[b] + size - 1) / size) : 0;
+      int32_t sum = own;                                   // inclusive
+#pragma unroll
+      for (int o = 1; o < kWave; o *= 2) {
+        const int32_t v = __shfl_up(sum, o, kWave);
+        if (tid % kWave >= o) sum += v;
+      }
+      if (b < buckets) out[b] = before + sum - own;
+      before += __shfl(sum, kWave - 1, kWave);
+    }
+    if (tid % kWave == 0) out[buckets] = before;
   }
 }
 
@@ -145,7 +144,9 @@ int xnn_group_plan(const int64_t* ids, int64_t n, int32_t n_groups, int32_t* pla
   while ((1 << bits) <= n_groups) ++bits;
   if (runs > 0)
     hipLaunchKernelGGL(group_count_kernel, dim3(runs), dim3(kWave), 0, s, ids, (int)n, n_groups, counts);
-  hipLaunchKernelGGL(group_place_kernel, dim3(1), dim3(1024), 0, s, counts, runs, n_groups, row_ptr);
+  int lanes = 1;                   // threads of a bucket's counts
+  while (lanes < runs && lanes * 2 * (n_groups + 1) <= 1024) lanes *= 2;
+  hipLaunchKernelGGL(group_place_kernel, dim3(1), dim3(1024), 0, s, counts, runs, n_groups, lanes, row_ptr);
   if (runs > 0)
     hipLaunchKernelGGL(group_scatter_kernel, dim3(runs), dim3(kWave), 0, s, ids, (int)n, n_groups, bits, counts,
                        row_ptr, plan);
