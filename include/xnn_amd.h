@@ -1291,21 +1291,28 @@ int xnn_group_plan_size(int64_t n, int32_t n_groups, size_t* plan_bytes, size_t*
 int xnn_group_plan(const int64_t* ids, int64_t n, int32_t n_groups, int32_t* plan, void* work,
                    size_t work_bytes, xnn_stream_t stream);
 
+/* Bytes of the workspace of xnn_linear (0 where it needs none: only a long reduction for few
+ * outputs is cut into parts that are added); grouped: with a plan. */
+int xnn_linear_work_size(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, int32_t n_groups,
+                         int32_t grouped, size_t* bytes);
+
 /* out (n_rows, n_out) = residual + activation(x weight + bias), weight (n_in, n_out), bias (n_out)
  * and residual (n_rows, n_out) contiguous, bias and residual may be NULL; row r of x at
  * x + r * x_stride. With a plan (xnn_group_plan of these rows) weight (n_groups, n_in, n_out) and
  * bias (n_groups, n_out) are those of each row's group, and a row of no group is NaN; without
  * (NULL) n_groups is 1. slope (n_rows, n_out), for the backward pass: the activation's derivative, of
  * 4 bytes an element for XNN_F32 and 2 for the others, in a form of its own (NULL: not wanted, and
- * where there is no activation). */
+ * where there is no activation). `work` is aligned to 16 bytes. */
 int xnn_linear(int dtype, const void* x, int64_t x_stride, int64_t n_rows, int32_t n_in, int32_t n_out,
                const void* weight, const void* bias, int32_t activation, const void* residual,
-               const int32_t* plan, int32_t n_groups, void* out, void* slope, xnn_stream_t stream);
+               const int32_t* plan, int32_t n_groups, void* out, void* slope, void* work, size_t work_bytes,
+               xnn_stream_t stream);
 
-/* Bytes of the workspace of xnn_linear_backward; grouped: with a plan; slope, weight, bias: with a
- * slope, with dweight, with dbias. */
+/* Bytes of the workspace of xnn_linear_backward; grouped: with a plan; slope, input, weight, bias:
+ * with a slope, with dx, with dweight, with dbias. */
 int xnn_linear_backward_work_size(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, int32_t n_groups,
-                                  int32_t grouped, int32_t slope, int32_t weight, int32_t bias, size_t* bytes);
+                                  int32_t grouped, int32_t slope, int32_t input, int32_t weight, int32_t bias,
+                                  size_t* bytes);
 
 /* Gradients for the cotangent `grad` (n_rows, n_out), contiguous: dx (n_rows, n_in; zero in rows of no
  * group), dweight and dbias as weight and bias (zero for a group without rows), each of which may be

@@ -69,11 +69,20 @@ def test_group_plan_arguments(lib):
 
 
 def test_linear_arguments(lib):
-    f = lib.xnn_linear
+    f, size = lib.xnn_linear, lib.xnn_linear_work_size
+    assert size(0, 100000, 64, 64, 1, 0, ctypes.byref(SIZE)) == 0 and SIZE.value == 0
+    assert size(0, 20, 4096, 64, 1, 0, ctypes.byref(SIZE)) == 0 and SIZE.value > 0     # a long sum for few outputs
+    need = SIZE.value
+    _refused(lib, size(0, 20, 4096, 64, 1, 0, None), b"NULL size")
+    _refused(lib, size(1, 20, 4096, 64, 1, 0, ctypes.byref(SIZE)), b"dtype")
 
-    def call(dtype=0, x=BUF, stride=8, rows=4, n_in=8, n_out=4, w=BUF, act=0, plan=None, groups=1, out=BUF,
-             slope=None):
-        return f(dtype, x, stride, rows, n_in, n_out, w, None, act, None, plan, groups, out, slope, None)
+    def call(dtype=0, x=BUF, stride=None, rows=4, n_in=8, n_out=4, w=BUF, act=0, plan=None, groups=1, out=BUF,
+             slope=None, work=BUF, room=0):
+        return f(dtype, x, n_in if stride is None else stride, rows, n_in, n_out, w, None, act, None, plan, groups,
+                 out, slope, work, room, None)
+    _refused(lib, call(rows=20, n_in=4096, n_out=64, room=need - 1), b"work too small")
+    _refused(lib, call(rows=20, n_in=4096, n_out=64, room=need, work=None), b"work too small")
+    _refused(lib, call(rows=20, n_in=4096, n_out=64, room=need, work=ctypes.addressof(BUF) + 4), b"aligned")
     _refused(lib, call(dtype=1), b"dtype")
     _refused(lib, call(rows=-1), b"n_rows")
     _refused(lib, call(rows=1 << 30), b"n_rows")
@@ -95,18 +104,18 @@ def test_linear_arguments(lib):
 
 def test_linear_backward_arguments(lib):
     def size(dtype, rows, groups, grouped=0, slope=0, weight=1, bias=0, out=None):
-        return lib.xnn_linear_backward_work_size(dtype, rows, 64, 64, groups, grouped, slope, weight, bias,
+        return lib.xnn_linear_backward_work_size(dtype, rows, 64, 64, groups, grouped, slope, 0, weight, bias,
                                                  ctypes.byref(SIZE) if out is None else out)
     assert size(0, 20, 1) == 0 and SIZE.value == 0
     assert size(2, 1000, 1, slope=1, weight=0) == 0 and SIZE.value == 0
-    assert lib.xnn_linear_backward_work_size(2, 1000, 200, 64, 1, 0, 1, 0, 0, ctypes.byref(SIZE)) == 0
+    assert lib.xnn_linear_backward_work_size(2, 1000, 200, 64, 1, 0, 1, 0, 0, 0, ctypes.byref(SIZE)) == 0
     assert SIZE.value == 1000 * 64 * 2                      # d
     assert size(0, 100000, 1) == 0
     need = SIZE.value
     assert need > 0
     _refused(lib, size(0, 20, 5000, 1), b"n_groups")
     _refused(lib, size(1, 20, 1), b"dtype")
-    _refused(lib, lib.xnn_linear_backward_work_size(0, 20, 64, 64, 1, 0, 0, 1, 0, None), b"NULL size")
+    _refused(lib, lib.xnn_linear_backward_work_size(0, 20, 64, 64, 1, 0, 0, 0, 1, 0, None), b"NULL size")
     f = lib.xnn_linear_backward
 
     def call(grad=BUF, slope=None, x=BUF, stride=64, rows=100000, w=BUF, dx=None, dw=BUF, db=None, work=BUF,

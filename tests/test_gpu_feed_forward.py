@@ -239,6 +239,14 @@ def test_linear_of_many_tiles(dtype, rows, n_in, n_out):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n_in,n_out", [(1, 4096, 70), (3, 70, 4097), (100, 3001, 130), (130, 200, 2900),
+                                             (64, 1030, 1030)])
+def test_linear_of_long_sums_for_few_outputs(dtype, rows, n_in, n_out):
+    _check_dense(dtype, _dense_case(dtype, rows, n_in, n_out, residual=True), "tanh")
+    _check_dense(dtype, _dense_case(dtype, rows, n_in, n_out, 5, some=[-1, 1, 1, 4]), "gelu")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,n_in,n_out", [(1, 5, 3), (70, 64, 64), (129, 33, 65)])
 def test_linear_of_a_part_of_wider_rows(dtype, rows, n_in, n_out):
     _check_dense(dtype, _dense_case(dtype, rows, n_in, n_out, strided=True), "gelu")
@@ -441,7 +449,7 @@ def test_rows_behind_the_output_are_left():
         x, w, _, _, _, _ = _dense_case("f32", rows, 24, n_out)
         out = torch.full((rows * n_out + 256,), -7.0, device=DEV)
         _lib.call("xnn_linear", 0, x.data_ptr(), 24, rows, 24, n_out, w.data_ptr(), None, 0, None, None, 1,
-                  out.data_ptr(), None, _lib.stream(torch.device(DEV)))
+                  out.data_ptr(), None, None, 0, _lib.stream(torch.device(DEV)))
         assert torch.equal(out[:rows * n_out].view(rows, n_out), xa.linear(x, w))
         assert (out[rows * n_out:] == -7.0).all()
 

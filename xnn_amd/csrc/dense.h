@@ -348,7 +348,7 @@ struct Operator {
     end = end_row - first_row;
     const bool whole = width % kPer == 0;
     most = ALONG || whole ? last : max(last - 1, 0);
-    fast = stride_ < kPer ? 0 : ALONG ? width / BK * BK : (whole ? end : end - 1) / BK * BK;
+    fast = stride_ < kPer ? 0 : ALONG ? (width - first_col) / BK * BK : (whole ? end : end - 1) / BK * BK;
     edges = 0;
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {
@@ -550,7 +550,7 @@ __device__ __forceinline__ void dense_product(A& a, B& b, int length, char* lds,
     a.fetch_fast(k);
     b.fetch_fast(k);
   };
-  const int fast = min(a.fast, b.fast);
+  const int fast = min(min(a.fast, b.fast), length);
   int k = 0;
   fetch(k);
   if constexpr (S::kStages == 2) {
@@ -670,6 +670,109 @@ __device__ __forceinline__ void store_row_part(T* row, int at, int width, const 
   }
 }
 
+// ---------------------------------------------------------------- outputs
+// What becomes of the sums of a row: residual + f(v + bias), and the slope
+struct Output {
+  const void *bias, *residual;     // NULL: none
+  void *out, *slope;
+  float* part;                     // (parts, rows, width): sums of parts of the reduction
+  GroupView groups;
+  int n_rows, width, activation;
+  float none;                      // in the rows of no group
+};
+
+template <typename T>
+__device__ __forceinline__ void load_bias(const Output& o, int group, int c, float (&bias)[16 / sizeof(T)]) {
+  constexpr int N = 16 / sizeof(T);
+#pragma unroll
+  for (int i = 0; i < N; ++i) bias[i] = 0.0f;
+  if (o.bias != nullptr && c < o.width)
+    load_row_part<T, N>((const T*)o.bias + (int64_t)group * o.width, c, o.width, bias);
+}
+
+template <typename T>
+__device__ __forceinline__ void put_row(const Output& o, int64_t row, int c, float (&v)[16 / sizeof(T)],
+                                        const float (&bias)[16 / sizeof(T)]) {
+  constexpr int N = 16 / sizeof(T);
+  typedef typename Slope<T>::type S;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] += bias[i];
+  if (o.activation != kNone) {
+    S slope[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float s;
+      activate(o.activation, v[i], v[i], s);
+      slope[i] = slope_stored<T>(s);
+    }
+    if (o.slope != nullptr) store_row_part<S, N>((S*)o.slope + row * o.width, c, o.width, slope);
+  }
+  if (o.residual != nullptr) {
+    float z[N];
+    load_row_part<T, N>((const T*)o.residual + row * o.width, c, o.width, z);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += z[i];
+  }
+  store_row_part<T, N>((T*)o.out + row * o.width, c, o.width, v);
+}
+
+// A tile's sums to where they go: the outputs, or the part's sums
+template <typename T, typename L>
+__device__ __forceinline__ void put_tile(char* lds, const f32x16 (&acc)[L::MT][L::NT], const Output& o, int parts,
+                                         int part, int group, const int32_t (&rows)[L::BM], int n0) {
+  int c;
+  if (parts > 1) {
+    float* to = o.part + (int64_t)part * o.n_rows * o.width;
+    dense_rows<L, 4>(
+        lds, acc, [&](int n) { c = n0 + n; },
+        [&](int m, float(&v)[4]) {
+          const int64_t row = rows[m];
+          if (row >= 0 && c < o.width) store_row_part<float, 4>(to + row * o.width, c, o.width, v);
+        });
+    return;
+  }
+  constexpr int N = 16 / sizeof(T);
+  float bias[N];
+  dense_rows<L, N>(
+      lds, acc,
+      [&](int n) {
+        c = n0 + n;
+        load_bias<T>(o, group, c, bias);
+      },
+      [&](int m, float(&v)[N]) {
+        const int64_t row = rows[m];
+        if (row >= 0 && c < o.width) put_row<T>(o, row, c, v, bias);
+      });
+}
+
+// The parts of a reduction added in their order: blocks of 32 sorted rows by 16 pieces of 16 bytes
+template <typename T>
+__global__ __launch_bounds__(256) void dense_parts_kernel(Output o, int parts, int columns) {
+  constexpr int N = 16 / sizeof(T);
+  const RowTile t = row_tile(o.groups, o.groups.n_groups + 1, o.n_rows, blockIdx.x / columns, 32);
+  if (t.group < 0) return;
+  const int c = (blockIdx.x % columns * 16 + threadIdx.x % 16) * N;
+  if (c >= o.width) return;
+  const bool none = o.groups.n_groups > 0 && t.group == o.groups.n_groups;   // rows of no group: done
+  float bias[N];
+  if (!none) load_bias<T>(o, t.group, c, bias);
+  for (int r = t.begin + threadIdx.x / 16; r < t.end && !none; r += 16) {
+    const int64_t row = group_row(o.groups, r);
+    if (row < 0 || row >= o.n_rows) continue;
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.0f;
+#pragma unroll 4
+    for (int n = 0; n < parts; ++n) {
+      float x[N];
+      load_row_part<float, N>(o.part + ((int64_t)n * o.n_rows + row) * o.width, c, o.width, x);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += x[i];
+    }
+    put_row<T>(o, row, c, v, bias);
+  }
+}
+
 // ---------------------------------------------------------------- host side
 // Tiles: 64 x 64; 128 x 128; in 16 bits 256 x 128, whose steps of 32 leave LDS and registers for two blocks a CU, one
 // in its products while the other loads or stores (24,000 x 1,024 x 4,096 in bfloat16 with gelu: 256 x 256, one
@@ -722,6 +825,40 @@ inline int group_level(int64_t rows) {
 // an upper bound of the tiles of `size` rows
 inline int64_t row_tiles(int64_t n_rows, int64_t n_groups, bool grouped, int64_t size) {
   return grouped ? n_rows / size + std::min<int64_t>(n_groups + 1, n_rows) : (n_rows + size - 1) / size;
+}
+
+// The parts of a reduction of `length` for an output of m x n: more than one where its tiles leave the card idle, as
+// many as the estimated time has its least with: steps of 0.6 us (their loads' latency), a launch that adds the parts, their
+// sums written and read at 4 TB/s. Each is of `steps` whole steps.
+struct Split {
+  int parts, steps;
+  size_t bytes;
+};
+inline Split dense_split(size_t size, int kind, int64_t m, int64_t n, int64_t length) {
+  const int64_t step = 128 / size, steps = (length + step - 1) / step;
+  Split best{1, (int)steps, 0};
+  if (kind != kTile64) return best;
+  const int64_t tiles = ((m + 63) / 64) * ((n + 63) / 64);
+  double least = 0.6 * (double)steps;
+  for (int64_t p = 2; p <= steps && p * tiles <= 1024; ++p) {
+    const int64_t each = (steps + p - 1) / p;
+    if ((p - 1) * each >= steps) continue;                 // the last part would be empty
+    const double time = 0.6 * (double)each * (p * tiles > 768 ? 2 : 1) + 4.0 + (double)(p * m * n) * 8 / 4e6;
+    if (time < least) {
+      least = time;
+      best = Split{(int)p, (int)each, (size_t)p * m * n * sizeof(float)};
+    }
+  }
+  return best;
+}
+
+template <typename T>
+static void parts_launch(const Output& o, const int32_t* plan, int n_groups, int parts, hipStream_t s) {
+  Output q = o;
+  q.groups = group_view(plan, o.n_rows, n_groups, 0);
+  const int columns = (o.width + 16 * (int)(16 / sizeof(T)) - 1) / (16 * (int)(16 / sizeof(T)));
+  const int64_t blocks = row_tiles(o.n_rows, n_groups, plan != nullptr, 32) * columns;
+  hipLaunchKernelGGL(dense_parts_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, q, parts, columns);
 }
 
 inline int dense_sizes(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, const int32_t* plan,

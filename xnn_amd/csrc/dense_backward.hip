@@ -93,36 +93,30 @@ __global__ __launch_bounds__(256) void dense_cotangent_kernel(BackwardArgs p, in
 
 // ---------------------------------------------------------------- the products
 template <typename T, typename L, bool TIMES>
-__global__ __launch_bounds__(kDenseThreads) void dense_input_kernel(BackwardArgs p) {
+__global__ __launch_bounds__(kDenseThreads) void dense_input_kernel(BackwardArgs p, Output o, int parts, int steps) {
   typedef DenseLds<L, T, true, true> S;
   __shared__ __align__(16) char lds[S::kBytes];
   __shared__ int32_t rows[L::BM];
   const int64_t slot = xcd_slot();
-  if (slot >= p.tiles) return;
-  const int n0 = (int)(slot % p.tiles_n) * L::BN;
-  const RowTile t = row_tile(p.groups, p.groups.n_groups + 1, p.n_rows, (int)(slot / p.tiles_n), L::BM);
+  if (slot >= p.tiles * parts) return;
+  const int part = (int)(slot / p.tiles), tile = (int)(slot % p.tiles);
+  const RowTile t = row_tile(o.groups, o.groups.n_groups + 1, o.n_rows, tile / p.tiles_n, L::BM);
   if (t.group < 0) return;
-  if (p.groups.n_groups > 0 && t.group == p.groups.n_groups) {   // rows of no group
-    fill_rows<T, L::BN>(p.groups, t, p.n_rows, (T*)p.dx, n0, p.n_in, (T)0.0f);
+  const int n0 = tile % p.tiles_n * L::BN;
+  if (o.groups.n_groups > 0 && t.group == o.groups.n_groups) {   // rows of no group
+    if (part == 0) fill_rows<T, L::BN>(o.groups, t, o.n_rows, (T*)o.out, n0, o.width, (T)o.none);
     return;
   }
-  note_rows(p.groups, t, p.n_rows, rows);
+  const int k0 = part * steps * L::BK, k1 = min(p.n_out, k0 + steps * L::BK);
+  note_rows(o.groups, t, o.n_rows, rows);
   Operator<T, L::BM, L::BK, true, TIMES> a;
   Operator<T, L::BN, L::BK, true> b;
-  a.init(p.g, p.groups.order, p.n_out, p.n_rows, p.n_out, t.begin, t.end, 0, p.slope);
+  a.init(p.g, o.groups.order, p.n_out, o.n_rows, p.n_out, t.begin, t.end, k0, p.slope);
   b.init((const T*)p.w + (int64_t)t.group * p.n_in * p.n_out, nullptr, p.n_out, p.n_in, p.n_out, n0,
-         min(n0 + L::BN, p.n_in), 0);
+         min(n0 + L::BN, p.n_in), k0);
   f32x16 acc[L::MT][L::NT];
-  dense_product<T, L, true, true>(a, b, p.n_out, lds, acc, [](int) {});
-  constexpr int N = 16 / sizeof(T);
-  int c;
-  dense_rows<L, N>(
-      lds, acc, [&](int n) { c = n0 + n; },
-      [&](int m, float(&v)[N]) {
-        const int64_t row = rows[m];
-        if (row < 0 || c >= p.n_in) return;
-        store_row_part<T, N>((T*)p.dx + row * p.n_in, c, p.n_in, v);
-      });
+  dense_product<T, L, true, true>(a, b, k1 - k0, lds, acc, [](int) {});
+  put_tile<T, L>(lds, acc, o, parts, part, t.group, rows, n0);
 }
 
 // the parts go to the XCDs in turn, a part's tiles to one
@@ -278,14 +272,15 @@ static Parts parts_of(int64_t n_rows, bool grouped, int64_t want, int64_t least)
 constexpr int kFormInProducts = 128;
 
 struct BackwardPlan {
-  int kind;                        // of the weight's tiles
+  int input_kind, kind;            // of the input's tiles, of the weight's
+  Split split;                     // of the input's reduction, whose sums are gone before the weight's are there
   Parts weight, bias;
   bool pass;                       // forms d
   size_t bytes;                    // of the weight's parts, the bias's, d
   size_t bias_at, d_at;
 };
 static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, int64_t n_groups,
-                                  bool grouped, bool slope, bool weight, bool bias) {
+                                  bool grouped, bool slope, bool input, bool weight, bool bias) {
   BackwardPlan b{};
   const int64_t size = storage_bytes(dtype);
   const auto tiles = [&](int64_t bm, int64_t bn) { return ((n_in + bm - 1) / bm) * ((n_out + bn - 1) / bn); };
@@ -316,11 +311,14 @@ static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32
     }
   }
   b.pass = slope && n_in > kFormInProducts;
+  b.input_kind = dense_tile(size, n_rows, n_in, grouped ? n_groups : 0);
+  if (slope && !b.pass) b.input_kind = std::min<int>(b.input_kind, kTile128);
+  b.split = dense_split(size, b.input_kind, n_rows, n_in, n_out);
   b.bias = b.weight;
   // eight blocks a CU of 512 bytes of the columns each
   if (b.pass) b.bias = parts_of(n_rows, grouped, std::max<int64_t>(1, 2048 / ((n_out * size + 511) / 512)), 64);
   const auto room = [](size_t n) { return (n + 255) / 256 * 256; };
-  b.bias_at = room((size_t)b.weight.slots * n_in * n_out * sizeof(float));
+  b.bias_at = std::max(room((size_t)b.weight.slots * n_in * n_out * sizeof(float)), input ? room(b.split.bytes) : 0);
   b.d_at = b.bias_at + (bias ? room((size_t)b.bias.slots * n_out * sizeof(float)) : 0);
   b.bytes = b.d_at + (b.pass ? (size_t)n_rows * n_out * size : 0);
   return b;
@@ -337,18 +335,18 @@ static void cotangent_launch(BackwardArgs p, const int32_t* plan, int n_groups, 
 }
 
 template <typename T, typename L>
-static void input_launch(BackwardArgs p, const int32_t* plan, int n_groups, hipStream_t s) {
-  p.groups = group_view(plan, p.n_rows, n_groups, group_level(L::BM));
+static void input_launch(BackwardArgs p, const Split& split, const int32_t* plan, int n_groups, hipStream_t s) {
+  Output o{nullptr, nullptr, p.dx, nullptr, p.part, GroupView{}, p.n_rows, p.n_in, kNone, 0.0f};
+  o.groups = group_view(plan, p.n_rows, n_groups, group_level(L::BM));
   p.tiles_n = (p.n_in + L::BN - 1) / L::BN;
   p.tiles = row_tiles(p.n_rows, n_groups, plan != nullptr, L::BM) * p.tiles_n;
-  const dim3 grid((unsigned)xcd_blocks(p.tiles));
-  if constexpr (L::BM <= 128) {
-    if (p.slope != nullptr) {
-      hipLaunchKernelGGL((dense_input_kernel<T, L, true>), grid, dim3(kDenseThreads), 0, s, p);
-      return;
-    }
-  }
-  hipLaunchKernelGGL((dense_input_kernel<T, L, false>), grid, dim3(kDenseThreads), 0, s, p);
+  const int steps = split.parts > 1 ? split.steps : (p.n_out + L::BK - 1) / L::BK;
+  const dim3 grid((unsigned)xcd_blocks(p.tiles * split.parts));
+  if (p.slope == nullptr)
+    hipLaunchKernelGGL((dense_input_kernel<T, L, false>), grid, dim3(kDenseThreads), 0, s, p, o, split.parts, steps);
+  else if constexpr (L::BM <= 128)
+    hipLaunchKernelGGL((dense_input_kernel<T, L, true>), grid, dim3(kDenseThreads), 0, s, p, o, split.parts, steps);
+  if (split.parts > 1) parts_launch<T>(o, plan, n_groups, split.parts, s);
 }
 
 // Groups of different sizes have parts of different lengths, the long ones next to each other: spread over the XCDs
@@ -377,12 +375,15 @@ using namespace xnn;
 extern "C" {
 
 int xnn_linear_backward_work_size(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, int32_t n_groups,
-                                  int32_t grouped, int32_t slope, int32_t weight, int32_t bias, size_t* bytes) {
+                                  int32_t grouped, int32_t slope, int32_t input, int32_t weight, int32_t bias,
+                                  size_t* bytes) {
   static const int32_t some = 0;
   const int status = dense_sizes(dtype, n_rows, n_in, n_out, &some, n_groups);
   if (status != XNN_OK) return status;
   XNN_REQUIRE(bytes != nullptr, "NULL size");
-  *bytes = backward_plan(dtype, n_rows, n_in, n_out, n_groups, grouped != 0, slope != 0, weight != 0, bias != 0).bytes;
+  *bytes = backward_plan(dtype, n_rows, n_in, n_out, n_groups, grouped != 0, slope != 0, input != 0, weight != 0,
+                         bias != 0)
+               .bytes;
   return XNN_OK;
 }
 
@@ -399,8 +400,8 @@ int xnn_linear_backward(int dtype, const void* grad, const void* slope, const vo
   XNN_REQUIRE(dbias == nullptr || dweight != nullptr, "the bias's gradient goes with the weight's");
   if (dweight == nullptr && (dx == nullptr || n_rows == 0)) return XNN_OK;
   const bool grouped = plan != nullptr && n_rows > 0;
-  const BackwardPlan b = backward_plan(dtype, n_rows, n_in, n_out, n_groups, grouped, slope != nullptr, dweight != nullptr,
-                                       dbias != nullptr);
+  const BackwardPlan b = backward_plan(dtype, n_rows, n_in, n_out, n_groups, grouped, slope != nullptr, dx != nullptr,
+                                       dweight != nullptr, dbias != nullptr);
   XNN_REQUIRE(b.bytes == 0 || (work && work_bytes >= b.bytes), "work too small");
   XNN_REQUIRE((uintptr_t)work % 16 == 0, "work must be aligned to 16 bytes");
   BackwardArgs p{};
@@ -424,8 +425,6 @@ int xnn_linear_backward(int dtype, const void* grad, const void* slope, const vo
   p.groups = group_view(order, n_rows, n_groups, grouped ? group_level(p.rows) : 0);
   p.bias_groups = group_view(order, n_rows, n_groups, grouped ? group_level(p.bias_rows) : 0);
   hipStream_t s = as_hip(stream);
-  int kind = dense_tile(storage_bytes(dtype), n_rows, n_in, grouped ? n_groups : 0);
-  if (slope != nullptr && !b.pass) kind = std::min<int>(kind, kTile128);
   p.sums = dbias != nullptr && !b.pass;
   XNN_STORAGE_DISPATCH(dtype, T, {
     if (b.pass && n_rows > 0) {
@@ -433,7 +432,7 @@ int xnn_linear_backward(int dtype, const void* grad, const void* slope, const vo
       p.g = p.d;
       p.slope = nullptr;
     }
-    if (n_rows > 0 && dx != nullptr) XNN_TILE_DISPATCH(kind, T, L, input_launch<T, L>(p, order, n_groups, s));
+    if (n_rows > 0 && dx != nullptr) XNN_TILE_DISPATCH(b.input_kind, T, L, input_launch<T, L>(p, b.split, order, n_groups, s));
     if (n_rows > 0 && dweight != nullptr)
       XNN_TILE_DISPATCH(b.kind, T, L, weight_launch<T, L>(p, order, n_groups, s));
     // groups without rows have zeros, parts have sums

@@ -3,7 +3,7 @@
 #define XNN_ENTRIES(X)                                                                           \
   X(xnn_last_error) X(xnn_layer_norm) X(xnn_layer_norm_backward_work_size)                       \
   X(xnn_layer_norm_backward) X(xnn_group_plan_size) X(xnn_group_plan) X(xnn_linear)              \
-  X(xnn_linear_backward_work_size) X(xnn_linear_backward)
+  X(xnn_linear_work_size) X(xnn_linear_backward_work_size) X(xnn_linear_backward)
 #define XNN_FAMILY "feed-forward"
 
 #include "native_ops.h"
@@ -292,9 +292,14 @@ Two dense_forward(XNN_DENSE_ARGUMENTS, bool keep) {
   if (keep)
     slope = at::empty(activation != XNN_NO_ACTIVATION ? at::IntArrayRef(d.out) : at::IntArrayRef({0}),
                       x.options().dtype(slope_type(x)));
+  Tensor work;
+  size_t need = 0;
+  check("xnn_linear_work_size", api.xnn_linear_work_size(storage_code(x), d.rows, (int32_t)d.n_in, (int32_t)d.n_out,
+                                                         (int32_t)d.groups, p.defined(), &need));
+  if (need > 0) work = bytes(x, need);
   XNN_CALL(xnn_linear, storage_code(x), data(rows), row_stride(rows), d.rows, (int32_t)d.n_in, (int32_t)d.n_out,
            data(w), data(b), (int32_t)activation, data(r), (const int32_t*)data(p), (int32_t)d.groups, data(out),
-           data_if(keep && activation != XNN_NO_ACTIVATION, slope), stream_of(x));
+           data_if(keep && activation != XNN_NO_ACTIVATION, slope), data(work), need, stream_of(x));
   return {out, slope};
 }
 
@@ -333,7 +338,8 @@ Three dense_backward_kernel(const Tensor& grad_, const MaybeTensor& slope_, cons
   size_t need = 0;
   check("xnn_linear_backward_work_size",
         api.xnn_linear_backward_work_size(storage_code(x), d.rows, (int32_t)d.n_in, (int32_t)d.n_out,
-                                          (int32_t)d.groups, p.defined(), slope.defined(), weights, biases, &need));
+                                          (int32_t)d.groups, p.defined(), slope.defined(), input, weights, biases,
+                                          &need));
   if (need > 0) work = bytes(x, need);
   XNN_CALL(xnn_linear_backward, storage_code(x), data(grad), data(slope), data(rows), row_stride(rows), d.rows,
            (int32_t)d.n_in, (int32_t)d.n_out, data(w), (const int32_t*)data(p), (int32_t)d.groups,
