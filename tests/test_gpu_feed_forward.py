@@ -239,6 +239,14 @@ def test_linear_of_many_tiles(dtype, rows, n_in, n_out):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 8, 9])
+@pytest.mark.parametrize("n_in,n_out", [(1, 3), (33, 1000), (1500, 65), (5000, 40), (64, 2100)])
+def test_linear_of_few_rows(dtype, rows, n_in, n_out):
+    _check_dense(dtype, _dense_case(dtype, rows, n_in, n_out, residual=rows % 2 == 0, strided=rows == 5), "silu")
+    _check_dense(dtype, _dense_case(dtype, rows, n_in, n_out, 3, some=[-1, 0, 2], bias=rows != 4), None)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,n_in,n_out", [(1, 4096, 70), (3, 70, 4097), (100, 3001, 130), (130, 200, 2900),
                                              (64, 1030, 1030)])
 def test_linear_of_long_sums_for_few_outputs(dtype, rows, n_in, n_out):

@@ -22,7 +22,7 @@ from .conv import ConvTensorProduct
 from .attention import (AttentionPlan, attention_plan, dropout_add, embedding, head_norm_rotate,
                         structure_attention)
 from .feed_forward import GroupPlan, group_plan, grouped_linear, layer_norm, linear
-from .atom_attention import AtomAttention, AtomAttentionPotential, SpeciesEmbedding
+from .atom_attention import AtomAttention, AtomAttentionPotential, AtomFeedForward, SpeciesEmbedding
 from .irreps import Irrep, Irreps, tp_out_irreps_with_instructions, wigner_3j
 
 __all__ = [
@@ -37,7 +37,7 @@ __all__ = [
     "register_model", "ForceStressOutput",
     "FullyConnectedNet", "RadialNet", "set_recompute_radial", "ConvTensorProduct",
     "AttentionPlan", "attention_plan", "dropout_add", "embedding", "head_norm_rotate",
-    "structure_attention", "AtomAttention", "AtomAttentionPotential", "SpeciesEmbedding",
+    "structure_attention", "AtomAttention", "AtomAttentionPotential", "AtomFeedForward", "SpeciesEmbedding",
     "GroupPlan", "group_plan", "grouped_linear", "layer_norm", "linear",
     "Irrep", "Irreps", "tp_out_irreps_with_instructions", "wigner_3j",
 ]

@@ -1,5 +1,5 @@
-"""An attention block over atoms and :class:`AtomAttentionPotential`, the model that runs the
-operators of :mod:`xnn_amd.attention` together.
+"""Attention and feed-forward blocks over atoms and :class:`AtomAttentionPotential`, the model that runs
+the operators of :mod:`xnn_amd.attention` and :mod:`xnn_amd.feed_forward` together.
 
 Every module has two evaluations of the same function, as the other fast-path modules
 (common/models/fast.py:73-91): the HIP kernels, and a PyTorch formulation that is differentiable
@@ -15,6 +15,7 @@ from torch import Tensor, nn
 
 from .attention import (AttentionPlan, attention_plan, dropout_add, embedding, head_norm_rotate,
                         structure_attention)
+from .feed_forward import GroupPlan, group_plan, grouped_linear, layer_norm, linear
 from .fast import MI355X_POLICY, FastPathModule, fast_modules, select
 from .models import ShEdgePotential, register_model
 
@@ -80,6 +81,31 @@ def structure_attention_torch(q: Tensor, k: Tensor, v: Tensor, n_atoms: Tensor) 
     # structures without atoms have rows of nothing, which no atom reads
     out = (p @ padded(v)).transpose(1, 2).reshape(B * L, *q.shape[1:])
     return out.index_select(0, rows)
+
+
+def layer_norm_torch(x: Tensor, weight: Tensor, bias: Tensor, eps: float) -> Tensor:
+    centered = x - x.mean(-1, keepdim=True)
+    return centered * torch.rsqrt(centered.square().mean(-1, keepdim=True) + eps) * weight + bias
+
+
+_ACTIVATIONS = {None: lambda z: z, "silu": nn.functional.silu, "gelu": nn.functional.gelu, "tanh": torch.tanh}
+
+
+def linear_torch(x: Tensor, weight: Tensor, bias: Tensor, activation: Optional[str],
+                 residual: Optional[Tensor] = None) -> Tensor:
+    y = _ACTIVATIONS[activation](x @ weight + bias)
+    return y if residual is None else residual + y
+
+
+def grouped_linear_torch(x: Tensor, weight: Tensor, ids: Tensor, bias: Tensor, activation: Optional[str],
+                         residual: Optional[Tensor] = None) -> Tensor:
+    """The rows of each group that has some with its weight."""
+    order = torch.argsort(ids, stable=True)
+    groups, counts = torch.unique(ids, return_counts=True)
+    parts = [_ACTIVATIONS[activation](x[rows] @ weight[g] + bias[g])
+             for g, rows in zip(groups.tolist(), order.split(counts.tolist()))]
+    y = torch.cat(parts)[torch.argsort(order)] if parts else x @ weight[0]
+    return y if residual is None else residual + y
 
 
 # --------------------------------------------------------------------------- modules
@@ -186,6 +212,60 @@ class AtomAttention(nn.Module, FastPathModule):
         return add(y, x, self.dropout, self.seed, offset)
 
 
+class AtomFeedForward(nn.Module, FastPathModule):
+    """``x + W_2 f(W_1 layer_norm(x) + b_1) + b_2``, the weights shared by all atoms or, with ``n_species``,
+    those of each atom's atomic number (below ``n_species``)."""
+
+    def __init__(self, channels: int, hidden: int, activation: Optional[str] = "silu",
+                 n_species: Optional[int] = None, eps: float = 1e-5,
+                 generator: Optional[torch.Generator] = None):
+        super().__init__()
+        if channels < 1 or hidden < 1 or (n_species is not None and n_species < 1):
+            raise ValueError(f"{channels} channels, {hidden} hidden ones and {n_species} species: each must be positive")
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"unknown activation {activation!r} (None, 'silu', 'gelu' or 'tanh')")
+        self.activation, self.n_species, self.eps = activation, n_species, float(eps)
+        self.fast_active = False
+        lead = () if n_species is None else (n_species,)
+
+        def weight(n_in, n_out):
+            return nn.Parameter(torch.randn(*lead, n_in, n_out, generator=generator) / n_in ** 0.5)
+        self.norm_weight = nn.Parameter(torch.ones(channels))
+        self.norm_bias = nn.Parameter(torch.zeros(channels))
+        self.up, self.up_bias = weight(channels, hidden), nn.Parameter(torch.zeros(*lead, hidden))
+        self.down, self.down_bias = weight(hidden, channels), nn.Parameter(torch.zeros(*lead, channels))
+
+    def fast_supported(self, device: torch.device, dtype: torch.dtype) -> bool:
+        return (_takes(device, dtype) and self.norm_weight.shape[0] <= 16384
+                and (self.n_species is None or self.n_species <= 4096))
+
+    def forward(self, x: Tensor, z: Optional[Tensor] = None, plan: Optional[GroupPlan] = None,
+                param_grads: bool = True) -> Tensor:
+        """``x`` (N, channels); with species ``z`` (N,), the atomic numbers, and ``plan`` of them for the
+        kernels (made here when None)."""
+        params = (self.norm_weight, self.norm_bias, self.up, self.up_bias, self.down, self.down_bias)
+        nw, nb, up, ub, down, db = (p.to(x.dtype) if param_grads else p.detach().to(x.dtype) for p in params)
+        if self.n_species is not None and z is None:
+            raise ValueError("weights of species need the atomic numbers")
+        if not self.fast_active:
+            n = layer_norm_torch(x, nw, nb, self.eps)
+            if self.n_species is None:
+                return linear_torch(linear_torch(n, up, ub, self.activation), down, db, None, x)
+            return grouped_linear_torch(grouped_linear_torch(n, up, z, ub, self.activation), down, z, db, None, x)
+        n, residual = layer_norm(x, nw, nb, self.eps), x
+        if torch.is_autocast_enabled("cuda") and x.dtype == torch.float32:
+            # under autocast the products are of its type; x keeps its own
+            low = torch.get_autocast_dtype("cuda")
+            n, up, ub, down, db = (t.to(low) for t in (n, up, ub, down, db))
+            residual = None
+        if self.n_species is None:
+            y = linear(linear(n, up, ub, self.activation), down, db, None, residual)
+        else:
+            plan = group_plan(z, self.n_species) if plan is None else plan
+            y = grouped_linear(grouped_linear(n, up, plan, ub, self.activation), down, plan, db, None, residual)
+        return y if residual is not None else x + y.to(x.dtype)
+
+
 @register_model("atom_attention")
 class AtomAttentionPotential(ShEdgePotential):
     """Edge messages, then attention among the atoms of a structure.
@@ -193,7 +273,9 @@ class AtomAttentionPotential(ShEdgePotential):
     The message sums ``A_i`` of :class:`~xnn_amd.models.ShEdgePotential` give each atom the invariants
     ``s_i = log(1 + sum_m A_i[c, l, m]^2)``; features ``x_i = s_i W + embedding(Z_i)`` pass through
     ``layers`` blocks of :class:`AtomAttention`, whose phases are linear in ``s_i`` (so the energy
-    does not change when the structure is turned, moved or its atoms reordered), and are read out as
+    does not change when the structure is turned, moved or its atoms reordered), each followed by an
+    :class:`AtomFeedForward` of ``feed_forward`` hidden channels where that is not zero (with the weights of
+    each atom's species where ``species_weights``), and are read out as
     ``E_i = <U, x_i> + atom_ref[Z_i]``. All geometry enters through the edge vectors: forces and
     stress come from the edge backward. ``use_fast=False``, a CPU or a training step on forces
     (``create_graph=True``) takes the PyTorch formulation.
@@ -207,7 +289,8 @@ class AtomAttentionPotential(ShEdgePotential):
                  channels: int = 128, cutoff: float = 5.0, heads: int = 4,
                  kv_heads: Optional[int] = None, layers: int = 2, dropout: float = 0.0,
                  embedding_scale: float = 1.0, seed: Optional[int] = 0,
-                 dropout_seed: Optional[int] = None, **kwargs):
+                 dropout_seed: Optional[int] = None, feed_forward: int = 0, species_weights: bool = False,
+                 activation: Optional[str] = "silu", **kwargs):
         super().__init__(species=species, n_rbf=n_rbf, l_max=l_max, channels=channels,
                          cutoff=cutoff, seed=seed, **kwargs)
         gen = torch.Generator().manual_seed(seed + 1) if seed is not None else None
@@ -223,6 +306,11 @@ class AtomAttentionPotential(ShEdgePotential):
         half = self.blocks[0].head_dim // 2 if layers else 0
         self.phase = nn.Parameter(torch.randn(n_inv, half, generator=gen) / n_inv ** 0.5)
         self.U = nn.Parameter(torch.randn(channels, generator=gen) / channels ** 0.5)
+        # after the weights that a model without them has: those draw the same numbers
+        self.feed_forward = nn.ModuleList(
+            AtomFeedForward(channels, feed_forward, activation, max(species) + 1 if species_weights else None,
+                            generator=gen)
+            for _ in range(layers if feed_forward else 0))
         orders = torch.cat([torch.full((2 * l + 1,), l) for l in range(l_max + 1)])
         self.register_buffer("per_order", torch.nn.functional.one_hot(orders).float())
 
@@ -241,8 +329,13 @@ class AtomAttentionPotential(ShEdgePotential):
         plan = None
         if self.blocks and self.blocks[0].fast_active:
             plan = data.attention_plan()                   # one host read a graph, not a step
-        for block in self.blocks:
+        species = None
+        if self.feed_forward and self.feed_forward[0].fast_active and self.feed_forward[0].n_species is not None:
+            species = data.species_plan(self.feed_forward[0].n_species)
+        for i, block in enumerate(self.blocks):
             x = block(x, cos, sin, data.n_atoms, plan, self.param_grads, offset)
+            if self.feed_forward:
+                x = self.feed_forward[i](x, data.atomic_numbers, species, self.param_grads)
         ref = self.atom_ref.to(x.dtype)
         if x.is_cuda and self.embed.fast_active:
             from .ops import node_readout_op

@@ -745,32 +745,42 @@ __device__ __forceinline__ void put_tile(char* lds, const f32x16 (&acc)[L::MT][L
       });
 }
 
-// The parts of a reduction added in their order: blocks of 32 sorted rows by 16 pieces of 16 bytes
+// The parts of a reduction added: a block has 4 sorted rows of 8 pieces of 16 bytes, eight threads an output, each with
+// every eighth part in order, then those sums in order (one thread an output waited 12 us for 32 parts, whose
+// lines other dies have written)
 template <typename T>
 __global__ __launch_bounds__(256) void dense_parts_kernel(Output o, int parts, int columns) {
   constexpr int N = 16 / sizeof(T);
-  const RowTile t = row_tile(o.groups, o.groups.n_groups + 1, o.n_rows, blockIdx.x / columns, 32);
+  __shared__ __align__(16) float sums[8][32][N];
+  const int lane = threadIdx.x % 8, line = threadIdx.x / 8 % 4, slice = threadIdx.x / 32;
+  const int quarter = blockIdx.x / columns % 8;
+  const RowTile t = row_tile(o.groups, o.groups.n_groups + 1, o.n_rows, blockIdx.x / (8 * columns), 32);
   if (t.group < 0) return;
-  const int c = (blockIdx.x % columns * 16 + threadIdx.x % 16) * N;
-  if (c >= o.width) return;
-  const bool none = o.groups.n_groups > 0 && t.group == o.groups.n_groups;   // rows of no group: done
-  float bias[N];
-  if (!none) load_bias<T>(o, t.group, c, bias);
-  for (int r = t.begin + threadIdx.x / 16; r < t.end && !none; r += 16) {
-    const int64_t row = group_row(o.groups, r);
-    if (row < 0 || row >= o.n_rows) continue;
-    float v[N];
+  if (o.groups.n_groups > 0 && t.group == o.groups.n_groups) return;   // rows of no group: done
+  const int c = (blockIdx.x % columns * 8 + lane) * N, r = t.begin + 4 * quarter + line;
+  const int64_t row = r < t.end ? group_row(o.groups, r) : -1;
+  const bool live = c < o.width && row >= 0 && row < o.n_rows;
+  float v[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = 0.0f;
+  for (int i = 0; i < N; ++i) v[i] = 0.0f;
+  if (live)
 #pragma unroll 4
-    for (int n = 0; n < parts; ++n) {
+    for (int n = slice; n < parts; n += 8) {
       float x[N];
       load_row_part<float, N>(o.part + ((int64_t)n * o.n_rows + row) * o.width, c, o.width, x);
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] += x[i];
     }
-    put_row<T>(o, row, c, v, bias);
-  }
+  store_pack<float, N>(sums[slice][threadIdx.x % 32], v);
+  __syncthreads();
+  if (slice != 0 || !live) return;
+  float bias[N];
+  load_bias<T>(o, t.group, c, bias);
+#pragma unroll
+  for (int q = 1; q < 8; ++q)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += sums[q][threadIdx.x][i];
+  put_row<T>(o, row, c, v, bias);
 }
 
 // ---------------------------------------------------------------- host side
@@ -828,8 +838,8 @@ inline int64_t row_tiles(int64_t n_rows, int64_t n_groups, bool grouped, int64_t
 }
 
 // The parts of a reduction of `length` for an output of m x n: more than one where its tiles leave the card idle, as
-// many as the estimated time has its least with: steps of 0.6 us (their loads' latency), a launch that adds the parts, their
-// sums written and read at 4 TB/s. Each is of `steps` whole steps.
+// many as the estimated time has its least with: steps of 0.7 us (their loads' latency), a launch that adds the parts,
+// their sums written and read at 4 TB/s. Each is of `steps` whole steps.
 struct Split {
   int parts, steps;
   size_t bytes;
@@ -839,11 +849,11 @@ inline Split dense_split(size_t size, int kind, int64_t m, int64_t n, int64_t le
   Split best{1, (int)steps, 0};
   if (kind != kTile64) return best;
   const int64_t tiles = ((m + 63) / 64) * ((n + 63) / 64);
-  double least = 0.6 * (double)steps;
+  double least = 0.7 * (double)steps;
   for (int64_t p = 2; p <= steps && p * tiles <= 1024; ++p) {
     const int64_t each = (steps + p - 1) / p;
     if ((p - 1) * each >= steps) continue;                 // the last part would be empty
-    const double time = 0.6 * (double)each * (p * tiles > 768 ? 2 : 1) + 4.0 + (double)(p * m * n) * 8 / 4e6;
+    const double time = 0.7 * (double)each * (p * tiles > 768 ? 2 : 1) + 6.0 + 0.03 * (double)p + (double)(p * m * n) * 8 / 4e6;
     if (time < least) {
       least = time;
       best = Split{(int)p, (int)each, (size_t)p * m * n * sizeof(float)};
@@ -856,8 +866,8 @@ template <typename T>
 static void parts_launch(const Output& o, const int32_t* plan, int n_groups, int parts, hipStream_t s) {
   Output q = o;
   q.groups = group_view(plan, o.n_rows, n_groups, 0);
-  const int columns = (o.width + 16 * (int)(16 / sizeof(T)) - 1) / (16 * (int)(16 / sizeof(T)));
-  const int64_t blocks = row_tiles(o.n_rows, n_groups, plan != nullptr, 32) * columns;
+  const int columns = (o.width + 8 * (int)(16 / sizeof(T)) - 1) / (8 * (int)(16 / sizeof(T)));
+  const int64_t blocks = row_tiles(o.n_rows, n_groups, plan != nullptr, 32) * 8 * columns;
   hipLaunchKernelGGL(dense_parts_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, q, parts, columns);
 }
 

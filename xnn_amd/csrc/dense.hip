@@ -55,6 +55,124 @@ static void forward_launch(ForwardArgs p, const int32_t* plan, int n_groups, hip
   if (p.parts > 1) parts_launch<T>(p.o, plan, n_groups, p.parts, s);
 }
 
+// ---------------------------------------------------------------- few rows
+// One or two rows (in groups each by itself): a stream of the weight, which bounds it. A block takes a strip of `lanes`
+// 16-byte pieces of the columns and the whole reduction, its 512 threads each every 512 / lanes-th row of the
+// weight, sixteen of them in flight before the first is used; x lies in LDS as float32. The sums of
+// the threads of a column are added across lanes and then waves, in a fixed order. float32 products are float32's
+// own here.
+constexpr int kFewThreads = 512;
+constexpr int kMaxFew = 2;
+
+// x[j] += x[j] of the lanes at distances from, 2 from, ... 32
+template <int N>
+__device__ __forceinline__ void add_lanes_from(float (&x)[N], int from) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (from <= 2) x[j] += dpp_move<0x4E>(x[j]);
+    if (from <= 4) x[j] += dpp_move<0x1B>(dpp_move<0x141>(x[j]));   // the half row mirrored, its quads turned back
+    if (from <= 8) x[j] += dpp_move<0x128>(x[j]);
+    x[j] = add_xor32(add_xor16(x[j]));
+  }
+}
+
+template <typename T, int MR>
+__global__ __launch_bounds__(kFewThreads) void dense_few_kernel(ForwardArgs p, int lanes) {
+  constexpr int N = 16 / sizeof(T), LOADS = 16, WAVES = kFewThreads / kWave;
+  constexpr int kRound = kFewThreads / 2 * LOADS;          // rows of the weight a round, for the fewest lanes
+  __shared__ float xs[MR][kRound];
+  __shared__ float sums[WAVES][8][MR * N];
+  const Output& o = p.o;
+  const int tid = threadIdx.x, lane = tid % lanes, slice = tid / lanes, slices = kFewThreads / lanes;
+  const int c = (blockIdx.x * lanes + lane) * N;
+  // the block's rows: all, or in groups the blockIdx.y-th in their order
+  int group = 0;
+  int64_t row0 = 0;
+  int rows = o.n_rows;
+  if (o.groups.n_groups > 0) {
+    const int g = find_group(o.groups.row_ptr, o.groups.n_groups + 1, blockIdx.y);
+    row0 = group_row(o.groups, blockIdx.y);
+    rows = 1;
+    if (row0 < 0 || row0 >= o.n_rows) return;
+    if (g == o.groups.n_groups) {
+      if (slice == 0)
+        for (int i = 0; i < N && c + i < o.width; ++i) ((T*)o.out)[row0 * o.width + c + i] = (T)o.none;
+      return;
+    }
+    group = g;
+  }
+  const T* x = (const T*)p.x + row0 * p.x_stride;
+  const T* w = (const T*)p.w + (int64_t)group * p.n_in * o.width;
+  float acc[MR * N];
+#pragma unroll
+  for (int i = 0; i < MR * N; ++i) acc[i] = 0.0f;
+  const int round = min(kRound, slices * LOADS);
+  for (int k0 = 0; k0 < p.n_in; k0 += round) {
+    u32x4 piece[LOADS];
+    const int length = min(round, p.n_in - k0);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int k = slice + i * slices;
+      piece[i] = u32x4{0, 0, 0, 0};
+      if (k < length && c < o.width)
+        piece[i] = load_raw<T>(reinterpret_cast<const char*>(w + (int64_t)(k0 + k) * o.width + c), o.width - c,
+                               k0 + k == p.n_in - 1 || o.width < N);
+    }
+    if (k0 > 0) __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+      for (int k = tid; k < length; k += kFewThreads)
+        xs[m][k] = m < rows ? (float)x[m * p.x_stride + k0 + k] : 0.0f;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      if (i * slices >= length) break;
+      const int k = min(slice + i * slices, length - 1);   // beyond the round the piece is zero
+      const Pack<T, N> v = __builtin_bit_cast(Pack<T, N>, piece[i]);
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        const float f = xs[m][k];
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[m * N + j] = fmaf(f, (float)v.v[j], acc[m * N + j]);
+      }
+    }
+  }
+  add_lanes_from<MR * N>(acc, lanes);
+  if (tid % kWave < lanes)
+#pragma unroll
+    for (int i = 0; i < MR * N; ++i) sums[tid / kWave][lane][i] = acc[i];
+  __syncthreads();
+  const int m = tid / lanes;
+  if (m >= rows || m >= MR || c >= o.width) return;
+  float v[N], bias[N];
+  load_bias<T>(o, group, c, bias);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = 0.0f;
+#pragma unroll 4
+  for (int q = 0; q < WAVES; ++q)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += sums[q][lane][m * N + i];
+  put_row<T>(o, row0 + m, c, v, bias);
+}
+
+template <typename T>
+static void few_launch(ForwardArgs p, const int32_t* plan, int n_groups, hipStream_t s) {
+  constexpr int N = 16 / sizeof(T);
+  const int rows = p.o.n_rows;
+  p.o.groups = group_view(plan, rows, n_groups, 0);
+  // strips of 128 bytes, a line each, where they make 64 blocks; else narrower ones
+  int lanes = 8;
+  while (lanes > 2 && (p.o.width + lanes * N - 1) / (lanes * N) < 64) lanes /= 2;
+  const dim3 grid((p.o.width + lanes * N - 1) / (lanes * N), plan != nullptr ? rows : 1);
+#define XNN_FEW_LAUNCH(MR) \
+  hipLaunchKernelGGL((dense_few_kernel<T, MR>), grid, dim3(kFewThreads), 0, s, p, lanes)
+  if (rows == 1 || plan != nullptr)
+    XNN_FEW_LAUNCH(1);
+  else
+    XNN_FEW_LAUNCH(2);
+#undef XNN_FEW_LAUNCH
+}
+
 }  // namespace xnn
 
 using namespace xnn;
@@ -68,7 +186,9 @@ int xnn_linear_work_size(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out,
   if (status != XNN_OK) return status;
   XNN_REQUIRE(bytes != nullptr, "NULL size");
   const size_t size = storage_bytes(dtype);
-  *bytes = dense_split(size, dense_tile(size, n_rows, n_out, grouped ? n_groups : 0), n_rows, n_out, n_in).bytes;
+  *bytes = 0;
+  if (n_rows > kMaxFew)
+    *bytes = dense_split(size, dense_tile(size, n_rows, n_out, grouped ? n_groups : 0), n_rows, n_out, n_in).bytes;
   return XNN_OK;
 }
 
@@ -84,8 +204,9 @@ int xnn_linear(int dtype, const void* x, int64_t x_stride, int64_t n_rows, int32
   XNN_REQUIRE(x && weight && out, "NULL input or output");
   XNN_REQUIRE(x_stride >= n_in, "rows of x overlap");
   const size_t size = storage_bytes(dtype);
+  const bool few = n_rows <= kMaxFew;
   const int kind = dense_tile(size, n_rows, n_out, plan != nullptr ? n_groups : 0);
-  const Split split = dense_split(size, kind, n_rows, n_out, n_in);
+  const Split split = few ? Split{1, 0, 0} : dense_split(size, kind, n_rows, n_out, n_in);
   XNN_REQUIRE(split.bytes == 0 || (work && work_bytes >= split.bytes), "work too small");
   XNN_REQUIRE((uintptr_t)work % 16 == 0, "work must be aligned to 16 bytes");
   ForwardArgs p{};
@@ -98,7 +219,12 @@ int xnn_linear(int dtype, const void* x, int64_t x_stride, int64_t n_rows, int32
   p.o = Output{bias,       residual, out, slope, (float*)work, GroupView{}, (int)n_rows, n_out,
                activation, __builtin_nanf("")};
   hipStream_t s = as_hip(stream);
-  XNN_STORAGE_DISPATCH(dtype, T, XNN_TILE_DISPATCH(kind, T, L, forward_launch<T, L>(p, plan, n_groups, s)));
+  XNN_STORAGE_DISPATCH(dtype, T, {
+    if (few)
+      few_launch<T>(p, plan, n_groups, s);
+    else
+      XNN_TILE_DISPATCH(kind, T, L, forward_launch<T, L>(p, plan, n_groups, s));
+  });
   XNN_LAUNCH_CHECK();
   return XNN_OK;
 }
