@@ -32,7 +32,7 @@
 
 namespace xnn {
 
-constexpr int kDenseThreads = 256;
+constexpr int kDenseThreads = 256;     // and two blocks a CU: two waves of at most 256 registers a SIMD
 constexpr int kDenseWaves = kDenseThreads / kWave;
 
 // ---------------------------------------------------------------- groups

@@ -18,7 +18,7 @@ struct ForwardArgs {
 };
 
 template <typename T, typename L>
-__global__ __launch_bounds__(kDenseThreads) void dense_forward_kernel(ForwardArgs p) {
+__global__ __launch_bounds__(kDenseThreads, 2) void dense_forward_kernel(ForwardArgs p) {
   typedef DenseLds<L, T, true, false> S;
   __shared__ __align__(16) char lds[S::kBytes];
   __shared__ int32_t rows[L::BM];

@@ -5,7 +5,7 @@
 // of one weight or of each row's group. Where both products need d once (a width of 128 at most in x), they form it as
 // they stage it; else a pass over g and the slope does, with db's sums. (Formed in the staging of 24,000 rows of
 // 1,024 -> 4,096 in bfloat16, both products 843 us, for the registers, against 529 and 110 for the pass; 72,000
-// rows of 128 -> 512 in float32: MEASURED.) A weight's reduction runs over all rows of its group: it is cut into
+// rows of 128 -> 512 in float32: 217 us, and 189 with 94 for the pass.) A weight's reduction runs over all rows of its group: it is cut into
 // parts, one a block, which are added in their order where there is more than one. Without the pass db's sums
 // are the weight's product's, taken from what it stages.
 #include <hip/hip_runtime.h>
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256) void dense_cotangent_kernel(BackwardArgs p, in
 
 // ---------------------------------------------------------------- the products
 template <typename T, typename L, bool TIMES>
-__global__ __launch_bounds__(kDenseThreads) void dense_input_kernel(BackwardArgs p, Output o, int parts, int steps) {
+__global__ __launch_bounds__(kDenseThreads, 2) void dense_input_kernel(BackwardArgs p, Output o, int parts, int steps) {
   typedef DenseLds<L, T, true, true> S;
   __shared__ __align__(16) char lds[S::kBytes];
   __shared__ int32_t rows[L::BM];
@@ -127,7 +127,7 @@ __device__ __forceinline__ int64_t slot_of_xcd(int64_t tiles, int64_t& tile) {
 }
 
 template <typename T, typename L, bool TIMES>
-__global__ __launch_bounds__(kDenseThreads) void dense_weight_kernel(BackwardArgs p) {
+__global__ __launch_bounds__(kDenseThreads, 2) void dense_weight_kernel(BackwardArgs p) {
   typedef DenseLds<L, T, false, false> S;
   __shared__ __align__(16) char lds[S::kBytes];
   const int64_t slot = xcd_slot();
@@ -287,20 +287,27 @@ static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32
   if (weight) {
     // The tiles and the number of parts with the least time, estimated from the rates of large products
     // (kinds 0, 1, 2: microseconds of 64 rows of a tile with all of a CU's blocks at work, and those blocks) and
-    // the parts' sums, written and read at 4 TB/s
-    static const double step16[] = {0.9, 1.5, 2.4}, step32[] = {2.9, 5.4, 0.0};
+    // the parts' sums, written and read at 4 TB/s. Parts of one length come in rounds; those of groups, of any, fill
+    // the card but for three quarters of a long one's time at its end, and the more of them the more what is around
+    // their products counts: wide weights take the large tiles (16,384 rows in 64 groups, 1,024 x 1,024 in bfloat16, a few
+    // large groups and even ones: 128 x 128 tiles 185 and 143 us, 256 x 128 170 and 117).
+    static const double step16[] = {0.9, 1.4, 2.2}, step32[] = {2.9, 5.4, 0.0};
     static const int per_cu[] = {3, 2, 2}, bm[] = {64, 128, 256}, bn[] = {64, 128, 128};
     const double sums = (double)n_in * n_out * 8 / 4e6;
     double best = 0.0;
     for (int kind = 0; kind < (size == 2 && !(slope && n_in <= kFormInProducts) ? 3 : 2); ++kind) {
-      const int64_t t = tiles(bm[kind], bn[kind]);
+      if (grouped && size == 2 && kind < 2 && n_in >= 256 && n_out >= 128)
+        continue;
+      const double t = (double)tiles(bm[kind], bn[kind]), blocks = 256.0 * per_cu[kind];
+      const double step = size == 2 ? step16[kind] : step32[kind];
       for (int64_t want = 1; want <= 1024; want += std::max<int64_t>(1, want / 4)) {
         const Parts parts = parts_of(n_rows, grouped, want, 256);
-        const int64_t n = row_tiles(n_rows, n_groups, false, parts.rows) + (grouped ? n_groups / 2 : 0);
-        const double rounds = std::max(1.0, std::ceil((double)(n * t) / (256 * per_cu[kind])));
+        const double n = (double)row_tiles(n_rows, 0, false, parts.rows), all = n + (grouped ? n_groups / 2 : 0);
         const double steps = (double)std::min<int64_t>(parts.rows, n_rows) / 64 + 2;   // and two for what is around
-        const double time = rounds * steps * (size == 2 ? step16[kind] : step32[kind]) +
-                            (parts.slots > 0 ? 5.0 + sums * (double)row_tiles(n_rows, 0, false, parts.rows) : 0.0);
+        double time = std::max(1.0, std::ceil(all * t / blocks)) * steps * step;
+        if (grouped && all * t > blocks)
+          time = ((double)n_rows / 64 + 2 * all) * t / blocks * step + 0.75 * steps * step;
+        if (parts.slots > 0) time += 5.0 + sums * n;
         if (best == 0.0 || time < best) {
           best = time;
           b.kind = kind;
@@ -350,7 +357,7 @@ static void input_launch(BackwardArgs p, const Split& split, const int32_t* plan
 }
 
 // Groups of different sizes have parts of different lengths, the long ones next to each other: spread over the XCDs
-// where there are enough of them (16,384 rows in 64 groups, 1,024 x 1,024 in bfloat16: MEASURED)
+// where there are enough of them (16,384 rows in 64 groups, 1,024 x 1,024 in bfloat16: 212 us, in turn 161)
 template <typename T, typename L>
 static void weight_launch(BackwardArgs p, const int32_t* plan, int n_groups, hipStream_t s) {
   p.tiles_m = (p.n_in + L::BM - 1) / L::BM;
