@@ -310,7 +310,7 @@ __device__ __forceinline__ u32x4 times_slope(u32x4 g, u32x4 slope) {
 // Steps that begin before `fast` are of whole pieces, one address each that the step before has left: along the rows
 // those that end within them; across them all but the last one where a piece may reach beyond its row (the
 // tensor's last row is the last of its group).
-template <typename T, int LEN, int BK, bool ALONG, bool TIMES = false>
+template <typename T, int LEN, int BK, bool ALONG, bool TIMES = false, bool ORDERED = ALONG>
 struct Operator {
   static constexpr int kPer = 16 / sizeof(T);
   static constexpr int kRows = ALONG ? LEN : BK, kCols = ALONG ? BK : LEN;   // of a staged step
@@ -327,7 +327,7 @@ struct Operator {
   int most;                        // the last row that a whole piece may begin in
   uint32_t edges;                  // ALONG: pieces of the tensor's last row
   const char* p[kCount];           // pieces of the next step; across rows in an order
-  int32_t index[ALONG ? 1 : kCount];   // those rows, whose loads have a step's time
+  int32_t index[!ALONG && ORDERED ? kCount : 1];   // those rows, whose loads have a step's time
   u32x4 x[kCount], y[TIMES ? kCount : 1];
 
   // rows [first_row, end_row), columns from first_col on
@@ -354,21 +354,20 @@ struct Operator {
     for (int n = 0; n < kCount; ++n) {
       const int i = row_of(row + n * kStep);
       if (ALONG && i == last) edges |= 1u << n;
-      if constexpr (!ALONG) index[n] = i;
+      if constexpr (!ALONG && ORDERED) index[n] = i;
       p[n] = column + i * stride;
     }
   }
   __device__ __forceinline__ int row_of(int r) const {
     r = min(r, end - 1);
-    return order == nullptr ? first + r : min(max(order[r], 0), last);
+    if (!ORDERED || (ALONG && order == nullptr)) return first + r;
+    return min(max(order[r], 0), last);
   }
   // the step from reduction index k0 < fast on
   __device__ __forceinline__ void fetch_fast(int k0) {
-    if constexpr (!ALONG)
-      if (order != nullptr) {
+    if constexpr (!ALONG && ORDERED)
 #pragma unroll
-        for (int n = 0; n < kCount; ++n) p[n] = column + min(index[n], most) * stride;
-      }
+      for (int n = 0; n < kCount; ++n) p[n] = column + min(index[n], most) * stride;
     const int64_t step = ALONG ? BK * (int)sizeof(T) : BK * stride;
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {
@@ -376,11 +375,9 @@ struct Operator {
       if constexpr (TIMES) y[n] = load_raw(p[n] + slope);
       p[n] += step;
     }
-    if constexpr (!ALONG)
-      if (order != nullptr) {
+    if constexpr (!ALONG && ORDERED)
 #pragma unroll
-        for (int n = 0; n < kCount; ++n) index[n] = row_of(k0 + BK + row + n * kStep);
-      }
+      for (int n = 0; n < kCount; ++n) index[n] = row_of(k0 + BK + row + n * kStep);
   }
   // any step
   __device__ __forceinline__ void fetch(int k0) {
@@ -797,17 +794,21 @@ using Tile256 = Shape<T, 256, 128, 2, 2, 32>;
 
 // The kind for an output of m x n, in `groups` of rows where they are grouped (then a group's last tile is half empty;
 // how many groups have rows is not known here, and that any has does not speak for smaller tiles).
-// 256 x 128 tiles pay where they come in full rounds of two a CU (9,000 x 512 x 2,048 with silu, 1.1 rounds: 78 us,
-// 128 x 128 57; 24,000 x 1,024 x 4,096, 5.9: 423 and 470), 64 x 64 where 128 x 128 are not one a CU
-// (1,000^3: 10 us, 128 x 128 21).
+// 256 x 128 tiles pay where they come in full rounds of two a CU, a last round of up to one a CU counting little more
+// than half (9,000 x 512 x 2,048 with silu, 1.1 rounds: 78 us, 128 x 128 57; 24,000 x 1,024 x 4,096, 5.9: 423 and
+// 470; 24,000 x 4,096 x 1,024, 1.5: 226 and 255); 64 x 64 where 128 x 128 are not one a CU (1,000^3: 10 us, 128 x 128
+// 21).
 inline int dense_tile(size_t size, int64_t m, int64_t n, int64_t groups) {
   const auto rounds = [&](int64_t bm, int64_t bn, int64_t more) {
     return (double)((m + bm - 1) / bm + more) * (double)((n + bn - 1) / bn) / 512;
   };
+  const auto whole = [](double r) {
+    const double f = r - std::floor(r);
+    return std::floor(r) + (f == 0.0 ? 0.0 : f <= 0.5 ? 0.6 : 1.0);
+  };
   if (n <= 64 || rounds(128, 128, 0) < 0.5) return kTile64;
   const int64_t more = groups / 2;
-  return size == 2 && 1.8 * std::ceil(rounds(256, 128, more)) <= std::ceil(rounds(128, 128, more)) ? kTile256
-                                                                                                 : kTile128;
+  return size == 2 && 1.8 * whole(rounds(256, 128, more)) <= whole(rounds(128, 128, more)) ? kTile256 : kTile128;
 }
 
 // call(Shape) for the kind
@@ -838,7 +839,7 @@ inline int64_t row_tiles(int64_t n_rows, int64_t n_groups, bool grouped, int64_t
 }
 
 // The parts of a reduction of `length` for an output of m x n: more than one where its tiles leave the card idle, as
-// many as the estimated time has its least with: steps of 0.7 us (their loads' latency), a launch that adds the parts,
+// many as the estimated time has its least with: steps of 0.3 us, in float32 0.5 (their loads' latency), a launch that adds the parts,
 // their sums written and read at 4 TB/s. Each is of `steps` whole steps.
 struct Split {
   int parts, steps;
@@ -849,11 +850,12 @@ inline Split dense_split(size_t size, int kind, int64_t m, int64_t n, int64_t le
   Split best{1, (int)steps, 0};
   if (kind != kTile64) return best;
   const int64_t tiles = ((m + 63) / 64) * ((n + 63) / 64);
-  double least = 0.7 * (double)steps;
+  const double one = size == 2 ? 0.3 : 0.5;
+  double least = one * (double)steps;
   for (int64_t p = 2; p <= steps && p * tiles <= 1024; ++p) {
     const int64_t each = (steps + p - 1) / p;
     if ((p - 1) * each >= steps) continue;                 // the last part would be empty
-    const double time = 0.7 * (double)each * (p * tiles > 768 ? 2 : 1) + 6.0 + 0.03 * (double)p + (double)(p * m * n) * 8 / 4e6;
+    const double time = one * (double)each * (p * tiles > 768 ? 2 : 1) + 5.0 + 0.03 * (double)p + (double)(p * m * n) * 8 / 4e6;
     if (time < least) {
       least = time;
       best = Split{(int)p, (int)each, (size_t)p * m * n * sizeof(float)};

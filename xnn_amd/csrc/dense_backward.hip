@@ -126,7 +126,7 @@ __device__ __forceinline__ int64_t slot_of_xcd(int64_t tiles, int64_t& tile) {
   return i / tiles * kXcds + blockIdx.x % kXcds;
 }
 
-template <typename T, typename L, bool TIMES>
+template <typename T, typename L, bool TIMES, bool ORDERED>
 __global__ __launch_bounds__(kDenseThreads, 2) void dense_weight_kernel(BackwardArgs p) {
   typedef DenseLds<L, T, false, false> S;
   __shared__ __align__(16) char lds[S::kBytes];
@@ -142,8 +142,8 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_weight_kernel(Backward
   const int m0 = (int)(tile / p.tiles_n) * L::BM, n0 = (int)(tile % p.tiles_n) * L::BN;
   const RowTile t = row_tile(p.groups, p.groups.n_groups, p.n_rows, (int)part, p.rows);
   if (t.group < 0) return;
-  typedef Operator<T, L::BN, L::BK, false, TIMES> B;
-  Operator<T, L::BM, L::BK, false> a;
+  typedef Operator<T, L::BN, L::BK, false, TIMES, ORDERED> B;
+  Operator<T, L::BM, L::BK, false, false, ORDERED> a;
   B b;
   a.init(p.x, p.groups.order, p.x_stride, p.n_rows, p.n_in, t.begin, t.end, m0);
   b.init(p.g, p.groups.order, p.n_out, p.n_rows, p.n_out, t.begin, t.end, n0, p.slope);
@@ -153,9 +153,11 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_weight_kernel(Backward
   float sums[B::kPer];
 #pragma unroll
   for (int i = 0; i < B::kPer; ++i) sums[i] = 0.0f;
-  dense_product<T, L, false, false>(a, b, length, lds, acc, [&](int k) {
-    if (bias) b.add_rows(k, length, sums);
-  });
+  // two loops: a branch in one would part its loads from its products (TIMES: of one row of tiles, one loop)
+  if (TIMES || bias)
+    dense_product<T, L, false, false>(a, b, length, lds, acc, [&](int k) { b.add_rows(k, length, sums); });
+  else
+    dense_product<T, L, false, false>(a, b, length, lds, acc, [](int) {});
   const bool only = part_alone(p.groups, p.n_rows, p.rows, t.group);
   const int64_t at =
       part_slot(p.groups, t.begin, p.rows, p.groups.n_groups > 0 && part == p.groups.tile_ptr[t.group]);
@@ -322,8 +324,8 @@ static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32
   if (slope && !b.pass) b.input_kind = std::min<int>(b.input_kind, kTile128);
   b.split = dense_split(size, b.input_kind, n_rows, n_in, n_out);
   b.bias = b.weight;
-  // eight blocks a CU of 512 bytes of the columns each
-  if (b.pass) b.bias = parts_of(n_rows, grouped, std::max<int64_t>(1, 2048 / ((n_out * size + 511) / 512)), 64);
+  // sixteen blocks a CU of 512 bytes of the columns each
+  if (b.pass) b.bias = parts_of(n_rows, grouped, std::max<int64_t>(1, 4096 / ((n_out * size + 511) / 512)), 64);
   const auto room = [](size_t n) { return (n + 255) / 256 * 256; };
   b.bias_at = std::max(room((size_t)b.weight.slots * n_in * n_out * sizeof(float)), input ? room(b.split.bytes) : 0);
   b.d_at = b.bias_at + (bias ? room((size_t)b.bias.slots * n_out * sizeof(float)) : 0);
@@ -366,13 +368,18 @@ static void weight_launch(BackwardArgs p, const int32_t* plan, int n_groups, hip
   p.spread = plan != nullptr && p.parts >= 4 * kXcds;
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   const int64_t blocks = p.spread ? xcd_blocks(p.parts) * tiles : xcd_blocks(p.parts * tiles);
-  if constexpr (L::BM <= 128) {
-    if (p.slope != nullptr) {
-      hipLaunchKernelGGL((dense_weight_kernel<T, L, true>), dim3((unsigned)blocks), dim3(kDenseThreads), 0, s, p);
-      return;
-    }
+  const dim3 grid((unsigned)blocks), threads(kDenseThreads);
+  if (p.slope == nullptr) {
+    if (plan != nullptr)
+      hipLaunchKernelGGL((dense_weight_kernel<T, L, false, true>), grid, threads, 0, s, p);
+    else
+      hipLaunchKernelGGL((dense_weight_kernel<T, L, false, false>), grid, threads, 0, s, p);
+  } else if constexpr (L::BM <= 128) {
+    if (plan != nullptr)
+      hipLaunchKernelGGL((dense_weight_kernel<T, L, true, true>), grid, threads, 0, s, p);
+    else
+      hipLaunchKernelGGL((dense_weight_kernel<T, L, true, false>), grid, threads, 0, s, p);
   }
-  hipLaunchKernelGGL((dense_weight_kernel<T, L, false>), dim3((unsigned)blocks), dim3(kDenseThreads), 0, s, p);
 }
 
 }  // namespace xnn
