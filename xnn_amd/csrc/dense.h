@@ -781,22 +781,23 @@ __global__ __launch_bounds__(256) void dense_parts_kernel(Output o, int parts, i
 }
 
 // ---------------------------------------------------------------- host side
-// Tiles: 64 x 64; 128 x 128; in 16 bits 256 x 128, whose steps of 32 leave LDS and registers for two blocks a CU, one
-// in its products while the other loads or stores (24,000 x 1,024 x 4,096 in bfloat16 with gelu: 256 x 256, one
-// block a CU, 495 us; 256 x 128 423; 128 x 128 in steps of 64 470).
+// Tiles: 64 x 64; 128 x 128; in 16 bits 256 x 128. Steps of 32 leave LDS and registers for two blocks a CU, of 128 x 128
+// in 16 bits three, one in its products while another loads or stores (24,000 x 1,024 x 4,096 in bfloat16 with
+// gelu: 256 x 256, one block a CU, 495 us; 256 x 128 398; 128 x 128 418, in steps of 64 470; 70,000 x 128 x 512 with silu:
+// 128 x 128 47, in steps of 64 58).
 enum TileKind : int { kTile64 = 0, kTile128 = 1, kTile256 = 2 };
 template <typename T>
 using Tile64 = Shape<T, 64, 64, 2, 2, 128 / sizeof(T)>;
 template <typename T>
-using Tile128 = Shape<T, 128, 128, 2, 2, 128 / sizeof(T)>;
+using Tile128 = Shape<T, 128, 128, 2, 2, 32>;
 template <typename T>
 using Tile256 = Shape<T, 256, 128, 2, 2, 32>;
 
 // The kind for an output of m x n, in `groups` of rows where they are grouped (then a group's last tile is half empty;
 // how many groups have rows is not known here, and that any has does not speak for smaller tiles).
 // 256 x 128 tiles pay where they come in full rounds of two a CU, a last round of up to one a CU counting little more
-// than half (9,000 x 512 x 2,048 with silu, 1.1 rounds: 78 us, 128 x 128 57; 24,000 x 1,024 x 4,096, 5.9: 423 and
-// 470; 24,000 x 4,096 x 1,024, 1.5: 226 and 255); 64 x 64 where 128 x 128 are not one a CU (1,000^3: 10 us, 128 x 128
+// than half (9,000 x 512 x 2,048 with silu, 1.1 rounds: 78 us, 128 x 128 44; 24,000 x 1,024 x 4,096, 5.9: 398 and
+// 418; 24,000 x 4,096 x 1,024, 1.5: 226 and 255); 64 x 64 where 128 x 128 are not one a CU (1,000^3: 10 us, 128 x 128
 // 21).
 inline int dense_tile(size_t size, int64_t m, int64_t n, int64_t groups) {
   const auto rounds = [&](int64_t bm, int64_t bn, int64_t more) {
