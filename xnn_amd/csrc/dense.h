@@ -653,13 +653,19 @@ __device__ __forceinline__ void load_row_part(const T* row, int at, int width, f
     for (int i = 0; i < N; ++i) out[i] = at + i < width ? (float)row[at + i] : 0.0f;
   }
 }
-template <typename T, int N, typename V>
+// (STREAM: past the caches, for what is not read soon)
+template <typename T, int N, bool STREAM = false, typename V>
 __device__ __forceinline__ void store_row_part(T* row, int at, int width, const V* in) {
   if (at + N <= width) {
     Pack<T, N> x;
 #pragma unroll
     for (int i = 0; i < N; ++i) x.v[i] = (T)in[i];
-    __builtin_memcpy(row + at, &x, sizeof(x));
+    if constexpr (STREAM) {
+      typedef uint32_t Words __attribute__((ext_vector_type(sizeof(x) / 4), aligned(sizeof(T))));
+      __builtin_nontemporal_store(__builtin_bit_cast(Words, x), reinterpret_cast<Words*>(row + at));
+    } else {
+      __builtin_memcpy(row + at, &x, sizeof(x));
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -676,7 +682,15 @@ struct Output {
   GroupView groups;
   int n_rows, width, activation;
   float none;                      // in the rows of no group
+  int stream;                      // out is larger than the caches of the dies
 };
+
+// An output that the L2 caches (4 MB a die) cannot hold for its reader goes past them, as the slope does, which the
+// backward pass reads (24,000 x 4,096 in bfloat16: 274 us without an activation, past them 256; with gelu 396,
+// the slope past them 376)
+inline int past_caches(int64_t rows, int64_t width, size_t size) {
+  return rows * width * (int64_t)size > ((int64_t)32 << 20);
+}
 
 template <typename T>
 __device__ __forceinline__ void load_bias(const Output& o, int group, int c, float (&bias)[16 / sizeof(T)]) {
@@ -702,7 +716,7 @@ __device__ __forceinline__ void put_row(const Output& o, int64_t row, int c, flo
       activate(o.activation, v[i], v[i], s);
       slope[i] = slope_stored<T>(s);
     }
-    if (o.slope != nullptr) store_row_part<S, N>((S*)o.slope + row * o.width, c, o.width, slope);
+    if (o.slope != nullptr) store_row_part<S, N, true>((S*)o.slope + row * o.width, c, o.width, slope);
   }
   if (o.residual != nullptr) {
     float z[N];
@@ -710,7 +724,10 @@ __device__ __forceinline__ void put_row(const Output& o, int64_t row, int c, flo
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] += z[i];
   }
-  store_row_part<T, N>((T*)o.out + row * o.width, c, o.width, v);
+  if (o.stream)
+    store_row_part<T, N, true>((T*)o.out + row * o.width, c, o.width, v);
+  else
+    store_row_part<T, N>((T*)o.out + row * o.width, c, o.width, v);
 }
 
 // A tile's sums to where they go: the outputs, or the part's sums

@@ -217,7 +217,7 @@ int xnn_linear(int dtype, const void* x, int64_t x_stride, int64_t n_rows, int32
   p.parts = split.parts;
   p.steps = split.steps;
   p.o = Output{bias,       residual, out, slope, (float*)work, GroupView{}, (int)n_rows, n_out,
-               activation, __builtin_nanf("")};
+               activation, __builtin_nanf(""), past_caches(n_rows, n_out, size)};
   hipStream_t s = as_hip(stream);
   XNN_STORAGE_DISPATCH(dtype, T, {
     if (few)

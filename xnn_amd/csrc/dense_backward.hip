@@ -345,7 +345,8 @@ static void cotangent_launch(BackwardArgs p, const int32_t* plan, int n_groups, 
 
 template <typename T, typename L>
 static void input_launch(BackwardArgs p, const Split& split, const int32_t* plan, int n_groups, hipStream_t s) {
-  Output o{nullptr, nullptr, p.dx, nullptr, p.part, GroupView{}, p.n_rows, p.n_in, kNone, 0.0f};
+  Output o{nullptr, nullptr, p.dx, nullptr, p.part, GroupView{}, p.n_rows, p.n_in, kNone, 0.0f,
+           past_caches(p.n_rows, p.n_in, sizeof(T))};
   o.groups = group_view(plan, p.n_rows, n_groups, group_level(L::BM));
   p.tiles_n = (p.n_in + L::BN - 1) / L::BN;
   p.tiles = row_tiles(p.n_rows, n_groups, plan != nullptr, L::BM) * p.tiles_n;
