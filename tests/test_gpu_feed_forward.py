@@ -294,6 +294,17 @@ def test_a_row_that_is_not_finite_reaches_no_other():
         assert torch.equal(got[keep], want[keep])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows", [1, 2, 3, 70])
+@pytest.mark.parametrize("n_in", [1, 2, 10, 33, 1000, 4097])
+def test_an_infinite_input_gives_infinities_of_its_weights_signs(dtype, rows, n_in):
+    """In 16 bits products are the type's own: an infinity in the last place of the sum meets no zero."""
+    x, w, _, _, _, _ = _dense_case(dtype, rows, n_in, 40, bias=False)
+    w = torch.where(w == 0, torch.ones_like(w), w)
+    x[:, -1] = math.inf
+    assert torch.equal(xa.linear(x, w), (w[-1].sign() * math.inf).expand(rows, 40))
+
+
 def test_what_lies_around_the_operands_is_not_read_into_sums():
     """Rows of a tensor that ends where they end, amid NaN: odd widths, whose 16-byte pieces reach beyond a row."""
     for dtype in TYPES:

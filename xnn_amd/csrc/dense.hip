@@ -127,11 +127,12 @@ __global__ __launch_bounds__(kFewThreads) void dense_few_kernel(ForwardArgs p, i
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       if (i * slices >= length) break;
-      const int k = min(slice + i * slices, length - 1);   // beyond the round the piece is zero
+      const int k = slice + i * slices;
+      const bool in = k < length;                          // else the piece is zero, and so is x, whatever it holds
       const Pack<T, N> v = __builtin_bit_cast(Pack<T, N>, piece[i]);
 #pragma unroll
       for (int m = 0; m < MR; ++m) {
-        const float f = xs[m][k];
+        const float f = in ? xs[m][min(k, length - 1)] : 0.0f;
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[m * N + j] = fmaf(f, (float)v.v[j], acc[m * N + j]);
       }
