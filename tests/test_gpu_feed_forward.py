@@ -395,6 +395,28 @@ def test_group_plan(rows, groups):
             assert np.array_equal(lists[1 + level], np.concatenate([[0], np.cumsum(tiles)])), level
 
 
+@pytest.mark.parametrize("rows,groups", [(2, 3), (2, 200), (300, 3), (300, 200), (5000, 70)])
+def test_a_plan_of_other_numbers_reaches_nothing_outside(rows, groups):
+    """The registered operators take a plan as it is given: every index of it is held to the rows and groups."""
+    gen = torch.Generator().manual_seed(rows)
+    for dtype in ("f32", "bf16"):
+        x, w, b, r, g, ids = _dense_case(dtype, rows, 72, 130, groups, residual=True)
+        plan = xa.group_plan(ids, groups)
+        want = xa.grouped_linear(x, w, plan, b, "silu", r)
+        around = [torch.full((1 << 16,), 5.0, device=DEV) for _ in range(8)]
+        n = plan.rows.numel()
+        for bad in (torch.full((n,), -1), torch.full((n,), 2 ** 31 - 1), torch.full((n,), -2 ** 31),
+                    torch.arange(n, 0, -1), torch.randint(-2 ** 31, 2 ** 31 - 1, (n,), generator=gen),
+                    torch.randint(-3, 2 * rows, (n,), generator=gen)):
+            bad = bad.to(torch.int32).to(DEV)
+            out, slope = torch.ops.xnn_amd.dense_slope(x, w, b, 1, r, bad)
+            dx, dw, db = torch.ops.xnn_amd.dense_backward(g, slope, x, w, bad, True, True, True)
+            torch.cuda.synchronize()
+            assert out.shape == want.shape and dx.shape == x.shape and dw.shape == w.shape and db.shape == b.shape
+        assert all((t == 5.0).all() for t in around)
+        assert torch.equal(xa.grouped_linear(x, w, plan, b, "silu", r), want)
+
+
 def test_the_species_plan_is_kept_with_the_graph():
     from xnn_amd import synthetic
     g = xa.structure_to_graph(synthetic.random_molecules(1, seed=2)[0].as_dict(), 4.0).to(DEV)

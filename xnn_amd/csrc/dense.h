@@ -73,7 +73,7 @@ __device__ __forceinline__ int find_group(const int32_t* __restrict__ p, int n, 
   while (len > 1) {
     const int step = (len + kWave - 1) / kWave, at = lane * step;
     const int v = at < len ? p[lo + at] : INT_MAX;
-    const int k = __popcll(__ballot(v <= t)) - 1;
+    const int k = max(__popcll(__ballot(v <= t)) - 1, 0);  // a list that is none of prefix sums: stays within it
     lo += k * step;
     len = min(step, len - k * step);
   }
