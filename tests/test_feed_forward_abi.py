@@ -134,6 +134,27 @@ def test_linear_backward_arguments(lib):
     assert f(0, None, None, None, 0, 0, 64, 64, None, None, 1, BUF, None, None, None, 0, None) == 0
 
 
+def test_sizes_whose_launches_pass_32_bits_of_threads(lib):
+    def forward(rows, n_in, n_out, groups):
+        return lib.xnn_linear_work_size(2, rows, n_in, n_out, groups, int(groups > 1), ctypes.byref(SIZE))
+
+    def backward(rows, n_in, n_out, groups, slope=0, weight=1, bias=1):
+        return lib.xnn_linear_backward_work_size(2, rows, n_in, n_out, groups, int(groups > 1), slope, 1, weight, bias,
+                                                 ctypes.byref(SIZE))
+    wide = (1 << 20) - 1
+    _refused(lib, forward((1 << 30) - 1, 1, 1, 1), b"too many tiles")
+    _refused(lib, forward(1, 1, wide, 4096), b"too many tiles")
+    _refused(lib, backward((1 << 30) - 1, 1, 1, 1), b"too many tiles")
+    assert forward(1 << 29, 1, 1, 1) == 0 and backward(1 << 29, 1, 1, 1) == 0
+    assert forward(5000, 1, wide, 200) == 0
+    # a weight of 2^37 elements; a bias of 2^28 in sixteens
+    _refused(lib, backward(100, 1 << 19, 1 << 18, 1), b"too many tiles")
+    assert backward(100, 1 << 18, 1 << 17, 1) == 0
+    _refused(lib, backward(100, 1, 1 << 17, 4000), b"too many tiles")
+    assert backward(100, 1, 1 << 15, 4000) == 0
+    assert backward(100, 1, 1 << 17, 4000, weight=0, bias=0) == 0
+
+
 def test_functions_refuse_cpu_tensors():
     import xnn_amd as xa
     x, w = torch.zeros(4, 8), torch.zeros(8, 8)

@@ -891,6 +891,9 @@ static void parts_launch(const Output& o, const int32_t* plan, int n_groups, int
   hipLaunchKernelGGL(dense_parts_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, q, parts, columns);
 }
 
+// blocks of a launch: its threads are numbered in 32 bits
+constexpr int64_t kMaxBlocks = ((int64_t)1 << 32) / kDenseThreads - kXcds;
+
 inline int dense_sizes(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, const int32_t* plan,
                        int32_t n_groups) {
   XNN_REQUIRE(is_storage(dtype), "dtype must be XNN_F32, XNN_BF16 or XNN_F16");
@@ -898,8 +901,7 @@ inline int dense_sizes(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, c
   XNN_REQUIRE(n_in >= 1 && n_in < (1 << 20) && n_out >= 1 && n_out < (1 << 20), "widths must be in [1, 2^20)");
   XNN_REQUIRE(n_groups >= 1 && n_groups <= kMaxGroups, "n_groups must be in [1, %d]", kMaxGroups);
   XNN_REQUIRE(plan != nullptr || n_groups == 1 || n_rows == 0, "groups need a plan");
-  XNN_REQUIRE(((n_rows >> 6) + n_groups + 2) * ((std::max(n_in, n_out) >> 6) + 1) < ((int64_t)1 << 31) - 8,
-              "too many tiles");
+  XNN_REQUIRE(((n_rows >> 6) + n_groups + 2) * ((std::max(n_in, n_out) >> 6) + 1) < kMaxBlocks, "too many tiles");
   return XNN_OK;
 }
 

@@ -273,6 +273,12 @@ static Parts parts_of(int64_t n_rows, bool grouped, int64_t want, int64_t least)
 // the width of x up to which the products form d themselves: a tile of both
 constexpr int kFormInProducts = 128;
 
+// the join's blocks of a group: of its weight, and of its bias
+static int64_t join_weight_blocks(int64_t n_in, int64_t n_out, int64_t n_groups) {
+  return std::max<int64_t>(1, std::min<int64_t>((n_in * n_out + 1023) / 1024, 65536 / n_groups));
+}
+static int64_t join_bias_blocks(int64_t n_out, bool bias) { return bias ? (n_out + 15) / 16 : 0; }
+
 struct BackwardPlan {
   int input_kind, kind;            // of the input's tiles, of the weight's
   Split split;                     // of the input's reduction, whose sums are gone before the weight's are there
@@ -280,6 +286,7 @@ struct BackwardPlan {
   bool pass;                       // forms d
   size_t bytes;                    // of the weight's parts, the bias's, d
   size_t bias_at, d_at;
+  int64_t blocks;                  // of the largest launch, at most
 };
 static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, int64_t n_groups,
                                   bool grouped, bool slope, bool input, bool weight, bool bias) {
@@ -326,6 +333,12 @@ static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32
   b.bias = b.weight;
   // sixteen blocks a CU of 512 bytes of the columns each
   if (b.pass) b.bias = parts_of(n_rows, grouped, std::max<int64_t>(1, 4096 / ((n_out * size + 511) / 512)), 64);
+  if (weight)
+    b.blocks = (row_tiles(n_rows, n_groups, grouped, b.weight.rows) + kXcds) *
+               (b.kind == kTile64 ? tiles(64, 64) : b.kind == kTile128 ? tiles(128, 128) : tiles(256, 128));
+  if (weight) b.blocks = std::max(b.blocks, (join_weight_blocks(n_in, n_out, n_groups) + join_bias_blocks(n_out, bias)) * n_groups);
+  if (b.pass)
+    b.blocks = std::max(b.blocks, row_tiles(n_rows, n_groups, grouped, b.bias.rows) * ((n_out * size + 511) / 512));
   const auto room = [](size_t n) { return (n + 255) / 256 * 256; };
   b.bias_at = std::max(room((size_t)b.weight.slots * n_in * n_out * sizeof(float)), input ? room(b.split.bytes) : 0);
   b.d_at = b.bias_at + (bias ? room((size_t)b.bias.slots * n_out * sizeof(float)) : 0);
@@ -396,9 +409,10 @@ int xnn_linear_backward_work_size(int dtype, int64_t n_rows, int32_t n_in, int32
   const int status = dense_sizes(dtype, n_rows, n_in, n_out, &some, n_groups);
   if (status != XNN_OK) return status;
   XNN_REQUIRE(bytes != nullptr, "NULL size");
-  *bytes = backward_plan(dtype, n_rows, n_in, n_out, n_groups, grouped != 0, slope != 0, input != 0, weight != 0,
-                         bias != 0)
-               .bytes;
+  const BackwardPlan b = backward_plan(dtype, n_rows, n_in, n_out, n_groups, grouped != 0, slope != 0, input != 0,
+                                       weight != 0, bias != 0);
+  XNN_REQUIRE(b.blocks < kMaxBlocks, "too many tiles");
+  *bytes = b.bytes;
   return XNN_OK;
 }
 
@@ -417,6 +431,7 @@ int xnn_linear_backward(int dtype, const void* grad, const void* slope, const vo
   const bool grouped = plan != nullptr && n_rows > 0;
   const BackwardPlan b = backward_plan(dtype, n_rows, n_in, n_out, n_groups, grouped, slope != nullptr, dx != nullptr,
                                        dweight != nullptr, dbias != nullptr);
+  XNN_REQUIRE(b.blocks < kMaxBlocks, "too many tiles");
   XNN_REQUIRE(b.bytes == 0 || (work && work_bytes >= b.bytes), "work too small");
   XNN_REQUIRE((uintptr_t)work % 16 == 0, "work must be aligned to 16 bytes");
   BackwardArgs p{};
@@ -453,9 +468,8 @@ int xnn_linear_backward(int dtype, const void* grad, const void* slope, const vo
     // groups without rows have zeros, parts have sums
     if (dweight != nullptr &&
         (grouped || b.weight.slots > 0 || n_rows == 0 || (dbias != nullptr && b.bias.slots > 0))) {
-      const int64_t all = ((int64_t)n_in * n_out + 1023) / 1024;
-      const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(all, 65536 / n_groups));
-      const int bias_blocks = dbias != nullptr ? (n_out + 15) / 16 : 0;
+      const int blocks = (int)join_weight_blocks(n_in, n_out, n_groups);
+      const int bias_blocks = (int)join_bias_blocks(n_out, dbias != nullptr);
       hipLaunchKernelGGL(dense_join_kernel<T>, dim3((unsigned)(blocks + bias_blocks) * (unsigned)n_groups), dim3(256),
                          0, s, p, blocks, bias_blocks);
     }
