@@ -73,7 +73,7 @@ __device__ __forceinline__ int find_group(const int32_t* __restrict__ p, int n, 
   while (len > 1) {
     const int step = (len + kWave - 1) / kWave, at = lane * step;
     const int v = at < len ? p[lo + at] : INT_MAX;
-    const int k = max(__popcll(__ballot(v <= t)) - 1, 0);  // a list that is none of prefix sums: stays within it
+    const int below = __popcll(__ballot(v <= t)), k = max(below - 1, 0);   // a list of other numbers: within it, too
     lo += k * step;
     len = min(step, len - k * step);
   }
@@ -107,8 +107,9 @@ __device__ __forceinline__ RowTile row_tile(const GroupView& v, int n_buckets, i
     from = v.row_ptr[g];
     to = v.row_ptr[g + 1];
   }
-  const int begin = max(0, from + (t - before) * size);
-  const int end = min(min(to, n_rows), begin + size);
+  // (unsigned: other numbers may wrap, and are then held to the rows)
+  const int begin = max(0, (int)((uint32_t)from + ((uint32_t)t - (uint32_t)before) * (uint32_t)size));
+  const int end = min(min(to, n_rows), (int)((uint32_t)begin + (uint32_t)size));
   return RowTile{begin, end, begin < end ? g : -1};
 }
 

@@ -203,7 +203,7 @@ __device__ __forceinline__ int group_parts(const GroupView& v, int n_rows, int r
   begin = 0;
   if (v.n_groups == 0) return (n_rows + rows - 1) / rows;
   begin = min(max(v.row_ptr[group], 0), n_rows);
-  return min(v.tile_ptr[group + 1] - v.tile_ptr[group], (n_rows - begin + rows - 1) / rows);
+  return min((int)((uint32_t)v.tile_ptr[group + 1] - (uint32_t)v.tile_ptr[group]), (n_rows - begin + rows - 1) / rows);
 }
 
 // The parts of a weight and of its bias added in their order, zeros where there is none; a group's only part is done.
