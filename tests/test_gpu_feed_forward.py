@@ -427,6 +427,37 @@ def test_the_species_plan_is_kept_with_the_graph():
     assert g.species_plan(9) is not plan
 
 
+def test_a_species_plan_that_a_capture_makes_is_not_kept():
+    """Its rows are there once the graph is replayed, and in the graph's memory; one that is kept serves a capture, and
+    another stream makes its own."""
+    from xnn_amd import synthetic
+    g = xa.structure_to_graph(synthetic.random_molecules(1, seed=2)[0].as_dict(), 4.0).to(DEV)
+    want = xa.group_plan(g.atomic_numbers, 9).rows
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = g.species_plan(9)
+    plan = g.species_plan(9)
+    assert plan is not inside and torch.equal(plan.rows, want)
+    for _ in range(3):
+        inside.rows.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(inside.rows, want) and g.species_plan(9) is plan
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert g.species_plan(9) is plan
+        rows = plan.rows + 1
+    graph.replay()
+    assert torch.equal(rows, want + 1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = g.species_plan(9)
+        assert other is not plan and g.species_plan(9) is other
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other.rows, want)
+
+
 # --------------------------------------------------------------------------- streams, graphs, refusals
 def test_the_same_bits_at_every_call_and_on_another_stream():
     x, w, b, r, g, ids = _dense_case("bf16", 5000, 128, 256, 5, residual=True)

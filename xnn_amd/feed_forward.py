@@ -111,15 +111,19 @@ def group_plan(ids: Tensor, n_groups: int) -> GroupPlan:
 
 def species_plan_for(graph, n_groups: int) -> GroupPlan:
     """The cached plan of an :class:`~xnn_amd.data.AtomicGraph`'s species (made again when its
-    ``atomic_numbers`` are another tensor or were written to, or for another number of groups)."""
+    ``atomic_numbers`` are another tensor or were written to, for another number of groups and on another
+    stream). A capture takes the one that is there; one that it makes is the captured graph's, and not kept."""
     ids = graph.atomic_numbers
     version = None if ids.is_inference() else ids._version
     key = (version, int(n_groups))
+    capturing = ids.is_cuda and torch.cuda.is_current_stream_capturing()
+    stream = torch.cuda.current_stream(ids.device).cuda_stream if ids.is_cuda else None
     cached = getattr(graph, "_xnn_species_plan", None)
-    if cached is not None and cached[0] is ids and cached[1] == key:
-        return cached[2]
+    if cached is not None and cached[0] is ids and cached[1] == key and (capturing or cached[2] == stream):
+        return cached[3]
     plan = group_plan(ids, n_groups)
-    object.__setattr__(graph, "_xnn_species_plan", (ids, key, plan))
+    if not capturing:
+        object.__setattr__(graph, "_xnn_species_plan", (ids, key, stream, plan))
     return plan
 
 
