@@ -213,6 +213,27 @@ def _check_dense(dtype, case, activation):
     assert out[~seen].isnan().all() and not grads[0][~seen].any()
 
 
+@pytest.mark.parametrize("n_in", [40, 300])
+def test_slopes_far_from_one_keep_their_digits_in_bfloat16(n_in):
+    """silu at z = -10 -+ 2: f' of 1e-3 to 1e-5, its error half a float16 step of it (2^-11) and, of the exponential,
+    |z| 2^-23 and two roundings of z itself; d and dx are rounded to the type."""
+    gen = torch.Generator().manual_seed(n_in)
+    x, g = _random(gen, (200, n_in), "bf16"), _random(gen, (200, 96), "bf16")
+    w = _random(gen, (n_in, 96), "bf16", 0.5 * n_in ** -0.5)
+    b = torch.full((96,), -10.0, device=DEV, dtype=torch.bfloat16)
+    leaf = x.detach().requires_grad_(True)
+    got, = torch.autograd.grad(xa.linear(leaf, w, b, "silu"), leaf, g)
+    z = (x.double() @ w.double() - 10).requires_grad_(True)
+    slope, = torch.autograd.grad(torch.nn.functional.silu(z).sum(), z)
+    z = z.detach()
+    d = g.double() * slope
+    dz = _term("bf16", n_in) * (x.double().abs() @ w.double().abs() + 10)
+    dd = d.abs() * (2.0 ** -11 + 2.0 ** -8 + z.abs() * 2.0 ** -22 + 4 * 2.0 ** -24 + 2 * dz) * 1.01
+    dx = d @ w.double().t()
+    bound = dd @ w.double().abs().t() + _term("bf16", 96) * (d.abs() @ w.double().abs().t()) + 2.0 ** -8 * dx.abs()
+    _close(got, dx, bound, "dx")
+
+
 SHAPES = [(1, 1, 1), (1, 8, 8), (1, 1024, 4096), (5, 3, 7), (2, 64, 1), (21, 128, 512), (64, 64, 64), (65, 129, 33),
           (300, 250, 511), (257, 40, 300), (31, 512, 17), (1000, 17, 129)]
 

@@ -177,9 +177,9 @@ __device__ __forceinline__ void activate(int kind, float z, float& y, float& slo
 }
 
 // f'(z) as the backward pass gets it, so that d = g f'(z) is rounded once and not twice (the gradients' error is 1.4
-// times an output's rounding, 1.7 with f' in the type): float32 as it is, for bfloat16 a float16; for float16 its
-// root with its sign in 15 bits of fixed point (f' is below 1.13), off by 2^-15 near 1, the number below -32,767
-// standing for NaN
+// times an output's rounding, 1.7 with f' in the type): float32 as it is; for bfloat16 2^15 times it in float16 (f'
+// is below 1.13), off by 2^-11 of it down to 2^-29; for float16 its root with its sign in 15 bits of fixed point, off by
+// 2^-15 near 1 and by 2^-15 root(f') below, the number below -32,767 standing for NaN
 template <typename T>
 struct Slope {
   typedef T type;
@@ -192,19 +192,23 @@ template <>
 struct Slope<f16_t> {
   typedef int16_t type;
 };
-constexpr float kSlopeUnit = 30000.0f;
+constexpr float kSlopeUnit = 30000.0f, kSlopeScale = 32768.0f;
 template <typename T>
 __device__ __forceinline__ typename Slope<T>::type slope_stored(float s) {
-  if constexpr (!__is_same(T, f16_t))
-    return (typename Slope<T>::type)s;
+  if constexpr (sizeof(T) == 4)
+    return s;
+  else if constexpr (__is_same(T, bf16_t))
+    return (f16_t)(s * kSlopeScale);
   else
     return s == s ? (int16_t)__float2int_rn(copysignf(kSlopeUnit * __builtin_amdgcn_sqrtf(fabsf(s)), s))
                   : (int16_t)-32768;
 }
 template <typename T>
 __device__ __forceinline__ float slope_value(typename Slope<T>::type s) {
-  if constexpr (!__is_same(T, f16_t))
-    return (float)s;
+  if constexpr (sizeof(T) == 4)
+    return s;
+  else if constexpr (__is_same(T, bf16_t))
+    return (float)s * (1.0f / kSlopeScale);
   else
     return s == -32768 ? __builtin_nanf("") : (float)s * fabsf((float)s) * (1.0f / (kSlopeUnit * kSlopeUnit));
 }
