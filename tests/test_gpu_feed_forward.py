@@ -535,6 +535,68 @@ def test_a_captured_step_replays_the_plan_the_layers_and_their_gradients():
             assert torch.equal(a.nan_to_num(7.0), c.nan_to_num(7.0))
 
 
+def test_operands_of_more_than_4_GB():
+    """Offsets beyond 32 bits: in rows of x and of the output, and in the weights of the last group."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    gen = torch.Generator(device=DEV).manual_seed(5)
+
+    def rand(*shape):
+        return torch.randn(shape, generator=gen, device=DEV, dtype=torch.bfloat16)
+    pick = [0, 1, 65_535, 65_536, 130_999, 131_071, 139_998, 139_999]
+    x = rand(140_000, 16_384)                               # 4.6 GB, 2.3e9 elements
+    nw, nb = rand(16_384), rand(16_384)
+    leaf = x.requires_grad_(True)
+    out = xa.layer_norm(leaf, nw, nb)
+    dx, = torch.autograd.grad(out, leaf, out.detach())
+    part = x.detach()[pick].requires_grad_(True)
+    alone = xa.layer_norm(part, nw, nb)
+    assert torch.equal(out[pick], alone)
+    assert torch.equal(dx[pick], torch.autograd.grad(alone, part, alone.detach())[0])
+    del out, dx, alone, part
+    w = rand(16_384, 40) / 128
+    leaf = x.detach().requires_grad_(True)
+    wl = w.detach().requires_grad_(True)
+    out = xa.linear(leaf, wl, None, "silu")
+    g = rand(140_000, 40)
+    dx, dw = torch.autograd.grad(out, (leaf, wl), g)
+    z = x.detach()[pick].double() @ w.double()
+    u = 2.0 ** -8
+    size = x.detach()[pick].double().abs() @ w.double().abs()
+    dz = _term("bf16", 16_384) * size
+    y = torch.nn.functional.silu(z)
+    _close(out.detach()[pick], y, 1.2 * dz + 2.0 ** -21 * (1 + z.abs()) + (u + 2.0 ** -23) * y.abs(), "out")
+    s = torch.sigmoid(z)
+    d = g[pick].double() * s * (1 + z * (1 - s))
+    dd = g[pick].double().abs() * (dz + 2.0 ** -21 * (1 + z.abs()) + 1.13 * 2.0 ** -11) + u * d.abs()
+    ref = d @ w.double().t()
+    _close(dx[pick], ref, dd @ w.double().abs().t() + _term("bf16", 40) * (d.abs() @ w.double().abs().t())
+           + u * ref.abs(), "dx")
+    # the weight's gradient: the rows behind the 32-bit offset alone, the others' cotangents zero
+    g[:132_000] = 0
+    dw, = torch.autograd.grad(xa.linear(leaf, wl), wl, g)
+    tail, gt = x.detach()[132_000:].double(), g[132_000:].double()
+    ref = tail.t() @ gt
+    _close(dw, ref, _term("bf16", 8_000) * (tail.abs().t() @ gt.abs()) + u * ref.abs(), "dw")
+    del x, leaf, out, dx, dw, tail, size
+    w = rand(4096, 1024, 600)                               # 5 GB of weights
+    ids = torch.tensor([4095, 0, 4095, 3500, 3600, 7], device=DEV)
+    x, g, plan = rand(6, 1024), rand(6, 600), xa.group_plan(ids, 4096)
+    wl, leaf = w.requires_grad_(True), x.requires_grad_(True)
+    out = xa.grouped_linear(leaf, wl, plan)
+    dx, dw = torch.autograd.grad(out, (leaf, wl), g)
+    for i, group in enumerate(ids.tolist()):
+        wd, xd, gd = w.detach()[group].double(), x.detach()[i].double(), g[i].double()
+        ref = xd @ wd
+        _close(out.detach()[i], ref, _term("bf16", 1024) * (xd.abs() @ wd.abs()) + u * ref.abs(), "grouped out")
+        ref = gd @ wd.t()
+        _close(dx[i], ref, _term("bf16", 600) * (gd.abs() @ wd.t().abs()) + u * ref.abs(), "grouped dx")
+        rows = (ids == group).nonzero()[:, 0]
+        ref = x.detach()[rows].double().t() @ g[rows].double()
+        _close(dw[group], ref, 2.0 ** -20 * ref.abs() + u * ref.abs() + 2.0 ** -20, "grouped dw")
+    assert not dw[1:7].any() and not dw[3601:4095].any()
+
+
 def test_rows_behind_the_output_are_left():
     """Outputs are written row by row: what follows the last row in memory stays."""
     from xnn_amd import _lib
