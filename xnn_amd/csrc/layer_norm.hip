@@ -4,12 +4,12 @@
 //   n = (x - mean x) r,  r = 1 / sqrt(mean (x - mean x)^2 + eps),  y = w n + b
 //   dx = r (g w - mean(g w) - n mean(g w n)),   dw = sum_rows g n,   db = sum_rows g
 //
-// A stream: a row lies in the registers of 2^k threads, U pieces of 16 bytes a thread, so that the
-// squares are of the centered values and nothing is read twice. A wave has a row of its own up to four pieces a
-// lane: its sums are exchanges in the vector unit and wait for no other wave (24,000 rows of 2,048 in bfloat16, a
-// piece a thread and four waves a row: forward 81 us, so 38, the rate of a large copy). Longer rows add their waves' sums through LDS. A
-// thread keeps its columns from row to row and adds up their gradients in registers; the blocks' sums are
-// added in their order. Arithmetic is float32.
+// A stream: a row lies in the registers of 2^k threads, U pieces of 16 bytes a thread, so that the squares are of
+// the centered values and nothing is read twice. A wave has a row of its own up to four pieces a lane: its sums are
+// exchanges in the vector unit and wait for no other wave (24,000 rows of 2,048 in bfloat16, a piece a thread and
+// four waves a row: forward 81 us, so 38, the rate of a large copy). Longer rows add their waves' sums through LDS.
+// A thread keeps its columns from row to row and adds up their gradients in registers; the blocks' sums are added
+// in their order. Arithmetic is float32. The backward pass of those rows takes 64 us (4.6 TB/s) and the join 5.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
