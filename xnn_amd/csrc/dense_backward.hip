@@ -105,9 +105,10 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_input_kernel(BackwardA
   typedef DenseLds<L, T, true, true> S;
   __shared__ __align__(16) char lds[S::kBytes];
   __shared__ int32_t rows[L::BM];
-  const int64_t slot = xcd_slot();
-  if (slot >= p.tiles * parts) return;
-  const int part = (int)(slot / p.tiles), tile = (int)(slot % p.tiles);
+  int64_t tiles;
+  const int64_t slot = tile_slot(o.groups, p.tiles, p.tiles_n, parts, tiles);
+  if (slot < 0) return;
+  const int part = (int)(slot / tiles), tile = (int)(slot % tiles);
   const RowTile t = row_tile(o.groups, o.groups.n_groups + 1, o.n_rows, tile / p.tiles_n, L::BM);
   if (t.group < 0) return;
   const int n0 = tile % p.tiles_n * L::BN;
