@@ -34,6 +34,7 @@ struct BackwardArgs {
   int rows, bias_rows;             // of a part of the weight's sums, of the bias's
   int spread;                      // parts of different lengths: to the XCDs in turn
   int sums;                        // the weight's product adds up db
+  int stream;                      // dw is larger than the caches of the dies
 };
 
 // Where the sums of the part of sorted rows from `begin` on stand: parts of one weight follow each other; among
@@ -193,7 +194,10 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_weight_kernel(Backward
     dense_rows<L, N>(
         lds, acc, [&](int n) { c = n0 + n; },
         [&](int m, float(&v)[N]) {
-          if (m0 + m < p.n_in && c < p.n_out)
+          if (m0 + m >= p.n_in || c >= p.n_out) return;
+          if (p.stream)
+            store_row_part<T, N, true>(dw + (int64_t)(m0 + m) * p.n_out, c, p.n_out, v);
+          else
             store_row_part<T, N>(dw + (int64_t)(m0 + m) * p.n_out, c, p.n_out, v);
         });
   } else {
@@ -465,6 +469,7 @@ int xnn_linear_backward(int dtype, const void* grad, const void* slope, const vo
   p.bias_groups = group_view(order, n_rows, n_groups, grouped ? group_level(p.bias_rows) : 0);
   hipStream_t s = as_hip(stream);
   p.sums = dbias != nullptr && !b.pass;
+  p.stream = past_caches((int64_t)n_groups * n_in, n_out, storage_bytes(dtype));
   XNN_STORAGE_DISPATCH(dtype, T, {
     if (b.pass && n_rows > 0) {
       cotangent_launch<T>(p, order, n_groups, s);
