@@ -12,9 +12,9 @@
 // Bounds: of large products the matrix cores' feed (8,192^3 in bfloat16 dx 955 to 970, dW 1,040 to 1,090 TFLOP/s:
 // dW reads both operands across their rows, by the transposing read, with a tenth of the LDS conflicts), of the
 // pass memory (24,000 x 4,096 in bfloat16, 590 MB in 137 us: 4.3 TB/s), of short reductions what is around the
-// products (72,000 rows of 128 -> 512 in float32, two species: dx 97 to 114 us, dW 75 to 87, join 14 to 16).
-// Weights of 64 uneven groups (16,384 rows, 1,024 x 1,024 in bfloat16): 153 us and a join of 39, for the 134 MB of
-// their gradient and the parts' sums.
+// products (72,000 rows of 128 -> 512 in float32, two species: dx 97 to 116 us, dW 77 to 86, join 10). Weights of
+// 64 uneven groups (16,384 rows, 1,024 x 1,024 in bfloat16): 126 us and a join of 11, for the 134 MB of their gradient
+// and the parts' sums.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -32,7 +32,7 @@ struct BackwardArgs {
   GroupView groups, bias_groups;
   int n_rows, n_in, n_out, tiles_m, tiles_n;
   int rows, bias_rows;             // of a part of the weight's sums, of the bias's
-  int spread;                      // parts of different lengths: to the XCDs in turn
+  int spread;                      // parts of different lengths: to the XCDs in turn (1), or a part's tiles, so many
   int sums;                        // the weight's product adds up db
   int stream;                      // dw is larger than the caches of the dies
 };
@@ -142,7 +142,11 @@ __global__ __launch_bounds__(kDenseThreads, 2) void dense_weight_kernel(Backward
   __shared__ __align__(16) char lds[S::kBytes];
   const int64_t slot = xcd_slot();
   int64_t part, tile;
-  if (p.spread) {
+  if (p.spread > 1) {
+    const int each = p.spread / kXcds, i = (int)(blockIdx.x / kXcds);
+    part = i / each;
+    tile = (int)(blockIdx.x % kXcds) * each + i % each;
+  } else if (p.spread) {
     part = slot_of_xcd(p.tiles_m * p.tiles_n, tile);
   } else {
     part = slot / (p.tiles_m * p.tiles_n);
@@ -420,7 +424,9 @@ static void input_launch(BackwardArgs p, const Split& split, const int32_t* plan
 }
 
 // Groups of different sizes have parts of different lengths, the long ones next to each other: spread over the XCDs
-// where there are enough of them (16,384 rows in 64 groups, 1,024 x 1,024 in bfloat16: 212 us, in turn 161)
+// where there are enough of them (16,384 rows in 64 uneven groups, 1,024 x 1,024 in bfloat16: 212 us, in turn 161), and
+// where a weight's tiles are a multiple of eight each part's over all XCDs, whose work is then the same (those in turn had
+// up to 1.7 times the mean: with the join 134 us, so 117; even groups 79 and 83, for x and d read by each XCD).
 template <typename T, typename L>
 static void weight_launch(BackwardArgs p, const int32_t* plan, int n_groups, hipStream_t s) {
   p.tiles_m = (p.n_in + L::BM - 1) / L::BM;
@@ -428,7 +434,8 @@ static void weight_launch(BackwardArgs p, const int32_t* plan, int n_groups, hip
   p.parts = row_tiles(p.n_rows, n_groups, plan != nullptr, p.rows);
   p.spread = plan != nullptr && p.parts >= 4 * kXcds;
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-  const int64_t blocks = p.spread ? xcd_blocks(p.parts) * tiles : xcd_blocks(p.parts * tiles);
+  if (p.spread && tiles % kXcds == 0) p.spread = (int)tiles;
+  const int64_t blocks = p.spread == 1 ? xcd_blocks(p.parts) * tiles : xcd_blocks(p.parts * tiles);
   const dim3 grid((unsigned)blocks), threads(kDenseThreads);
   if (p.slope == nullptr) {
     if (plan != nullptr)
