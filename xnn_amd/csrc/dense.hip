@@ -6,7 +6,7 @@
 // x 4,096 x 4,096 194 (as six products 1,160). What leaves costs beside them: 24,000 x 1,024 -> 4,096 in bfloat16
 // 275 us, with gelu and its slope 376 to 388 (31 vector instructions an element, two of them of four times the
 // cycles; 375 MB written). Short reductions are bound by it: 72,000 x 128 -> 512 in float32 with silu and its slope
-// 118 to 137 us, 281 MB written.
+// 120 to 137 us, 281 MB written.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
