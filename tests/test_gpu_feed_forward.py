@@ -297,6 +297,22 @@ def test_grouped_linear_of_many_tiles(dtype, rows, n_in, n_out):
     _check_dense(dtype, _dense_case(dtype, rows, n_in, n_out, 7, some=[0, 0, 0, 1, 1, 3, 6], strided=True), "silu")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("groups", [62, 63, 64, 65, 254, 255, 256, 257, 300])
+def test_grouped_linear_of_as_many_groups_as_lanes(dtype, groups):
+    """Tiles are found in lists of up to a wave's lanes, up to four of them, and longer ones."""
+    some = [0, 1, groups - 1, groups - 1, groups - 1, groups // 2, -1, groups]
+    _check_dense(dtype, _dense_case(dtype, 700, 40, 72, groups, residual=True, some=some), "gelu")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_in,n_out", [(256, 1024), (130, 900), (100, 520)])
+def test_grouped_linear_of_uneven_groups_with_many_parts(dtype, n_in, n_out):
+    """The weight's gradient in parts of different lengths, a weight's tiles a multiple of the dies and not."""
+    some = [3] * 30 + [20] * 18 + list(range(4, 20)) + [-1]
+    _check_dense(dtype, _dense_case(dtype, 12000, n_in, n_out, 24, some=some), "silu")
+
+
 def test_a_row_that_is_not_finite_reaches_no_other():
     for dtype in TYPES:
         x, w, b, r, g, ids = _dense_case(dtype, 200, 70, 90, 4)
@@ -497,6 +513,30 @@ def test_the_same_bits_at_every_call_and_on_another_stream():
     torch.cuda.current_stream().wait_stream(side)
     for a, c, d in zip(want, got, once()):
         assert torch.equal(a, c) and torch.equal(a, d)
+
+
+def test_two_streams_at_once():
+    """Calls in flight on two streams, forward and backward, share no workspace and no state."""
+    cases = [_dense_case("f32", 3000, 256, 96, 6, residual=True, seed=1), _dense_case("bf16", 40, 4096, 64, 3, seed=2)]
+
+    def once(case):
+        x, w, b, r, g, ids = case
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        out = xa.grouped_linear(leaves[0], leaves[1], xa.group_plan(ids, w.shape[0]), leaves[2], "silu", r)
+        return [out.detach(), *torch.autograd.grad(out, leaves, g)]
+    want = [once(c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for stream in streams:
+        stream.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(6):
+        for case, stream, ref in zip(cases, streams, want):
+            with torch.cuda.stream(stream):
+                got.append((once(case), ref))
+    torch.cuda.synchronize()
+    for a, ref in got:
+        for t, u in zip(a, ref):
+            assert torch.equal(t, u)
 
 
 def test_a_captured_step_replays_the_plan_the_layers_and_their_gradients():
