@@ -13,8 +13,8 @@
 // dW reads both operands across their rows, by the transposing read, with a tenth of the LDS conflicts), of the
 // pass memory (24,000 x 4,096 in bfloat16, 590 MB in 137 us: 4.3 TB/s), of short reductions what is around the
 // products (72,000 rows of 128 -> 512 in float32, two species: dx 97 to 116 us, dW 77 to 86, join 10). Weights of
-// 64 uneven groups (16,384 rows, 1,024 x 1,024 in bfloat16): 126 us and a join of 11, for the 134 MB of their gradient
-// and the parts' sums.
+// 64 uneven groups (16,384 rows, 1,024 x 1,024 in bfloat16): with the join 103, for the 134 MB of their gradient and the
+// parts' sums.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -349,16 +349,16 @@ static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32
     // The tiles and the number of parts with the least time, estimated from the rates of large products (kinds 0,
     // 1, 2: microseconds of 64 rows of a tile with all of a CU's blocks at work, and those blocks) and the parts'
     // sums, written and read at 4 TB/s. Parts of one length come in rounds; those of groups, of any, fill the card
-    // but for three quarters of a long one's time at its end, and the more of them the more what is around their
-    // products counts: wide weights take the large tiles (16,384 rows in 64 groups, 1,024 x 1,024 in bfloat16, a
-    // few large groups and even ones: 128 x 128 tiles 185 and 143 us, 256 x 128 170 and 117).
+    // but for about one long one's time and a half at its end. Wide weights of groups take 128 x 128 tiles, three
+    // blocks a CU, of which others work while one looks up its rows (16,384 rows, 1,024 x 1,024 in bfloat16, with the
+    // join: 64 uneven groups 103 us, 256 x 128 117; four even ones 88 and 114; 32,768 in eight, 4,096 x 4,096: 2,015
+    // and 2,270).
     static const double step16[] = {0.9, 1.4, 2.2}, step32[] = {2.9, 5.4, 0.0};
     static const int per_cu[] = {3, 2, 2}, bm[] = {64, 128, 256}, bn[] = {64, 128, 128};
     const double sums = (double)n_in * n_out * 8 / 4e6;
     double best = 0.0;
     for (int kind = 0; kind < (size == 2 && !(slope && n_in <= kFormInProducts) ? 3 : 2); ++kind) {
-      if (grouped && size == 2 && kind < 2 && n_in >= 256 && n_out >= 128)
-        continue;
+      if (grouped && size == 2 && kind != kTile128 && n_in >= 256 && n_out >= 128) continue;
       const double t = (double)tiles(bm[kind], bn[kind]), blocks = 256.0 * per_cu[kind];
       const double step = size == 2 ? step16[kind] : step32[kind];
       for (int64_t want = 1; want <= 1024; want += std::max<int64_t>(1, want / 4)) {
@@ -367,7 +367,7 @@ static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32
         const double steps = (double)std::min<int64_t>(parts.rows, n_rows) / 64 + 2;   // and two for what is around
         double time = std::max(1.0, std::ceil(all * t / blocks)) * steps * step;
         if (grouped && all * t > blocks)
-          time = ((double)n_rows / 64 + 2 * all) * t / blocks * step + 0.75 * steps * step;
+          time = ((double)n_rows / 64 + 2 * all) * t / blocks * step + 1.4 * steps * step;
         if (parts.slots > 0) time += 5.0 + sums * n;
         if (best == 0.0 || time < best) {
           best = time;
