@@ -349,7 +349,7 @@ static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32
     // The tiles and the number of parts with the least time, estimated from the rates of large products (kinds 0,
     // 1, 2: microseconds of 64 rows of a tile with all of a CU's blocks at work, and those blocks) and the parts'
     // sums, written and read at 4 TB/s. Parts of one length come in rounds; those of groups, of any, fill the card
-    // but for about one long one's time and a half at its end. Wide weights of groups take 128 x 128 tiles, three
+    // but for about one long one's time and a half at its end. Weights of groups take tiles of up to 128 x 128, wide ones those, three
     // blocks a CU, of which others work while one looks up its rows (16,384 rows, 1,024 x 1,024 in bfloat16, with the
     // join: 64 uneven groups 103 us, 256 x 128 117; four even ones 88 and 114; 32,768 in eight, 4,096 x 4,096: 2,015
     // and 2,270).
@@ -357,8 +357,8 @@ static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32
     static const int per_cu[] = {3, 2, 2}, bm[] = {64, 128, 256}, bn[] = {64, 128, 128};
     const double sums = (double)n_in * n_out * 8 / 4e6;
     double best = 0.0;
-    for (int kind = 0; kind < (size == 2 && !(slope && n_in <= kFormInProducts) ? 3 : 2); ++kind) {
-      if (grouped && size == 2 && kind != kTile128 && n_in >= 256 && n_out >= 128) continue;
+    for (int kind = 0; kind < (size == 2 && !grouped && !(slope && n_in <= kFormInProducts) ? 3 : 2); ++kind) {
+      if (grouped && size == 2 && kind == kTile64 && n_in >= 256 && n_out >= 128) continue;
       const double t = (double)tiles(bm[kind], bn[kind]), blocks = 256.0 * per_cu[kind];
       const double step = size == 2 ? step16[kind] : step32[kind];
       for (int64_t want = 1; want <= 1024; want += std::max<int64_t>(1, want / 4)) {
@@ -437,16 +437,16 @@ static void weight_launch(BackwardArgs p, const int32_t* plan, int n_groups, hip
   if (p.spread && tiles % kXcds == 0) p.spread = (int)tiles;
   const int64_t blocks = p.spread == 1 ? xcd_blocks(p.parts) * tiles : xcd_blocks(p.parts * tiles);
   const dim3 grid((unsigned)blocks), threads(kDenseThreads);
-  if (p.slope == nullptr) {
-    if (plan != nullptr)
+  // 256 x 128 tiles are of one weight, and of a d that is there
+  if (plan == nullptr && p.slope == nullptr) {
+    hipLaunchKernelGGL((dense_weight_kernel<T, L, false, false>), grid, threads, 0, s, p);
+  } else if constexpr (L::BM <= 128) {
+    if (plan == nullptr)
+      hipLaunchKernelGGL((dense_weight_kernel<T, L, true, false>), grid, threads, 0, s, p);
+    else if (p.slope == nullptr)
       hipLaunchKernelGGL((dense_weight_kernel<T, L, false, true>), grid, threads, 0, s, p);
     else
-      hipLaunchKernelGGL((dense_weight_kernel<T, L, false, false>), grid, threads, 0, s, p);
-  } else if constexpr (L::BM <= 128) {
-    if (plan != nullptr)
       hipLaunchKernelGGL((dense_weight_kernel<T, L, true, true>), grid, threads, 0, s, p);
-    else
-      hipLaunchKernelGGL((dense_weight_kernel<T, L, true, false>), grid, threads, 0, s, p);
   }
 }
 
