@@ -18,6 +18,7 @@ They are differentiable once. The per-edge reference path has no counterpart.
 """
 from __future__ import annotations
 
+import ctypes
 import os
 from dataclasses import dataclass
 from typing import Optional
@@ -109,21 +110,60 @@ def group_plan(ids: Tensor, n_groups: int) -> GroupPlan:
     return GroupPlan(ids.shape[0], int(n_groups), rows)
 
 
+class _KeptPlans:
+    """A graph's plans by stream and number of groups, of one tensor of species at one version."""
+
+    def __init__(self, ids=None, version=None):
+        self.ids, self.version, self.plans = ids, version, {}
+
+
+class _CapturedPlans(list):
+    """Plans that captured graphs write and read, held by their species as long as those are there."""
+
+
+def _form_again(plan: GroupPlan, ids: Tensor) -> None:
+    """``plan`` formed in its own memory once more (from other ids, of another content)."""
+    ids = ids.to(torch.int64).contiguous()
+    sizes = [ctypes.c_size_t(), ctypes.c_size_t()]
+    _lib.call("xnn_group_plan_size", plan.n_rows, plan.n_groups, *map(ctypes.byref, sizes))
+    work = torch.empty(sizes[1].value, dtype=torch.uint8, device=ids.device)
+    with torch.cuda.device(ids.device):
+        _lib.call("xnn_group_plan", ids.data_ptr(), plan.n_rows, plan.n_groups, plan.rows.data_ptr(),
+                  work.data_ptr(), work.numel(), _lib.stream(ids.device))
+
+
 def species_plan_for(graph, n_groups: int) -> GroupPlan:
-    """The cached plan of an :class:`~xnn_amd.data.AtomicGraph`'s species (made again when its
-    ``atomic_numbers`` are another tensor or were written to, for another number of groups and on another
-    stream). A capture takes the one that is there; one that it makes is the captured graph's, and not kept."""
+    """The plan of an :class:`~xnn_amd.data.AtomicGraph`'s species, kept for each stream and number of groups, and
+    made again when its ``atomic_numbers`` are another tensor or were written to.
+
+    What a capture uses is formed in it, so that each replay follows the atomic numbers as they are then: a new plan
+    in the captured graph's memory, or a kept one in its own, which serves no later call and stays as long as the
+    species that the captured kernels read."""
     ids = graph.atomic_numbers
+    if not ids.is_cuda:
+        return group_plan(ids, n_groups)                   # (refused)
     version = None if ids.is_inference() else ids._version
-    key = (version, int(n_groups))
-    capturing = ids.is_cuda and torch.cuda.is_current_stream_capturing()
-    stream = torch.cuda.current_stream(ids.device).cuda_stream if ids.is_cuda else None
-    cached = getattr(graph, "_xnn_species_plan", None)
-    if cached is not None and cached[0] is ids and cached[1] == key and (capturing or cached[2] == stream):
-        return cached[3]
-    plan = group_plan(ids, n_groups)
-    if not capturing:
-        object.__setattr__(graph, "_xnn_species_plan", (ids, key, stream, plan))
+    with torch.cuda.device(ids.device):
+        capturing = torch.cuda.is_current_stream_capturing()
+    kept = getattr(graph, "_xnn_species_plan", None)
+    if kept is None or kept.ids is not ids or kept.version != version:
+        kept = _KeptPlans(ids, version)
+        if not capturing:
+            object.__setattr__(graph, "_xnn_species_plan", kept)
+    if capturing:
+        key = next((k for k in kept.plans if k[1] == n_groups), None)
+        if key is None:
+            return group_plan(ids, n_groups)
+        plan = kept.plans.pop(key)
+        if not hasattr(ids, "_xnn_captured_plans"):
+            ids._xnn_captured_plans = _CapturedPlans()
+        ids._xnn_captured_plans.append(plan)
+        _form_again(plan, ids)
+        return plan
+    key = (torch.cuda.current_stream(ids.device).cuda_stream, int(n_groups))
+    plan = kept.plans.get(key)
+    if plan is None:
+        plan = kept.plans[key] = group_plan(ids, n_groups)
     return plan
 
 
