@@ -113,6 +113,12 @@ def test_streams_and_numbers_of_groups_keep_a_plan_each(card):
     assert card.made == 4
 
 
+def test_numbers_without_a_version_have_a_new_plan_each_time(card):
+    """A write to an inference tensor can't be noticed."""
+    graph = Graph(inference=True)
+    assert FF.species_plan_for(graph, 9) is not FF.species_plan_for(graph, 9)
+
+
 # --------------------------------------------------------------------------- on the GPU
 def _graph(n=4):
     from xnn_amd import synthetic
@@ -180,3 +186,14 @@ def test_a_captured_model_with_weights_of_species_follows_them(kept):
         torch.cuda.synchronize()
         for key, value in got.items():
             assert torch.equal(value, eager[key]), (k, key)
+
+
+@pytest.mark.gpu
+def test_inference_numbers_that_were_written_to():
+    with torch.inference_mode():
+        ids = torch.tensor([1, 6, 8, 1], device="cuda")
+        g = Graph()
+        g.atomic_numbers = ids
+        FF.species_plan_for(g, 9)
+        ids[0] = 8
+        assert torch.equal(FF.species_plan_for(g, 9).rows, xa.group_plan(ids, 9).rows)

@@ -134,20 +134,20 @@ def _form_again(plan: GroupPlan, ids: Tensor) -> None:
 
 def species_plan_for(graph, n_groups: int) -> GroupPlan:
     """The plan of an :class:`~xnn_amd.data.AtomicGraph`'s species, kept for each stream and number of groups, and
-    made again when its ``atomic_numbers`` are another tensor or were written to.
+    made again when its ``atomic_numbers`` are another tensor or were written to (of an inference tensor, which
+    does not tell, at every call).
 
     What a capture uses is formed in it, so that each replay follows the atomic numbers as they are then: a new plan
     in the captured graph's memory, or a kept one in its own, which serves no later call and stays as long as the
     species that the captured kernels read."""
     ids = graph.atomic_numbers
-    if not ids.is_cuda:
-        return group_plan(ids, n_groups)                   # (refused)
-    version = None if ids.is_inference() else ids._version
+    if not ids.is_cuda or ids.is_inference():
+        return group_plan(ids, n_groups)                   # (refused on a CPU)
     with torch.cuda.device(ids.device):
         capturing = torch.cuda.is_current_stream_capturing()
     kept = getattr(graph, "_xnn_species_plan", None)
-    if kept is None or kept.ids is not ids or kept.version != version:
-        kept = _KeptPlans(ids, version)
+    if kept is None or kept.ids is not ids or kept.version != ids._version:
+        kept = _KeptPlans(ids, ids._version)
         if not capturing:
             object.__setattr__(graph, "_xnn_species_plan", kept)
     if capturing:
