@@ -2,6 +2,7 @@
 plan's kernels; on the GPU the replays of captured steps."""
 import copy
 import gc
+import pickle
 import types
 import weakref
 
@@ -117,6 +118,20 @@ def test_numbers_without_a_version_have_a_new_plan_each_time(card):
     """A write to an inference tensor can't be noticed."""
     graph = Graph(inference=True)
     assert FF.species_plan_for(graph, 9) is not FF.species_plan_for(graph, 9)
+
+
+@pytest.mark.parametrize("other", [copy.deepcopy, lambda graph: pickle.loads(pickle.dumps(graph))])
+def test_a_copied_graph_makes_its_own(card, other):
+    """The version of copied numbers starts again, and may come to that of the numbers which the plan is of."""
+    graph = Graph()
+    graph.atomic_numbers._version = 2
+    FF.species_plan_for(graph, 9)
+    _captured(graph, card)
+    FF.species_plan_for(graph, 9)
+    made, another = card.made, other(graph)
+    another.atomic_numbers._version = 2                     # 1 after the copy, and one write
+    FF.species_plan_for(another, 9)
+    assert card.made == made + 1
 
 
 # --------------------------------------------------------------------------- on the GPU

@@ -111,14 +111,21 @@ def group_plan(ids: Tensor, n_groups: int) -> GroupPlan:
 
 
 class _KeptPlans:
-    """A graph's plans by stream and number of groups, of one tensor of species at one version."""
+    """A graph's plans by stream and number of groups, of one tensor of species at one version. Copied or pickled it is
+    empty: versions start again there."""
 
     def __init__(self, ids=None, version=None):
         self.ids, self.version, self.plans = ids, version, {}
 
+    def __reduce__(self):
+        return _KeptPlans, ()
+
 
 class _CapturedPlans(list):
     """Plans that captured graphs write and read, held by their species as long as those are there."""
+
+    def __reduce__(self):
+        return _CapturedPlans, ()
 
 
 def _form_again(plan: GroupPlan, ids: Tensor) -> None:
