@@ -186,15 +186,15 @@ __device__ __forceinline__ void activate(int kind, float z, float& y, float& slo
     y = z * c;
     slope = fmaf(z * 0.39894228040143268f, e, c);
   } else if (kind == kTanh) {
-    // by the exponential; near zero, where that loses it, the series
+    // by the exponential; y near zero, where that loses it, by the series (1 - y^2 would lose the slope where y is near 1)
     const float a = fabsf(z), e = __builtin_amdgcn_exp2f(-2.0f * kLog2e * a), w = z * z;
-    const float far = copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), z);
+    const float r = __builtin_amdgcn_rcpf(1.0f + e), far = copysignf((1.0f - e) * r, z);
     float q = fmaf(w, 62.0f / 2835.0f, -17.0f / 315.0f);
     q = fmaf(w, q, 2.0f / 15.0f);
     q = fmaf(w, q, -1.0f / 3.0f);
     const float near = fmaf(z * w, q, z);
     y = a < 0.25f ? near : far;
-    slope = fmaf(-y, y, 1.0f);
+    slope = 4.0f * e * r * r;
   } else {
     y = z;
     slope = 1.0f;
