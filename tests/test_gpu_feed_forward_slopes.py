@@ -102,3 +102,30 @@ def _check_tail(dtype, name):
 def test_tanh_far_from_zero(dtype):
     """f' is 4 e / (1 + e)^2, e = exp(-2 |z|): 1 - y^2 has lost it where y is near 1."""
     _check_tail(dtype, "tanh")
+
+
+@pytest.mark.parametrize("name", TAILS)
+def test_float16_far_from_one(name):
+    """Small f' keep the type's digits: a loss scale makes their gradients large."""
+    _check_tail("f16", name)
+
+
+@pytest.mark.parametrize("name", TAILS)
+def test_every_slope_of_float16_as_it_is_kept(name):
+    """Over the whole range, the largest and the least among them: 1.13 and -0.13 of gelu at -+1.414, zeros, and the
+    borders between the forms."""
+    z = torch.cat([torch.linspace(-20, 20, 20001), torch.linspace(-1.5, -1.2, 2000), torch.linspace(1.3, 2.5, 2000),
+                   torch.linspace(3.0, 3.2, 500), torch.zeros(3)])
+    for width in (64, 192):
+        _check("f16", name, z, width, 1.0)
+
+
+def test_slopes_that_are_not_numbers_stay_so():
+    for dtype, t in TYPES.items():
+        for width in (64, 192):
+            x = torch.randn(40, width, generator=torch.Generator().manual_seed(1)).to(t).to(DEV)
+            x[3] = float("nan")
+            leaf = x.clone().requires_grad_(True)
+            out = xa.linear(leaf, torch.eye(width, dtype=t, device=DEV), None, "tanh")
+            got, = torch.autograd.grad(out, leaf, torch.ones_like(out))
+            assert got[3].isnan().all() and got[:3].isfinite().all() and got[4:].isfinite().all()

@@ -203,8 +203,12 @@ __device__ __forceinline__ void activate(int kind, float z, float& y, float& slo
 
 // f'(z) as the backward pass gets it, so that d = g f'(z) is rounded once and not twice (the gradients' error is
 // 1.4 times an output's rounding, 1.7 with f' in the type): float32 as it is; for bfloat16 2^15 times it in float16
-// (f' is below 1.13), off by 2^-11 of it down to 2^-29; for float16 its root with its sign in 15 bits of fixed
-// point, off by 2^-15 near 1 and by 2^-15 root(f') below, the number below -32,767 standing for NaN
+// (f' is below 1.13), off by 2^-11 of it down to 2^-29; for float16 in 16 bits that are fine where f' is large and never
+// coarser than the type where it is small (a loss scale makes such d large):
+//   |f'| >= 2^-7   its root in steps of 1 / 30,000, off by 2^-14.8 root(f'): 2^-14.8 of it near 1, 2^-11.3 at 2^-7
+//   below          2^5 times it in float16, off by 2^-11 of it down to 2^-19, by 2^-30 below
+// Of 65,536 numbers the first 13,313 are the float16 ones, then roots up to 1.13's; a negative f', whose root is below
+// 0.36, has the complement of its size's number, and what is between the two ends stands for NaN.
 template <typename T>
 struct Slope {
   typedef T type;
@@ -215,18 +219,28 @@ struct Slope<bf16_t> {
 };
 template <>
 struct Slope<f16_t> {
-  typedef int16_t type;
+  typedef uint16_t type;
 };
-constexpr float kSlopeUnit = 30000.0f, kSlopeScale = 32768.0f;
+constexpr float kSlopeScale = 32768.0f;
+constexpr float kSlopeUnit = 30000.0f, kSlopeFine = 0x1p-7f, kSlopeFineScale = 32.0f;
+constexpr int kSlopeFineLast = 0x3400;             // 2^5 2^-7 in float16
+constexpr int kSlopeRoots = 10662;                 // the root of 2^-7, 2,652 steps, comes after it
+constexpr int kSlopeNan = 43000;
+static_assert(kSlopeRoots + 2652 == kSlopeFineLast + 2 && kSlopeRoots + 31950 < kSlopeNan &&
+                  65535 - (kSlopeRoots + 10850) > kSlopeNan, "");
 template <typename T>
 __device__ __forceinline__ typename Slope<T>::type slope_stored(float s) {
   if constexpr (sizeof(T) == 4)
     return s;
   else if constexpr (__is_same(T, bf16_t))
     return (f16_t)(s * kSlopeScale);
-  else
-    return s == s ? (int16_t)__float2int_rn(copysignf(kSlopeUnit * __builtin_amdgcn_sqrtf(fabsf(s)), s))
-                  : (int16_t)-32768;
+  else {
+    const float a = fabsf(s);
+    const int fine = __builtin_bit_cast(uint16_t, (f16_t)(a * kSlopeFineScale));
+    const int root = kSlopeRoots + __float2int_rn(kSlopeUnit * __builtin_amdgcn_sqrtf(a));
+    const int n = a < kSlopeFine ? fine : root;
+    return (uint16_t)(s == s ? (s < 0.0f ? ~n : n) : kSlopeNan);
+  }
 }
 template <typename T>
 __device__ __forceinline__ float slope_value(typename Slope<T>::type s) {
@@ -234,8 +248,14 @@ __device__ __forceinline__ float slope_value(typename Slope<T>::type s) {
     return s;
   else if constexpr (__is_same(T, bf16_t))
     return (float)s * (1.0f / kSlopeScale);
-  else
-    return s == -32768 ? __builtin_nanf("") : (float)s * fabsf((float)s) * (1.0f / (kSlopeUnit * kSlopeUnit));
+  else {
+    const bool negative = s > kSlopeNan;
+    const uint16_t n = negative ? (uint16_t)~s : s;
+    const float root = (float)((int)n - kSlopeRoots) * (1.0f / kSlopeUnit);
+    const float fine = (float)__builtin_bit_cast(f16_t, n) * (1.0f / kSlopeFineScale);
+    const float a = n <= kSlopeFineLast ? fine : root * root;
+    return s == kSlopeNan ? __builtin_nanf("") : negative ? -a : a;
+  }
 }
 
 // ---------------------------------------------------------------- sizes

@@ -236,7 +236,7 @@ Three dense_backward(const Tensor& grad, const MaybeTensor& slope, const Tensor&
   return op.call(grad, slope, x, weight, plan, input, weights, biases);
 }
 
-// the slope's own form: float32, float16 beside bfloat16, fixed point beside float16
+// the slope's own form: float32, float16 beside bfloat16, 16 bits of its own beside float16
 at::ScalarType slope_type(const Tensor& x) {
   return x.scalar_type() == at::kFloat ? at::kFloat : x.scalar_type() == at::kBFloat16 ? at::kHalf : at::kShort;
 }

@@ -81,8 +81,8 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     ``"gelu"`` (``z Phi(z)``, by the error function) or ``"tanh"``. Rows of ``x`` may be strided.
 
     Where a gradient is wanted the forward pass keeps ``f'(z)`` (beside the 16-bit types in 16 bits of a form of its
-    own: off by 2^-11 of it in bfloat16, by 2^-15 of its root in float16), and the backward pass rounds ``d = grad f'(z)`` to ``x``'s type once, between
-    ``f'`` and the two products. float32 operands enter the products as three
+    own: off by 2^-11 of it at most down to 2^-29 in bfloat16; in float16 by 2^-14.8 of it near 1 and 2^-11 down to
+    2^-19), and the backward pass rounds ``d = grad f'(z)`` to ``x``'s type once, between ``f'`` and the two products. float32 operands enter the products as three
     planes of 8 bits: one that is not finite makes the outputs it reaches NaN."""
     code = _activation(activation)
     if is_compiling():
