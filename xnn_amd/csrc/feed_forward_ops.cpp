@@ -149,8 +149,8 @@ struct LayerNormBackward : Node {
     const bool wanted[] = {task_should_compute_output(0), task_should_compute_output(1),
                            task_should_compute_output(2)};
     at::AutoDispatchBelowADInplaceOrView below;            // no derivative of its own
-    const Three all = layer_norm_backward(grads[0], x.unpack(), maybe(weight.unpack()), stats.unpack(), wanted[0],
-                                          wanted[1], wanted[2]);
+    const Three all = layer_norm_backward(grads[0], x.unpack(), wanted[0] ? maybe(weight.unpack()) : MaybeTensor(),
+                                          stats.unpack(), wanted[0], wanted[1], wanted[2]);
     if (wanted[0]) out[0] = std::get<0>(all);
     if (wanted[1]) out[1] = std::get<1>(all);
     if (wanted[2]) out[2] = std::get<2>(all);
@@ -176,7 +176,7 @@ Tensor layer_norm_autograd(XNN_NORM_ARGUMENTS) {
   }
   auto node = node_of<LayerNormBackward>(x, w, b);
   node->x = SavedVariable(x, false);
-  node->weight = SavedVariable(w, false);
+  if (x.requires_grad()) node->weight = SavedVariable(w, false);   // of dx alone
   node->stats = SavedVariable(stats, false);
   set_history(out, node);
   return out;
