@@ -206,8 +206,13 @@ Tensor group_plan_kernel(const Tensor& ids_, int64_t n_groups) {
 }
 
 // as xnn_group_plan_size: the rows, where the groups begin, and fifty-two lists of their tiles
+constexpr int kPlanLists = 53;
 Tensor group_plan_shape(const Tensor& ids, int64_t n_groups) {
-  return at::empty_symint({ids.sym_numel() + 53 * (n_groups + 2)}, ids.options().dtype(at::kInt));
+  return at::empty_symint({ids.sym_numel() + kPlanLists * (n_groups + 2)}, ids.options().dtype(at::kInt));
+}
+template <typename N>
+N groups_of(const N& plan, const N& rows) {
+  return (plan - rows) / kPlanLists - 2;
 }
 
 // ---------------------------------------------------------------- dense layers
@@ -229,9 +234,10 @@ Two dense_slope(XNN_DENSE_ARGUMENTS) {
 }
 
 // the gradients of x, weight and bias; those that are not wanted are empty
-Three dense_backward(const Tensor& grad, const MaybeTensor& slope, const Tensor& x, const Tensor& weight,
+// (x is needed for the last two alone, weight for the first)
+Three dense_backward(const Tensor& grad, const MaybeTensor& slope, const MaybeTensor& x, const MaybeTensor& weight,
                      const MaybeTensor& plan, bool input, bool weights, bool biases) {
-  XNN_OPERATOR("dense_backward", Three(const Tensor&, const MaybeTensor&, const Tensor&, const Tensor&,
+  XNN_OPERATOR("dense_backward", Three(const Tensor&, const MaybeTensor&, const MaybeTensor&, const MaybeTensor&,
                                        const MaybeTensor&, bool, bool, bool));
   return op.call(grad, slope, x, weight, plan, input, weights, biases);
 }
@@ -246,6 +252,20 @@ struct Dense {
   int64_t rows, n_in, n_out, groups;
   std::vector<int64_t> out, bias;
 };
+
+void check_sizes(const Dense& d, const Tensor& plan) {
+  if (plan.defined()) {
+    TORCH_CHECK_VALUE(d.groups >= 1, "no groups");
+    size_t plan_bytes = 0, need = 0;
+    check("xnn_group_plan_size",
+          api.xnn_group_plan_size(d.rows, (int32_t)std::min<int64_t>(d.groups, 1 << 30), &plan_bytes, &need));
+    TORCH_CHECK_VALUE(plan.scalar_type() == at::kInt && plan.dim() == 1 && plan.is_contiguous() &&
+                          plan.size(0) == (int64_t)(plan_bytes / sizeof(int32_t)),
+                      "the plan is not of ", d.rows, " rows and ", d.groups, " groups");
+  }
+  TORCH_CHECK_VALUE(d.n_in < (1 << 20) && d.n_out < (1 << 20), "widths must be below 2^20, got ", d.n_in, " and ",
+                    d.n_out);
+}
 
 Dense check_dense(const Tensor& x, const Tensor& weight, const Tensor& plan) {
   check_rows(x);
@@ -265,17 +285,7 @@ Dense check_dense(const Tensor& x, const Tensor& weight, const Tensor& plan) {
   d.out.back() = d.n_out;
   if (lead) d.bias.push_back(d.groups);
   d.bias.push_back(d.n_out);
-  if (plan.defined()) {
-    TORCH_CHECK_VALUE(d.groups >= 1, "no groups");
-    size_t plan_bytes = 0, need = 0;
-    check("xnn_group_plan_size",
-          api.xnn_group_plan_size(d.rows, (int32_t)std::min<int64_t>(d.groups, 1 << 30), &plan_bytes, &need));
-    TORCH_CHECK_VALUE(plan.scalar_type() == at::kInt && plan.dim() == 1 && plan.is_contiguous() &&
-                          plan.size(0) == (int64_t)(plan_bytes / sizeof(int32_t)),
-                      "the plan is not of ", d.rows, " rows and ", d.groups, " groups");
-  }
-  TORCH_CHECK_VALUE(d.n_in < (1 << 20) && d.n_out < (1 << 20), "widths must be below 2^20, got ", d.n_in, " and ",
-                    d.n_out);
+  check_sizes(d, plan);
   return d;
 }
 
@@ -321,39 +331,74 @@ Two dense_slope_shape(XNN_DENSE_ARGUMENTS) {
   return {out, activation != XNN_NO_ACTIVATION ? at::empty_symint(out.sym_sizes(), options) : at::empty({0}, options)};
 }
 
-Three dense_backward_kernel(const Tensor& grad_, const MaybeTensor& slope_, const Tensor& x, const Tensor& weight,
-                            const MaybeTensor& plan, bool input, bool weights, bool biases) {
-  const Tensor slope = contiguous(slope_), p = or_none(plan);
-  check_tensors({&x, &grad_, &slope, &weight, &p});
-  const Dense d = check_dense(x, weight, p);
-  check_like(grad_, x, d.out, "the cotangent");
-  TORCH_CHECK_VALUE(!slope.defined() || (slope.sizes() == d.out && slope.scalar_type() == slope_type(x)),
-                    "the slope is not that of the forward pass");
+// the operation's sizes from the cotangent and one of x and the weight
+Dense check_one(const Tensor& grad, const Tensor& x, const Tensor& weight, const Tensor& plan) {
+  Dense d;
+  check_rows(grad);
+  if (x.defined()) check_rows(x);
+  TORCH_CHECK_VALUE(!weight.defined() || weight.dim() == (plan.defined() ? 3 : 2), "weight must be (",
+                    plan.defined() ? "groups, " : "", "inputs, outputs), got ", weight.sizes());
+  d.n_in = x.defined() ? x.size(-1) : weight.size(-2);
+  d.n_out = grad.size(-1);
+  d.rows = grad.numel() / d.n_out;
+  d.groups = !plan.defined() ? 1 : weight.defined() ? weight.size(0) : groups_of(plan.numel(), d.rows);
+  d.out = grad.sizes().vec();
+  if (plan.defined()) d.bias.push_back(d.groups);
+  d.bias.push_back(d.n_out);
+  check_sizes(d, plan);
+  return d;
+}
+
+Three dense_backward_kernel(const Tensor& grad_, const MaybeTensor& slope_, const MaybeTensor& x_,
+                            const MaybeTensor& weight_, const MaybeTensor& plan, bool input, bool weights,
+                            bool biases) {
+  const Tensor slope = contiguous(slope_), p = or_none(plan), x = or_none(x_), weight = or_none(weight_);
+  check_tensors({&grad_, &x, &slope, &weight, &p});
   weights = weights || biases;                             // the weight's product has the bias's sums
-  const c10::DeviceGuard guard(x.device());
-  const Tensor rows = as_rows(x), w = weight.contiguous(), grad = grad_.contiguous();
-  const Tensor dx = empty_if(input, x.sizes(), x), dw = empty_if(weights, weight.sizes(), x),
-               db = empty_if(biases, d.bias, x);
+  TORCH_CHECK_VALUE(x.defined() || !weights, "the weight's and the bias's gradients need x");
+  TORCH_CHECK_VALUE(weight.defined() || !input, "x's gradient needs the weight");
+  const int code = storage_code(grad_);
+  if (!input && !weights) return {empty_if(false, {}, grad_), empty_if(false, {}, grad_), empty_if(false, {}, grad_)};
+  const Dense d = x.defined() && weight.defined() ? check_dense(x, weight, p) : check_one(grad_, x, weight, p);
+  std::vector<int64_t> in = d.out, shape = d.bias;
+  in.back() = d.n_in;
+  shape.insert(shape.end() - 1, d.n_in);
+  check_like(grad_, x.defined() ? x : weight, d.out, "the cotangent");
+  TORCH_CHECK_VALUE(!x.defined() || x.sizes() == in, "x must be ", in, ", got ", x.sizes());
+  TORCH_CHECK_VALUE(!weight.defined() || weight.sizes() == shape, "weight must be ", shape, ", got ", weight.sizes());
+  TORCH_CHECK_VALUE(!slope.defined() || (slope.sizes() == d.out && slope.scalar_type() == slope_type(grad_)),
+                    "the slope is not that of the forward pass");
+  const c10::DeviceGuard guard(grad_.device());
+  const Tensor rows = x.defined() ? as_rows(x) : Tensor(), w = contiguous(weight_), grad = grad_.contiguous();
+  const Tensor dx = empty_if(input, in, grad), dw = empty_if(weights, shape, grad), db = empty_if(biases, d.bias, grad);
   Tensor work;
   size_t need = 0;
   check("xnn_linear_backward_work_size",
-        api.xnn_linear_backward_work_size(storage_code(x), d.rows, (int32_t)d.n_in, (int32_t)d.n_out,
-                                          (int32_t)d.groups, p.defined(), slope.defined(), input, weights, biases,
-                                          &need));
-  if (need > 0) work = bytes(x, need);
-  XNN_CALL(xnn_linear_backward, storage_code(x), data(grad), data(slope), data(rows), row_stride(rows), d.rows,
-           (int32_t)d.n_in, (int32_t)d.n_out, data(w), (const int32_t*)data(p), (int32_t)d.groups,
-           data_if(input, dx), data_if(weights, dw), data_if(biases, db), data(work), need, stream_of(x));
+        api.xnn_linear_backward_work_size(code, d.rows, (int32_t)d.n_in, (int32_t)d.n_out, (int32_t)d.groups,
+                                          p.defined(), slope.defined(), input, weights, biases, &need));
+  if (need > 0) work = bytes(grad, need);
+  XNN_CALL(xnn_linear_backward, code, data(grad), data(slope), data(rows), x.defined() ? row_stride(rows) : d.n_in,
+           d.rows, (int32_t)d.n_in, (int32_t)d.n_out, data(w), (const int32_t*)data(p), (int32_t)d.groups,
+           data_if(input, dx), data_if(weights, dw), data_if(biases, db), data(work), need, stream_of(grad));
   return {dx, dw, db};
 }
 
-Three dense_backward_shape(const Tensor&, const MaybeTensor&, const Tensor& x, const Tensor& weight,
-                           const MaybeTensor& plan, bool input, bool weights, bool biases) {
-  std::vector<c10::SymInt> bias;
-  if (or_none(plan).defined()) bias.push_back(weight.sym_size(0));
-  bias.push_back(weight.sym_size(-1));
-  return {empty_shape(input, x), empty_shape(weights || biases, weight),
-          biases ? at::empty_symint(bias, x.options()) : at::empty({0}, x.options())};
+Three dense_backward_shape(const Tensor& grad, const MaybeTensor&, const MaybeTensor& x_, const MaybeTensor& weight_,
+                           const MaybeTensor& plan_, bool input, bool weights, bool biases) {
+  const Tensor x = or_none(x_), weight = or_none(weight_), plan = or_none(plan_);
+  const auto none = [&] { return at::empty({0}, grad.options()); };
+  if (!x.defined() && !weight.defined()) return {none(), none(), none()};
+  const c10::SymInt n_in = x.defined() ? x.sym_size(-1) : weight.sym_size(-2);
+  std::vector<c10::SymInt> bias, in = grad.sym_sizes().vec();
+  if (plan.defined())
+    bias.push_back(weight.defined() ? weight.sym_size(0) : groups_of(plan.sym_numel(), rows_of(grad)));
+  bias.push_back(grad.sym_size(-1));
+  std::vector<c10::SymInt> shape = bias;
+  shape.insert(shape.end() - 1, n_in);
+  in.back() = n_in;
+  return {input ? at::empty_symint(in, grad.options()) : none(),
+          weights || biases ? at::empty_symint(shape, grad.options()) : none(),
+          biases ? at::empty_symint(bias, grad.options()) : none()};
 }
 
 struct DenseBackward : Node {
@@ -368,8 +413,11 @@ struct DenseBackward : Node {
     if (!wanted[0] && !wanted[1] && !wanted[2]) return out;
     once_differentiable();
     at::AutoDispatchBelowADInplaceOrView below;            // no derivative of its own
-    const Three all = dense_backward(grads[0], maybe(slope.unpack()), x.unpack(), weight.unpack(),
-                                     maybe(plan.unpack()), wanted[0], wanted[1], wanted[2]);
+    // (unpacking asks whether a tensor was written to: only of those that these gradients need)
+    const Three all = dense_backward(grads[0], maybe(slope.unpack()),
+                                     wanted[1] || wanted[2] ? maybe(x.unpack()) : MaybeTensor(),
+                                     wanted[0] ? maybe(weight.unpack()) : MaybeTensor(), maybe(plan.unpack()),
+                                     wanted[0], wanted[1], wanted[2]);
     if (wanted[0]) out[0] = std::get<0>(all);
     if (wanted[1]) out[1] = std::get<1>(all);
     if (wanted[2]) out[2] = std::get<2>(all);
@@ -395,8 +443,8 @@ Tensor dense_autograd(XNN_DENSE_ARGUMENTS) {
   }
   if (!wanted({&x, &weight, &b, &r})) return out;
   auto node = node_of<DenseBackward>(x, weight, b, r);
-  node->x = SavedVariable(x, false);
-  node->weight = SavedVariable(weight, false);
+  if (wanted({&weight, &b})) node->x = SavedVariable(x, false);
+  if (x.requires_grad()) node->weight = SavedVariable(weight, false);
   node->slope = SavedVariable(slope, false);
   node->plan = SavedVariable(p, false);
   set_history(out, node);
@@ -426,7 +474,7 @@ TORCH_LIBRARY_FRAGMENT(xnn_amd, m) {
   m.def("group_plan(Tensor ids, int n_groups) -> Tensor");
   m.def("dense(" XNN_DENSE_SCHEMA ") -> Tensor");
   m.def("dense_slope(" XNN_DENSE_SCHEMA ") -> (Tensor, Tensor)");
-  m.def("dense_backward(Tensor grad, Tensor? slope, Tensor x, Tensor weight, Tensor? plan, bool input, "
+  m.def("dense_backward(Tensor grad, Tensor? slope, Tensor? x, Tensor? weight, Tensor? plan, bool input, "
         "bool weights, bool biases) -> (Tensor, Tensor, Tensor)");
 }
 
