@@ -236,7 +236,7 @@ class AtomFeedForward(nn.Module, FastPathModule):
         self.down, self.down_bias = weight(hidden, channels), nn.Parameter(torch.zeros(*lead, channels))
 
     def fast_supported(self, device: torch.device, dtype: torch.dtype) -> bool:
-        return (_takes(device, dtype) and self.norm_weight.shape[0] <= 16384
+        return (_takes(device, dtype) and self.norm_weight.shape[0] <= 16384 and self.up.shape[-1] < 1 << 20
                 and (self.n_species is None or self.n_species <= 4096))
 
     def forward(self, x: Tensor, z: Optional[Tensor] = None, plan: Optional[GroupPlan] = None,
