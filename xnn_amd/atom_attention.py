@@ -99,10 +99,11 @@ def linear_torch(x: Tensor, weight: Tensor, bias: Tensor, activation: Optional[s
 
 def grouped_linear_torch(x: Tensor, weight: Tensor, ids: Tensor, bias: Tensor, activation: Optional[str],
                          residual: Optional[Tensor] = None) -> Tensor:
-    """The rows of each group that has some with its weight."""
+    """The rows of each group that has some with its weight; NaN for those of no group."""
     order = torch.argsort(ids, stable=True)
     groups, counts = torch.unique(ids, return_counts=True)
-    parts = [_ACTIVATIONS[activation](x[rows] @ weight[g] + bias[g])
+    parts = [_ACTIVATIONS[activation](x[rows] @ weight[g] + bias[g]) if 0 <= g < weight.shape[0]
+             else x.new_full((len(rows), weight.shape[2]), float("nan"), dtype=(x[:0] @ weight[0]).dtype)
              for g, rows in zip(groups.tolist(), order.split(counts.tolist()))]
     y = torch.cat(parts)[torch.argsort(order)] if parts else x @ weight[0]
     return y if residual is None else residual + y
