@@ -83,7 +83,8 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     Where a gradient is wanted the forward pass keeps ``f'(z)`` (beside the 16-bit types in 16 bits of a form of its
     own: off by 2^-11 of it at most down to 2^-29 in bfloat16; in float16 by 2^-14.8 of it near 1 and 2^-11 down to
     2^-19), and the backward pass rounds ``d = grad f'(z)`` to ``x``'s type once, between ``f'`` and the two products. float32 operands enter the products as three
-    planes of 8 bits: one that is not finite makes the outputs it reaches NaN."""
+    planes of 8 bits: one that is not finite makes the outputs it reaches NaN (the forward pass of one or two rows of
+    up to 1,500 inputs multiplies in float32, and gives infinities where that does)."""
     code = _activation(activation)
     if is_compiling():
         return torch.ops.xnn_amd.dense(x, weight, bias, code, residual, None)
