@@ -13,8 +13,8 @@
 // dW reads both operands across their rows, by the transposing read, with a tenth of the LDS conflicts), of the
 // pass memory (24,000 x 4,096 in bfloat16, 590 MB in 137 us: 4.3 TB/s), of short reductions what is around the
 // products (72,000 rows of 128 -> 512 in float32, two species: dx 97 to 116 us, dW 77 to 86, join 10). Weights of
-// 64 uneven groups (16,384 rows, 1,024 x 1,024 in bfloat16): with the join 103, for the 134 MB of their gradient and the
-// parts' sums.
+// 64 uneven groups (16,384 rows, 1,024 x 1,024 in bfloat16): with the join 98 to 106 back to back, 115 to 124 within a step, whose
+// other kernels have the caches; 134 MB of gradients, and the parts' sums.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -349,18 +349,20 @@ static BackwardPlan backward_plan(int dtype, int64_t n_rows, int32_t n_in, int32
     // The tiles and the number of parts with the least time, estimated from the rates of large products (kinds 0,
     // 1, 2: microseconds of 64 rows of a tile with all of a CU's blocks at work, and those blocks) and the parts'
     // sums, written and read at 4 TB/s. Parts of one length come in rounds; those of groups, of any, fill the card
-    // but for about one long one's time and a half at its end. Weights of groups take tiles of up to 128 x 128, wide ones those, three
-    // blocks a CU, of which others work while one looks up its rows (16,384 rows, 1,024 x 1,024 in bfloat16, with the
-    // join: 64 uneven groups 103 us, 256 x 128 117; four even ones 88 and 114; 32,768 in eight, 4,096 x 4,096: 2,015
-    // and 2,270).
-    static const double step16[] = {0.9, 1.4, 2.2}, step32[] = {2.9, 5.4, 0.0};
+    // but for about one long one's time and a half at its end. Weights of groups take tiles of up to 128 x 128 (256 x 128
+    // cost 14 % at 64 uneven groups, 30 % at four even ones). 64 x 64 tiles of groups cost a third more than of one
+    // weight, for each looks up its rows: bfloat16, with the join, 64 x 64 and 128 x 128 (chosen: *) of 5,000 rows of
+    // four species, 256 -> 128 10.8* and 13.7 us, 256 -> 512 20.7 and 19.5*; 72,000 of two, 256 -> 128 33 and 27*, 512 ->
+    // 512 120 and 78*; 16,384 of 64 uneven groups 128 -> 128 12.8* and 14.9, 256 -> 128 18.6* and 17.3, 1,024 -> 1,024
+    // 147 and 98*. Of one weight 40 sizes from 21 x 128 -> 128 to 72,000 x 2,048 -> 2,048 take the better kind or one within
+    // 4 %. (In 16 bits a third block of 128 x 128 fits a CU; the step counted is that of two, which it does not change.)
+    static const double step16[] = {0.9, 1.4, 2.2}, step32[] = {2.9, 5.4, 0.0}, grouped16 = 1.2;
     static const int per_cu[] = {3, 2, 2}, bm[] = {64, 128, 256}, bn[] = {64, 128, 128};
     const double sums = (double)n_in * n_out * 8 / 4e6;
     double best = 0.0;
     for (int kind = 0; kind < (size == 2 && !grouped && !(slope && n_in <= kFormInProducts) ? 3 : 2); ++kind) {
-      if (grouped && size == 2 && kind == kTile64 && n_in >= 256 && n_out >= 128) continue;
       const double t = (double)tiles(bm[kind], bn[kind]), blocks = 256.0 * per_cu[kind];
-      const double step = size == 2 ? step16[kind] : step32[kind];
+      const double step = size == 4 ? step32[kind] : grouped && kind == kTile64 ? grouped16 : step16[kind];
       for (int64_t want = 1; want <= 1024; want += std::max<int64_t>(1, want / 4)) {
         const Parts parts = parts_of(n_rows, grouped, want, 256);
         const double n = (double)row_tiles(n_rows, 0, false, parts.rows), all = n + (grouped ? n_groups / 2 : 0);
