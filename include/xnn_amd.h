@@ -1314,6 +1314,16 @@ int xnn_linear_backward_work_size(int dtype, int64_t n_rows, int32_t n_in, int32
                                   int32_t grouped, int32_t slope, int32_t input, int32_t weight, int32_t bias,
                                   size_t* bytes);
 
+/* What calls of these sizes run, for tests and measurements: rows of a tile (64, 128 or 256; 0: the
+ * stream of the weight that few rows take) and parts of the reduction (of a weight's, at most) of the
+ * forward pass, of dx and of dweight, the rows of a part of dweight's, and whether a pass of its own
+ * forms the activation's cotangent. */
+typedef struct {
+  int32_t forward_tile, forward_parts, input_tile, input_parts, weight_tile, weight_parts, weight_rows, pass;
+} xnn_linear_variant;
+int xnn_linear_variants(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, int32_t n_groups,
+                        int32_t grouped, int32_t slope, xnn_linear_variant* out);
+
 /* Gradients for the cotangent `grad` (n_rows, n_out), contiguous: dx (n_rows, n_in; zero in rows of no
  * group), dweight and dbias as weight and bias (zero for a group without rows), each of which may be
  * NULL (dbias with dweight only). slope: the forward pass's, NULL

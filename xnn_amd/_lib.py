@@ -297,6 +297,7 @@ _SIGNATURES = {
     "xnn_linear_work_size": [c_int, i64, i32, i32, i32, i32, vp],
     "xnn_linear": [c_int, vp, i64, i64, i32, i32, vp, vp, i32, vp, vp, i32, vp, vp, vp, sz, vp],
     "xnn_linear_backward_work_size": [c_int, i64, i32, i32, i32, i32, i32, i32, i32, i32, vp],
+    "xnn_linear_variants": [c_int, i64, i32, i32, i32, i32, i32, vp],
     "xnn_linear_backward": [c_int, vp, vp, vp, i64, i64, i32, i32, vp, vp, i32, vp, vp, vp, vp, sz, vp],
 }
 _RESTYPES = {"xnn_last_error": ctypes.c_char_p, "xnn_scan_workspace_bytes": sz,

@@ -68,14 +68,7 @@ static void forward_launch(ForwardArgs p, const int32_t* plan, int n_groups, hip
 // weight, sixteen of them in flight before the first is used; x lies in LDS as float32. The sums of
 // the threads of a column are added across lanes and then waves, in a fixed order. float32 products are float32's
 // own here.
-//
-// Against tiles, whose reduction is cut into parts that all CUs take (one row, 1,024 outputs): 1,024 inputs in bfloat16
-// 5.7 us, tiles 10.5, in float32 5.4 and 7.3; 1,500 inputs 7.0 and 7.4, 6.6 and 8.3; 2,048 8.3 and 7.2, 7.8 and 8.9;
-// 4,096 13.3 and 8.4, 19.1 and 12.3. Two rows cost 1 us more, tiles the same; of three (accumulators for four) 1,024
-// inputs take 8.4 us in bfloat16 and 7.1 in float32, tiles 10.5 and 7.3, but 128 inputs 5.9 and tiles 4.2.
 constexpr int kFewThreads = 512;
-constexpr int kMaxFew = 2, kMaxFewInputs = 1500;
-static bool few_rows(int64_t n_rows, int32_t n_in) { return n_rows <= kMaxFew && n_in <= kMaxFewInputs; }
 
 // x[j] += x[j] of the lanes at distances from, 2 from, ... 32
 template <int N>

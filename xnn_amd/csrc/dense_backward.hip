@@ -472,6 +472,24 @@ int xnn_linear_backward_work_size(int dtype, int64_t n_rows, int32_t n_in, int32
   return XNN_OK;
 }
 
+int xnn_linear_variants(int dtype, int64_t n_rows, int32_t n_in, int32_t n_out, int32_t n_groups, int32_t grouped,
+                        int32_t slope, xnn_linear_variant* out) {
+  static const int32_t some = 0;
+  const int status = dense_sizes(dtype, n_rows, n_in, n_out, &some, n_groups);
+  if (status != XNN_OK) return status;
+  XNN_REQUIRE(n_rows > 0, "no rows");
+  XNN_REQUIRE(out != nullptr, "NULL variant");
+  const size_t size = storage_bytes(dtype);
+  const bool few = few_rows(n_rows, n_in);
+  const int kind = dense_tile(size, n_rows, n_out, grouped ? n_groups : 0);
+  const BackwardPlan b =
+      backward_plan(dtype, n_rows, n_in, n_out, n_groups, grouped != 0, slope != 0, true, true, true);
+  *out = xnn_linear_variant{few ? 0 : 64 << kind, few ? 1 : dense_split(size, kind, n_rows, n_out, n_in).parts,
+                            64 << b.input_kind, b.split.parts, 64 << b.kind,
+                            (int32_t)row_tiles(n_rows, n_groups, grouped != 0, b.weight.rows), b.weight.rows, b.pass};
+  return XNN_OK;
+}
+
 int xnn_linear_backward(int dtype, const void* grad, const void* slope, const void* x, int64_t x_stride,
                         int64_t n_rows, int32_t n_in, int32_t n_out, const void* weight, const int32_t* plan,
                         int32_t n_groups, void* dx, void* dweight, void* dbias, void* work,
