@@ -32,6 +32,7 @@ from torch import Tensor
 from torch.compiler import is_compiling
 
 from . import _lib
+from .plan import capturing, hold_captured
 
 _native, _failure = None, None
 try:
@@ -172,12 +173,14 @@ def attention_plan(n_atoms: Tensor, n_tokens: Optional[int] = None) -> Attention
 
 def plan_for(graph) -> AttentionPlan:
     """The cached plan of an :class:`~xnn_amd.data.AtomicGraph` (made again when ``n_atoms`` is another tensor
-    or was written to, or the number of atoms changes)."""
+    or was written to, or the number of atoms changes). One that a capture takes stays as long as ``n_atoms``."""
     n_atoms = graph.n_atoms
     version = None if n_atoms.is_inference() else n_atoms._version
     key = (version, graph.num_nodes)
     cached = getattr(graph, "_xnn_attention_plan", None)
     if cached is not None and cached[0] is n_atoms and cached[1] == key:
+        if capturing(n_atoms.device):
+            hold_captured(n_atoms, cached[2])
         return cached[2]
     plan = attention_plan(n_atoms, graph.num_nodes)
     object.__setattr__(graph, "_xnn_attention_plan", (n_atoms, key, plan))

@@ -28,6 +28,7 @@ from torch import Tensor
 from torch.compiler import is_compiling
 
 from . import _lib
+from .plan import capturing, hold_captured
 
 _native, _failure = None, None
 try:
@@ -122,13 +123,6 @@ class _KeptPlans:
         return _KeptPlans, ()
 
 
-class _CapturedPlans(list):
-    """Plans that captured graphs write and read, held by their species as long as those are there."""
-
-    def __reduce__(self):
-        return _CapturedPlans, ()
-
-
 def _form_again(plan: GroupPlan, ids: Tensor) -> None:
     """``plan`` formed in its own memory once more (from other ids, of another content)."""
     ids = ids.to(torch.int64).contiguous()
@@ -151,21 +145,18 @@ def species_plan_for(graph, n_groups: int) -> GroupPlan:
     ids = graph.atomic_numbers
     if not ids.is_cuda or ids.is_inference():
         return group_plan(ids, n_groups)                   # (refused on a CPU)
-    with torch.cuda.device(ids.device):
-        capturing = torch.cuda.is_current_stream_capturing()
+    captured = capturing(ids.device)
     kept = getattr(graph, "_xnn_species_plan", None)
     if kept is None or kept.ids is not ids or kept.version != ids._version:
         kept = _KeptPlans(ids, ids._version)
-        if not capturing:
+        if not captured:
             object.__setattr__(graph, "_xnn_species_plan", kept)
-    if capturing:
+    if captured:
         key = next((k for k in kept.plans if k[1] == n_groups), None)
         if key is None:
             return group_plan(ids, n_groups)
         plan = kept.plans.pop(key)
-        if not hasattr(ids, "_xnn_captured_plans"):
-            ids._xnn_captured_plans = _CapturedPlans()
-        ids._xnn_captured_plans.append(plan)
+        hold_captured(ids, plan)
         _form_again(plan, ids)
         return plan
     key = (torch.cuda.current_stream(ids.device).cuda_stream, int(n_groups))

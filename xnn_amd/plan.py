@@ -26,6 +26,26 @@ from torch import Tensor
 from . import _lib
 
 
+def capturing(device: torch.device) -> bool:
+    """Whether the current stream of ``device`` captures a HIP graph."""
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
+class _CapturedPlans(list):
+    """Not copied or pickled with the tensor that has it."""
+
+    def __reduce__(self):
+        return _CapturedPlans, ()
+
+
+def hold_captured(tensor: Tensor, plan) -> None:
+    """Keeps ``plan``, whose memory captured kernels use, as long as the ``tensor`` that it is of."""
+    held = tensor.__dict__.setdefault("_xnn_captured_plans", _CapturedPlans())
+    if not any(p is plan for p in held):
+        held.append(plan)
+
+
 @dataclass
 class EdgePlan:
     n_nodes: int
