@@ -239,8 +239,9 @@ __device__ __forceinline__ void activate(int kind, float z, float& y, float& slo
 // coarser than the type where it is small (a loss scale makes such d large):
 //   |f'| >= 2^-7   its root in steps of 1 / 30,000, off by 2^-14.8 root(f'): 2^-14.8 of it near 1, 2^-11.3 at 2^-7
 //   below          2^5 times it in float16, off by 2^-11 of it down to 2^-19, by 2^-30 below
-// Of 65,536 numbers the first 13,313 are the float16 ones, then roots up to 1.13's; a negative f', whose root is below
-// 0.36, has the complement of its size's number, and what is between the two ends stands for NaN.
+// Of 65,536 numbers, counted from one for zero, 13,312 are the float16 ones and then the roots up to 1.13's above it, and as
+// many and the roots up to 0.13's below (no f' is less); the last one stands for NaN. (Both passes of 72,000 x 128 -> 512 with
+// silu 153 us, 139 with the root alone, which was off by 0.4 % for silu at z = -12 and by 5 % for tanh at 8.)
 template <typename T>
 struct Slope {
   typedef T type;
@@ -257,9 +258,9 @@ constexpr float kSlopeScale = 32768.0f;
 constexpr float kSlopeUnit = 30000.0f, kSlopeFine = 0x1p-7f, kSlopeFineScale = 32.0f;
 constexpr int kSlopeFineLast = 0x3400;             // 2^5 2^-7 in float16
 constexpr int kSlopeRoots = 10662;                 // the root of 2^-7, 2,652 steps, comes after it
-constexpr int kSlopeNan = 43000;
-static_assert(kSlopeRoots + 2652 == kSlopeFineLast + 2 && kSlopeRoots + 31950 < kSlopeNan &&
-                  65535 - (kSlopeRoots + 10850) > kSlopeNan, "");
+constexpr int kSlopeZero = 21600, kSlopeNan = 65535;
+static_assert(kSlopeRoots + 2652 == kSlopeFineLast + 2 && kSlopeZero + kSlopeRoots + 31950 < kSlopeNan &&
+                  kSlopeZero > kSlopeRoots + 10850, "");
 template <typename T>
 __device__ __forceinline__ typename Slope<T>::type slope_stored(float s) {
   if constexpr (sizeof(T) == 4)
@@ -271,7 +272,7 @@ __device__ __forceinline__ typename Slope<T>::type slope_stored(float s) {
     const int fine = __builtin_bit_cast(uint16_t, (f16_t)(a * kSlopeFineScale));
     const int root = kSlopeRoots + __float2int_rn(kSlopeUnit * __builtin_amdgcn_sqrtf(a));
     const int n = a < kSlopeFine ? fine : root;
-    return (uint16_t)(s == s ? (s < 0.0f ? ~n : n) : kSlopeNan);
+    return (uint16_t)(s == s ? kSlopeZero + (s < 0.0f ? -n : n) : kSlopeNan);
   }
 }
 template <typename T>
@@ -281,12 +282,11 @@ __device__ __forceinline__ float slope_value(typename Slope<T>::type s) {
   else if constexpr (__is_same(T, bf16_t))
     return (float)s * (1.0f / kSlopeScale);
   else {
-    const bool negative = s > kSlopeNan;
-    const uint16_t n = negative ? (uint16_t)~s : s;
-    const float root = (float)((int)n - kSlopeRoots) * (1.0f / kSlopeUnit);
-    const float fine = (float)__builtin_bit_cast(f16_t, n) * (1.0f / kSlopeFineScale);
-    const float a = n <= kSlopeFineLast ? fine : root * root;
-    return s == kSlopeNan ? __builtin_nanf("") : negative ? -a : a;
+    const float m = (float)s - (float)kSlopeZero, a = fabsf(m);
+    const float root = fmaf(a, 1.0f / kSlopeUnit, -kSlopeRoots / kSlopeUnit);
+    const float fine = (float)__builtin_bit_cast(f16_t, (uint16_t)a) * (1.0f / kSlopeFineScale);
+    const float f = copysignf(a <= (float)kSlopeFineLast ? fine : root * root, m);
+    return m > (float)(kSlopeNan - kSlopeZero - 1) ? __builtin_nanf("") : f;
   }
 }
 
