@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from xnn_amd import attention
+from xnn_amd.plan import captured_plans, hold_captured
 
 
 class Thing:
@@ -41,5 +42,28 @@ def test_a_plan_that_a_capture_takes_lives_on(monkeypatch, act):
         graph.n_atoms._version += 1
     attention.plan_for(graph)
     gc.collect()
-    assert plan() is not None and len(graph.n_atoms._xnn_captured_plans) == 1
-    assert not copy.deepcopy(graph).n_atoms._xnn_captured_plans
+    assert plan() is not None and len(captured_plans(graph.n_atoms)) == 1
+    assert not captured_plans(copy.deepcopy(graph).n_atoms)
+    del graph
+    gc.collect()
+    assert plan() is None
+
+
+def test_a_tensor_that_plans_are_held_for_is_saved_as_any_other():
+    import io
+    counts = torch.tensor([3, 4])
+    hold_captured(counts, Thing())
+    file = io.BytesIO()
+    torch.save(counts, file)
+    file.seek(0)
+    assert torch.equal(torch.load(file, weights_only=True), counts) and not captured_plans(torch.tensor([3, 4]))
+    # an object of Python that went and came back, the tensor having stayed
+    plan = weakref.ref(captured_plans(counts)[0])
+    holder = torch.nn.Module()
+    holder.register_buffer("counts", counts)
+    del counts
+    gc.collect()
+    assert captured_plans(holder.counts)[0] is plan()
+    del holder
+    gc.collect()
+    assert plan() is None

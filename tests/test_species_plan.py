@@ -89,8 +89,13 @@ def test_a_replay_follows_the_atomic_numbers_whether_a_plan_was_kept_or_not(card
     assert FF.species_plan_for(graph, 9) is kept and not card.again
     _captured(graph, card)
     assert len(card.again) == 1 and card.again[0] is kept
-    # the replays write to that one: calls outside them have another
-    assert FF.species_plan_for(graph, 9) is not kept
+    # the replays write to that one: calls outside them have another, and so has a second capture, of its own
+    other = FF.species_plan_for(graph, 9)
+    assert other is not kept
+    made = card.made
+    for _ in range(3):
+        assert _captured(graph, card)() is not other.rows
+    assert card.made == made + 3 and len(card.again) == 1 and FF.species_plan_for(graph, 9) is other
 
 
 def test_a_plan_of_numbers_that_were_written_to_is_not_taken_by_a_capture(card):

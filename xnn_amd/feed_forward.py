@@ -28,7 +28,7 @@ from torch import Tensor
 from torch.compiler import is_compiling
 
 from . import _lib
-from .plan import capturing, hold_captured
+from .plan import captured_plans, capturing, hold_captured
 
 _native, _failure = None, None
 try:
@@ -140,8 +140,8 @@ def species_plan_for(graph, n_groups: int) -> GroupPlan:
     does not tell, at every call).
 
     What a capture uses is formed in it, so that each replay follows the atomic numbers as they are then: a new plan
-    in the captured graph's memory, or a kept one in its own, which serves no later call and stays as long as the
-    species that the captured kernels read."""
+    in the captured graph's memory, or, the first time, a kept one in its own, which serves no later call and stays as
+    long as the species that the captured kernels read."""
     ids = graph.atomic_numbers
     if not ids.is_cuda or ids.is_inference():
         return group_plan(ids, n_groups)                   # (refused on a CPU)
@@ -153,7 +153,7 @@ def species_plan_for(graph, n_groups: int) -> GroupPlan:
             object.__setattr__(graph, "_xnn_species_plan", kept)
     if captured:
         key = next((k for k in kept.plans if k[1] == n_groups), None)
-        if key is None:
+        if key is None or any(p.n_groups == n_groups for p in captured_plans(ids)):
             return group_plan(ids, n_groups)
         plan = kept.plans.pop(key)
         hold_captured(ids, plan)

@@ -22,6 +22,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.utils.weak import WeakIdKeyDictionary
 
 from . import _lib
 
@@ -32,16 +33,19 @@ def capturing(device: torch.device) -> bool:
         return torch.cuda.is_current_stream_capturing()
 
 
-class _CapturedPlans(list):
-    """Not copied or pickled with the tensor that has it."""
+# plans whose memory captured kernels use, by the tensors that they are of (beside them: what is pickled with a tensor
+# stays what it was)
+_captured = WeakIdKeyDictionary()
 
-    def __reduce__(self):
-        return _CapturedPlans, ()
+
+def captured_plans(tensor: Tensor) -> list:
+    """The plans of ``tensor`` that captured kernels use."""
+    return _captured.get(tensor, [])
 
 
 def hold_captured(tensor: Tensor, plan) -> None:
     """Keeps ``plan``, whose memory captured kernels use, as long as the ``tensor`` that it is of."""
-    held = tensor.__dict__.setdefault("_xnn_captured_plans", _CapturedPlans())
+    held = _captured.setdefault(tensor, [])
     if not any(p is plan for p in held):
         held.append(plan)
 
