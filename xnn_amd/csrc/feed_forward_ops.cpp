@@ -148,9 +148,10 @@ struct LayerNormBackward : Node {
     if (!grads[0].defined()) return out;
     const bool wanted[] = {task_should_compute_output(0), task_should_compute_output(1),
                            task_should_compute_output(2)};
+    // unpacked first: a checkpoint computes the forward pass again then, with its derivatives
+    const Tensor x_ = x.unpack(), weight_ = wanted[0] ? weight.unpack() : Tensor(), stats_ = stats.unpack();
     at::AutoDispatchBelowADInplaceOrView below;            // no derivative of its own
-    const Three all = layer_norm_backward(grads[0], x.unpack(), wanted[0] ? maybe(weight.unpack()) : MaybeTensor(),
-                                          stats.unpack(), wanted[0], wanted[1], wanted[2]);
+    const Three all = layer_norm_backward(grads[0], x_, maybe(weight_), stats_, wanted[0], wanted[1], wanted[2]);
     if (wanted[0]) out[0] = std::get<0>(all);
     if (wanted[1]) out[1] = std::get<1>(all);
     if (wanted[2]) out[2] = std::get<2>(all);
@@ -412,12 +413,13 @@ struct DenseBackward : Node {
     if (task_should_compute_output(3)) out[3] = grads[0];
     if (!wanted[0] && !wanted[1] && !wanted[2]) return out;
     once_differentiable();
+    // Unpacked first: a checkpoint computes the forward pass again then, with its derivatives. (Unpacking asks whether a
+    // tensor was written to: only of those that these gradients need.)
+    const Tensor slope_ = slope.unpack(), plan_ = plan.unpack();
+    const Tensor x_ = wanted[1] || wanted[2] ? x.unpack() : Tensor(), weight_ = wanted[0] ? weight.unpack() : Tensor();
     at::AutoDispatchBelowADInplaceOrView below;            // no derivative of its own
-    // (unpacking asks whether a tensor was written to: only of those that these gradients need)
-    const Three all = dense_backward(grads[0], maybe(slope.unpack()),
-                                     wanted[1] || wanted[2] ? maybe(x.unpack()) : MaybeTensor(),
-                                     wanted[0] ? maybe(weight.unpack()) : MaybeTensor(), maybe(plan.unpack()),
-                                     wanted[0], wanted[1], wanted[2]);
+    const Three all = dense_backward(grads[0], maybe(slope_), maybe(x_), maybe(weight_), maybe(plan_), wanted[0],
+                                     wanted[1], wanted[2]);
     if (wanted[0]) out[0] = std::get<0>(all);
     if (wanted[1]) out[1] = std::get<1>(all);
     if (wanted[2]) out[2] = std::get<2>(all);
