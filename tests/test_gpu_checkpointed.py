@@ -50,3 +50,21 @@ def test_a_feed_forward_block(species):
     block.fast_active = True
     z = torch.tensor([1, 6, 7, 8], device=DEV)[torch.arange(40, device=DEV) % 4]
     _same(lambda x: block(x, z), (_normal(40, 12),), False)
+
+
+def _attention(name):
+    plan = xa.attention_plan(torch.tensor([17, 3, 20], device=DEV)) if name == "structure_attention" else None
+    ids = torch.arange(40, device=DEV) % 5
+    phase = torch.linspace(0, 3, 160, device=DEV).view(40, 4)
+    return {"structure_attention": (lambda q, k, v: xa.structure_attention(q, k, v, plan),
+                                    (_normal(40, 4, 8), _normal(40, 2, 8), _normal(2, 40, 8).transpose(0, 1))),
+            "head_norm_rotate": (lambda q, k, a, b: torch.cat(xa.head_norm_rotate(q, k, a, b, phase.cos(), phase.sin()), 1),
+                                 (_normal(40, 4, 8), _normal(40, 2, 8), _normal(8), _normal(1, 8)[0])),
+            "embedding": (lambda w: xa.embedding(ids, w), (_normal(5, 12),)),
+            "dropout_add": (lambda x, r: xa.dropout_add(x, r, 0.3, 7, 11), (_normal(40, 12), _normal(1, 40, 12)[0]))}[name]
+
+
+@pytest.mark.parametrize("name", ["structure_attention", "head_norm_rotate", "embedding", "dropout_add"])
+@pytest.mark.parametrize("use_reentrant", [False, True])
+def test_attention(name, use_reentrant):
+    _same(*_attention(name), use_reentrant)

@@ -557,10 +557,12 @@ struct AttentionBackward : Node {
     once_differentiable();
     variable_list result(3);
     if (!grads[0].defined()) return result;
+    // unpacked first: a checkpoint computes the forward pass again then, with its derivatives
+    const Tensor out_ = out.unpack(shared_from_this()), lse_ = lse.unpack(), q_ = q.unpack(), k_ = k.unpack(),
+                 v_ = v.unpack(), t32 = tiles32.unpack(), t128 = tiles128.unpack(), mask_ = mask.unpack();
     at::AutoDispatchBelowADInplaceOrView below;            // no derivative of its own
-    const Three all = structure_attention_backward(
-        grads[0], out.unpack(shared_from_this()), lse.unpack(), q.unpack(), k.unpack(), v.unpack(),
-        tiles32.unpack(), tiles128.unpack(), maybe(mask.unpack()), n_tokens, max_atoms, scale);
+    const Three all = structure_attention_backward(grads[0], out_, lse_, q_, k_, v_, t32, t128, maybe(mask_), n_tokens,
+                                                   max_atoms, scale);
     if (task_should_compute_output(0)) result[0] = std::get<0>(all);
     if (task_should_compute_output(1)) result[1] = std::get<1>(all);
     if (task_should_compute_output(2)) result[2] = std::get<2>(all);
