@@ -182,7 +182,8 @@ def plan_for(graph) -> AttentionPlan:
         if capturing(n_atoms.device):
             hold_captured(n_atoms, cached[2])
         return cached[2]
-    plan = attention_plan(n_atoms, graph.num_nodes)
+    with torch.inference_mode(False):                      # it serves a training step, too
+        plan = attention_plan(n_atoms, graph.num_nodes)
     object.__setattr__(graph, "_xnn_attention_plan", (n_atoms, key, plan))
     return plan
 

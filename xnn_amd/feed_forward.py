@@ -162,7 +162,8 @@ def species_plan_for(graph, n_groups: int) -> GroupPlan:
     key = (torch.cuda.current_stream(ids.device).cuda_stream, int(n_groups))
     plan = kept.plans.get(key)
     if plan is None:
-        plan = kept.plans[key] = group_plan(ids, n_groups)
+        with torch.inference_mode(False):                  # it serves a training step, too
+            plan = kept.plans[key] = group_plan(ids, n_groups)
     return plan
 
 

@@ -159,8 +159,10 @@ def plan_for(graph) -> EdgePlan:
     if (cached is not None and cached[0] is graph.edge_index and cached[1] is graph.cell_shifts
             and cached[2] == graph.num_nodes):
         return cached[3]
-    plan = build_plan(graph.edge_index, graph.cell_shifts, graph.num_nodes, graph.batch,
-                      graph.n_atoms, graph.pos, graph.cell)
+    # a plan that an evaluation in inference mode makes serves a training step, too
+    with torch.inference_mode(False):
+        plan = build_plan(graph.edge_index, graph.cell_shifts, graph.num_nodes, graph.batch,
+                          graph.n_atoms, graph.pos, graph.cell)
     object.__setattr__(graph, "_xnn_plan",
                        (graph.edge_index, graph.cell_shifts, graph.num_nodes, plan))
     return plan
