@@ -209,6 +209,22 @@ def test_a_captured_model_with_weights_of_species_follows_them(kept):
 
 
 @pytest.mark.gpu
+def test_a_backward_pass_whose_plan_a_capture_took_raises():
+    """Replays after a write to the numbers would give it others' weights."""
+    g = _graph()
+    x = torch.randn(g.num_nodes, 8, device="cuda", requires_grad=True)
+    w = torch.randn(9, 8, 8, device="cuda")
+    out = xa.grouped_linear(x, w, g.species_plan(9))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        g.species_plan(9)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        out.sum().backward()
+    xa.grouped_linear(x, w, g.species_plan(9)).sum().backward()
+    assert x.grad.isfinite().all()
+
+
+@pytest.mark.gpu
 def test_inference_numbers_that_were_written_to():
     with torch.inference_mode():
         ids = torch.tensor([1, 6, 8, 1], device="cuda")

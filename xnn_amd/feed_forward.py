@@ -124,7 +124,9 @@ class _KeptPlans:
 
 
 def _form_again(plan: GroupPlan, ids: Tensor) -> None:
-    """``plan`` formed in its own memory once more (from other ids, of another content)."""
+    """``plan`` formed in its own memory once more (from other ids, of another content). A backward pass of before that
+    has kept it is told, and raises."""
+    torch.autograd.graph.increment_version(plan.rows)
     ids = ids.to(torch.int64).contiguous()
     sizes = [ctypes.c_size_t(), ctypes.c_size_t()]
     _lib.call("xnn_group_plan_size", plan.n_rows, plan.n_groups, *map(ctypes.byref, sizes))
